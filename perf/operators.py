@@ -405,11 +405,16 @@ def _logprobs(s: dict) -> dict:
 # -- from the definitions, in 64 bits --------------------------------------------------------------
 
 
+def _power64(e: torch.Tensor) -> torch.Tensor:
+    """2^e from its bits: exact, as torch.ldexp on a GPU is not."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _stored64(x: torch.Tensor, largest: float) -> torch.Tensor:
     """What the format keeps of 64-bit rows: the nearest value of the block's grid, ties to the even code."""
     x = x.clamp(-largest, largest).unflatten(-1, (-1, BLOCK))
     m, e = torch.frexp(x.abs().amax(-1, keepdim=True))  # the maximum is m 2^e, m in [0.5, 1)
-    unit = torch.ldexp(torch.ones_like(m), (e - 3 + (m >= 0.875).to(e.dtype)).clamp(-125, 126))
+    unit = _power64((e - 3 + (m >= 0.875).to(e.dtype)).clamp(-125, 126))
     y = (x / unit).abs()
     # the step of the grid at y: 0.5 below 2, 1 below 4, 2 from there
     step = torch.where(y < 2, 0.5, torch.where(y < 4, 1.0, 2.0))
@@ -420,9 +425,9 @@ def _decoded64(code: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
     """The values of E2M1 bytes in 64 bits, from sign, exponent and mantissa bits."""
     nib = torch.stack((code & 15, code >> 4), dim=-1).flatten(-2).to(torch.int16)
     e, m = (nib >> 1) & 3, (nib & 1).double()
-    mag = torch.where(e == 0, 0.5 * m, torch.ldexp(1 + 0.5 * m, (e - 1).clamp(min=0)))
+    mag = torch.where(e == 0, 0.5 * m, (1 + 0.5 * m) * _power64((e - 1).clamp(min=0)))
     val = torch.where(nib >= 8, -mag, mag)
-    return val * torch.ldexp(torch.ones((), dtype=torch.float64, device=code.device), s.int() - 127).repeat_interleave(BLOCK, -1)
+    return val * _power64(s.int() - 127).repeat_interleave(BLOCK, -1)
 
 
 def _exact_rows(case: dict, seed: int) -> dict:
