@@ -103,6 +103,46 @@ KVH_API int kvh_reshape_and_cache_fp8(const void* k, int64_t k_tok_stride, int64
                               int32_t dtype, float k_scale, float v_scale, void* stream);
 
 /*
+ * MXFP4 KV cache (OCP microscaling). k_cache / v_cache hold E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and a sign), two to a byte, element 2i in the low nibble: [num_blocks, block_size, num_kv_heads,
+ * head_dim / 2] bytes, strides {block, slot, head} in BYTES. k_scale / v_scale hold one E8M0 byte s
+ * (the factor 2^(s - 127); 255: NaN) for every 32 consecutive elements of a row: [num_blocks,
+ * block_size, num_kv_heads, head_dim / 32] bytes with strides of their own. The last dimension is
+ * contiguous; pages that hold each head's tokens together (head stride above slot stride) are read
+ * in whole lines. The reference has no 4-bit cache; this one takes 4.25 bits an element.
+ *
+ * reshape_and_cache_fp4: kvh_reshape_and_cache into an MXFP4 cache; dtype is that of k and v (fp32,
+ * fp16 or bf16). Elements are clamped to +-1.5 2^15 (fp16) or +-1.5 2^127 (bf16, fp32), the largest
+ * value the format and the type both hold. With a the block's largest magnitude, s - 127 =
+ * floor(log2 a) - 2, one more where a >= 1.75 2^floor(log2 a) (no element is then off by more than
+ * half a step), s at least 2; elements are x / 2^(s - 127) rounded to nearest even, at most 6. A block
+ * with a NaN is stored under s = 255. head_dim a multiple of 32 up to 1024; k, v 16-byte aligned with
+ * strides multiples of 16 bytes; caches 4-byte aligned with strides multiples of 4; a page's rows
+ * within 2 GiB.
+ */
+KVH_API int kvh_reshape_and_cache_fp4(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                              const void* v, int64_t v_tok_stride, int64_t v_head_stride,
+                              void* k_cache, const int64_t k_cache_strides[3],
+                              void* k_scale, const int64_t k_scale_strides[3],
+                              void* v_cache, const int64_t v_cache_strides[3],
+                              void* v_scale, const int64_t v_scale_strides[3],
+                              const int64_t* slot_mapping, int64_t num_tokens, int64_t num_blocks,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                              int32_t dtype, void* stream);
+
+/* read_cache_fp4: the rows of an MXFP4 cache at slot_mapping as values of dtype (fp32, fp16 or bf16):
+ * k[t, h, :] and v[t, h, :] = e2m1 2^(s - 127) converted to dtype, zeros for slots outside the pool.
+ * Shapes and alignments as kvh_reshape_and_cache_fp4. */
+KVH_API int kvh_read_cache_fp4(const void* k_cache, const int64_t k_cache_strides[3],
+                       const void* k_scale, const int64_t k_scale_strides[3],
+                       const void* v_cache, const int64_t v_cache_strides[3],
+                       const void* v_scale, const int64_t v_scale_strides[3],
+                       const int64_t* slot_mapping, void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                       void* v, int64_t v_tok_stride, int64_t v_head_stride,
+                       int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t block_size, int32_t dtype, void* stream);
+
+/*
  * rope_and_cache: the step before attention in one pass. From this step's fused QKV
  * projection qkv [num_tokens, (num_heads + 2 num_kv_heads) head_dim] (token stride
  * qkv_tok_stride; query heads first, then key heads, then value heads) it computes, for
@@ -140,6 +180,20 @@ KVH_API int kvh_rope_and_cache_fp8(const void* qkv, int64_t qkv_tok_stride, cons
                            const int64_t* slot_mapping, int64_t num_tokens, int64_t num_blocks,
                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                            int32_t dtype, float k_scale, float v_scale, void* stream);
+
+/* rope_and_cache into MXFP4 caches (see reshape_and_cache_fp4). The rotation is computed in fp32 (two
+ * products and their sum, each rounded to fp32) and rounded once: the queries to dtype, the keys to the
+ * cache's format. head_dim a multiple of 64 up to 1024; the tables 16-byte aligned. */
+KVH_API int kvh_rope_and_cache_fp4(const void* qkv, int64_t qkv_tok_stride, const int64_t* positions,
+                           const float* cos_table, const float* sin_table, int64_t max_positions,
+                           void* q_out, int64_t q_tok_stride, int64_t q_head_stride,
+                           void* k_cache, const int64_t k_cache_strides[3],
+                           void* k_scale, const int64_t k_scale_strides[3],
+                           void* v_cache, const int64_t v_cache_strides[3],
+                           void* v_scale, const int64_t v_scale_strides[3],
+                           const int64_t* slot_mapping, int64_t num_tokens, int64_t num_blocks,
+                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                           int32_t dtype, void* stream);
 
 /*
  * prepare_metadata: one step's attention metadata, built on the device from block tables that
@@ -264,6 +318,27 @@ KVH_API int kvh_paged_attention_fp8(const void* q, int64_t q_tok_stride, int64_t
                             int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale,
                             float k_scale, float v_scale, int32_t dtype,
                             void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * kvh_paged_attention over MXFP4 caches (see reshape_and_cache_fp4). q and out are fp16 or bf16 (dtype);
+ * keys and values are converted to dtype for the MFMA contractions (exact in bf16; in fp16 where it
+ * holds them), P is rounded to dtype before P.V as in the 16-bit path. head_dim 64 or 128, block_size a
+ * multiple of 16; cache rows aligned to head_dim / 8 bytes, as their strides; workspace as
+ * kvh_paged_attention_workspace_size for the same shape and dtype. The bytes of slots past a sequence's
+ * end, scales included, may be anything.
+ */
+KVH_API int kvh_paged_attention_fp4(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                            const void* k_cache, const int64_t k_cache_strides[3],
+                            const void* k_scale, const int64_t k_scale_strides[3],
+                            const void* v_cache, const int64_t v_cache_strides[3],
+                            const void* v_scale, const int64_t v_scale_strides[3],
+                            int64_t num_blocks,
+                            void* out, int64_t o_tok_stride, int64_t o_head_stride,
+                            const int64_t* block_tables, int64_t bt_row_stride, int32_t max_blocks_per_seq,
+                            const int64_t* seq_lens, const int64_t* query_start_loc,
+                            int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale,
+                            int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Engine-harness kernels (no counterpart in the attention path; they serve the Llama layer

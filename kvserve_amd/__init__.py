@@ -15,6 +15,7 @@ from kvserve_amd.attention import (
     AttentionMetadata,
     HipAttention,
     build_metadata,
+    fp4_caches,
     get_backend,
     hip_available,
     hip_eligible,
@@ -26,6 +27,7 @@ __all__ = [
     "AttentionMetadata",
     "HipAttention",
     "build_metadata",
+    "fp4_caches",
     "get_backend",
     "hip_available",
     "hip_eligible",

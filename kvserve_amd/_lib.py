@@ -41,6 +41,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _f32,
          _vp],
     ),
+    "kvh_reshape_and_cache_fp4": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _i64, _vp, _i64, _i64,  # k, v
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p,  # caches, each with its scales
+            _vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp,  # slots, sizes, dtype, stream
+        ],  # fmt: skip
+    ),
+    "kvh_read_cache_fp4": (
+        ctypes.c_int,
+        [
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p,  # caches, each with its scales
+            _vp, _vp, _i64, _i64, _vp, _i64, _i64,  # slots, k, v
+            _i64, _i64, _i32, _i32, _i32, _i32, _vp,  # sizes, dtype, stream
+        ],  # fmt: skip
+    ),
     "kvh_rope_and_cache": (
         ctypes.c_int,
         [
@@ -57,6 +73,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _vp, _i64, _i64,  # q_out
             _vp, _i64p, _vp, _i64p,  # caches
             _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _vp,  # slots, sizes, dtype, scales, stream
+        ],  # fmt: skip
+    ),
+    "kvh_rope_and_cache_fp4": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _vp, _vp, _vp, _i64,  # qkv, positions, cos/sin tables
+            _vp, _i64, _i64,  # q_out
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p,  # caches, each with its scales
+            _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp,  # slots, sizes, dtype, stream
         ],  # fmt: skip
     ),
     "kvh_gemv_rope_and_cache": (
@@ -113,6 +138,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _vp, _i64, _i32,  # block tables
             _vp, _vp,  # seq_lens, query_start_loc
             _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _f32, _i32,  # sizes, scales, dtype
+            _vp, _sz, _vp,  # workspace, stream
+        ],  # fmt: skip
+    ),
+    "kvh_paged_attention_fp4": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _i64,  # q
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _i64,  # caches, each with its scales, num_blocks
+            _vp, _i64, _i64,  # out
+            _vp, _i64, _i32,  # block tables
+            _vp, _vp,  # seq_lens, query_start_loc
+            _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,  # sizes, scale, dtype
             _vp, _sz, _vp,  # workspace, stream
         ],  # fmt: skip
     ),

@@ -117,6 +117,8 @@ FP8 = torch.float8_e4m3fn
 def _kv_format(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float, v_scale: float) -> bool:
     """True for E4M3 caches (scales positive and finite); 16-bit / fp32 caches take no scales."""
     fp8 = k_cache.dtype == FP8
+    for s in (k_scale, v_scale):
+        _require(not (isinstance(s, torch.Tensor) and s.dtype == E8M0), "E8M0 scales belong to float4_e2m1fn_x2 caches")
     _require(v_cache.dtype == k_cache.dtype, f"k/v cache dtypes differ: {k_cache.dtype}, {v_cache.dtype}")
     if fp8:
         _require(all(0.0 < float(x) < float("inf") for x in (k_scale, v_scale)), "FP8 scales must be positive, finite")
@@ -125,9 +127,151 @@ def _kv_format(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float, v_s
     return fp8
 
 
+# MXFP4 KV caches (the *_fp4 entry points): float4_e2m1fn_x2 tensors, two elements to a byte, with a float8_e8m0fnu
+# tensor each that holds one power of two for every 32 elements of a row.
+FP4 = torch.float4_e2m1fn_x2
+E8M0 = torch.float8_e8m0fnu
+FP4_BLOCK = 32
+
+
+def fp4_caches(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+               device: torch.device | str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+    """(k_cache, v_cache, k_scale, v_scale) of an empty MXFP4 cache: float4_e2m1fn_x2 tensors [num_blocks, block_size,
+    kv_heads, D / 2] and float8_e8m0fnu tensors [.., D / 32]. A page holds each head's tokens together (the tensors
+    are permuted views of [num_blocks, kv_heads, block_size, ..]), so that the attention reads whole lines: a token's
+    row of one head is only 64 bytes at D = 128. Any other strides with a contiguous last dim are taken too."""
+    _require(head_dim > 0 and head_dim % FP4_BLOCK == 0, f"4-bit caches need head sizes in 32s, not {head_dim}")
+
+    def pages(width: int, dtype: torch.dtype) -> torch.Tensor:
+        raw = torch.zeros((num_blocks, num_kv_heads, block_size, width), dtype=torch.uint8, device=device)
+        return raw.permute(0, 2, 1, 3).view(dtype)
+
+    k, v = (pages(head_dim // 2, FP4) for _ in range(2))
+    k_scale, v_scale = (pages(head_dim // FP4_BLOCK, E8M0) for _ in range(2))
+    return k, v, k_scale, v_scale
+
+
+def _fp4_layout(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> tuple:
+    """(num_blocks, block_size, kv_heads, head_dim, device index) of MXFP4 caches and their scales, checked."""
+    _require(v_cache.dtype == FP4, f"k/v cache dtypes differ: {k_cache.dtype}, {v_cache.dtype}")
+    for s in (k_scale, v_scale):
+        _require(isinstance(s, torch.Tensor) and s.dtype == E8M0,
+                 "float4_e2m1fn_x2 caches need k_scale and v_scale as float8_e8m0fnu tensors")  # fmt: skip
+    _check_cache(k_cache, v_cache)
+    num_blocks, block_size, num_kv_heads, packed = k_cache.shape
+    head_dim = 2 * packed
+    _require(head_dim % FP4_BLOCK == 0, f"4-bit caches need head sizes in 32s, not {head_dim}")
+    want = (num_blocks, block_size, num_kv_heads, head_dim // FP4_BLOCK)
+    for s in (k_scale, v_scale):
+        _require(s.shape == want and s.stride(-1) == 1, f"scales must be {list(want)} with a contiguous last dim")
+    dev = k_cache.get_device()
+    _on_device(dev, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    return num_blocks, block_size, num_kv_heads, head_dim, dev
+
+
+def _fp4_args(*caches: torch.Tensor) -> list:
+    """Address and strides of each, as the C ABI takes them."""
+    return [x for t in caches for x in (t.data_ptr(), _lib.i64x3(t.stride()[:3]))]
+
+
+def _write_kv_fp4(k_cache, v_cache, k, v, slots, k_scale, v_scale) -> None:
+    num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
+    _on_device(dev, k=k, v=v, slot_mapping=slots)
+    _require(k.dim() == 3 and k.shape == v.shape, "k and v must be [T, kv_heads, head_dim]")
+    _require(k.shape[1:] == (num_kv_heads, head_dim), f"k/v rows {tuple(k.shape[1:])} != cache rows")
+    _require(k.stride(-1) == 1 and v.stride(-1) == 1, "k/v last dim must be contiguous")
+    _check_index(slots, "slot_mapping", 1)
+    _require(slots.shape[0] == k.shape[0], "one slot per token")
+    st = _lib.load().kvh_reshape_and_cache_fp4(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.shape[0], num_blocks, num_kv_heads,
+        head_dim, block_size, _dtype_code(k, v), _stream_handle(k_cache.device),
+    )  # fmt: skip
+    _lib.check(st, "kvh_reshape_and_cache_fp4")
+
+
+def _rope_and_cache_fp4(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, out, k_scale,
+                        v_scale) -> torch.Tensor:  # fmt: skip
+    num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
+    out = _check_rope(qkv, positions, cos, sin, slots, num_heads, num_kv_heads, head_dim, dev, out)
+    dtype = _dtype_code(qkv, out)
+    if qkv.shape[0] == 0:
+        return out
+    st = _lib.load().kvh_rope_and_cache_fp4(
+        qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        out.data_ptr(), out.stride(0), out.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale),
+        slots.data_ptr(), qkv.shape[0], num_blocks, num_heads, num_kv_heads, head_dim, block_size, dtype,
+        _stream_handle(qkv.device),
+    )  # fmt: skip
+    _lib.check(st, "kvh_rope_and_cache_fp4")
+    return out
+
+
+def _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale) -> torch.Tensor:
+    num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
+    out, tables, seq_lens, qsl = _check_attention(q, meta, num_kv_heads, head_dim, dev, out)
+    _require(q.dtype != torch.float32, "float4_e2m1fn_x2 caches need bf16 or fp16 queries")
+    dtype = _dtype_code(q, out)
+    num_tokens, num_heads, _ = q.shape
+    num_seqs, width = tables.shape
+    if num_tokens == 0 or num_seqs == 0:
+        return out
+    lib = _lib.load()
+    max_q = int(meta.max_query_len)
+    ws_bytes = _workspace_size(lib, num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, width, block_size, max_q,
+                               dtype)  # fmt: skip
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    st = lib.kvh_paged_attention_fp4(
+        q.data_ptr(), q.stride(0), q.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale), num_blocks,
+        out.data_ptr(), out.stride(0), out.stride(1), tables.data_ptr(), tables.stride(0), width,
+        seq_lens.data_ptr(), qsl.data_ptr(), num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+        max_q, float(scale), dtype, ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(q.device),
+    )  # fmt: skip
+    _lib.check(st, "kvh_paged_attention_fp4")
+    return out
+
+
 def _check_index(t: torch.Tensor, name: str, dim: int) -> None:
     _require(t.dtype == torch.int64, f"{name} must be int64 (got {t.dtype})")
     _require(t.dim() == dim and t.stride(-1) == 1, f"{name} must be {dim}-d with a contiguous last dim")
+
+
+def _check_rope(qkv, positions, cos, sin, slots, num_heads, num_kv_heads, head_dim, dev, out) -> torch.Tensor:
+    """rope_and_cache's arguments, whatever the cache; returns the output (a new one where `out` is None)."""
+    _on_device(dev, qkv=qkv, positions=positions, cos=cos, sin=sin, slot_mapping=slots)
+    _require(qkv.dim() == 2 and qkv.stride(-1) == 1, "qkv must be [T, (H + 2 Hkv) D] with a contiguous last dim")
+    _require(qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim, "qkv width != (H + 2 Hkv) D")
+    _require(cos.dtype == torch.float32 and sin.dtype == torch.float32, "cos/sin tables must be fp32")
+    _require(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == head_dim, "cos/sin must be [P, D]")
+    _require(cos.is_contiguous() and sin.is_contiguous(), "cos/sin tables must be contiguous")
+    _check_index(positions, "positions", 1)
+    _check_index(slots, "slot_mapping", 1)
+    num_tokens = qkv.shape[0]
+    _require(positions.shape[0] == num_tokens and slots.shape[0] == num_tokens, "one position and slot per token")
+    if out is None:
+        out = torch.empty((num_tokens, num_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+    _on_device(dev, out=out)
+    _require(out.shape == (num_tokens, num_heads, head_dim) and out.stride(-1) == 1, "out must be [T, H, D]")
+    return out
+
+
+def _check_attention(q, meta, num_kv_heads, head_dim, dev, out) -> tuple:
+    """forward's arguments, whatever the cache; returns the output (a new one where `out` is None) and the metadata."""
+    tables, seq_lens, qsl = meta.block_tables, meta.seq_lens, meta.query_start_loc
+    _on_device(dev, q=q, block_tables=tables, seq_lens=seq_lens, query_start_loc=qsl)
+    _require(q.dim() == 3 and q.shape[2] == head_dim, "q must be [T, H, head_dim]")
+    _require(q.stride(-1) == 1, "q last dim must be contiguous")
+    _require(q.shape[1] % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
+    _check_index(tables, "block_tables", 2)
+    _check_index(seq_lens, "seq_lens", 1)
+    _check_index(qsl, "query_start_loc", 1)
+    num_seqs = tables.shape[0]
+    _require(seq_lens.shape[0] == num_seqs and qsl.shape[0] == num_seqs + 1, "metadata sizes disagree")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _on_device(dev, out=out)
+    _require(out.shape == q.shape and out.stride(-1) == 1, "out must match q with a contiguous last dim")
+    return out, tables, seq_lens, qsl
 
 
 def _calls():
@@ -166,7 +310,11 @@ class HipAttention:
         any token/head stride (v is typically a strided view of the fused QKV output).
         Slots outside the pool are skipped instead of raising. float8_e4m3fn caches store
         (x / scale).clamp(-448, 448).to(float8_e4m3fn) with the given scales, bit for bit.
+        float4_e2m1fn_x2 caches [num_blocks, block_size, kv_heads, D / 2] store MXFP4 rows, their powers of two
+        in k_scale and v_scale (float8_e8m0fnu [.., D / 32]; kvh_reshape_and_cache_fp4).
         """
+        if k_cache.dtype == FP4:
+            return _write_kv_fp4(k_cache, v_cache, k, v, slots, k_scale, v_scale)
         calls = _calls()
         if calls is not None:
             r = calls.write_kv(k_cache, v_cache, k, v, slots, k_scale, v_scale)
@@ -202,6 +350,32 @@ class HipAttention:
         )  # fmt: skip
         _lib.check(st, "kvh_reshape_and_cache")
 
+    @staticmethod
+    def read_kv(
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        slots: torch.Tensor,
+        dtype: torch.dtype,
+        k_scale: torch.Tensor,
+        v_scale: torch.Tensor,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [T, kv_heads, D] in `dtype` (bf16, fp16 or fp32): the rows of a float4_e2m1fn_x2 cache at `slots`,
+        zeros for slots outside the pool. (The other caches' rows are cache.flatten(0, 1)[slots] in torch.)"""
+        _require(k_cache.dtype == FP4, f"read_kv reads float4_e2m1fn_x2 caches, not {k_cache.dtype}")
+        num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
+        _on_device(dev, slots=slots)
+        _check_index(slots, "slots", 1)
+        _require(dtype in _lib.KVH_DTYPE, f"unsupported dtype {dtype} (float32, float16, bfloat16)")
+        shape = (slots.shape[0], num_kv_heads, head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+        st = _lib.load().kvh_read_cache_fp4(
+            *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), slots.shape[0], num_blocks, num_kv_heads, head_dim, block_size,
+            _lib.KVH_DTYPE[dtype], _stream_handle(k_cache.device),
+        )  # fmt: skip
+        _lib.check(st, "kvh_read_cache_fp4")
+        return k, v
+
     # Extension beyond the reference's interface: RoPE + QKV split + write_kv in one kernel.
     fused_rope_cache = True
 
@@ -226,8 +400,12 @@ class HipAttention:
         positions: int64 [T]; cos, sin: fp32 [max_positions, head_dim] (RotaryEmbedding's
         tables). Writes RoPE(k) and v into the caches at `slots` (as write_kv) and returns
         RoPE(q) as [T, num_heads, head_dim] (in `out` if given), bit-identical to the
-        reference's bf16/fp16/fp32 torch operations.
+        reference's bf16/fp16/fp32 torch operations. Over float4_e2m1fn_x2 caches (scales as write_kv) the
+        rotation is computed in fp32 and rounded once, q to its type, k to the cache's.
         """
+        if k_cache.dtype == FP4:
+            return _rope_and_cache_fp4(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, out, k_scale,
+                                       v_scale)  # fmt: skip
         calls = _calls()
         if calls is not None:
             r = calls.rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, out, k_scale, v_scale)
@@ -237,20 +415,8 @@ class HipAttention:
                 return r
         num_blocks, block_size, num_kv_heads, head_dim, kcs, vcs, dev = _cache_layout(k_cache, v_cache)
         fp8 = _kv_format(k_cache, v_cache, k_scale, v_scale)
-        _on_device(dev, qkv=qkv, positions=positions, cos=cos, sin=sin, slot_mapping=slots)
-        _require(qkv.dim() == 2 and qkv.stride(-1) == 1, "qkv must be [T, (H + 2 Hkv) D] with a contiguous last dim")
-        _require(qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim, "qkv width != (H + 2 Hkv) D")
-        _require(cos.dtype == torch.float32 and sin.dtype == torch.float32, "cos/sin tables must be fp32")
-        _require(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == head_dim, "cos/sin must be [P, D]")
-        _require(cos.is_contiguous() and sin.is_contiguous(), "cos/sin tables must be contiguous")
-        _check_index(positions, "positions", 1)
-        _check_index(slots, "slot_mapping", 1)
+        out = _check_rope(qkv, positions, cos, sin, slots, num_heads, num_kv_heads, head_dim, dev, out)
         num_tokens = qkv.shape[0]
-        _require(positions.shape[0] == num_tokens and slots.shape[0] == num_tokens, "one position and slot per token")
-        if out is None:
-            out = torch.empty((num_tokens, num_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
-        _on_device(dev, out=out)
-        _require(out.shape == (num_tokens, num_heads, head_dim) and out.stride(-1) == 1, "out must be [T, H, D]")
         dtype = _dtype_code(qkv, out) if fp8 else _dtype_code(qkv, k_cache, v_cache, out)
         if num_tokens == 0:
             return out
@@ -285,7 +451,8 @@ class HipAttention:
         """rope_and_cache(x @ w_qkv.T, ...) in one kernel (kvh_gemv_rope_and_cache) for at most
         GEMV_ROPE_MAX_ROWS rows of 16-bit x: the same bits as the projection on kvh_gemv (up to 4
         rows) or kvh_gemm_skinny (more; hidden % 1024 == 0, head_dim % 16 == 0) followed by
-        rope_and_cache. x: [T, hidden]; w_qkv: [(H + 2 Hkv) D, hidden], contiguous."""
+        rope_and_cache. x: [T, hidden]; w_qkv: [(H + 2 Hkv) D, hidden], contiguous. Not over 4-bit caches."""
+        _require(k_cache.dtype != FP4, "gemv_rope_and_cache does not write float4_e2m1fn_x2 caches: use rope_and_cache")
         num_blocks, block_size, num_kv_heads, head_dim, kcs, vcs, dev = _cache_layout(k_cache, v_cache)
         fp8 = _kv_format(k_cache, v_cache, k_scale, v_scale)
         _on_device(dev, x=x, w_qkv=w_qkv, positions=positions, cos=cos, sin=sin, slot_mapping=slots)
@@ -328,7 +495,10 @@ class HipAttention:
         v_scale: float = 1.0,
     ) -> torch.Tensor:
         """q: [T, H, D]; caches: [num_blocks, block_size, H_kv, D]. Returns [T, H, D] (in `out` if given).
-        float8_e4m3fn caches hold keys / values as e4m3 * k_scale / v_scale (q and out bf16 or fp16)."""
+        float8_e4m3fn caches hold keys / values as e4m3 * k_scale / v_scale (q and out bf16 or fp16);
+        float4_e2m1fn_x2 caches as MXFP4, k_scale and v_scale their float8_e8m0fnu tensors (see write_kv)."""
+        if k_cache.dtype == FP4:
+            return _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale)
         calls = _calls()
         if calls is not None:
             r = calls.forward(q, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.query_start_loc,
@@ -339,21 +509,9 @@ class HipAttention:
                 return r
         num_blocks, block_size, num_kv_heads, head_dim, kcs, vcs, dev = _cache_layout(k_cache, v_cache)
         fp8 = _kv_format(k_cache, v_cache, k_scale, v_scale)
-        tables, seq_lens, qsl = meta.block_tables, meta.seq_lens, meta.query_start_loc
-        _on_device(dev, q=q, block_tables=tables, seq_lens=seq_lens, query_start_loc=qsl)
-        _require(q.dim() == 3 and q.shape[2] == head_dim, "q must be [T, H, head_dim]")
-        _require(q.stride(-1) == 1, "q last dim must be contiguous")
+        out, tables, seq_lens, qsl = _check_attention(q, meta, num_kv_heads, head_dim, dev, out)
         num_tokens, num_heads, _ = q.shape
-        _require(num_heads % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
-        _check_index(tables, "block_tables", 2)
-        _check_index(seq_lens, "seq_lens", 1)
-        _check_index(qsl, "query_start_loc", 1)
         num_seqs = tables.shape[0]
-        _require(seq_lens.shape[0] == num_seqs and qsl.shape[0] == num_seqs + 1, "metadata sizes disagree")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _on_device(dev, out=out)
-        _require(out.shape == q.shape and out.stride(-1) == 1, "out must match q with a contiguous last dim")
         dtype = _dtype_code(q, out) if fp8 else _dtype_code(q, k_cache, v_cache, out)
         _require(not fp8 or q.dtype != torch.float32, "float8_e4m3fn caches need bf16 or fp16 queries")
         if num_tokens == 0 or num_seqs == 0:

@@ -32,11 +32,13 @@ LIB = LIB_DIR / "libkvhip.so"
 INCLUDE = PKG.parent / "include"
 
 SOURCES = [
+    "cache_fp4.hip",
     "engine_ops.hip",
     "kvh_api.hip",
     "metadata.hip",
     "paged_attention.hip",
     "paged_attention_f32.hip",
+    "paged_attention_kv4.hip",
     "probes.hip",
     "reshape_and_cache.hip",
     "rope_and_cache.hip",
@@ -45,8 +47,13 @@ SOURCES = [
 # Per-source additions. The MFMA kernels treat scores as finite (masked keys become -inf by
 # selects, never by arithmetic on NaN), so fmaxf needs no sNaN canonicalisation: without
 # -fno-honor-nans every max of an MFMA result costs an extra v_max_f32 x, x, x.
-# rope_and_cache reproduces PyTorch's separately rounded multiply and add: no FMA contraction.
-SOURCE_FLAGS = {"paged_attention.hip": ["-fno-honor-nans"], "rope_and_cache.hip": ["-ffp-contract=off"]}
+# rope_and_cache and cache_fp4 reproduce PyTorch's separately rounded multiply and add: no FMA contraction.
+SOURCE_FLAGS = {
+    "paged_attention.hip": ["-fno-honor-nans"],
+    "paged_attention_kv4.hip": ["-fno-honor-nans"],
+    "rope_and_cache.hip": ["-ffp-contract=off"],
+    "cache_fp4.hip": ["-ffp-contract=off"],
+}
 
 # -packed-fp32-ops: keep hipcc from emitting v_pk_{add,mul,fma}_f32 (unreliable on these
 # hosts); the host pass warns that it does not know the feature, which is harmless.
@@ -164,8 +171,8 @@ def build(
 
     jobs = min(len(SOURCES), int(os.environ.get("MAX_JOBS", "8")), 16)
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
-        # the slowest compilation (paged_attention) starts first
-        order = sorted(SOURCES, key=lambda s: s != "paged_attention.hip")
+        # the slowest compilations (paged_attention*) start first
+        order = sorted(SOURCES, key=lambda s: not s.startswith("paged_attention"))
         futs = {s: ex.submit(compile_one, s) for s in order}
         built = [futs[s].result() for s in SOURCES]
     objs = [obj for obj, _ in built]

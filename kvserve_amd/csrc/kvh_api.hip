@@ -196,6 +196,124 @@ int kvh_reshape_and_cache_fp8(const void* k, int64_t k_tok_stride, int64_t k_hea
 
 }  // extern "C"
 
+// The caches of the *_fp4 entry points: packed rows of head_dim / 2 bytes in 4-byte granules (`wide`: the
+// attention's loads of an eighth of head_dim bytes), E8M0 rows of head_dim / 32 bytes.
+static int fp4_caches(int32_t head_dim, int32_t block_size, void* k_cache, const int64_t k_cache_strides[3], void* k_scale, const int64_t k_scale_strides[3], void* v_cache,
+                      const int64_t v_cache_strides[3], void* v_scale, const int64_t v_scale_strides[3], bool wide,
+                      Fp4Cache* kc, Fp4Cache* vc) {
+  if (!k_cache || !k_cache_strides || !k_scale || !k_scale_strides || !v_cache || !v_cache_strides || !v_scale ||
+      !v_scale_strides)
+    return KVH_E_NULL;
+  const int64_t* const rows[] = {k_cache_strides, v_cache_strides};
+  const int64_t* const scales[] = {k_scale_strides, v_scale_strides};
+  const int align = wide ? (head_dim >= 128 ? 16 : 8) : 4;
+  for (const int64_t* st : rows)
+    for (int i = 0; i < 3; ++i) {
+      if (st[i] < 0) return KVH_E_SHAPE;
+      if (st[i] % align) return KVH_E_ALIGN;
+    }
+  for (const int64_t* st : scales)
+    for (int i = 0; i < 3; ++i)
+      if (st[i] < 0) return KVH_E_SHAPE;
+  // a page's rows lie within 2 GiB (32-bit offsets inside a page)
+  for (const int64_t* const* set : {rows, scales})
+    for (int i = 0; i < 2; ++i)
+      if (set[i][1] > 0x7fffffffLL / block_size) return KVH_E_UNSUPPORTED;
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) & (uintptr_t)(align - 1)) return KVH_E_ALIGN;
+  *kc = Fp4Cache{(uint8_t*)k_cache, k_cache_strides[0], k_cache_strides[1], k_cache_strides[2],
+                 (uint8_t*)k_scale, k_scale_strides[0], k_scale_strides[1], k_scale_strides[2]};
+  *vc = Fp4Cache{(uint8_t*)v_cache, v_cache_strides[0], v_cache_strides[1], v_cache_strides[2],
+                 (uint8_t*)v_scale, v_scale_strides[0], v_scale_strides[1], v_scale_strides[2]};
+  return KVH_OK;
+}
+
+static int check_fp4_rows(int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t block_size, int32_t dtype) {
+  if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
+  if (num_tokens < 0 || num_blocks < 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0) return KVH_E_SHAPE;
+  if (num_tokens > 0x7fffffffLL || num_blocks > INT64_MAX / block_size) return KVH_E_SHAPE;
+  if (head_dim % kFp4Block != 0 || head_dim > 1024 || num_kv_heads > 65535) return KVH_E_UNSUPPORTED;
+  return KVH_OK;
+}
+
+// Rows of 16-byte vectors at p, token and head strides in elements.
+static int check_fp4_tensor(const void* p, int64_t tok_stride, int64_t head_stride, int32_t dtype) {
+  if (!p) return KVH_E_NULL;
+  const int vec = 16 / elem_bytes(dtype);
+  if (tok_stride < 0 || head_stride < 0) return KVH_E_SHAPE;
+  return tok_stride % vec || head_stride % vec || !aligned16(p) ? KVH_E_ALIGN : KVH_OK;
+}
+
+extern "C" {
+
+int kvh_reshape_and_cache_fp4(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                              int64_t v_tok_stride, int64_t v_head_stride, void* k_cache,
+                              const int64_t k_cache_strides[3], void* k_scale, const int64_t k_scale_strides[3],
+                              void* v_cache, const int64_t v_cache_strides[3], void* v_scale,
+                              const int64_t v_scale_strides[3], const int64_t* slot_mapping, int64_t num_tokens,
+                              int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                              int32_t dtype, void* stream) {
+  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  if (st != KVH_OK || num_tokens == 0) return st;
+  if ((st = check_fp4_tensor(k, k_tok_stride, k_head_stride, dtype)) != KVH_OK) return st;
+  if ((st = check_fp4_tensor(v, v_tok_stride, v_head_stride, dtype)) != KVH_OK) return st;
+  if (!slot_mapping) return KVH_E_NULL;
+  Fp4Cache kc, vc;
+  st = fp4_caches(head_dim, block_size, k_cache, k_cache_strides, k_scale, k_scale_strides, v_cache,
+                  v_cache_strides, v_scale, v_scale_strides, false, &kc, &vc);
+  if (st != KVH_OK) return st;
+  return launch_reshape_and_cache_fp4(k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride, kc, vc,
+                                      slot_mapping, num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype,
+                                      (hipStream_t)stream);
+}
+
+int kvh_rope_and_cache_fp4(const void* qkv, int64_t qkv_tok_stride, const int64_t* positions, const float* cos_table,
+                           const float* sin_table, int64_t max_positions, void* q_out, int64_t q_tok_stride,
+                           int64_t q_head_stride, void* k_cache, const int64_t k_cache_strides[3], void* k_scale,
+                           const int64_t k_scale_strides[3], void* v_cache, const int64_t v_cache_strides[3],
+                           void* v_scale, const int64_t v_scale_strides[3], const int64_t* slot_mapping,
+                           int64_t num_tokens, int64_t num_blocks, int32_t num_heads, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t block_size, int32_t dtype, void* stream) {
+  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  if (st != KVH_OK) return st;
+  if (num_heads <= 0 || max_positions <= 0) return KVH_E_SHAPE;
+  if (head_dim % (2 * kFp4Block) != 0 || num_heads > 65535) return KVH_E_UNSUPPORTED;  // half a row is whole blocks
+  if (num_tokens == 0) return KVH_OK;
+  if (!positions || !cos_table || !sin_table || !slot_mapping) return KVH_E_NULL;
+  if (((uintptr_t)cos_table | (uintptr_t)sin_table) & 15u) return KVH_E_ALIGN;
+  if ((st = check_fp4_tensor(qkv, qkv_tok_stride, 0, dtype)) != KVH_OK) return st;
+  if ((st = check_fp4_tensor(q_out, q_tok_stride, q_head_stride, dtype)) != KVH_OK) return st;
+  if (qkv_tok_stride < ((int64_t)num_heads + 2 * (int64_t)num_kv_heads) * head_dim) return KVH_E_SHAPE;
+  Fp4Cache kc, vc;
+  st = fp4_caches(head_dim, block_size, k_cache, k_cache_strides, k_scale, k_scale_strides, v_cache,
+                  v_cache_strides, v_scale, v_scale_strides, false, &kc, &vc);
+  if (st != KVH_OK) return st;
+  return launch_rope_and_cache_fp4(qkv, qkv_tok_stride, positions, cos_table, sin_table, max_positions, q_out,
+                                   q_tok_stride, q_head_stride, kc, vc, slot_mapping, num_tokens, num_blocks,
+                                   num_heads, num_kv_heads, head_dim, block_size, dtype, (hipStream_t)stream);
+}
+
+int kvh_read_cache_fp4(const void* k_cache, const int64_t k_cache_strides[3], const void* k_scale,
+                       const int64_t k_scale_strides[3], const void* v_cache, const int64_t v_cache_strides[3],
+                       const void* v_scale, const int64_t v_scale_strides[3], const int64_t* slot_mapping, void* k,
+                       int64_t k_tok_stride, int64_t k_head_stride, void* v, int64_t v_tok_stride,
+                       int64_t v_head_stride, int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads,
+                       int32_t head_dim, int32_t block_size, int32_t dtype, void* stream) {
+  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  if (st != KVH_OK || num_tokens == 0) return st;
+  if ((st = check_fp4_tensor(k, k_tok_stride, k_head_stride, dtype)) != KVH_OK) return st;
+  if ((st = check_fp4_tensor(v, v_tok_stride, v_head_stride, dtype)) != KVH_OK) return st;
+  if (!slot_mapping) return KVH_E_NULL;
+  Fp4Cache kc, vc;
+  st = fp4_caches(head_dim, block_size, (void*)k_cache, k_cache_strides, (void*)k_scale, k_scale_strides,
+                  (void*)v_cache, v_cache_strides, (void*)v_scale, v_scale_strides, false, &kc, &vc);
+  if (st != KVH_OK) return st;
+  return launch_read_cache_fp4(kc, vc, slot_mapping, k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride,
+                               num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"
+
 static int rope_and_cache_impl(const void* qkv, int64_t qkv_tok_stride, const int64_t* positions,
                                const float* cos_table, const float* sin_table, int64_t max_positions, void* q_out,
                                int64_t q_tok_stride, int64_t q_head_stride, void* k_cache,
@@ -332,7 +450,8 @@ size_t kvh_paged_attention_workspace_size(int64_t num_tokens, int32_t num_seqs, 
 
 }  // extern "C"
 
-// kvh_paged_attention and kvh_paged_attention_fp8 (kv8: E4M3 caches with scales k_scale, v_scale).
+// kvh_paged_attention (kv: kKv16), kvh_paged_attention_fp8 (kKv8: E4M3 caches with scales k_scale, v_scale) and
+// kvh_paged_attention_fp4 (kKv4: MXFP4 caches, whose E8M0 bytes are kx, vx).
 static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
                                 const int64_t k_cache_strides[3], const void* v_cache,
                                 const int64_t v_cache_strides[3], int64_t num_blocks, void* out, int64_t o_tok_stride,
@@ -340,8 +459,9 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int32_t max_blocks_per_seq, const int64_t* seq_lens, const int64_t* query_start_loc,
                                 int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                 int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale,
-                                int32_t dtype, bool kv8, float k_scale, float v_scale, void* workspace,
-                                size_t workspace_bytes, void* stream) {
+                                int32_t dtype, int32_t kv, float k_scale, float v_scale, const void* kx,
+                                const int64_t kx_strides[3], const void* vx, const int64_t vx_strides[3],
+                                void* workspace, size_t workspace_bytes, void* stream) {
   // the timing hook covers exactly one call, whatever its outcome
   LaunchLog log;
   void* armed[8];
@@ -359,8 +479,8 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
     return KVH_E_NULL;
   // num_blocks >= 1: the kernels read block 0 in place of an absent tile (and mask it out)
   if (num_blocks < 1 || bt_row_stride < max_blocks_per_seq) return KVH_E_SHAPE;
-  if (kv8) {
-    // E4M3 caches feed the 16-bit MFMA path only
+  if (kv != kKv16) {
+    // E4M3 and MXFP4 caches feed the 16-bit MFMA path only
     if (dtype == KVH_DTYPE_F32 || !mfma_shape(head_dim, block_size, num_heads / num_kv_heads))
       return KVH_E_UNSUPPORTED;
     if (!(k_scale > 0.f && k_scale < INFINITY && v_scale > 0.f && v_scale < INFINITY)) return KVH_E_SHAPE;
@@ -372,9 +492,19 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   for (int i = 0; i < 10; ++i) {
     if (strides[i] < 0) return KVH_E_SHAPE;
     // E4M3 cache rows are read 16 bytes at a time: 16 one-byte elements
-    if (strides[i] % (kv8 && i >= 4 ? 16 : vec_elems)) return KVH_E_ALIGN;
+    // (MXFP4: fp4_caches)
+    if (kv != kKv4 || i < 4)
+      if (strides[i] % (kv == kKv8 && i >= 4 ? 16 : vec_elems)) return KVH_E_ALIGN;
   }
-  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return KVH_E_ALIGN;
+  if (!aligned16(q) || !aligned16(out)) return KVH_E_ALIGN;
+  Fp4Cache kc{}, vc{};
+  if (kv == kKv4) {
+    st = fp4_caches(head_dim, block_size, (void*)k_cache, k_cache_strides, (void*)kx, kx_strides,
+                    (void*)v_cache, v_cache_strides, (void*)vx, vx_strides, true, &kc, &vc);
+    if (st != KVH_OK) return st;
+  } else if (!aligned16(k_cache) || !aligned16(v_cache)) {
+    return KVH_E_ALIGN;
+  }
 
   const Plan plan = make_plan(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, max_blocks_per_seq, block_size,
                               max_query_len, dtype);
@@ -409,8 +539,16 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   p.G = plan.G;
   p.BS = block_size;
   p.scale = scale;
-  p.qk_scale = scale * kLog2e * (kv8 ? k_scale : 1.f);
-  p.v_scale = kv8 ? v_scale : 1.f;
+  p.qk_scale = scale * kLog2e * (kv == kKv8 ? k_scale : 1.f);
+  p.v_scale = kv == kKv8 ? v_scale : 1.f;
+  p.kx = kc.x;
+  p.kx_sb = kc.xsb;
+  p.kx_ss = kc.xss;
+  p.kx_sh = kc.xsh;
+  p.vx = vc.x;
+  p.vx_sb = vc.xsb;
+  p.vx_ss = vc.xss;
+  p.vx_sh = vc.xsh;
   p.QS = plan.QS;
   p.RS = plan.RS;
   p.HGW = plan.HGW;
@@ -418,7 +556,7 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   p.NUP = 0;  // set by the prefill launcher likewise
   p.CASC = 0;  // set by the launcher when the plan has the cascade path
   {
-    const int nx = cascade_tiles(plan.NX, kv8);  // cascade prefix group: 16-row tiles (see make_plan)
+    const int nx = cascade_tiles(plan.NX, kv != kKv16);  // cascade prefix group: 16-row tiles (see make_plan)
     p.XR = 16 * nx;
     p.SG = cascade_group(plan.RS, nx);
   }
@@ -460,7 +598,7 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   if (dtype == KVH_DTYPE_F32 || !mfma_shape(head_dim, block_size, plan.G))
     st = launch_paged_attention_valu(p, head_dim, dtype, max_query_len < 1 ? 1 : max_query_len, s, log);
   else
-    st = launch_paged_attention_mfma(p, plan, head_dim, dtype, kv8, max_query_len < 1 ? 1 : max_query_len, s, log);
+    st = launch_paged_attention_mfma(p, plan, head_dim, dtype, kv, max_query_len < 1 ? 1 : max_query_len, s, log);
   g_prof.last_count = log.launched;
   for (int i = 0; i < 8; ++i) g_prof.last_kinds[i] = log.kinds[i];
   return st;
@@ -525,7 +663,8 @@ int kvh_paged_attention_static(const void* q, int64_t q_tok_stride, int64_t q_he
   return paged_attention_impl(q, q_tok_stride, q_head_stride, k_cache, k_cache_strides, v_cache, v_cache_strides,
                               num_blocks, out, o_tok_stride, o_head_stride, block_tables, bt_row_stride,
                               max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
-                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, false, 1.f, 1.f, ws,
+                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, kKv16, 1.f, 1.f, nullptr, nullptr,
+                              nullptr, nullptr, ws,
                               need > 0 ? (size_t)KVH_STATIC_SCRATCH_BYTES : 0, stream);
 }
 
@@ -540,8 +679,8 @@ int kvh_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stri
   return paged_attention_impl(q, q_tok_stride, q_head_stride, k_cache, k_cache_strides, v_cache, v_cache_strides,
                               num_blocks, out, o_tok_stride, o_head_stride, block_tables, bt_row_stride,
                               max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
-                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, false, 1.f, 1.f,
-                              workspace, workspace_bytes, stream);
+                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, kKv16, 1.f, 1.f, nullptr, nullptr,
+                              nullptr, nullptr, workspace, workspace_bytes, stream);
 }
 
 int kvh_paged_attention_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
@@ -555,8 +694,24 @@ int kvh_paged_attention_fp8(const void* q, int64_t q_tok_stride, int64_t q_head_
   return paged_attention_impl(q, q_tok_stride, q_head_stride, k_cache, k_cache_strides, v_cache, v_cache_strides,
                               num_blocks, out, o_tok_stride, o_head_stride, block_tables, bt_row_stride,
                               max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
-                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, true, k_scale, v_scale,
-                              workspace, workspace_bytes, stream);
+                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, kKv8, k_scale, v_scale, nullptr,
+                              nullptr, nullptr, nullptr, workspace, workspace_bytes, stream);
+}
+
+int kvh_paged_attention_fp4(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
+                            const int64_t k_cache_strides[3], const void* k_scale, const int64_t k_scale_strides[3],
+                            const void* v_cache, const int64_t v_cache_strides[3], const void* v_scale,
+                            const int64_t v_scale_strides[3], int64_t num_blocks, void* out, int64_t o_tok_stride,
+                            int64_t o_head_stride, const int64_t* block_tables, int64_t bt_row_stride,
+                            int32_t max_blocks_per_seq, const int64_t* seq_lens, const int64_t* query_start_loc,
+                            int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale, int32_t dtype,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_attention_impl(q, q_tok_stride, q_head_stride, k_cache, k_cache_strides, v_cache, v_cache_strides,
+                              num_blocks, out, o_tok_stride, o_head_stride, block_tables, bt_row_stride,
+                              max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
+                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, kKv4, 1.f, 1.f, k_scale,
+                              k_scale_strides, v_scale, v_scale_strides, workspace, workspace_bytes, stream);
 }
 
 static bool a16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

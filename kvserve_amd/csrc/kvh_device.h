@@ -43,6 +43,12 @@ struct BF16 {
   static __device__ __forceinline__ uint32_t from_fp8x2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
   }
+  // Two E2M1 values (byte B of w) times the power of two `scale`, as a packed bf16 pair, the low nibble in the low
+  // half: exact, and NaN under the E8M0 NaN (scale bits 255 << 23).
+  template <int B>
+  static __device__ __forceinline__ uint32_t from_fp4x2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, B));
+  }
   // acc + lo + hi of a packed pair (v_dot2_f32_bf16 against {1, 1})
   static __device__ __forceinline__ float dot2_ones(uint32_t x, float acc) {
     typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -70,6 +76,11 @@ struct F16 {
   static __device__ __forceinline__ uint32_t from_fp8x2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
   }
+  // Two scaled E2M1 values as a packed fp16 pair (one rounding where fp16's range ends).
+  template <int B>
+  static __device__ __forceinline__ uint32_t from_fp4x2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, B));
+  }
   // acc + lo + hi of a packed pair (v_dot2_f32_f16 against {1, 1})
   static __device__ __forceinline__ float dot2_ones(uint32_t x, float acc) {
     typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -95,6 +106,14 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
+
+// OCP MXFP4: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, element 2i in the low
+// nibble, and one E8M0 byte s (the factor 2^(s - 127); 255: NaN) for every kFp4Block consecutive
+// elements of a row: the storage format of the *_fp4 entry points.
+constexpr int kFp4Block = 32;
+
+// The factor of an E8M0 byte as the conversion instructions read it (they take the exponent field alone).
+__device__ __forceinline__ float fp4_scale(uint32_t s) { return __uint_as_float(s << 23); }
 
 // Interleave the low (SEL = 0) or high (SEL = 1) 16-bit halves of two dwords:
 // result = {half(a), half(b)} with half(a) in the low 16 bits.

@@ -9,6 +9,9 @@
 
 namespace kvh {
 
+// Storage formats of the KV caches: the element type of q, E4M3 with a scale per tensor, MXFP4.
+constexpr int kKv16 = 0, kKv8 = 1, kKv4 = 2;
+
 // Upper bound on the waves one decode launch uses (256 CUs x 8 waves per SIMD x 4 SIMDs
 // would be 8192); the workspace is sized for it, so its size never depends on the device.
 constexpr int32_t kMaxDecodeWaves = 8192;
@@ -86,6 +89,11 @@ struct PAParams {
   float* ws_xml;         // [xslots, HGW, XR, 2]
   int32_t* ws_xjob;      // [B * Hkv / HGW, kJobInts] merge jobs per (sequence, head group)
   int32_t LINES;         // mixed batch in one launch: K's token rows lie where whole-line reads pay
+  // MXFP4 caches: the E8M0 bytes of K and V, strides {block, slot, head} in bytes
+  const uint8_t* kx;
+  int64_t kx_sb, kx_ss, kx_sh;
+  const uint8_t* vx;
+  int64_t vx_sb, vx_ss, vx_sh;
 };
 
 // Launch plan: a pure function of static shapes (graph-capture safe).
@@ -104,8 +112,8 @@ struct Plan {
 // Cascade: decode-class sequences per prefix group of nx 16-row tiles, RS rows each.
 inline int32_t cascade_group(int32_t RS, int32_t nx) { return RS >= 16 * nx ? 1 : 16 * nx / RS; }
 // 16-row tiles of a cascade prefix group: the plan's NX (4 or 1) over 16-bit caches, at most 2
-// over E4M3 caches.
-inline int32_t cascade_tiles(int32_t NX, bool kv8) { return kv8 && NX > 2 ? 2 : NX; }
+// over E4M3 and MXFP4 caches (`packed`).
+inline int32_t cascade_tiles(int32_t NX, bool packed) { return packed && NX > 2 ? 2 : NX; }
 
 Plan make_plan(int64_t T, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t W, int32_t BS, int32_t max_q,
                int32_t dtype);
@@ -119,8 +127,10 @@ struct LaunchLog {
   void after_launch(int kind, hipStream_t s);
 };
 
-int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, bool kv8, int32_t max_q,
+int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t kv, int32_t max_q,
                                 hipStream_t s, LaunchLog& log);
+int launch_paged_attention_kv4(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
+                               LaunchLog& log);
 // Whether a 16-bit launch takes the MFMA kernels: head sizes 64 and 128, pages a whole number
 // of 16-token tiles, GQA groups of at most 64 rows per token (four 16-row tiles). Every other
 // 16-bit shape, and fp32, takes the vector-ALU kernel (no workspace).
@@ -185,6 +195,26 @@ int launch_gemv_rope_and_cache(const void* x, int64_t x_rs, const void* w, int64
                                const int64_t* vcs, const int64_t* slots, int64_t num_blocks, int32_t H, int32_t Hkv,
                                int32_t D, int32_t BS, int32_t dtype, bool kv8, float k_scale, float v_scale,
                                hipStream_t s);
+// MXFP4 caches (cache_fp4.hip). kcs / vcs and kxs / vxs: {block, slot, head} byte strides of the packed rows and of
+// their E8M0 bytes.
+struct Fp4Cache {
+  uint8_t* c;
+  int64_t sb, ss, sh;
+  uint8_t* x;
+  int64_t xsb, xss, xsh;
+};
+int launch_reshape_and_cache_fp4(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                                 const Fp4Cache& kc, const Fp4Cache& vc, const int64_t* slots, int64_t T,
+                                 int64_t num_blocks, int32_t Hkv, int32_t D, int32_t BS, int32_t dtype, hipStream_t s);
+int launch_rope_and_cache_fp4(const void* qkv, int64_t qkv_ts, const int64_t* positions, const float* cos_t,
+                              const float* sin_t, int64_t max_pos, void* q_out, int64_t q_ts, int64_t q_hs,
+                              const Fp4Cache& kc, const Fp4Cache& vc, const int64_t* slots, int64_t T,
+                              int64_t num_blocks, int32_t H, int32_t Hkv, int32_t D, int32_t BS, int32_t dtype,
+                              hipStream_t s);
+int launch_read_cache_fp4(const Fp4Cache& kc, const Fp4Cache& vc, const int64_t* slots, void* k, int64_t k_ts,
+                          int64_t k_hs, void* v, int64_t v_ts, int64_t v_hs, int64_t T, int64_t num_blocks, int32_t Hkv,
+                          int32_t D, int32_t BS, int32_t dtype, hipStream_t s);
+
 int launch_reshape_and_cache_fp8(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
                                  int64_t v_hs, void* kc, const int64_t* kcs, void* vc, const int64_t* vcs,
                                  const int64_t* slots, int64_t T, int64_t num_blocks, int32_t Hkv, int32_t D,

@@ -47,10 +47,10 @@ constexpr int kChunk = 32;  // tokens per wave iteration
 static_assert(kPlanChunk == kChunk, "the prefill plan counts the tiles' chunks");
 constexpr int kWavesPerWG = 4;
 // 16-row tiles per prefill wave: 3 over 16-bit caches (48 rows, 238 VGPRs at D = 128, 2 workgroups per
-// CU), 2 over E4M3 caches (whose conversion registers leave no room for a third)
-template <bool KV8>
+// CU), 2 over the others (whose conversion registers leave no room for a third)
+template <int KV>
 constexpr int prefill_nt() {
-  return KV8 ? 2 : 3;
+  return KV == kKv16 ? 3 : 2;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -105,7 +105,7 @@ struct VRegs {
   uint32_t v[8][VW / 2];             // token t8 = 4 tile + e  <->  chunk token 16 tile + 4j + e
 };
 
-// The same chunk from an E4M3 cache (KV8), as loaded; converted to 16-bit MFMA operands at
+// The same chunk from an E4M3 cache, as loaded; converted to 16-bit MFMA operands at
 // use. K: 16 bytes per lane per pair of operands: lane (j, n) holds token 16t + n, bytes
 // d = 64c + 16j .. +15, and operand 2c + h takes d = 64c + 16j + 8h .. +7 (the query operand
 // uses the same k-slot order). V: lane (j, m) holds d = VW m .. VW m + VW - 1 of 8 tokens.
@@ -118,6 +118,35 @@ struct VRegs8 {
   static constexpr int VW = D / 16;
   uint32_t v[8][VW / 4];  // token t8 as in VRegs, 4 E4M3 values per dword
 };
+
+// The same chunk from an MXFP4 cache (kKv4). K: lane (j, n) holds row n of tile t, D / 4 elements from d = (D / 4) j
+// on, all under one scale, and operand c takes d = (D / 4) j + 8c .. +7. V: lane (j, m) holds d = VW m .. VW m + VW - 1
+// of 8 tokens, and the scale of the token that its place in its quad names (slot 4 tile + m % 4).
+// Row 4j + e of a tile is token 4e + j (tile_token): a V load e then reads the four whole rows of tokens 4e .. 4e + 3,
+// at D = 128 with a head's tokens together in a page two whole lines, not half a row of eight.
+template <int D>
+struct KRegs4 {
+  static constexpr int KW = D / 32;  // dwords
+  uint32_t k[2][KW];
+  uint32_t x[2];  // E8M0 byte
+};
+template <int D>
+struct VRegs4 {
+  uint32_t v[8];  // VW nibbles
+  uint32_t x[2];
+};
+
+// Token of a 16-token tile that row 4j + e of S^T and V slot e of lanes (j, *) stand for.
+template <int KV>
+__device__ __forceinline__ int tile_token(int j, int e) {
+  return KV == kKv4 ? 4 * e + j : 4 * j + e;
+}
+template <class KR>
+constexpr int regs_format = kKv16;
+template <int D>
+constexpr int regs_format<KRegs8<D>> = kKv8;
+template <int D>
+constexpr int regs_format<KRegs4<D>> = kKv4;
 
 // Uniform description of a chunk: first token and the block of each 16-token tile.
 struct ChunkRef {
@@ -141,6 +170,7 @@ __device__ __forceinline__ ChunkRef chunk_ref(PageWindow& pw, const PAParams& p,
 struct LaneOffsets {
   uint32_t k;  // (n * k_ss + 8 j) * 2
   uint32_t v;  // (4j * v_ss + VW n) * 2
+  uint32_t kx, vx;  // MXFP4: the scale bytes
 };
 
 // Whole-line K reads (LINES), for up to 8 query rows (R <= 8, one tile): an instruction reads 128
@@ -151,17 +181,26 @@ struct LaneOffsets {
 // as before. A non-temporal load does not keep the line's other half for the next instruction, so
 // half-line reads ask the L2 twice for every line. Rows of 128 bytes or more (can_read_lines); where they pay is
 // in line_reads.h.
-template <int D, bool KV8 = false, bool LINES = false>
+template <int D, int KV = kKv16, bool LINES = false>
 __device__ __forceinline__ LaneOffsets lane_offsets(const PAParams& p) {
   const int lane = threadIdx.x & 63;
   const int j = lane >> 4, n = lane & 15;
   LaneOffsets o;
-  if (LINES) {  // token n % 8 of a group of 8, 16-byte chunk 2 j + n / 8 of the line
-    o.k = (uint32_t)((n & 7) * (uint32_t)p.k_ss) * (KV8 ? 1u : 2u) + 16u * (uint32_t)(2 * j + (n >> 3));
-    o.v = (uint32_t)(4 * j * (uint32_t)p.v_ss + (D / 16) * n) * (KV8 ? 1u : 2u);
+  o.kx = o.vx = 0;
+  if (KV == kKv4) {  // strides in bytes
+    const uint32_t tok = (uint32_t)tile_token<KV>(n >> 2, n & 3);
+    o.k = tok * (uint32_t)p.k_ss + (uint32_t)(D / 8 * j);
+    o.kx = tok * (uint32_t)p.kx_ss + (uint32_t)(D / 4 * j / kFp4Block);
+    o.v = (uint32_t)j * (uint32_t)p.v_ss + (uint32_t)(D / 32 * n);
+    o.vx = (uint32_t)tile_token<KV>(j, n & 3) * (uint32_t)p.vx_ss + (uint32_t)(D / 16 * n / kFp4Block);
     return o;
   }
-  if (KV8) {  // one byte per element
+  if (LINES) {  // token n % 8 of a group of 8, 16-byte chunk 2 j + n / 8 of the line
+    o.k = (uint32_t)((n & 7) * (uint32_t)p.k_ss) * (KV == kKv8 ? 1u : 2u) + 16u * (uint32_t)(2 * j + (n >> 3));
+    o.v = (uint32_t)(4 * j * (uint32_t)p.v_ss + (D / 16) * n) * (KV == kKv8 ? 1u : 2u);
+    return o;
+  }
+  if (KV == kKv8) {  // one byte per element
     o.k = (uint32_t)(n * (uint32_t)p.k_ss + 16 * j);
     o.v = (uint32_t)(4 * j * (uint32_t)p.v_ss + (D / 16) * n);
   } else {
@@ -189,7 +228,8 @@ __device__ __forceinline__ T stream_load(const void* p) {
 // and is masked out of the scores and zeroed out of V like any invalid key.
 // LINES: r.k[t][g D / 64 + cc] is line cc of the 8-token group g of tile t.
 template <int D, bool NTL, bool LINES>
-__device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t k_lane) {
+__device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
+  const uint32_t k_lane = lo.k;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -209,7 +249,8 @@ __device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const Chu
 }
 
 template <int D, bool NTL>
-__device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t v_lane) {
+__device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
+  const uint32_t v_lane = lo.v;
   constexpr int VD = D / 32;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -235,7 +276,8 @@ __device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const Chu
 }
 
 template <int D, bool NTL, bool LINES>
-__device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t k_lane) {
+__device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
+  const uint32_t k_lane = lo.k;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -249,7 +291,8 @@ __device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const Ch
 }
 
 template <int D, bool NTL>
-__device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t v_lane) {
+__device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
+  const uint32_t v_lane = lo.v;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -267,6 +310,58 @@ __device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const Ch
       }
     }
   }
+}
+
+template <int D, bool NTL, bool LINES>
+__device__ __forceinline__ void load_k(KRegs4<D>& r, const PAParams& p, const ChunkRef& c, int kvh,
+                                       const LaneOffsets& lo) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
+    const int slot0 = (c.tok0 + 16 * t) % p.BS;
+    const char* page = (const char*)p.kc + blk * p.k_sb + (int64_t)kvh * p.k_sh + (int64_t)slot0 * p.k_ss;
+    const uint8_t* sc = p.kx + blk * p.kx_sb + (int64_t)kvh * p.kx_sh + (int64_t)slot0 * p.kx_ss;
+    r.x[t] = sc[lo.kx];
+    if constexpr (D == 128) {
+      const u32x4 w = stream_load<u32x4, NTL>(page + lo.k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.k[t][i] = w[i];
+    } else {
+      const u32x2 w = stream_load<u32x2, NTL>(page + lo.k);
+      r.k[t][0] = w[0];
+      r.k[t][1] = w[1];
+    }
+  }
+}
+
+template <int D, bool NTL>
+__device__ __forceinline__ void load_v(VRegs4<D>& r, const PAParams& p, const ChunkRef& c, int kvh,
+                                       const LaneOffsets& lo) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
+    const int slot0 = (c.tok0 + 16 * t) % p.BS;
+    const char* page = (const char*)p.vc + blk * p.v_sb + (int64_t)kvh * p.v_sh + (int64_t)slot0 * p.v_ss;
+    const uint8_t* sc = p.vx + blk * p.vx_sb + (int64_t)kvh * p.vx_sh + (int64_t)slot0 * p.vx_ss;
+    r.x[t] = sc[lo.vx];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const char* src = page + (int64_t)e * 4 * p.v_ss + lo.v;
+      if constexpr (D == 128)
+        r.v[4 * t + e] = stream_load<uint32_t, NTL>(src);
+      else
+        r.v[4 * t + e] = stream_load<uint16_t, NTL>(src);
+    }
+  }
+}
+
+// K operand cc of tile `tile` of an MXFP4 chunk: one conversion for two elements, scale included.
+template <class E, int D>
+__device__ __forceinline__ u32x4 k_operand(const KRegs4<D>& r, int tile, int cc) {
+  const uint32_t w = r.k[tile][cc];
+  const float f = fp4_scale(r.x[tile]);
+  return u32x4{E::template from_fp4x2<0>(w, f), E::template from_fp4x2<1>(w, f), E::template from_fp4x2<2>(w, f),
+               E::template from_fp4x2<3>(w, f)};
 }
 
 // K operand cc of tile `tile` of an E4M3 chunk, converted (exactly) to E's type.
@@ -288,10 +383,17 @@ struct WaveState {
   float thr[NT], nsh[NT]; // prefill only: raw-score bound that moves m, and -m (0 while m = -inf)
 };
 
+// First of the 8 elements of d that lanes (j, *) hold of query operand c: the K operands' order.
+template <int D, int KV>
+__device__ __forceinline__ int q_slot(int c, int j) {
+  if constexpr (KV == kKv4) return D / 4 * j + 8 * c;
+  return KV == kKv8 ? 64 * (c >> 1) + 16 * j + 8 * (c & 1) : 32 * c + 8 * j;
+}
+
 // Q rows of tile t: global row r = row0 + 16t + n, valid when r < R.
 // LINES: the operand's column n is row n % 8 at chunk n / 8 (see can_read_lines); D / 64 operands
 // are used (two over E4M3 caches), and columns 8 .. 15 see no key.
-template <int D, int NT, bool KV8 = false, bool LINES = false>
+template <int D, int NT, int KV = kKv16, bool LINES = false>
 __device__ __forceinline__ void load_q(WaveState<D, NT>& s, const PAParams& p, int64_t q_start, int R, int row0,
                                        int kvh, int64_t ctx, int64_t kv_total) {
   const int lane = threadIdx.x & 63;
@@ -313,8 +415,8 @@ __device__ __forceinline__ void load_q(WaveState<D, NT>& s, const PAParams& p, i
       const int qi = in ? rr / p.G : 0, g = in ? rr % p.G : 0;
       const uint16_t* qp = q + (q_start + qi) * p.q_ts + (int64_t)(kvh * p.G + g) * p.q_hs;
 #pragma unroll
-      for (int c = 0; c < (KV8 ? 2 : D / 64); ++c) {
-        const u32x4 x = *(const u32x4*)(qp + (KV8 ? 32 * j + 16 * hb + 8 * c : 64 * c + 16 * j + 8 * hb));
+      for (int c = 0; c < (KV == kKv8 ? 2 : D / 64); ++c) {
+        const u32x4 x = *(const u32x4*)(qp + (KV == kKv8 ? 32 * j + 16 * hb + 8 * c : 64 * c + 16 * j + 8 * hb));
 #pragma unroll
         for (int w = 0; w < 4; ++w) s.q[t][c][w] = in ? x[w] : 0u;
       }
@@ -326,9 +428,7 @@ __device__ __forceinline__ void load_q(WaveState<D, NT>& s, const PAParams& p, i
       const uint16_t* qp = q + (q_start + qi) * p.q_ts + (int64_t)(kvh * p.G + g) * p.q_hs;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        // operand c holds d = 32c + 8j .. +7, or with an E4M3 cache 64(c / 2) + 16j + 8(c % 2) .. +7
-        const int d0 = KV8 ? 64 * (c >> 1) + 16 * j + 8 * (c & 1) : 32 * c + 8 * j;
-        s.q[t][c] = *(const u32x4*)(qp + d0);
+        s.q[t][c] = *(const u32x4*)(qp + q_slot<D, KV>(c, j));
       }
       s.limit[t] = (int)clamp64(ctx + qi + 1, 0, kv_total);
     } else {
@@ -398,7 +498,7 @@ __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, 
         for (int cc = 0; cc < D / 32; ++cc) a = E::mfma(kr.k[tile][cc], s.q[t][cc], a);
         st[t][tile] = a;
       }
-  } else {  // E4M3: convert each tile's operands once for all row tiles
+  } else {  // E4M3, MXFP4: convert each tile's operands once for all row tiles
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
       u32x4 k[D / 32];
@@ -422,7 +522,7 @@ __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, 
       for (int e = 0; e < 4; ++e) {
         float x = st[t][tile][e] * p.qk_scale;
         if (MASKED) {
-          const int tok = c.tok0 + 16 * tile + 4 * j + e;
+          const int tok = c.tok0 + 16 * tile + tile_token<regs_format<KR>>(j, e);
           if (!(c.blk[tile] >= 0 && tok < s.limit[t])) x = -INFINITY;
         }
         st[t][tile][e] = x;
@@ -611,24 +711,63 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs8<D>& vr, con
     }
 }
 
+// O^T += V^T P^T from an MXFP4 V chunk: the scales of a quad's four tokens are read across it (DPP), the nibbles
+// convert to the 16-bit chunk's registers. A masked token's scale becomes 2^-127: its elements are then
+// finite whatever its bytes (an E2M1 code has no NaN), and its P is 0.
+template <class E, int D, int NT, bool MASKED>
+__device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs4<D>& vr, const ChunkRef& c, int data_end,
+                                         const u32x4 pt[NT]) {
+  const int lane = threadIdx.x & 63, j = lane >> 4;
+  VRegs<D> v;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    uint32_t x = vr.x[t] << 23;
+    if (MASKED) {
+      const int tok = c.tok0 + 16 * t + tile_token<kKv4>(j, lane & 3);
+      x = c.blk[t] >= 0 && tok < data_end ? x : 0u;
+    }
+    const int f[4] = {__builtin_amdgcn_update_dpp(0, (int)x, 0x00, 0xf, 0xf, false),
+                      __builtin_amdgcn_update_dpp(0, (int)x, 0x55, 0xf, 0xf, false),
+                      __builtin_amdgcn_update_dpp(0, (int)x, 0xaa, 0xf, 0xf, false),
+                      __builtin_amdgcn_update_dpp(0, (int)x, 0xff, 0xf, 0xf, false)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = vr.v[4 * t + e];
+      const float sc = __int_as_float(f[e]);
+      v.v[4 * t + e][0] = E::template from_fp4x2<0>(w, sc);
+      v.v[4 * t + e][1] = E::template from_fp4x2<1>(w, sc);
+      if constexpr (D == 128) {
+        v.v[4 * t + e][2] = E::template from_fp4x2<2>(w, sc);
+        v.v[4 * t + e][3] = E::template from_fp4x2<3>(w, sc);
+      }
+    }
+  }
+  chunk_pv<E, D, NT, false>(s, v, c, data_end, pt);
+}
+
+template <int D, int KV>
+using KChunk = std::conditional_t<KV == kKv4, KRegs4<D>, std::conditional_t<KV == kKv8, KRegs8<D>, KRegs<D>>>;
+template <int D, int KV>
+using VChunk = std::conditional_t<KV == kKv4, VRegs4<D>, std::conditional_t<KV == kKv8, VRegs8<D>, VRegs<D>>>;
+
 // Chunk loop of one wave over tokens tok_begin, tok_begin + stride, ... < tok_hi.
 // The body is straight-line (masks always applied, loads unconditional) and the loads are
 // pinned in the order K(c+1), V(c+1) with scheduling barriers, so each s_waitcnt waits for
 // exactly the operand it guards while the other half of the next chunk stays in flight.
-template <class E, int D, int NT, bool KV8 = false, bool NTL = true, bool LINES = false>
+template <class E, int D, int NT, int KV = kKv16, bool NTL = true, bool LINES = false>
 __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
                                            int tok_begin, int stride, int tok_hi, int data_end) {
   if (tok_begin >= tok_hi) return;
   const int page_end = (tok_hi + p.BS - 1) / p.BS;
-  const LaneOffsets lo = lane_offsets<D, KV8, LINES>(p);
+  const LaneOffsets lo = lane_offsets<D, KV, LINES>(p);
   PageWindow pw;
   load_window(pw, p, btrow, tok_begin / p.BS, page_end);
   ChunkRef c = chunk_ref(pw, p, btrow, tok_begin, tok_hi, page_end);
-  std::conditional_t<KV8, KRegs8<D>, KRegs<D>> kr;
-  std::conditional_t<KV8, VRegs8<D>, VRegs<D>> vr;
-  load_k<D, NTL, LINES>(kr, p, c, kvh, lo.k);
+  KChunk<D, KV> kr;
+  VChunk<D, KV> vr;
+  load_k<D, NTL, LINES>(kr, p, c, kvh, lo);
   __builtin_amdgcn_sched_barrier(0);
-  load_v<D, NTL>(vr, p, c, kvh, lo.v);
+  load_v<D, NTL>(vr, p, c, kvh, lo);
   __builtin_amdgcn_sched_barrier(0);
   // Every iteration has a next chunk, so its loads are unconditional; the last chunk is
   // peeled off below the loop.
@@ -637,11 +776,11 @@ __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& 
     u32x4 pt[NT];
     chunk_scores<E, D, NT, true, LINES>(s, kr, p, c, pt);
     __builtin_amdgcn_sched_barrier(0);
-    load_k<D, NTL, LINES>(kr, p, cn, kvh, lo.k);
+    load_k<D, NTL, LINES>(kr, p, cn, kvh, lo);
     __builtin_amdgcn_sched_barrier(0);
     chunk_pv<E, D, NT, true>(s, vr, c, data_end, pt);
     __builtin_amdgcn_sched_barrier(0);
-    load_v<D, NTL>(vr, p, cn, kvh, lo.v);
+    load_v<D, NTL>(vr, p, cn, kvh, lo);
     __builtin_amdgcn_sched_barrier(0);
     c = cn;
   }
@@ -948,7 +1087,7 @@ constexpr int kShareLdsList = 1024;  // members whose ids stay in LDS for the co
 constexpr int kShareCols = 4;        // columns per thread and pass
 constexpr int kShareRows = 16;       // member rows loaded together
 
-__global__ __launch_bounds__(kPlanThreads) void pa_share_kernel(PAParams p) {
+static __global__ __launch_bounds__(kPlanThreads) void pa_share_kernel(PAParams p) {
   __shared__ int s_wsum[kPlanThreads / 64];
   __shared__ int red[kPlanThreads / 64];
   __shared__ int s_list[kShareLdsList];
@@ -1049,7 +1188,7 @@ __global__ __launch_bounds__(kPlanThreads) void pa_share_kernel(PAParams p) {
 // Q rows of a prefix group (NX 16-row tiles, XR = 16 NX rows): row r = 16 t + n is member
 // r / RS of group grp (its decode-list index grp SG + r / RS), row r % RS of that sequence;
 // every valid row sees all L shared keys. Same k-slot order as load_q.
-template <int D, int NX, bool KV8>
+template <int D, int NX, int KV>
 __device__ __forceinline__ void load_q_group(WaveState<D, NX>& s, const PAParams& p, int grp, int nd, int L,
                                              int kvh) {
   const int lane = threadIdx.x & 63;
@@ -1074,8 +1213,7 @@ __device__ __forceinline__ void load_q_group(WaveState<D, NX>& s, const PAParams
       const uint16_t* qp = (const uint16_t*)p.q + (sv.qs + qi) * p.q_ts + (int64_t)(kvh * p.G + g) * p.q_hs;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        const int d0 = KV8 ? 64 * (c >> 1) + 16 * j + 8 * (c & 1) : 32 * c + 8 * j;
-        s.q[t][c] = *(const u32x4*)(qp + d0);
+        s.q[t][c] = *(const u32x4*)(qp + q_slot<D, KV>(c, j));
       }
       s.limit[t] = L;
     } else {
@@ -1103,10 +1241,10 @@ __device__ __forceinline__ void write_job_x(int32_t* job, int pieces, int64_t sl
 }
 
 // Decode class: NU * HGW / 4 workgroups of 4 waves; wave w of workgroup `block` is head w % HGW
-// of unit (4 block + w) / HGW. KV8: the cache is E4M3. NX: 16-row tiles of a cascade prefix
+// of unit (4 block + w) / HGW. KV: the caches' format. NX: 16-row tiles of a cascade prefix
 // group (XR = 16 NX rows; 1 outside the cascade).
 // LINES: whole-line K reads where the launch's mean unit asks for them (line_units).
-template <class E, int D, int NT, bool KV8, int NX, bool LINES>
+template <class E, int D, int NT, int KV, int NX, bool LINES>
 __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool may_read_lines = true) {
   static_assert(!LINES || (NT == 1 && NX == 1));
   const int lane = threadIdx.x & 63;
@@ -1157,12 +1295,12 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
   const int64_t NUa = active_units(C, p.NU);
   if (unit >= NUa) return;
   const bool weighted = NX == 4 && P > 0;
-  const bool rounds = KV8 && p.R1 < NUa;  // E4M3, two workgroups per CU: second-round shares
+  const bool rounds = KV != kKv16 && p.R1 < NUa;  // E4M3, two workgroups per CU: second-round shares
   const CostSplit split(P, C, NUa, weighted ? kPrefix64Cost : 1, weighted ? kChunkCost : 1, p.R1,
                         rounds ? kRound1Share : 1, rounds ? kRound2Share : 1);
   const int64_t a = split.begin(unit), b = split.begin(unit + 1);
   if (a >= b) return;
-  const bool lines = LINES && may_read_lines && wide == 0 && line_units(KV8, C, NUa);
+  const bool lines = LINES && may_read_lines && wide == 0 && line_units(KV == kKv8, C, NUa);
 
   int64_t pos = a;
   if constexpr (NT == 1) {
@@ -1175,12 +1313,12 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
       const int64_t y = b < seg_end ? b : seg_end;
       const int kvh = hg * p.HGW + hw;
       WaveState<D, NX> st;
-      load_q_group<D, NX, KV8>(st, p, grp, nd, L, kvh);
+      load_q_group<D, NX, KV>(st, p, grp, nd, L, kvh);
       const int64_t* btrow = p.bt + (int64_t)r0 * p.bt_rs;
       // 16- and 32-row groups each read the shared keys: ordinary loads, so the other groups'
       // reads hit the Infinity Cache (non-temporal ones ran C4 over E4M3 103 -> 108 us with
       // 16-row groups)
-      run_chunks<E, D, NX, KV8, (NX > 2)>(st, p, btrow, kvh, (int)(pos - seg_beg) * kChunk, kChunk,
+      run_chunks<E, D, NX, KV, (NX > 2)>(st, p, btrow, kvh, (int)(pos - seg_beg) * kChunk, kChunk,
                                           (int)(y - seg_beg) * kChunk, L);
       SeqView none{};
       write_rows<E, D, NX>(st, p, none, 16 * NX, 0, kvh, true, p.ws_xacc, p.ws_xml,
@@ -1224,17 +1362,17 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
     const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
     if constexpr (LINES) {
       if (lines) {
-        load_q<D, NT, KV8, true>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-        run_chunks<E, D, NT, KV8, true, true>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
+        load_q<D, NT, KV, true>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
+        run_chunks<E, D, NT, KV, true, true>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
       }
     }
     if (!lines) {
-      load_q<D, NT, KV8>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-      run_chunks<E, D, NT, KV8>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
+      load_q<D, NT, KV>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
+      run_chunks<E, D, NT, KV>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
     }
     const bool whole = pos == seg_beg && y == seg_end && !member;
     const int64_t slot = (int64_t)seq * NHG + hg + unit;
-    write_rows<E, D, NT, (KV8 && NT > 1)>(st, p, sv, R, 0, kvh, !whole, p.ws_acc, p.ws_ml, (slot * p.HGW + hw) * p.RS,
+    write_rows<E, D, NT, (KV != kKv16 && NT > 1)>(st, p, sv, R, 0, kvh, !whole, p.ws_acc, p.ws_ml, (slot * p.HGW + hw) * p.RS,
                                          p.RS);
     if (L > 0) {
       if (hw == 0 && lane == 0 && pos == seg_beg) {
@@ -1275,7 +1413,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
 // workspace and no merge launch follows: a batch this small is bound by latency, and the
 // merge launch was a third of it.
 // LINES: whole-line, non-temporal K/V loads for up to 8 rows (launch_mfma_typed).
-template <class E, int D, bool KV8, bool LINES>
+template <class E, int D, int KV, bool LINES>
 __global__ __launch_bounds__(256) void pa_decode_short_kernel(PAParams p) {
   constexpr int NI = D / 16;
   __shared__ f32x4 x_acc[kWavesPerWG - 1][NI][64];
@@ -1289,11 +1427,11 @@ __global__ __launch_bounds__(256) void pa_decode_short_kernel(PAParams p) {
   WaveState<D, 1> st;
   const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
   if (LINES && R <= kLineRows) {
-    load_q<D, 1, KV8, LINES>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-    run_chunks<E, D, 1, KV8, true, LINES>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
+    load_q<D, 1, KV, LINES>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
+    run_chunks<E, D, 1, KV, true, LINES>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
   } else {
-    load_q<D, 1, KV8>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-    run_chunks<E, D, 1, KV8, false>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
+    load_q<D, 1, KV>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
+    run_chunks<E, D, 1, KV, false>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
   }
   if (w > 0) {
 #pragma unroll
@@ -1504,11 +1642,11 @@ __device__ __forceinline__ void merge_job(const PAParams& p, const int32_t* job,
 // MIXED: the batch has prefill-class sequences (prefill records after the decode units);
 // decode and prefill jobs then both take 2 float4 per thread (16 rows at D = 128).
 template <class E, int D, bool MIXED, bool BLK>
-__global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
+static __global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
   constexpr int F = MIXED ? 4 : 1;
   constexpr int MR = merge_rows<D, F>();
-  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<false>()) % MR == 0 &&
-                           (kWavesPerWG * 16 * prefill_nt<true>()) % MR == 0),
+  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16>()) % MR == 0 &&
+                           (kWavesPerWG * 16 * prefill_nt<kKv8>()) % MR == 0),
                 "a prefill tile's rows split into whole merge chunks");
   const int CD = (p.HGW * p.RS + MR - 1) / MR;
   const int b = blockIdx.x;
@@ -1590,21 +1728,32 @@ struct PfLoads {
   int lstride;        // LDS bytes from one load to the next
   uint32_t ustep;     // global bytes from one load to the next (wave-uniform)
   uint32_t loff;      // the lane's global byte offset in the first load
+  // MXFP4: the same of the scale bytes
+  const uint8_t* scales;
+  int64_t xsb, xss;
+  uint32_t xstep, xoff;
 };
 
-// EB: bytes per cache element (2; 1 for an E4M3 cache, whose granules are the same 8
-// elements in 8 bytes, converted on their way to the 16-bit stage).
-template <int D, int EB = 2>
+// The granules of 8 elements are 16 bytes of a 16-bit cache, 8 of an E4M3 one and 4 of an MXFP4 one; the
+// latter two convert on their way to the 16-bit stage.
+template <int D, int KV = kKv16>
 __device__ __forceinline__ void pf_loads_init(PfLoads<D>& pl, const PAParams& p, int w, int kvh) {
   using L = PrefillLds<D>;
+  constexpr uint32_t GB = KV == kKv16 ? 16 : (KV == kKv8 ? 8 : 4);  // bytes of a granule
+  constexpr int SB = KV == kKv16 ? 2 : 1;                           // bytes of a stride's unit
   const int lane = threadIdx.x & 63;
   const int row_in = lane / L::kSlots, slot = lane % L::kSlots;
   const int g0 = w * L::kLoadsPerWave;
   const bool v = g0 / L::kLoadsPerTile != 0;
   const int i0 = g0 % L::kLoadsPerTile;
-  pl.sb2 = EB * (v ? p.v_sb : p.k_sb);
-  pl.ss2 = EB * (v ? p.v_ss : p.k_ss);
-  pl.cache = (const char*)(v ? p.vc : p.kc) + (int64_t)kvh * (v ? p.v_sh : p.k_sh) * EB;
+  pl.sb2 = SB * (v ? p.v_sb : p.k_sb);
+  pl.ss2 = SB * (v ? p.v_ss : p.k_ss);
+  pl.cache = (const char*)(v ? p.vc : p.kc) + (int64_t)kvh * (v ? p.v_sh : p.k_sh) * SB;
+  if constexpr (KV == kKv4) {
+    pl.xsb = v ? p.vx_sb : p.kx_sb;
+    pl.xss = v ? p.vx_ss : p.kx_ss;
+    pl.scales = (v ? p.vx : p.kx) + (int64_t)kvh * (v ? p.vx_sh : p.kx_sh);
+  }
   pl.h = i0 * L::kRowsPerLoad / 16;
   if (!v) {
     // load k fills row group i0 + k: rows (i0 + k) R + row_in of the chunk, token
@@ -1612,7 +1761,11 @@ __device__ __forceinline__ void pf_loads_init(PfLoads<D>& pl, const PAParams& p,
     pl.dst = i0 * L::kKLoadBytes;
     pl.lstride = L::kKLoadBytes;
     pl.ustep = (uint32_t)(L::kRowsPerLoad * pl.ss2);
-    pl.loff = (uint32_t)(row_in * pl.ss2) + 8u * EB * (uint32_t)(slot ^ row_in);
+    pl.loff = (uint32_t)(row_in * pl.ss2) + GB * (uint32_t)(slot ^ row_in);
+    if constexpr (KV == kKv4) {
+      pl.xstep = (uint32_t)(L::kRowsPerLoad * pl.xss);
+      pl.xoff = (uint32_t)(row_in * pl.xss) + (uint32_t)(slot ^ row_in) / (kFp4Block / 8);
+    }
   } else {
     // V stage layout: blocks b = h (D/16) + i of 512 bytes, block b holding d = 16i .. 16i+15
     // of the 16 tokens of half h, token-major (32 bytes per token). 16-byte granule P of the
@@ -1623,8 +1776,12 @@ __device__ __forceinline__ void pf_loads_init(PfLoads<D>& pl, const PAParams& p,
     const int b = (64 * i0 + lane) / 32, tok = (lane % 32) / 2, chunk = 2 * (b % (D / 16)) + lane % 2;
     pl.dst = L::kKBytes + i0 * 1024;
     pl.lstride = 1024;
-    pl.ustep = 32u * EB;
-    pl.loff = (uint32_t)(tok * pl.ss2) + 8u * EB * (uint32_t)chunk;
+    pl.ustep = 4 * GB;
+    pl.loff = (uint32_t)(tok * pl.ss2) + GB * (uint32_t)chunk;
+    if constexpr (KV == kKv4) {  // 4 granules on: the next scale
+      pl.xstep = 1;
+      pl.xoff = (uint32_t)(tok * pl.xss) + (uint32_t)chunk / (kFp4Block / 8);
+    }
   }
 }
 
@@ -1635,13 +1792,16 @@ __device__ __forceinline__ void pf_loads_init(PfLoads<D>& pl, const PAParams& p,
 // the tile's key range (a missing half is read from block 0 and masked).
 struct PfWindow {
   uint32_t off_lo, off_hi;  // VGPRs
+  uint32_t x_lo, x_hi;      // MXFP4: the same offset in the scales
   uint64_t ok0, ok1;        // SGPRs
   int c0;
   int first_bad;            // first chunk >= c0 with a missing half (c0 + 64 when none)
 };
 
+template <int KV = kKv16>
 __device__ __forceinline__ void pf_window(PfWindow& win, const PAParams& p, const int64_t* btrow, int c0, int c_end,
-                                          int page_end, int hmine, int64_t sb2, int64_t ss2) {
+                                          int page_end, int hmine, int64_t sb2, int64_t ss2, int64_t xsb = 0,
+                                          int64_t xss = 0) {
   const int lane = threadIdx.x & 63;
   const int c = c0 + lane;
   const int r = p.BS / 16;  // 16-token halves per page (BS % 16 == 0)
@@ -1675,6 +1835,11 @@ __device__ __forceinline__ void pf_window(PfWindow& win, const PAParams& p, cons
   const uint64_t o = (uint64_t)(uint32_t)idm * (uint64_t)sb2 + (uint64_t)(uint32_t)offm * (uint64_t)ss2;
   win.off_lo = (uint32_t)o;
   win.off_hi = (uint32_t)(o >> 32);
+  if constexpr (KV == kKv4) {
+    const uint64_t x = (uint64_t)(uint32_t)idm * (uint64_t)xsb + (uint64_t)(uint32_t)offm * (uint64_t)xss;
+    win.x_lo = (uint32_t)x;
+    win.x_hi = (uint32_t)(x >> 32);
+  }
   win.c0 = c0;
 }
 
@@ -1933,7 +2098,7 @@ template <class E, int D>
 __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                              int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                              int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<false>();
+  constexpr int NT = prefill_nt<kKv16>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   c_lo = uni(c_lo);
@@ -2056,18 +2221,18 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
   pf_write_rows<E, D, NT>(s, p, sv, R, row0, kvh, partial, slot * PRW - wg_row0);
 }
 
-// prefill_tile over an E4M3 cache. Direct global->LDS loads cannot convert, so each lane
-// loads, as E4M3, the 8-element granules the DMA would have moved (half the bytes, the
-// same offsets halved), converts them exactly to E's 16-bit type and writes them to the LDS
+// prefill_tile over an E4M3 or MXFP4 cache. Direct global->LDS loads cannot convert, so each lane
+// loads, as stored, the 8-element granules the DMA would have moved (8 bytes of E4M3; 4 of MXFP4
+// and their scale), converts them exactly to E's 16-bit type and writes them to the LDS
 // positions the DMA would have filled: the stage layout, the operand reads and the compute
 // are those of prefill_tile. Two register sets keep the loads two chunks ahead; chunk i is
 // converted and written right before the barrier that publishes it, so two LDS stages
 // suffice (stage i % 2 was last read by chunk i - 2, before the previous barrier).
-template <class E, int D>
-__device__ __forceinline__ void prefill_tile_kv8(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
-                                                 int kvh, int t, int c_lo, int c_hi, int w, bool partial,
-                                                 int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<true>();
+template <class E, int D, int KV>
+__device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
+                                                     int kvh, int t, int c_lo, int c_hi, int w, bool partial,
+                                                     int64_t slot, int rest, int total) {
+  constexpr int NT = prefill_nt<KV>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   constexpr int KLW = L::kLoadsPerWave;
@@ -2088,9 +2253,9 @@ __device__ __forceinline__ void prefill_tile_kv8(char* lds, const PAParams& p, c
   const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
   const int page_end = (kv_lim + p.BS - 1) / p.BS;
   PfLoads<D> pl;
-  pf_loads_init<D, 1>(pl, p, w, kvh);
+  pf_loads_init<D, KV>(pl, p, w, kvh);
   PfWindow win;
-  pf_window(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2);
+  pf_window<KV>(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2, pl.xsb, pl.xss);
   WaveState<D, NT> s;
   load_q<D, NT>(s, p, sv.qs, R, row0, kvh, sv.ctx, sv.kv_total);
   uint32_t ka[D / 32];
@@ -2104,8 +2269,11 @@ __device__ __forceinline__ void prefill_tile_kv8(char* lds, const PAParams& p, c
   const int n_my = max(0, min(n, (my_lim + kChunk - 1) / kChunk - c_lo));
   int n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
 
-  u32x2 raw[2][KLW];
-  auto issue = [&](u32x2 (&r)[KLW], int ci) {
+  struct Raw {
+    std::conditional_t<KV == kKv8, u32x2, uint32_t> g[KLW];
+    uint32_t x[KLW];  // MXFP4: E8M0 bytes
+  } raw[2];
+  auto issue = [&](Raw& r, int ci) {
     const int rel = ci - win.c0;
     const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(win.off_hi, rel) << 32) |
                        (uint32_t)__builtin_amdgcn_readlane(win.off_lo, rel);
@@ -2115,7 +2283,19 @@ __device__ __forceinline__ void prefill_tile_kv8(char* lds, const PAParams& p, c
     for (int k = 0; k < KLW; ++k) {
       uint64_t base = (uint64_t)(uintptr_t)pl.cache + o + (uint64_t)k * pl.ustep;
       asm volatile("" : "+s"(base));
-      r[k] = *(const u32x2*)((const char*)(uintptr_t)base + off);
+      r.g[k] = *(const std::remove_reference_t<decltype(r.g[k])>*)((const char*)(uintptr_t)base + off);
+    }
+    if constexpr (KV == kKv4) {
+      const uint64_t xo = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(win.x_hi, rel) << 32) |
+                          (uint32_t)__builtin_amdgcn_readlane(win.x_lo, rel);
+      uint32_t xoff = pl.xoff;
+      asm volatile("" : "+v"(xoff));
+#pragma unroll
+      for (int k = 0; k < KLW; ++k) {
+        uint64_t base = (uint64_t)(uintptr_t)pl.scales + xo + (uint64_t)k * pl.xstep;
+        asm volatile("" : "+s"(base));
+        r.x[k] = *((const uint8_t*)(uintptr_t)base + xoff);
+      }
     }
   };
   issue(raw[0], c_lo);
@@ -2130,22 +2310,29 @@ __device__ __forceinline__ void prefill_tile_kv8(char* lds, const PAParams& p, c
     if (i >= prio.next_drop) prio.set(i, n, rest, total);
     const int ci2 = c_lo + i + 2;
     if (i + 2 < n && ci2 - win.c0 >= 64) {
-      pf_window(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2);
+      pf_window<KV>(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2, pl.xsb, pl.xss);
       // the unmasked run reaches as far as the new window allows (the old window's end
       // capped it; a missing page before this point has already ended the run)
       n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
     }
     __builtin_amdgcn_sched_barrier(0);
     if (i + 1 < n)
-      wait_vm<KLW>();  // chunk i + 1 may stay in flight
+      wait_vm<(KV == kKv4 ? 2 : 1) * KLW>();  // chunk i + 1 may stay in flight
     else
       wait_vm<0>();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < KLW; ++k) {
-      const u32x2 r = raw[S][k];
-      const u32x4 o = {E::template from_fp8x2<false>(r[0]), E::template from_fp8x2<true>(r[0]),
-                       E::template from_fp8x2<false>(r[1]), E::template from_fp8x2<true>(r[1])};
+      const auto r = raw[S].g[k];
+      u32x4 o;
+      if constexpr (KV == kKv4) {
+        const float f = fp4_scale(raw[S].x[k]);
+        o = u32x4{E::template from_fp4x2<0>(r, f), E::template from_fp4x2<1>(r, f), E::template from_fp4x2<2>(r, f),
+                  E::template from_fp4x2<3>(r, f)};
+      } else {
+        o = u32x4{E::template from_fp8x2<false>(r[0]), E::template from_fp8x2<true>(r[0]),
+                  E::template from_fp8x2<false>(r[1]), E::template from_fp8x2<true>(r[1])};
+      }
       *(lds_u32x4_ptr)(uintptr_t)((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds +
                                   (uint32_t)(S * L::kStageBytes + pl.dst + k * pl.lstride + 16 * lane)) = o;
     }
@@ -2343,14 +2530,14 @@ __device__ __forceinline__ bool prefill_start(const PAParams& p, int b, PreStart
 // / 4) + NUP): each writes where a prefill unit starts, under the decode work, and the prefill
 // launch behind it begins with one load. (Computed by the prefill workgroups themselves it was
 // on that launch's path: 512 decodes and four 384-token chunks over E4M3 caches 483 -> 492 us.)
-template <class E, int D, int NT, bool KV8, int NX, bool LINES>
+template <class E, int D, int NT, int KV, int NX, bool LINES>
 __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
   const int b = blockIdx.x;
   if constexpr (NX == 1) {
     if (p.ND > 0 && b >= p.ND) {
       __shared__ PreStart st;
       __shared__ int64_t wsum[kPlanThreads / 64];
-      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV8>()>(p, b - p.ND, &st, wsum);
+      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV>()>(p, b - p.ND, &st, wsum);
       if (threadIdx.x == 0) {
         if (!work) st.u = -1;  // idle, rewritten on every call
         ((PreStart*)p.ws_plan)[b - p.ND] = st;
@@ -2358,7 +2545,7 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
       return;
     }
   }
-  decode_unit<E, D, NT, KV8, NX, LINES>(p, b);
+  decode_unit<E, D, NT, KV, NX, LINES>(p, b);
 }
 
 // Stream-K over the prefill-class work: a flat space of (sequence, kv head, tile, chunk),
@@ -2448,28 +2635,28 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
 }
 
 // LDS of a prefill workgroup: the ring's stages (3 over 16-bit caches, 2 over E4M3 caches).
-template <int D, bool KV8>
+template <int D, int KV>
 constexpr int prefill_lds_bytes() {
-  return (KV8 ? 2 : PrefillLds<D>::kStages) * PrefillLds<D>::kStageBytes;
+  return (KV == kKv16 ? PrefillLds<D>::kStages : 2) * PrefillLds<D>::kStageBytes;
 }
 
-template <class E, int D, bool KV8, bool PLANNED>
+template <class E, int D, int KV, bool PLANNED>
 __device__ __forceinline__ void prefill_unit(const PAParams& p, int block, char* lds) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  prefill_units<kWavesPerWG * 16 * prefill_nt<KV8>(), PLANNED>(p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
+  prefill_units<kWavesPerWG * 16 * prefill_nt<KV>(), PLANNED>(p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
                                    int64_t slot, int rest, int total) {
-    if constexpr (KV8)
-      prefill_tile_kv8<E, D>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
+    if constexpr (KV != kKv16)
+      prefill_tile_convert<E, D, KV>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
     else
       prefill_tile<E, D>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
   });
 }
 
 // 4-wave workgroups of 64 NT rows (PAParams::PR), 2 per CU.
-template <class E, int D, bool KV8>
+template <class E, int D, int KV>
 __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV8>()];
-  prefill_unit<E, D, KV8, true>(p, blockIdx.x, lds);
+  __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
+  prefill_unit<E, D, KV, true>(p, blockIdx.x, lds);
 }
 
 // A mixed batch in one launch: the first ND workgroups are its decode units, the next NUP its
@@ -2477,14 +2664,14 @@ __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
 // (launch_mixed): its workgroups leave their places at once, and no launch runs ahead of the
 // prefill work. Four prompts of 300-2500 tokens (D = 128, bf16): step 201 -> 176 us; two chunks
 // of 900-1024 tokens over 4000-10000 cached ones, E4M3: 328 -> 310 us.
-template <class E, int D, bool KV8>
+template <class E, int D, int KV>
 __global__ __launch_bounds__(256, 2) void pa_mixed_kernel(PAParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV8>()];
+  __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
   const int b = blockIdx.x;
   if (b < p.ND)
-    decode_unit<E, D, 1, KV8, 1, line_dim(D) && !KV8>(p, b, p.LINES);  // (E4M3: its units are too short for lines)
+    decode_unit<E, D, 1, KV, 1, line_dim(D) && KV == kKv16>(p, b, p.LINES);  // (E4M3: its units are too short for lines)
   else
-    prefill_unit<E, D, KV8, false>(p, b - p.ND, lds);
+    prefill_unit<E, D, KV, false>(p, b - p.ND, lds);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -2563,28 +2750,28 @@ static int decode_units(PAParams& p, int resident, int per_cu, bool kv8) {
   return wgs;
 }
 
-template <class E, int D, int NT, bool KV8, int NX = 1, bool LINES = false>
+template <class E, int D, int NT, int KV, int NX = 1, bool LINES = false>
 static int launch_decode_nt(PAParams& p, hipStream_t s) {
   int per_cu = 1;
-  const int resident = resident_blocks((const void*)&pa_decode_kernel<E, D, NT, KV8, NX, LINES>, 256, &per_cu);
-  const int wgs = decode_units(p, resident, per_cu, KV8);
+  const int resident = resident_blocks((const void*)&pa_decode_kernel<E, D, NT, KV, NX, LINES>, 256, &per_cu);
+  const int wgs = decode_units(p, resident, per_cu, KV != kKv16);
   p.ND = p.NUP > 0 ? wgs : 0;  // NUP > 0: the workgroups behind the decode units plan the prefill launch
-  hipLaunchKernelGGL((pa_decode_kernel<E, D, NT, KV8, NX, LINES>), dim3(wgs + p.NUP), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pa_decode_kernel<E, D, NT, KV, NX, LINES>), dim3(wgs + p.NUP), dim3(256), 0, s, p);
   return (int)hipGetLastError();
 }
 
 // The decode launch of a batch whose decode-class sequences take NT 16-row tiles (no cascade).
-template <class E, int D, bool KV8>
+template <class E, int D, int KV>
 static int launch_decode(PAParams& p, int NT, hipStream_t s) {
   switch (NT) {
     case 1:
-      if constexpr (line_dim(D))
-        if (line_launch(D, p.NUP > 0 ? 0 : p.RS, p.k_ss * (KV8 ? 1 : 2)))
-          return launch_decode_nt<E, D, 1, KV8, 1, true>(p, s);
-      return launch_decode_nt<E, D, 1, KV8>(p, s);
-    case 2: return launch_decode_nt<E, D, 2, KV8>(p, s);
-    case 3: return launch_decode_nt<E, D, 3, KV8>(p, s);
-    case 4: return launch_decode_nt<E, D, 4, KV8>(p, s);
+      if constexpr (line_dim(D) && KV != kKv4)
+        if (line_launch(D, p.NUP > 0 ? 0 : p.RS, p.k_ss * (KV == kKv8 ? 1 : 2)))
+          return launch_decode_nt<E, D, 1, KV, 1, true>(p, s);
+      return launch_decode_nt<E, D, 1, KV>(p, s);
+    case 2: return launch_decode_nt<E, D, 2, KV>(p, s);
+    case 3: return launch_decode_nt<E, D, 3, KV>(p, s);
+    case 4: return launch_decode_nt<E, D, 4, KV>(p, s);
     default: return (int)hipErrorInvalidValue;
   }
 }
@@ -2599,9 +2786,9 @@ constexpr int64_t kFusedUnitChunks = 4;
 // of 255-4095 keys beside four 384-token chunks 851 us in one launch, 816 apart; 100 decodes of
 // 255-2000 keys beside the same chunks 216 and 188; 512 decodes beside one 17-token chunk 721
 // and 741). Apart as well when a decode row needs more than one 16-row tile (GQA groups above 16).
-template <class E, int D, bool KV8>
+template <class E, int D, int KV>
 static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
-  p.PR = kWavesPerWG * 16 * prefill_nt<KV8>();
+  p.PR = kWavesPerWG * 16 * prefill_nt<KV>();
   // units x 2 partial slots x tile rows stay within the workspace's kMaxPrefillUnits x 2 x kPrefillRows
   const int cap = kMaxPrefillUnits * kPrefillRows / p.PR;
   // sequences that can be decode class: each of the others takes at most max_q of the T tokens
@@ -2610,34 +2797,35 @@ static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, Launc
   const int64_t n_dec = p.B > n_pre ? p.B - n_pre : 0;
   const int64_t dec_chunks = n_dec * (p.Hkv / p.HGW) * (((int64_t)p.W * p.BS + kChunk - 1) / kChunk);
   int err, per_cu = 1;
-  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV8>, 256, &per_cu);
-  const int wgs = decode_units(p, resident, per_cu, KV8);
+  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV>, 256, &per_cu);
+  const int wgs = decode_units(p, resident, per_cu, KV != kKv16);
   if (NT > 1 || dec_chunks > kFusedUnitChunks * p.NU) {
-    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV8>), cap) / 8 * 8);
-    if ((err = launch_decode<E, D, KV8>(p, NT, s))) return err;
+    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV>), cap) / 8 * 8);
+    if ((err = launch_decode<E, D, KV>(p, NT, s))) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
-    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV8>), dim3(p.NUP), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV>), dim3(p.NUP), dim3(256), 0, s, p);
     if ((err = (int)hipGetLastError())) return err;
     log.after_launch(KVH_KERNEL_PREFILL, s);
     return 0;
   }
   p.NUP = std::max(8, std::min(resident, cap) / 8 * 8);
-  p.LINES = line_launch(D, 0, p.k_ss * (KV8 ? 1 : 2));
+  p.LINES = KV == kKv16 && line_launch(D, 0, p.k_ss * 2);
   p.ND = (wgs + 7) / 8 * 8;  // prefill workgroup b keeps XCD b % 8
-  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV8>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
   if ((err = (int)hipGetLastError())) return err;
   log.after_launch(KVH_KERNEL_MIXED, s);
   return 0;
 }
 
-template <class E, int D, bool KV8>
+template <class E, int D, int KV>
 static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipStream_t s, LaunchLog& log) {
   int err = 0;
   if (plan.short_decode) {
-    if (line_short(D, KV8, (int64_t)p.B * p.Hkv * D, (int64_t)p.W * p.BS))
-      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV8, can_read_lines(D, KV8)>), dim3(p.Hkv, p.B), dim3(256), 0, s, p);
+    if (KV != kKv4 && line_short(D, KV == kKv8, (int64_t)p.B * p.Hkv * D, (int64_t)p.W * p.BS))
+      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, KV != kKv4 && can_read_lines(D, KV == kKv8)>),
+                         dim3(p.Hkv, p.B), dim3(256), 0, s, p);
     else
-      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV8, false>), dim3(p.Hkv, p.B), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, false>), dim3(p.Hkv, p.B), dim3(256), 0, s, p);
     if ((err = (int)hipGetLastError())) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
     return 0;
@@ -2649,11 +2837,11 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
     log.after_launch(KVH_KERNEL_SHARE, s);
   }
   if (plan.launch_prefill) {
-    if ((err = launch_mixed<E, D, KV8>(p, plan.NT, max_q, s, log))) return err;
+    if ((err = launch_mixed<E, D, KV>(p, plan.NT, max_q, s, log))) return err;
   } else {
-    constexpr int NX = KV8 ? 2 : 4;  // 64-row prefix groups (32 over E4M3 caches)
-    err = plan.cascade && p.XR == 16 * NX ? launch_decode_nt<E, D, 1, KV8, NX>(p, s)
-                                          : launch_decode<E, D, KV8>(p, plan.NT, s);
+    constexpr int NX = KV == kKv16 ? 4 : 2;  // 64-row prefix groups (32 over E4M3 caches)
+    err = plan.cascade && p.XR == 16 * NX ? launch_decode_nt<E, D, 1, KV, NX>(p, s)
+                                          : launch_decode<E, D, KV>(p, plan.NT, s);
     if (err) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
   }
@@ -2662,10 +2850,13 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
   const int nseg = plan.cascade ? p.B * (p.Hkv / p.HGW) : 0;  // cascade records
   const dim3 mg((p.NU > nseg ? p.NU : nseg) * cd + p.NUP * (p.PR / merge_rows<D, 4>()));
   // the partials' layout: tile blocks where the decode kernel wrote them so (write_rows<...,
-  // KV8 && NT > 1>: multi-tile rows over E4M3 caches), whole rows otherwise
-  if (plan.launch_prefill)
+  // KV != kKv16 && NT > 1>: multi-tile rows over E4M3 and MXFP4 caches), whole rows otherwise
+  const bool blk = KV != kKv16 && plan.NT > 1;
+  if (plan.launch_prefill && blk)  // GQA groups above 16
+    hipLaunchKernelGGL((pa_merge_kernel<E, D, true, true>), mg, dim3(256), 0, s, p);
+  else if (plan.launch_prefill)
     hipLaunchKernelGGL((pa_merge_kernel<E, D, true, false>), mg, dim3(256), 0, s, p);
-  else if (KV8 && plan.NT > 1)
+  else if (blk)
     hipLaunchKernelGGL((pa_merge_kernel<E, D, false, true>), mg, dim3(256), 0, s, p);
   else
     hipLaunchKernelGGL((pa_merge_kernel<E, D, false, false>), mg, dim3(256), 0, s, p);
@@ -2674,23 +2865,31 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
   return 0;
 }
 
-template <bool KV8>
+template <int KV>
 static int launch_mfma_kv(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
                           LaunchLog& log) {
   const bool bf = dtype == 2;
   if (D == 128)
-    return bf ? launch_mfma_typed<BF16, 128, KV8>(p, plan, max_q, s, log)
-              : launch_mfma_typed<F16, 128, KV8>(p, plan, max_q, s, log);
+    return bf ? launch_mfma_typed<BF16, 128, KV>(p, plan, max_q, s, log)
+              : launch_mfma_typed<F16, 128, KV>(p, plan, max_q, s, log);
   if (D == 64)
-    return bf ? launch_mfma_typed<BF16, 64, KV8>(p, plan, max_q, s, log)
-              : launch_mfma_typed<F16, 64, KV8>(p, plan, max_q, s, log);
+    return bf ? launch_mfma_typed<BF16, 64, KV>(p, plan, max_q, s, log)
+              : launch_mfma_typed<F16, 64, KV>(p, plan, max_q, s, log);
   return (int)hipErrorInvalidValue;
 }
 
-int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, bool kv8, int32_t max_q,
-                                hipStream_t s, LaunchLog& log) {
-  return kv8 ? launch_mfma_kv<true>(p, plan, D, dtype, max_q, s, log)
-             : launch_mfma_kv<false>(p, plan, D, dtype, max_q, s, log);
+#ifdef KVH_KV4_OBJECT
+int launch_paged_attention_kv4(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
+                               LaunchLog& log) {
+  return launch_mfma_kv<kKv4>(p, plan, D, dtype, max_q, s, log);
 }
+#else
+int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t kv, int32_t max_q,
+                                hipStream_t s, LaunchLog& log) {
+  if (kv == kKv4) return launch_paged_attention_kv4(p, plan, D, dtype, max_q, s, log);
+  return kv == kKv8 ? launch_mfma_kv<kKv8>(p, plan, D, dtype, max_q, s, log)
+                    : launch_mfma_kv<kKv16>(p, plan, D, dtype, max_q, s, log);
+}
+#endif
 
 }  // namespace kvh
