@@ -22,10 +22,12 @@ from kvserve_amd.attention import (
     last_launch_kernels,
     last_launches,
 )
+from kvserve_amd.logprobs import TokenLogprobs, token_logprobs
 
 __all__ = [
     "AttentionMetadata",
     "HipAttention",
+    "TokenLogprobs",
     "build_metadata",
     "fp4_caches",
     "get_backend",
@@ -33,4 +35,5 @@ __all__ = [
     "hip_eligible",
     "last_launch_kernels",
     "last_launches",
+    "token_logprobs",
 ]

@@ -35,6 +35,7 @@ SOURCES = [
     "cache_fp4.hip",
     "engine_ops.hip",
     "kvh_api.hip",
+    "logprobs.hip",
     "metadata.hip",
     "paged_attention.hip",
     "paged_attention_f32.hip",

@@ -831,6 +831,37 @@ int kvh_gemm_skinny_silu_mul(const void* x, int64_t x_row_stride, const void* w_
                             (hipStream_t)stream);
 }
 
+static int check_logprobs(int64_t rows, int32_t vocab, int32_t top, int32_t dtype) {
+  if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
+  if (rows < 0 || vocab <= 0 || top < 0 || top > vocab) return KVH_E_SHAPE;
+  // workgroups of a launch, and a row's bytes, within 32 bits
+  if (top > kMaxLogprobTop || rows > 0x7fffffffLL / kMaxLogprobSplits || vocab > 0x1fffffff) return KVH_E_UNSUPPORTED;
+  return KVH_OK;
+}
+
+size_t kvh_token_logprobs_workspace_size(int64_t num_rows, int32_t vocab, int32_t top, int32_t dtype) {
+  if (check_logprobs(num_rows, vocab, top, dtype) != KVH_OK) return 0;
+  const int32_t s = logprob_splits(num_rows, vocab, dtype);
+  return s > 1 ? (size_t)num_rows * s * (sizeof(float4) + (size_t)top * sizeof(uint64_t)) : 0;
+}
+
+int kvh_token_logprobs(const void* logits, int64_t row_stride, const int64_t* tokens, float* logprobs, float* entropy,
+                       float* top_logprobs, int64_t* top_ids, int64_t num_rows, int32_t vocab, int32_t top,
+                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_logprobs(num_rows, vocab, top, dtype);
+  if (st != KVH_OK) return st;
+  if (num_rows == 0) return KVH_OK;
+  if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return KVH_E_NULL;
+  if (row_stride < 0 || row_stride > INT64_MAX / 4) return KVH_E_SHAPE;
+  if ((uintptr_t)logits & (uintptr_t)(elem_bytes(dtype) - 1)) return KVH_E_ALIGN;
+  if (((uintptr_t)tokens | (uintptr_t)top_ids) & 7u) return KVH_E_ALIGN;
+  if (((uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_logprobs) & 3u) return KVH_E_ALIGN;
+  const size_t need = kvh_token_logprobs_workspace_size(num_rows, vocab, top, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || !a16(workspace))) return KVH_E_WORKSPACE;
+  return launch_token_logprobs(logits, row_stride, tokens, logprobs, entropy, top_logprobs, top_ids, num_rows, vocab,
+                               top, dtype, workspace, (hipStream_t)stream);
+}
+
 int kvh_profile_arm(void* const* events, int32_t num_events) {
   if (!events || num_events <= 0) {
     g_prof.num_events = 0;

@@ -184,6 +184,13 @@ int launch_gemm_skinny(const void* x, int64_t x_rs, const void* w, int64_t w_rs,
 int launch_gemv_silu_mul(const void* x, int64_t x_rs, const void* w, int64_t w_rs, void* y, int64_t y_rs, int32_t m,
                          int32_t inter, int32_t k, int32_t dtype, hipStream_t s);
 
+// Log probabilities (logprobs.hip): segments of a row and alternatives at most.
+constexpr int kMaxLogprobSplits = 64, kMaxLogprobTop = 64;
+int32_t logprob_splits(int64_t rows, int32_t V, int32_t dtype);
+int launch_token_logprobs(const void* logits, int64_t row_stride, const int64_t* tokens, float* logprobs,
+                          float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int32_t V, int32_t top,
+                          int32_t dtype, void* ws, hipStream_t s);
+
 int launch_rope_and_cache(const void* qkv, int64_t qkv_ts, const int64_t* positions, const float* cos_t,
                           const float* sin_t, int64_t max_pos, void* q_out, int64_t q_ts, int64_t q_hs, void* kc,
                           const int64_t* kcs, void* vc, const int64_t* vcs, const int64_t* slots, int64_t T,
