@@ -18,6 +18,7 @@ graph of cuda_graph.py:79-102) and called between piecewise-graph replays
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -174,7 +175,19 @@ def _fp4_args(*caches: torch.Tensor) -> list:
     return [x for t in caches for x in (t.data_ptr(), _lib.i64x3(t.stride()[:3]))]
 
 
+def _current(dev: int):
+    """The caches' device as the current one: a kernel is launched there."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
 def _write_kv_fp4(k_cache, v_cache, k, v, slots, k_scale, v_scale) -> None:
+    calls = _calls()
+    if calls is not None:
+        r = calls.write_kv_fp4(k_cache, v_cache, k, v, slots, k_scale, v_scale)
+        if r is True:
+            return
+        if r is not None:
+            _lib.check(r, "kvh_reshape_and_cache_fp4")
     num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
     _on_device(dev, k=k, v=v, slot_mapping=slots)
     _require(k.dim() == 3 and k.shape == v.shape, "k and v must be [T, kv_heads, head_dim]")
@@ -182,32 +195,50 @@ def _write_kv_fp4(k_cache, v_cache, k, v, slots, k_scale, v_scale) -> None:
     _require(k.stride(-1) == 1 and v.stride(-1) == 1, "k/v last dim must be contiguous")
     _check_index(slots, "slot_mapping", 1)
     _require(slots.shape[0] == k.shape[0], "one slot per token")
-    st = _lib.load().kvh_reshape_and_cache_fp4(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.shape[0], num_blocks, num_kv_heads,
-        head_dim, block_size, _dtype_code(k, v), _stream_handle(k_cache.device),
-    )  # fmt: skip
+    dtype = _dtype_code(k, v)
+    with _current(dev):
+        st = _lib.load().kvh_reshape_and_cache_fp4(
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.shape[0], num_blocks, num_kv_heads,
+            head_dim, block_size, dtype, _stream_handle(k_cache.device),
+        )  # fmt: skip
     _lib.check(st, "kvh_reshape_and_cache_fp4")
 
 
 def _rope_and_cache_fp4(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, out, k_scale,
                         v_scale) -> torch.Tensor:  # fmt: skip
+    calls = _calls()
+    if calls is not None:
+        r = calls.rope_and_cache_fp4(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, out, k_scale, v_scale)
+        if type(r) is int:
+            _lib.check(r, "kvh_rope_and_cache_fp4")
+        if r is not None:
+            return r
     num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
     out = _check_rope(qkv, positions, cos, sin, slots, num_heads, num_kv_heads, head_dim, dev, out)
     dtype = _dtype_code(qkv, out)
     if qkv.shape[0] == 0:
         return out
-    st = _lib.load().kvh_rope_and_cache_fp4(
-        qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        out.data_ptr(), out.stride(0), out.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale),
-        slots.data_ptr(), qkv.shape[0], num_blocks, num_heads, num_kv_heads, head_dim, block_size, dtype,
-        _stream_handle(qkv.device),
-    )  # fmt: skip
+    with _current(dev):
+        st = _lib.load().kvh_rope_and_cache_fp4(
+            qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            out.data_ptr(), out.stride(0), out.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale),
+            slots.data_ptr(), qkv.shape[0], num_blocks, num_heads, num_kv_heads, head_dim, block_size, dtype,
+            _stream_handle(qkv.device),
+        )  # fmt: skip
     _lib.check(st, "kvh_rope_and_cache_fp4")
     return out
 
 
 def _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale) -> torch.Tensor:
+    calls = _calls()
+    if calls is not None:
+        r = calls.forward_fp4(q, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.query_start_loc,
+                              meta.max_query_len, scale, out, k_scale, v_scale)  # fmt: skip
+        if type(r) is int:
+            _lib.check(r, "kvh_paged_attention_fp4")
+        if r is not None:
+            return r
     num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
     out, tables, seq_lens, qsl = _check_attention(q, meta, num_kv_heads, head_dim, dev, out)
     _require(q.dtype != torch.float32, "float4_e2m1fn_x2 caches need bf16 or fp16 queries")
@@ -221,12 +252,13 @@ def _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale) -> tor
     ws_bytes = _workspace_size(lib, num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, width, block_size, max_q,
                                dtype)  # fmt: skip
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    st = lib.kvh_paged_attention_fp4(
-        q.data_ptr(), q.stride(0), q.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale), num_blocks,
-        out.data_ptr(), out.stride(0), out.stride(1), tables.data_ptr(), tables.stride(0), width,
-        seq_lens.data_ptr(), qsl.data_ptr(), num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
-        max_q, float(scale), dtype, ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(q.device),
-    )  # fmt: skip
+    with _current(dev):
+        st = lib.kvh_paged_attention_fp4(
+            q.data_ptr(), q.stride(0), q.stride(1), *_fp4_args(k_cache, k_scale, v_cache, v_scale), num_blocks,
+            out.data_ptr(), out.stride(0), out.stride(1), tables.data_ptr(), tables.stride(0), width,
+            seq_lens.data_ptr(), qsl.data_ptr(), num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+            max_q, float(scale), dtype, ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(q.device),
+        )  # fmt: skip
     _lib.check(st, "kvh_paged_attention_fp4")
     return out
 
@@ -362,17 +394,25 @@ class HipAttention:
         """(k, v) [T, kv_heads, D] in `dtype` (bf16, fp16 or fp32): the rows of a float4_e2m1fn_x2 cache at `slots`,
         zeros for slots outside the pool. (The other caches' rows are cache.flatten(0, 1)[slots] in torch.)"""
         _require(k_cache.dtype == FP4, f"read_kv reads float4_e2m1fn_x2 caches, not {k_cache.dtype}")
+        calls = _calls()
+        if calls is not None:
+            r = calls.read_kv_fp4(k_cache, v_cache, slots, _lib.KVH_DTYPE.get(dtype), k_scale, v_scale)
+            if type(r) is int:
+                _lib.check(r, "kvh_read_cache_fp4")
+            if r is not None:
+                return r
         num_blocks, block_size, num_kv_heads, head_dim, dev = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
         _on_device(dev, slots=slots)
         _check_index(slots, "slots", 1)
         _require(dtype in _lib.KVH_DTYPE, f"unsupported dtype {dtype} (float32, float16, bfloat16)")
         shape = (slots.shape[0], num_kv_heads, head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
-        st = _lib.load().kvh_read_cache_fp4(
-            *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), slots.shape[0], num_blocks, num_kv_heads, head_dim, block_size,
-            _lib.KVH_DTYPE[dtype], _stream_handle(k_cache.device),
-        )  # fmt: skip
+        with _current(dev):
+            st = _lib.load().kvh_read_cache_fp4(
+                *_fp4_args(k_cache, k_scale, v_cache, v_scale), slots.data_ptr(), k.data_ptr(), k.stride(0),
+                k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.shape[0], num_blocks, num_kv_heads, head_dim,
+                block_size, _lib.KVH_DTYPE[dtype], _stream_handle(k_cache.device),
+            )  # fmt: skip
         _lib.check(st, "kvh_read_cache_fp4")
         return k, v
 

@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from kvserve_amd import _lib
-from kvserve_amd.attention import _check_index, _require, _stream_handle
+from kvserve_amd.attention import _calls, _check_index, _current, _require, _stream_handle
 
 MAX_TOP = 64  # alternatives of a row at most
 
@@ -26,6 +26,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
     Statistics in fp32 whatever the logits' type. A logit of -inf is a token that cannot be; a row with a NaN or a +inf,
     or of -inf alone, gives NaN, as does a token outside the vocabulary (its row's other outputs are unaffected)."""
+    calls = _calls()
+    if calls is not None:
+        r = calls.token_logprobs(logits, tokens, top)
+        if r is not None:
+            return TokenLogprobs(*r)
     _require(logits.dim() == 2 and logits.stride(-1) == 1, "logits must be [T, vocab] with a contiguous last dim")
     _require(logits.is_cuda, "logits must be on a HIP device")
     _require(logits.dtype in _lib.KVH_DTYPE, f"unsupported dtype {logits.dtype} (float32, float16, bfloat16)")
@@ -45,10 +50,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     lib = _lib.load()
     need = lib.kvh_token_logprobs_workspace_size(rows, vocab, top, dtype)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    st = lib.kvh_token_logprobs(
-        logits.data_ptr(), logits.stride(0), tokens.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * rows,
-        top_logprobs.data_ptr() if top else None, top_ids.data_ptr() if top else None, rows, vocab, top, dtype,
-        ws.data_ptr() if ws is not None else None, need, _stream_handle(dev),
-    )  # fmt: skip
+    with _current(logits.get_device()):
+        st = lib.kvh_token_logprobs(
+            logits.data_ptr(), logits.stride(0), tokens.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * rows,
+            top_logprobs.data_ptr() if top else None, top_ids.data_ptr() if top else None, rows, vocab, top, dtype,
+            ws.data_ptr() if ws is not None else None, need, _stream_handle(dev),
+        )  # fmt: skip
     _lib.check(st, "kvh_token_logprobs")
     return got

@@ -519,3 +519,39 @@ def test_refusals_on_the_device(hip_device):
         HipAttention.forward(rows.float()[:1], k, v, meta, 1.0, None, ks, vs)
     with pytest.raises(ValueError, match="head_dim"):
         HipAttention.forward(rows[:1, :, :32], k, v, meta, 1.0, None, ks, vs)
+
+
+def test_step_by_step_path_gives_the_same_bits(hip_device, monkeypatch):
+    """The methods without the C++ calls on tensors (_kvhtorch), and what those leave to the methods."""
+    from kvserve_amd import _lib
+
+    dev = hip_device
+    w = workloads.custom("calls", [1, 3, 40], [30, 500, 7], 32, 8, 64, 16, seed=1)
+    caches = _random_pool(w.num_blocks, 16, 8, 64, dev, "head", seed=1)
+    meta = _meta(w, dev)
+    q = torch.randn(w.num_tokens, 32, 64, device=dev).to(torch.bfloat16)
+    qkv = torch.randn(w.num_tokens, 48 * 64, device=dev).to(torch.bfloat16)
+    k, v = qkv[:, : 8 * 64].view(-1, 8, 64), qkv[:, 8 * 64 : 16 * 64].view(-1, 8, 64)
+    cos, sin = _tables(64, 64, dev)
+    pos = torch.arange(w.num_tokens, device=dev)
+
+    def everything():
+        pools = [[_bytes(c).clone().view(c.dtype) for c in caches] for _ in range(2)]
+        r = HipAttention.rope_and_cache(qkv, pos, cos, sin, *pools[0][:2], meta.slot_mapping, 32, None, *pools[0][2:])
+        HipAttention.write_kv(*pools[1][:2], k, v, meta.slot_mapping, *pools[1][2:])
+        rk, rv = HipAttention.read_kv(*pools[1][:2], meta.slot_mapping, torch.float32, *pools[1][2:])
+        out = HipAttention.forward(q, *pools[0][:2], meta, 0.125, None, *pools[0][2:])
+        return [r, rk, rv, out, *(_bytes(c) for p in pools for c in p)]
+
+    calls = _lib.calls()
+    a = [k, v, meta.slot_mapping]
+    assert calls.write_kv_fp4(*caches[:2], *a, *caches[2:]) is True
+    assert calls.write_kv_fp4(*caches[:2], *a, caches[2], 1.0) is None
+    assert calls.read_kv_fp4(*caches[:2], meta.slot_mapping.int(), 2, *caches[2:]) is None
+    assert calls.forward_fp4(q.float(), *caches[:2], meta.block_tables, meta.seq_lens, meta.query_start_loc, 40, 0.1, None,
+                             *caches[2:]) is None  # fmt: skip
+    got = everything()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_calls", None)
+        want = everything()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

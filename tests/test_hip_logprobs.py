@@ -186,3 +186,16 @@ def test_graph_replays(hip_device, T):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, token_logprobs(x, tok, 5)))
         _check(x[:4], tok[:4], 5, type(out)(*(f[:4] for f in got)))
+
+
+def test_step_by_step_path_gives_the_same_bits(hip_device, monkeypatch):
+    from kvserve_amd import _lib
+
+    x, tok = _logits(30, 5000, torch.bfloat16, hip_device)
+    assert _lib.calls().token_logprobs(x, tok, 5) is not None
+    assert _lib.calls().token_logprobs(x, tok.int(), 5) is None and _lib.calls().token_logprobs(x, tok, 65) is None
+    got = token_logprobs(x, tok, 5)
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_calls", None)
+        want = token_logprobs(x, tok, 5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
