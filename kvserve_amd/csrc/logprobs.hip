@@ -1,33 +1,43 @@
 // token_logprobs: for every row x[0..V) of a step's logits the log probability of one given token, the entropy of the
 // row's distribution and its `top` largest entries with their log probabilities, in one pass over the logits:
 //
-//   m = max_j x_j,  s = sum_j e^(x_j - m),  t = sum_j e^(x_j - m) (x_j - m)
-//   log p_j = (x_j - m) - ln s,   entropy = -sum_j p_j log p_j = ln s - t / s
+//   m = max_j x_j,  s = sum_j e^(x_j - m),  t = sum_j e^(x_j - m) (x_j - m) / ln 2
+//   log p_j = (x_j - m) - ln s,   entropy = -sum_j p_j log p_j = ln s - ln 2 t / s
 //
-// m, s, t are running values of a thread (fp32), rescaled where its maximum moves, then joined over lanes, waves
-// and segments; x_j - m is taken before the product with log2 e, so the terms near the maximum are exact.
+// m, s, t are running values of a thread (fp32), rescaled where its maximum moves, then joined over lanes, waves and
+// segments. With c = log2 e a term's exponent is d_j = c x_j - r, one FMA against the rounded r = fl(c m): rounded
+// once relative to itself. What r is off by, delta = c m - r, is exact in one FMA and taken out at the end. Where |m| is
+// above kFar, delta would be no small number: there d_j = c (x_j - m).
 //
-// HBM-bound on the logits. A row is cut into S segments of whole 256-vector chunks, a workgroup each, so that few rows
-// fill the chip too; a second launch joins the segments (S = 1: none).
+// HBM-bound on the logits, with the vector units close behind (8 issue slots an element: widening, maximum, FMA,
+// exponential, two sums). A row is cut into S segments of whole 256-vector chunks, a workgroup each, so that few
+// rows fill the chip too; a second launch joins the segments (S = 1: none).
 //
-// The largest entries cost the pass one select per vector: a thread only remembers where its maximum was first seen.
-// Entries are ordered by a 64-bit key, value first, then the lower index, so keys differ and the order is total. The
-// `top`-th largest of the 64 maxima over four threads each is a lower bound of the segment's `top`-th largest key, and
-// at least `top` entries, rarely many more (24 expected of 20 asked for), lie at or above it, all of them in threads
-// whose maximum does: those threads walk their entries again (in the caches), the entries found are ranked by
-// counting. Where more than kList are found (the largest entries all in few threads' strides), `top` rounds of a
-// whole maximum take their place.
+// The largest entries: the pass keeps the maxima of up to 16 x 64 cells, a cell being what four neighbouring threads read
+// in a sixteenth of it (one more maximum a vector). The `top`-th largest of the 64 maxima over a quad of threads each
+// is a lower bound thr of the segment's `top`-th largest entry, and rarely many more than `top` entries reach it (24
+// expected of 20 asked for). They lie in cells whose maximum does, so those cells alone are read again (20 cells of a
+// 256 KB row: 10 KB), and the entries found are ranked by counting, ties by the lower index. Where entries equal to thr
+// abound (a row of few values, or masked with -inf but for fewer than `top`), the larger ones are ranked and the
+// equal ones taken in index order; where more than kList are larger than thr (the largest entries all in few
+// cells), `top` rounds of a whole maximum take their place.
 //
-// NaN counts as -inf in the order and makes the row's m, s, t NaN; an infinite or all -inf row gives NaN as well.
+// NaN counts as -inf in the order and makes the row's s and t NaN; an infinite or all -inf row gives NaN as well.
+#include <type_traits>
+
 #include "kvh_device.h"
 #include "kvh_internal.h"
+
+// on a lambda: what it captures stays in registers
+#define INLINE __attribute__((always_inline))
 
 namespace kvh {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kGroups = 64;  // threads' maxima are ranked in groups of four
-constexpr int kList = 2048, kJoinList = kMaxLogprobSplits * kMaxLogprobTop;
+constexpr int kGroups = 64, kSpans = 16;  // quads of threads, parts of the pass
+constexpr int kCellsRead = 512;           // cells at or above thr, beyond which ties are taken in index order
+constexpr int kList = 1024, kJoinList = kMaxLogprobSplits * kMaxLogprobTop;
 constexpr int kUnroll = 4;
 
 struct LogprobArgs {
@@ -82,20 +92,23 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
   return (uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)x, o);
 }
 
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFar = 1048576.f;
+
 struct Sums {
   float m, s, t;
 };
 // Both relative to the larger maximum (0 while that is -inf).
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
-  const float da = a.m - ref, db = b.m - ref;
-  const float wa = fast_exp2(da * kLog2e), wb = fast_exp2(db * kLog2e);
-  Sums r;
-  r.m = m;
-  r.s = wa * a.s + wb * b.s;
+  const float da = (a.m - ref) * kLog2e, db = (b.m - ref) * kLog2e;
+  const float wa = fast_exp2(da), wb = fast_exp2(db);
+  Sums v;
+  v.m = m;
+  v.s = wa * a.s + wb * b.s;
   // an empty side weighs nothing (its d is -inf)
-  r.t = (wa > 0.f ? wa * __builtin_fmaf(da, a.s, a.t) : 0.f) + (wb > 0.f ? wb * __builtin_fmaf(db, b.s, b.t) : 0.f);
-  return r;
+  v.t = (wa > 0.f ? wa * __builtin_fmaf(da, a.s, a.t) : 0.f) + (wb > 0.f ? wb * __builtin_fmaf(db, b.s, b.t) : 0.f);
+  return v;
 }
 __device__ __forceinline__ Sums wave_join(Sums v) {
 #pragma unroll
@@ -110,7 +123,19 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, con
   const bool in = tok >= 0 && tok < a.V;
   const float x = Vec<DT>::one(a.x + row * a.row_bytes + (in ? tok : 0) * Vec<DT>::EB);
   a.logprobs[row] = in ? x - v.m - ln_s : __uint_as_float(0x7fc00000u);
-  a.entropy[row] = ln_s - v.t / v.s;
+  a.entropy[row] = ln_s - kLn2 * (v.t / v.s);
+}
+
+// max / min of three with no canonicalisation of the operands first (a NaN among them is dropped)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // Ranks the n keys of `list` (distinct): emit(rank, key) for the first `top`.
@@ -124,18 +149,15 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int top, 
   }
 }
 
-// A thread's entries in the order of their indexes: an element of the row's unaligned head, vectors v0 + tid,
-// v0 + tid + 256, ... of its aligned middle, an element of its tail.
-constexpr int kNone = -3, kTail = -2, kHead = -1;
-
 template <int DT, bool FINAL>
-__global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
   using X = Vec<DT>;
   constexpr int N = X::N, EB = X::EB;
   __shared__ Sums s_sums[kWaves];
-  __shared__ uint64_t s_group[kGroups], s_thr, s_best[kWaves];
-  __shared__ uint64_t s_list[kList];
-  __shared__ int s_n;
+  __shared__ float s_cell[kSpans][kGroups], s_group[kGroups], s_thr;
+  __shared__ uint64_t s_best[kWaves], s_list[kList];
+  __shared__ uint16_t s_cand[kSpans * kGroups];
+  __shared__ int s_n, s_nc, s_count[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = FINAL ? blockIdx.x : blockIdx.x / (unsigned)a.S;
   const int seg = FINAL ? 0 : (int)(blockIdx.x % (unsigned)a.S);
@@ -147,82 +169,108 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   const u32x4* mid = (const u32x4*)(x + head * EB);
   const int tail0 = head + nvec * N;
 
-  float m = -INFINITY, s = 0.f, t = 0.f;
-  int at = has_head ? kHead : (v0 + tid < v1 ? v0 + tid : (has_tail ? kTail : kNone));
-  // an entry or vector whose maximum is mx, first at `where`: moves m
-  auto raise = [&](float mx, int where) {
-    at = mx > m ? where : at;
+  // the sums' reference is r = c m - delta (0 while m is -inf); entries below lo take the careful sum
+  float m = -INFINITY, r = 0.f, delta = 0.f, lo = -kFar, s = 0.f, t = 0.f;
+  float cell = -INFINITY;  // the thread's maximum in this span
+  // an entry or vector whose maximum is mx: moves m
+  auto raise = [&](float mx) INLINE {
+    cell = fmaxf(cell, mx);
     if (__builtin_amdgcn_ballot_w64(mx > m)) {
-      const float mn = fmaxf(m, mx), d = m - mn;
-      const float w = mn == -INFINITY ? 1.f : fast_exp2(d * kLog2e);
-      t = w > 0.f ? w * __builtin_fmaf(mx > m ? d : 0.f, s, t) : 0.f;
+      const float mn = fmaxf(m, mx);
+      const bool none = mn == -INFINITY, far = fabsf(mn) > kFar && !none;
+      const float rn = none ? 0.f : mn * kLog2e, dn = none || far ? 0.f : __builtin_fmaf(mn, kLog2e, -rn);
+      // (an m that was -inf: nothing to rescale, d = -inf)
+      const float d = none ? 0.f : (m - mn) * kLog2e - delta + dn, w = fast_exp2(d);
+      t = w > 0.f ? w * __builtin_fmaf(d, s, t) : 0.f;
       s *= w;
       m = mn;
+      r = rn;
+      delta = dn;
+      lo = far ? INFINITY : -kFar;
     }
   };
-  auto add = [&](float v, float ref) {
-    const float d = v - ref;
-    const float e = fast_exp2(d * kLog2e);  // NaN stays
+  auto add = [&](float v) INLINE {
+    const float d = __builtin_fmaf(v, kLog2e, -r);
+    const float e = fast_exp2(d);  // NaN stays
     s += e;
-    t = __builtin_fmaf(e, fmaxf(d, -1000.f), t);  // e is 0 there: -inf adds nothing
+    t = __builtin_fmaf(e, d, t);
   };
-  auto vector = [&](const u32x4& w, int where) {
+  // also for -inf, the types' lowest values and maxima far from 0: an exponential of 0 meets a finite d
+  auto add_careful = [&](float v) INLINE {
+    const float d = lo == INFINITY ? (v - m) * kLog2e : __builtin_fmaf(v, kLog2e, -r);
+    const float e = fast_exp2(d);
+    s += e;
+    t = __builtin_fmaf(e, fmaxf(d, -1000.f), t);
+  };
+  auto vector = [&](const u32x4& w) INLINE {
     float f[N];
     X::unpack(w, f);
-    float mx = fmaxf(f[0], f[1]);
+    float mx = max3(f[0], f[1], f[2]), mn = min3(f[0], f[1], f[2]);
 #pragma unroll
-    for (int i = 2; i < N; ++i) mx = fmaxf(mx, f[i]);
-    raise(mx, where);
-    const float ref = m == -INFINITY ? 0.f : m;
+    for (int i = 3; i < N; i += 2) {
+      mx = max3(mx, f[i], i + 1 < N ? f[i + 1] : f[i]);
+      mn = min3(mn, f[i], i + 1 < N ? f[i + 1] : f[i]);
+    }
+    raise(mx);
+    if (__builtin_amdgcn_ballot_w64(mn < lo)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) add(f[i], ref);
+      for (int i = 0; i < N; ++i) add_careful(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) add(f[i]);
+    }
+  };
+  // spans of `quads` rounds of kUnroll vectors a thread; the last has the rest
+  const int quads = (v1 - v0) / (kThreads * kUnroll) / kSpans + 1;
+  int span = 0, left = quads;
+  auto end_span = [&]() INLINE {
+    float q = fmaxf(cell, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(cell), 0xB1, 0xf, 0xf, false)));
+    q = fmaxf(q, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(q), 0x4E, 0xf, 0xf, false)));
+    if ((tid & 3) == 0) s_cell[span][tid >> 2] = q;
+    cell = -INFINITY;
+    ++span;
+    left = quads;
   };
   if (has_head) {
     const float v = X::one(x + tid * EB);
-    raise(v, kHead);
-    add(v, m == -INFINITY ? 0.f : m);
+    raise(v);
+    add_careful(v);
   }
-  int i = v0 + tid;
-  for (; i - tid + kThreads * kUnroll <= v1; i += kThreads * kUnroll) {
-    u32x4 w[kUnroll];
+  // rounds of kUnroll vectors, the next one's loads in flight under this one's sums
+  const int rounds = (v1 - v0) / (kThreads * kUnroll);
+  u32x4 even[kUnroll], odd[kUnroll];
+  auto load = [&](u32x4 (&w)[kUnroll], int round) INLINE {
+    const u32x4* src = mid + v0 + round * (kThreads * kUnroll) + tid;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u] = mid[i + kThreads * u];
+    for (int u = 0; u < kUnroll; ++u) w[u] = __builtin_nontemporal_load(src + kThreads * u);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto sum = [&](const u32x4 (&w)[kUnroll]) INLINE {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) vector(w[u], i + kThreads * u);
+    for (int u = 0; u < kUnroll; ++u) vector(w[u]);
+    if (--left == 0) end_span();
+  };
+  if (rounds > 0) load(even, 0);
+  int round = 0;
+  for (; round + 2 <= rounds; round += 2) {
+    load(odd, round + 1);
+    sum(even);
+    load(even, min(round + 2, rounds - 1));
+    sum(odd);
   }
-  for (; i < v1; i += kThreads) vector(mid[i], i);
+  if (round < rounds) sum(even);
+  for (int i = v0 + rounds * (kThreads * kUnroll) + tid; i < v1; i += kThreads) vector(mid[i]);
   if (has_tail) {
     const float v = X::one(x + (tail0 + tid) * EB);
-    raise(v, kTail);
-    add(v, m == -INFINITY ? 0.f : m);
+    raise(v);
+    add_careful(v);
   }
+  end_span();
 
-  const Sums ws = wave_join(Sums{m, s, t});
+  const float back = fast_exp2(-delta);  // from r to c m
+  const Sums ws = wave_join(Sums{m, s * back, back * __builtin_fmaf(-delta, s, t)});
   if (lane == 0) s_sums[wave] = ws;
-  if (tid == 0) {
-    s_n = 0;
-    s_thr = 1;
-  }
-  // the key of the thread's maximum at its first place
-  uint64_t mine = 0;
-  if (a.top > 0) {
-    if (at == kHead) {
-      mine = entry_key(m, tid);
-    } else if (at == kTail) {
-      mine = entry_key(m, tail0 + tid);
-    } else if (at >= 0) {
-      float f[N];
-      X::unpack(mid[at], f);
-      int k = 0;
-#pragma unroll
-      for (int j = N - 1; j >= 0; --j) k = f[j] == m ? j : k;
-      if (m == -INFINITY) k = 0;  // nothing above -inf, NaNs among it
-      mine = entry_key(m, head + at * N + k);
-    }
-    uint64_t g = max64(mine, shfl_xor64(mine, 1));
-    g = max64(g, shfl_xor64(g, 2));
-    if ((tid & 3) == 0) s_group[tid >> 2] = g;
-  }
+  if (tid == 0) s_n = s_nc = 0;
   __syncthreads();
   Sums v = s_sums[0];
 #pragma unroll
@@ -236,43 +284,76 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
   }
   if (a.top == 0) return;
   if (wave == 0) {
-    const uint64_t g = s_group[lane];
-    int r = 0;
-    for (int k = 0; k < kGroups; ++k) r += s_group[k] > g;
-    if (r == a.top - 1 && g != 0) s_thr = g;  // of distinct keys one at most
+    float g = s_cell[0][lane];
+    for (int k = 1; k < span; ++k) g = fmaxf(g, s_cell[k][lane]);
+    s_group[lane] = g;
+    if (lane == 0) s_thr = -INFINITY;
+    __builtin_amdgcn_wave_barrier();
+    int above = 0, reach = 0;
+    for (int k = 0; k < kGroups; ++k) {
+      above += s_group[k] > g;
+      reach += s_group[k] >= g;
+    }
+    if (above < a.top && a.top <= reach) s_thr = g;  // of lanes of one value
   }
   __syncthreads();
-  const uint64_t thr = s_thr;
-  const float thr_x = thr == 1 ? -INFINITY : key_value(thr);
+  const float thr = s_thr;
 
-  // f(key) for every entry of the thread at or above `low` in value
-  auto walk = [&](float low, auto&& f) {
-    if (has_head) f(entry_key(X::one(x + tid * EB), tid));
-    for (int i = v0 + tid; i < v1; i += kThreads * kUnroll) {
-      u32x4 w[kUnroll];
+  // which of a vector's entries are above, or at, low
+  auto hits = [&](const u32x4& w, float low, bool equal) INLINE {
+    float e[N];
+    X::unpack(w, e);
+    uint32_t hit = 0;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) w[u] = mid[min(i + kThreads * u, v1 - 1)];
+    for (int j = 0; j < N; ++j) {
+      const float v = e[j] == e[j] ? e[j] : -INFINITY;
+      hit |= (uint32_t)(v > low || (equal && v == low)) << j;
+    }
+    return hit;
+  };
+  auto edge_hit = [&](int j, float low, bool equal) INLINE {
+    const float e = X::one(x + j * EB), v = e == e ? e : -INFINITY;
+    return v > low || (equal && v == low);
+  };
+  auto key_of = [&](int j) INLINE { return entry_key(X::one(x + (int64_t)j * EB), j); };
+  // this thread's share of the listed cells' vectors, then its own head and tail
+  auto walk = [&](float low, bool equal, auto&& f) INLINE {
+    const int len = 4 * kUnroll * quads, items = s_nc * len;
+    for (int w0 = tid; w0 < items; w0 += kThreads * kUnroll) {
+      u32x4 w[kUnroll];
+      int i[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        if (i + kThreads * u >= v1) continue;
-        float e[N];
-        X::unpack(w[u], e);
+        const int q = min(w0 + kThreads * u, items - 1), c = q / len, k = q - c * len, cell = s_cand[c];
+        i[u] = v0 + (cell / kGroups * kUnroll * quads + k / 4) * kThreads + cell % kGroups * 4 + k % 4;
+        w[u] = mid[min(i[u], v1 - 1)];
+      }
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (!(e[j] < low)) f(entry_key(e[j], head + (i + kThreads * u) * N + j));
+      for (int u = 0; u < kUnroll; ++u) {
+        uint32_t hit = w0 + kThreads * u < items && i[u] < v1 ? hits(w[u], low, equal) : 0;
+        for (; hit; hit &= hit - 1) f(key_of(head + i[u] * N + __builtin_ctz(hit)));
       }
     }
-    if (has_tail) f(entry_key(X::one(x + (tail0 + tid) * EB), tail0 + tid));
+    if (has_head && edge_hit(tid, low, equal)) f(key_of(tid));
+    if (has_tail && edge_hit(tail0 + tid, low, equal)) f(key_of(tail0 + tid));
   };
-  if (mine >= thr)
-    walk(thr_x, [&](uint64_t k) {
-      if (k < thr) return;
+  // lists the cells (of a segment with vectors) whose maximum is above, or at, thr
+  auto list_cells = [&](bool equal) INLINE {
+    for (int c = tid; c < span * kGroups && v0 < v1; c += kThreads) {
+      const float g = s_cell[c / kGroups][c % kGroups];
+      if (g > thr || (equal && g == thr)) s_cand[atomicAdd(&s_nc, 1)] = (uint16_t)c;
+    }
+    __syncthreads();
+  };
+  auto list_entries = [&](bool equal) INLINE {
+    walk(thr, equal, [&](uint64_t k) INLINE {
       const int p = atomicAdd(&s_n, 1);
       if (p < kList) s_list[p] = k;
     });
-  __syncthreads();
-  const int n = s_n;
-  auto emit = [&](int r, uint64_t k) {
+    __syncthreads();
+    return s_n;
+  };
+  auto emit = [&](int r, uint64_t k) INLINE {
     if constexpr (FINAL) {
       a.top_logprobs[row * a.top + r] = key_value(k) - v.m - ln_s;
       a.top_ids[row * a.top + r] = key_index(k);
@@ -280,18 +361,61 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       a.keys[(row * a.S + seg) * a.top + r] = k;
     }
   };
+  list_cells(true);
+  int n = s_nc > kCellsRead ? kList + 1 : list_entries(true);
   if (n <= kList) {
     rank_list(s_list, n, a.top, emit);
     if constexpr (!FINAL)
       for (int r = n + tid; r < a.top; r += kThreads) emit(r, 0);
     return;
   }
-  // more entries than the list holds: each round takes the largest key below the last one
+  __syncthreads();
+  if (tid == 0) s_n = s_nc = 0;
+  __syncthreads();
+  list_cells(false);
+  n = list_entries(false);
+  if (n <= kList) {
+    rank_list(s_list, n, a.top, emit);
+    // the rest: entries equal to thr (there are enough) in index order
+    int found = n;
+    auto take = [&](uint32_t hit, int first) INLINE {  // bit j: entry first + j is such a one
+      const int count = __builtin_popcount(hit);
+      int before = count;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(before, o);
+        before += lane >= o ? y : 0;
+      }
+      if (lane == 63) s_count[wave] = before;
+      before -= count;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) {
+        before += k < wave ? s_count[k] : 0;
+        all += s_count[k];
+      }
+      __syncthreads();
+      for (int r = found + before; hit && r < a.top; ++r, hit &= hit - 1)
+        emit(r, entry_key(thr, first + __builtin_ctz(hit)));
+      found += all;
+    };
+    auto equals = [&](uint32_t at_or_above, uint32_t above) INLINE { return at_or_above & ~above; };
+    take(has_head ? equals(edge_hit(tid, thr, true), edge_hit(tid, thr, false)) : 0, tid);
+    for (int b = v0; b < v1 && found < a.top; b += kThreads) {
+      const u32x4 w = mid[min(b + tid, v1 - 1)];
+      take(b + tid < v1 ? equals(hits(w, thr, true), hits(w, thr, false)) : 0, head + (b + tid) * N);
+    }
+    if (found < a.top)
+      take(has_tail ? equals(edge_hit(tail0 + tid, thr, true), edge_hit(tail0 + tid, thr, false)) : 0, tail0 + tid);
+    if constexpr (!FINAL)
+      for (int r = found + tid; r < a.top; r += kThreads) emit(r, 0);
+    return;
+  }
   uint64_t last = ~0ull;
-  for (int r = 0; r < a.top; ++r) {
+  for (int r = 0; r < a.top; ++r) {  // the largest key below the last one
     uint64_t best = 0;
-    if (mine >= thr)  // the others' entries lie below thr
-      walk(thr_x, [&](uint64_t k) { best = k < last ? max64(best, k) : best; });
+    walk(thr, false, [&](uint64_t k) INLINE { best = k < last ? max64(best, k) : best; });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) best = max64(best, shfl_xor64(best, o));
     if (lane == 0) s_best[wave] = best;
@@ -303,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
 }
 
 // Joins a row's segments: the sums over lanes, the alternatives as above (the segments' largest keys in the place of
-// the threads' maxima).
+// the cells' maxima).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   __shared__ Sums s_sums;
@@ -317,13 +441,15 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     s_n = 0;
     s_thr = 1;
   }
-  if (tid < kMaxLogprobSplits) {
+  // the segments' q-th largest keys: the (top / q)-th largest of them has `top` keys at or above it
+  const int q = min(a.top, (2 * a.top + a.S - 1) / a.S);
+  if (tid < 64) {
     Sums v{-INFINITY, 0.f, 0.f};
     if (tid < a.S) {
       const float4 p = a.part[row * a.S + tid];
       v = Sums{p.x, p.y, p.z};
     }
-    if (a.top > 0) s_first[tid] = tid < a.S ? keys[(int64_t)tid * a.top] : 0;
+    if (a.top > 0 && tid < kMaxLogprobSplits) s_first[tid] = tid < a.S ? keys[(int64_t)tid * a.top + q - 1] : 0;
     v = wave_join(v);
     if (tid == 0) {
       s_sums = v;
@@ -336,7 +462,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     const uint64_t g = s_first[tid];
     int r = 0;
     for (int k = 0; k < kMaxLogprobSplits; ++k) r += s_first[k] > g;
-    if (r == a.top - 1 && g != 0) s_thr = g;
+    if (r == (a.top + q - 1) / q - 1 && g != 0) s_thr = g;
   }
   __syncthreads();
   const uint64_t thr = s_thr;
@@ -357,11 +483,14 @@ int vec_elems(int32_t dtype) { return dtype == 0 ? 4 : 8; }
 
 }  // namespace
 
-// Segments of a row: about kTarget workgroups in all (eight of a CU's, all resident), whole chunks of 256 vectors each.
+// Segments of a row, whole chunks of 256 vectors each: up to kTarget workgroups in all, where a row to itself leaves the
+// chip idle. A segment pays for its own alternatives and the joining launch, so no more (bf16, 128256 entries, 5
+// alternatives, us by segments: 512 rows 1: 28.8, 2: 34.1; 300 rows 27.1, 27.5; 128 rows 1: 20.1, 2: 18.4, 4: 17.8,
+// 8: 18.2; 64 rows 2: 17.7, 4: 15.1, 8: 14.5, 16: 15.0; 8 rows 8: 11.9, 32: 11.5, 63: 11.6).
 int32_t logprob_splits(int64_t rows, int32_t V, int32_t dtype) {
-  constexpr int64_t kTarget = 2048;
+  constexpr int64_t kTarget = 512;
   const int64_t chunks = (V / vec_elems(dtype) + kThreads - 1) / kThreads;
-  int64_t s = rows > 0 ? (kTarget + rows - 1) / rows : 1;
+  int64_t s = rows > 0 ? kTarget / rows : 1;
   if (s > chunks) s = chunks;
   if (s > kMaxLogprobSplits) s = kMaxLogprobSplits;
   return s < 1 ? 1 : (int32_t)s;

@@ -76,6 +76,14 @@ def test_one_row_seen_many_times(hip_device):
 
 
 @pytest.mark.parametrize("T", [2, 2100])
+@pytest.mark.parametrize("offset", [-30000.0, 30000.0, -3e37, 3e37])
+def test_far_from_zero(hip_device, T, offset):
+    """Logits far from 0 (their differences are whole numbers, exact there): the reference cancels whatever its size."""
+    x = torch.randint(-20, 20, (T, 3000), device=hip_device).float() * max(1.0, abs(offset) / 2**22)
+    _check(x + offset, torch.arange(T, device=hip_device), 9)
+
+
+@pytest.mark.parametrize("T", [2, 2100])
 @pytest.mark.parametrize("V", [515, 40000])
 def test_ties_go_to_the_lowest_id(hip_device, T, V):
     x, tok = _logits(T, V, torch.bfloat16, hip_device, seed=V)
@@ -106,7 +114,9 @@ def test_masked_vocabulary_and_special_rows(hip_device, dtype, T, V):
     x[6, 3] = torch.finfo(dtype).max
     r = _check(x, tok, 20)
     assert r.logprobs[2].isnan() and r.logprobs[3].isnan() and r.logprobs[4].isnan()
-    assert r.logprobs[1] == -inf and r.logprobs[5] == 0 and r.entropy[5] == 0
+    assert r.logprobs[1] == -inf
+    # the one term is 2^delta taken back by 2^-delta, an ulp each: ln s within 2^-22 of 0, ln 2 t / s within as much
+    assert r.logprobs[5].abs() <= 2.0**-22 and r.entropy[5].abs() <= 2.0**-21
     assert r.top_ids[2].tolist() == list(range(20))
     assert r.top_ids[0, :4].tolist() == [V // 2, 5, V - 1, 0] and (r.top_logprobs[0, 3:] == -inf).all()
     ids = r.top_ids[4]

@@ -33,10 +33,11 @@ def test_refusals(over, want):
 
 def test_workspace_size():
     f = _lib.load().kvh_token_logprobs_workspace_size
-    assert f(4, 1000, 5, 2) == 0  # one segment a row
+    assert f(4, 1000, 5, 2) == 0 and f(300, 128256, 5, 2) == 0  # one segment a row
     assert f(4096, 128256, 20, 2) == 0
-    assert f(8, 128256, 5, 2) == 8 * 63 * (16 + 5 * 8)  # 63 chunks of 2048 logits
-    assert f(1023, 128256, 20, 2) == 1023 * 3 * (16 + 20 * 8)
+    assert f(8, 128256, 5, 2) == 8 * 32 * (16 + 5 * 8)
+    assert f(100, 128256, 20, 2) == 100 * 5 * (16 + 20 * 8)  # 512 workgroups in all
+    assert f(8, 20000, 5, 0) == 8 * 20 * (16 + 5 * 8)  # chunks of 1024 fp32 logits
     assert f(8, 128256, 65, 2) == 0 and f(-1, 10, 1, 2) == 0  # refused anyway
 
 
