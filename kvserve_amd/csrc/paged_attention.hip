@@ -122,7 +122,7 @@ struct VRegs8 {
 // The same chunk from an MXFP4 cache (kKv4). K: lane (j, n) holds row n of tile t, D / 4 elements from d = (D / 4) j
 // on, all under one scale, and operand c takes d = (D / 4) j + 8c .. +7. V: lane (j, m) holds d = VW m .. VW m + VW - 1
 // of 8 tokens, and the scale of the token that its place in its quad names (slot 4 tile + m % 4).
-// Row 4j + e of a tile is token 4e + j (tile_token): a V load e then reads the four whole rows of tokens 4e .. 4e + 3,
+// Row 4j + e of a tile is token 4e + j (kv4_token): a V load e then reads the four whole rows of tokens 4e .. 4e + 3,
 // at D = 128 with a head's tokens together in a page two whole lines, not half a row of eight.
 template <int D>
 struct KRegs4 {
@@ -136,18 +136,7 @@ struct VRegs4 {
   uint32_t x[2];
 };
 
-// Token of a 16-token tile that row 4j + e of S^T and V slot e of lanes (j, *) stand for.
-template <int KV>
-__device__ __forceinline__ int tile_token(int j, int e) {
-  return KV == kKv4 ? 4 * e + j : 4 * j + e;
-}
-template <class KR>
-constexpr int regs_format = kKv16;
-template <int D>
-constexpr int regs_format<KRegs8<D>> = kKv8;
-template <int D>
-constexpr int regs_format<KRegs4<D>> = kKv4;
-
+__device__ __forceinline__ int kv4_token(int j, int e) { return 4 * e + j; }
 // Uniform description of a chunk: first token and the block of each 16-token tile.
 struct ChunkRef {
   int tok0;
@@ -170,7 +159,6 @@ __device__ __forceinline__ ChunkRef chunk_ref(PageWindow& pw, const PAParams& p,
 struct LaneOffsets {
   uint32_t k;  // (n * k_ss + 8 j) * 2
   uint32_t v;  // (4j * v_ss + VW n) * 2
-  uint32_t kx, vx;  // MXFP4: the scale bytes
 };
 
 // Whole-line K reads (LINES), for up to 8 query rows (R <= 8, one tile): an instruction reads 128
@@ -186,15 +174,6 @@ __device__ __forceinline__ LaneOffsets lane_offsets(const PAParams& p) {
   const int lane = threadIdx.x & 63;
   const int j = lane >> 4, n = lane & 15;
   LaneOffsets o;
-  o.kx = o.vx = 0;
-  if (KV == kKv4) {  // strides in bytes
-    const uint32_t tok = (uint32_t)tile_token<KV>(n >> 2, n & 3);
-    o.k = tok * (uint32_t)p.k_ss + (uint32_t)(D / 8 * j);
-    o.kx = tok * (uint32_t)p.kx_ss + (uint32_t)(D / 4 * j / kFp4Block);
-    o.v = (uint32_t)j * (uint32_t)p.v_ss + (uint32_t)(D / 32 * n);
-    o.vx = (uint32_t)tile_token<KV>(j, n & 3) * (uint32_t)p.vx_ss + (uint32_t)(D / 16 * n / kFp4Block);
-    return o;
-  }
   if (LINES) {  // token n % 8 of a group of 8, 16-byte chunk 2 j + n / 8 of the line
     o.k = (uint32_t)((n & 7) * (uint32_t)p.k_ss) * (KV == kKv8 ? 1u : 2u) + 16u * (uint32_t)(2 * j + (n >> 3));
     o.v = (uint32_t)(4 * j * (uint32_t)p.v_ss + (D / 16) * n) * (KV == kKv8 ? 1u : 2u);
@@ -228,8 +207,7 @@ __device__ __forceinline__ T stream_load(const void* p) {
 // and is masked out of the scores and zeroed out of V like any invalid key.
 // LINES: r.k[t][g D / 64 + cc] is line cc of the 8-token group g of tile t.
 template <int D, bool NTL, bool LINES>
-__device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
-  const uint32_t k_lane = lo.k;
+__device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t k_lane) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -249,8 +227,7 @@ __device__ __forceinline__ void load_k(KRegs<D>& r, const PAParams& p, const Chu
 }
 
 template <int D, bool NTL>
-__device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
-  const uint32_t v_lane = lo.v;
+__device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t v_lane) {
   constexpr int VD = D / 32;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -276,8 +253,7 @@ __device__ __forceinline__ void load_v(VRegs<D>& r, const PAParams& p, const Chu
 }
 
 template <int D, bool NTL, bool LINES>
-__device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
-  const uint32_t k_lane = lo.k;
+__device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t k_lane) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -291,8 +267,7 @@ __device__ __forceinline__ void load_k(KRegs8<D>& r, const PAParams& p, const Ch
 }
 
 template <int D, bool NTL>
-__device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, const LaneOffsets& lo) {
-  const uint32_t v_lane = lo.v;
+__device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const ChunkRef& c, int kvh, uint32_t v_lane) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
@@ -308,49 +283,6 @@ __device__ __forceinline__ void load_v(VRegs8<D>& r, const PAParams& p, const Ch
       } else {
         r.v[4 * t + e][0] = stream_load<uint32_t, NTL>(src);
       }
-    }
-  }
-}
-
-template <int D, bool NTL, bool LINES>
-__device__ __forceinline__ void load_k(KRegs4<D>& r, const PAParams& p, const ChunkRef& c, int kvh,
-                                       const LaneOffsets& lo) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
-    const int slot0 = (c.tok0 + 16 * t) % p.BS;
-    const char* page = (const char*)p.kc + blk * p.k_sb + (int64_t)kvh * p.k_sh + (int64_t)slot0 * p.k_ss;
-    const uint8_t* sc = p.kx + blk * p.kx_sb + (int64_t)kvh * p.kx_sh + (int64_t)slot0 * p.kx_ss;
-    r.x[t] = sc[lo.kx];
-    if constexpr (D == 128) {
-      const u32x4 w = stream_load<u32x4, NTL>(page + lo.k);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.k[t][i] = w[i];
-    } else {
-      const u32x2 w = stream_load<u32x2, NTL>(page + lo.k);
-      r.k[t][0] = w[0];
-      r.k[t][1] = w[1];
-    }
-  }
-}
-
-template <int D, bool NTL>
-__device__ __forceinline__ void load_v(VRegs4<D>& r, const PAParams& p, const ChunkRef& c, int kvh,
-                                       const LaneOffsets& lo) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int64_t blk = c.blk[t] >= 0 ? c.blk[t] : 0;
-    const int slot0 = (c.tok0 + 16 * t) % p.BS;
-    const char* page = (const char*)p.vc + blk * p.v_sb + (int64_t)kvh * p.v_sh + (int64_t)slot0 * p.v_ss;
-    const uint8_t* sc = p.vx + blk * p.vx_sb + (int64_t)kvh * p.vx_sh + (int64_t)slot0 * p.vx_ss;
-    r.x[t] = sc[lo.vx];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const char* src = page + (int64_t)e * 4 * p.v_ss + lo.v;
-      if constexpr (D == 128)
-        r.v[4 * t + e] = stream_load<uint32_t, NTL>(src);
-      else
-        r.v[4 * t + e] = stream_load<uint16_t, NTL>(src);
     }
   }
 }
@@ -434,7 +366,7 @@ __device__ __forceinline__ void load_q(WaveState<D, NT>& s, const PAParams& p, i
     } else {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) s.q[t][c] = u32x4{0, 0, 0, 0};
-      s.limit[t] = 0;
+      s.limit[t] = KV == kKv4 ? INT32_MAX : 0;  // (run_chunks_kv4: a row that is not stored limits nothing)
     }
   }
 }
@@ -498,7 +430,7 @@ __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, 
         for (int cc = 0; cc < D / 32; ++cc) a = E::mfma(kr.k[tile][cc], s.q[t][cc], a);
         st[t][tile] = a;
       }
-  } else {  // E4M3, MXFP4: convert each tile's operands once for all row tiles
+  } else {  // E4M3: convert each tile's operands once for all row tiles
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
       u32x4 k[D / 32];
@@ -522,7 +454,7 @@ __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, 
       for (int e = 0; e < 4; ++e) {
         float x = st[t][tile][e] * p.qk_scale;
         if (MASKED) {
-          const int tok = c.tok0 + 16 * tile + tile_token<regs_format<KR>>(j, e);
+          const int tok = c.tok0 + 16 * tile + 4 * j + e;
           if (!(c.blk[tile] >= 0 && tok < s.limit[t])) x = -INFINITY;
         }
         st[t][tile][e] = x;
@@ -711,44 +643,9 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs8<D>& vr, con
     }
 }
 
-// O^T += V^T P^T from an MXFP4 V chunk: the scales of a quad's four tokens are read across it (DPP), the nibbles
-// convert to the 16-bit chunk's registers. A masked token's scale becomes 2^-127: its elements are then
-// finite whatever its bytes (an E2M1 code has no NaN), and its P is 0.
-template <class E, int D, int NT, bool MASKED>
-__device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs4<D>& vr, const ChunkRef& c, int data_end,
-                                         const u32x4 pt[NT]) {
-  const int lane = threadIdx.x & 63, j = lane >> 4;
-  VRegs<D> v;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    uint32_t x = vr.x[t] << 23;
-    if (MASKED) {
-      const int tok = c.tok0 + 16 * t + tile_token<kKv4>(j, lane & 3);
-      x = c.blk[t] >= 0 && tok < data_end ? x : 0u;
-    }
-    const int f[4] = {__builtin_amdgcn_update_dpp(0, (int)x, 0x00, 0xf, 0xf, false),
-                      __builtin_amdgcn_update_dpp(0, (int)x, 0x55, 0xf, 0xf, false),
-                      __builtin_amdgcn_update_dpp(0, (int)x, 0xaa, 0xf, 0xf, false),
-                      __builtin_amdgcn_update_dpp(0, (int)x, 0xff, 0xf, 0xf, false)};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t w = vr.v[4 * t + e];
-      const float sc = __int_as_float(f[e]);
-      v.v[4 * t + e][0] = E::template from_fp4x2<0>(w, sc);
-      v.v[4 * t + e][1] = E::template from_fp4x2<1>(w, sc);
-      if constexpr (D == 128) {
-        v.v[4 * t + e][2] = E::template from_fp4x2<2>(w, sc);
-        v.v[4 * t + e][3] = E::template from_fp4x2<3>(w, sc);
-      }
-    }
-  }
-  chunk_pv<E, D, NT, false>(s, v, c, data_end, pt);
-}
-
-template <int D, int KV>
-using KChunk = std::conditional_t<KV == kKv4, KRegs4<D>, std::conditional_t<KV == kKv8, KRegs8<D>, KRegs<D>>>;
-template <int D, int KV>
-using VChunk = std::conditional_t<KV == kKv4, VRegs4<D>, std::conditional_t<KV == kKv8, VRegs8<D>, VRegs<D>>>;
+template <class E, int D, int NT, bool NTL>
+__device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
+                                               int tok_begin, int stride, int tok_hi, int data_end);
 
 // Chunk loop of one wave over tokens tok_begin, tok_begin + stride, ... < tok_hi.
 // The body is straight-line (masks always applied, loads unconditional) and the loads are
@@ -757,17 +654,21 @@ using VChunk = std::conditional_t<KV == kKv4, VRegs4<D>, std::conditional_t<KV =
 template <class E, int D, int NT, int KV = kKv16, bool NTL = true, bool LINES = false>
 __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
                                            int tok_begin, int stride, int tok_hi, int data_end) {
+  if constexpr (KV == kKv4) {
+    run_chunks_kv4<E, D, NT, NTL>(s, p, btrow, kvh, tok_begin, stride, tok_hi, data_end);
+    return;
+  }
   if (tok_begin >= tok_hi) return;
   const int page_end = (tok_hi + p.BS - 1) / p.BS;
   const LaneOffsets lo = lane_offsets<D, KV, LINES>(p);
   PageWindow pw;
   load_window(pw, p, btrow, tok_begin / p.BS, page_end);
   ChunkRef c = chunk_ref(pw, p, btrow, tok_begin, tok_hi, page_end);
-  KChunk<D, KV> kr;
-  VChunk<D, KV> vr;
-  load_k<D, NTL, LINES>(kr, p, c, kvh, lo);
+  std::conditional_t<KV == kKv8, KRegs8<D>, KRegs<D>> kr;
+  std::conditional_t<KV == kKv8, VRegs8<D>, VRegs<D>> vr;
+  load_k<D, NTL, LINES>(kr, p, c, kvh, lo.k);
   __builtin_amdgcn_sched_barrier(0);
-  load_v<D, NTL>(vr, p, c, kvh, lo);
+  load_v<D, NTL>(vr, p, c, kvh, lo.v);
   __builtin_amdgcn_sched_barrier(0);
   // Every iteration has a next chunk, so its loads are unconditional; the last chunk is
   // peeled off below the loop.
@@ -776,17 +677,251 @@ __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& 
     u32x4 pt[NT];
     chunk_scores<E, D, NT, true, LINES>(s, kr, p, c, pt);
     __builtin_amdgcn_sched_barrier(0);
-    load_k<D, NTL, LINES>(kr, p, cn, kvh, lo);
+    load_k<D, NTL, LINES>(kr, p, cn, kvh, lo.k);
     __builtin_amdgcn_sched_barrier(0);
     chunk_pv<E, D, NT, true>(s, vr, c, data_end, pt);
     __builtin_amdgcn_sched_barrier(0);
-    load_v<D, NTL>(vr, p, cn, kvh, lo);
+    load_v<D, NTL>(vr, p, cn, kvh, lo.v);
     __builtin_amdgcn_sched_barrier(0);
     c = cn;
   }
   u32x4 pt[NT];
   chunk_scores<E, D, NT, true, LINES>(s, kr, p, c, pt);
   chunk_pv<E, D, NT, true>(s, vr, c, data_end, pt);
+}
+
+// ---------------------------------------------------------------------------------------
+// MXFP4 caches. A chunk is a quarter of the 16-bit one's bytes, so run_chunks' own addresses and masks weigh four times
+// as much (254 of its 550 instructions a chunk were scalar: 64 decodes of 1023-8191 keys 75.6 us, here 70.2; 32
+// sequences of 6 queries 46.6, here 43.8). Here the page offsets of 64 tiles are computed one a lane, the loads take a
+// scalar base and 32-bit lane offsets, chunks that every row sees whole take no masks, and a score costs one FMA and
+// one exponential. What bounds it now are the loads: with scores, softmax and values left out the walk still takes
+// 67-70 us, and 128 decodes of 8000-16000 keys (1.72 GB) 315 of 319 us, 5.4 TB/s. The window's offsets cost a short
+// walk 1.3 us (16 decodes 22.9 us, 21.6), and pages with a token's heads together, where a row of 64 bytes stands by
+// itself, are slower (89.6 us, 83.4): the documented layout keeps a head's rows together.
+//
+// Byte offsets, from the cache's and the scales' first, of tiles tile0 .. tile0 + 63, one a lane; the values' are
+// apart only where their strides differ from the keys'. ok: the tiles that are there.
+struct Kv4Window {
+  uint64_t k, kx, v, vx;
+  uint64_t ok;
+  int tile0;
+};
+
+__device__ __forceinline__ bool kv4_same_strides(const PAParams& p) {
+  return p.k_sb == p.v_sb && p.k_ss == p.v_ss && p.kx_sb == p.vx_sb && p.kx_ss == p.vx_ss;
+}
+
+__device__ __forceinline__ void kv4_window(Kv4Window& w, const PAParams& p, const int64_t* btrow, int tile0,
+                                           int tile_end, bool same) {
+  const int tile = tile0 + (threadIdx.x & 63), r = p.BS / 16, page = tile / r;
+  const bool in = tile < tile_end;
+  const int64_t raw = btrow[in ? page : 0];  // every lane loads: no divergent branch
+  const bool ok = in && raw >= 0 && raw < p.num_blocks;
+  const uint64_t b = ok ? (uint64_t)raw : 0, slot = (uint64_t)((tile - page * r) * 16);
+  w.ok = __builtin_amdgcn_ballot_w64(ok);
+  w.k = b * (uint64_t)p.k_sb + slot * (uint64_t)p.k_ss;
+  w.kx = b * (uint64_t)p.kx_sb + slot * (uint64_t)p.kx_ss;
+  if (!same) {
+    w.v = b * (uint64_t)p.v_sb + slot * (uint64_t)p.v_ss;
+    w.vx = b * (uint64_t)p.vx_sb + slot * (uint64_t)p.vx_ss;
+  }
+  w.tile0 = tile0;
+}
+
+// Offsets of a chunk's two tiles (`rel` and the next of the window; an absent tile's are block 0's).
+struct Kv4Chunk {
+  uint64_t k[2], kx[2], v[2], vx[2];
+};
+
+__device__ __forceinline__ uint64_t lane_u64(uint64_t x, int l) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
+}
+
+// This wave's lane offsets and bases of a kv head.
+template <int D>
+struct Kv4Lanes {
+  uint64_t kc, kx, vc, vx;         // addresses at the kv head
+  uint32_t ko, kxo, vo[4], vxo;    // lane offsets in bytes; vo[e]: V load e of a tile
+  __device__ __forceinline__ Kv4Lanes(const PAParams& p, int kvh) {
+    const int lane = threadIdx.x & 63, j = lane >> 4, n = lane & 15;
+    kc = (uint64_t)(uintptr_t)p.kc + (uint64_t)kvh * (uint64_t)p.k_sh;
+    kx = (uint64_t)(uintptr_t)p.kx + (uint64_t)kvh * (uint64_t)p.kx_sh;
+    vc = (uint64_t)(uintptr_t)p.vc + (uint64_t)kvh * (uint64_t)p.v_sh;
+    vx = (uint64_t)(uintptr_t)p.vx + (uint64_t)kvh * (uint64_t)p.vx_sh;
+    const uint32_t tok = (uint32_t)kv4_token(n >> 2, n & 3);
+    ko = tok * (uint32_t)p.k_ss + (uint32_t)(D / 8 * j);
+    kxo = tok * (uint32_t)p.kx_ss + (uint32_t)(D / 4 * j / kFp4Block);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vo[e] = (uint32_t)kv4_token(j, e) * (uint32_t)p.v_ss + (uint32_t)(D / 32 * n);
+    vxo = (uint32_t)kv4_token(j, n & 3) * (uint32_t)p.vx_ss + (uint32_t)(D / 16 * n / kFp4Block);
+  }
+};
+
+__device__ __forceinline__ Kv4Chunk kv4_chunk(const Kv4Window& w, int rel, bool same) {
+  Kv4Chunk c;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    c.k[t] = c.v[t] = lane_u64(w.k, rel + t);
+    c.kx[t] = c.vx[t] = lane_u64(w.kx, rel + t);
+    if (!same) {
+      c.v[t] = lane_u64(w.v, rel + t);
+      c.vx[t] = lane_u64(w.vx, rel + t);
+    }
+  }
+  return c;
+}
+
+// One load at a scalar base and a 32-bit lane offset (the empty asm keeps the two apart, as in pf_issue; `off` is passed
+// through its own in place).
+template <class T, bool NTL>
+__device__ __forceinline__ T kv4_load(uint64_t base, uint32_t& off) {
+  asm volatile("" : "+s"(base));
+  asm volatile("" : "+v"(off));
+  typedef const __attribute__((address_space(1))) char* global_bytes;
+  typedef const __attribute__((address_space(1))) T* global_t;
+  if constexpr (NTL)
+    return __builtin_nontemporal_load((global_t)((global_bytes)base + off));
+  else
+    return *(global_t)((global_bytes)base + off);
+}
+
+template <int D, bool NTL>
+__device__ __forceinline__ void kv4_load_k(KRegs4<D>& r, Kv4Lanes<D>& l, const Kv4Chunk& c) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if constexpr (D == 128) {
+      const u32x4 w = kv4_load<u32x4, NTL>(l.kc + c.k[t], l.ko);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.k[t][i] = w[i];
+    } else {
+      const u32x2 w = kv4_load<u32x2, NTL>(l.kc + c.k[t], l.ko);
+      r.k[t][0] = w[0];
+      r.k[t][1] = w[1];
+    }
+    r.x[t] = kv4_load<uint8_t, false>(l.kx + c.kx[t], l.kxo);
+  }
+}
+
+template <int D, bool NTL>
+__device__ __forceinline__ void kv4_load_v(VRegs4<D>& r, Kv4Lanes<D>& l, const Kv4Chunk& c) {
+  using W = std::conditional_t<D == 128, uint32_t, uint16_t>;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[4 * t + e] = kv4_load<W, NTL>(l.vc + c.v[t], l.vo[e]);
+    r.x[t] = kv4_load<uint8_t, false>(l.vx + c.vx[t], l.vxo);
+  }
+}
+
+// Raw scores of a chunk.
+template <class E, int D, int NT>
+__device__ __forceinline__ void kv4_scores(const WaveState<D, NT>& s, const KRegs4<D>& kr, f32x4 (&st)[NT][2]) {
+#pragma unroll
+  for (int tile = 0; tile < 2; ++tile) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) st[t][tile] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int cc = 0; cc < D / 32; ++cc) {
+      const u32x4 k = k_operand<E, D>(kr, tile, cc);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) st[t][tile] = E::mfma(k, s.q[t][cc], st[t][tile]);
+    }
+  }
+}
+
+// -inf where row and key do not meet (bits: the tiles that are there). The values of a token that is not there take the
+// scale 2^-127: finite whatever their bytes (an E2M1 code has no NaN), for its P of 0.
+template <int D, int NT>
+__device__ __forceinline__ void kv4_mask(const WaveState<D, NT>& s, VRegs4<D>& vr, int tok0, int bits, int data_end,
+                                         f32x4 (&st)[NT][2]) {
+  const int lane = threadIdx.x & 63, j = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const bool in = ((bits >> t) & 1) && tok0 + 16 * t + kv4_token(j, lane & 3) < data_end;
+    vr.x[t] = in ? vr.x[t] : 0u;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      const int lim = (bits >> tile) & 1 ? s.limit[t] - (tok0 + 16 * tile + j) : INT32_MIN;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[t][tile][e] = 4 * e < lim ? st[t][tile][e] : -INFINITY;
+    }
+}
+
+// Online-softmax update from (masked) raw scores, c > 0: pf_softmax with a shift that is always the row's maximum (in
+// thr as a raw score), so that the largest P is 1 and no rounding meets it: with the prefill's slack a softmax of few
+// large terms was off by 2.4e-3 instead of 1.7e-3 in bf16 (2-norm). A maximum moves some ten times in thousands of keys.
+template <class E, int D, int NT>
+__device__ __forceinline__ void kv4_softmax(WaveState<D, NT>& s, const f32x4 (&st)[NT][2], float c, u32x4 (&pt)[NT]) {
+  float mx[NT];
+  pf_lanemax<NT>(st, mx);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (__builtin_amdgcn_ballot_w64(mx[t] > s.thr[t])) {
+      const float top = fmaxf(s.thr[t], max_over_groups(mx[t]));
+      const bool empty = top == -INFINITY;  // the ballot is wave-wide
+      const float nsh = empty ? 0.f : -top * c;
+      const float alpha = s.thr[t] == -INFINITY ? 0.f : fast_exp2(nsh - s.nsh[t]);
+      s.l[t] *= alpha;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s.acc[t][i] *= alpha;
+      s.thr[t] = top;
+      s.nsh[t] = nsh;
+      s.m[t] = empty ? -INFINITY : -nsh;
+    }
+    float pv[8];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pv[4 * tile + e] = fast_exp2(__builtin_fmaf(st[t][tile][e], c, s.nsh[t]));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      pt[t][w] = E::pack2(pv[2 * w], pv[2 * w + 1]);
+      s.l[t] = E::dot2_ones(pt[t][w], s.l[t]);
+    }
+  }
+}
+
+// O^T += V^T P^T: the scales of a quad's four tokens are read across it (DPP); a byte of each token's converts to a
+// neighbouring pair of its elements, and the halves of two tokens' make the operands' dwords.
+template <class E, int D, int NT>
+__device__ __forceinline__ void kv4_pv(WaveState<D, NT>& s, const VRegs4<D>& vr, const u32x4 (&pt)[NT]) {
+  float f[8];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint32_t x = vr.x[t] << 23;
+    f[4 * t] = __int_as_float(__builtin_amdgcn_update_dpp(0, (int)x, 0x00, 0xf, 0xf, false));
+    f[4 * t + 1] = __int_as_float(__builtin_amdgcn_update_dpp(0, (int)x, 0x55, 0xf, 0xf, false));
+    f[4 * t + 2] = __int_as_float(__builtin_amdgcn_update_dpp(0, (int)x, 0xaa, 0xf, 0xf, false));
+    f[4 * t + 3] = __int_as_float(__builtin_amdgcn_update_dpp(0, (int)x, 0xff, 0xf, 0xf, false));
+  }
+  auto pair = [&](auto X) __attribute__((always_inline)) {
+    constexpr int x = decltype(X)::value;
+    uint32_t c[8];
+#pragma unroll
+    for (int t8 = 0; t8 < 8; ++t8) c[t8] = E::template from_fp4x2<x>(vr.v[t8], f[t8]);
+    u32x4 lo, hi;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      lo[w] = pick_halves<0>(c[2 * w], c[2 * w + 1]);
+      hi[w] = pick_halves<1>(c[2 * w], c[2 * w + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s.acc[t][2 * x] = E::mfma(lo, pt[t], s.acc[t][2 * x]);
+      s.acc[t][2 * x + 1] = E::mfma(hi, pt[t], s.acc[t][2 * x + 1]);
+    }
+  };
+  pair(std::integral_constant<int, 0>{});
+  pair(std::integral_constant<int, 1>{});
+  if constexpr (D == 128) {
+    pair(std::integral_constant<int, 2>{});
+    pair(std::integral_constant<int, 3>{});
+  }
 }
 
 template <class E, int VW>
@@ -1219,7 +1354,7 @@ __device__ __forceinline__ void load_q_group(WaveState<D, NX>& s, const PAParams
     } else {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) s.q[t][c] = u32x4{0, 0, 0, 0};
-      s.limit[t] = 0;
+      s.limit[t] = KV == kKv4 ? INT32_MAX : 0;
     }
   }
 }
@@ -2084,6 +2219,65 @@ __device__ __forceinline__ float pf_q_ready(WaveState<D, NT>& s, const PAParams&
   return c;
 }
 
+// run_chunks over an MXFP4 cache: the next chunk's K and V are in flight while this one is computed.
+template <class E, int D, int NT, bool NTL>
+__device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
+                                               int tok_begin, int stride, int tok_hi, int data_end) {
+  if (tok_begin >= tok_hi) return;
+  const bool same = kv4_same_strides(p);
+  const int tile_end = (tok_hi + 15) / 16;
+  Kv4Window win;
+  kv4_window(win, p, btrow, tok_begin / 16, tile_end, same);
+  Kv4Lanes<D> lanes(p, kvh);
+  KRegs4<D> kr;
+  VRegs4<D> vr;
+  int tok0 = tok_begin;
+  int bits = (int)(win.ok & 3);
+  {
+    const Kv4Chunk n = kv4_chunk(win, 0, same);
+    kv4_load_k<D, NTL>(kr, lanes, n);
+    __builtin_amdgcn_sched_barrier(0);
+    kv4_load_v<D, NTL>(vr, lanes, n);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const float c = pf_q_ready<E, D, NT>(s, p);
+  // keys that every row sees
+  int seen = min(tok_hi, data_end);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) seen = min(seen, s.limit[t]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) seen = min(seen, __shfl_xor(seen, o));
+  seen = uni(seen);
+  auto step = [&](auto more) __attribute__((always_inline)) {
+    constexpr bool MORE = decltype(more)::value;
+    const int next = tok0 + stride;
+    Kv4Chunk n;
+    int nbits = 0;
+    if (MORE) {
+      if (next / 16 + 2 - win.tile0 > 64) kv4_window(win, p, btrow, next / 16, tile_end, same);
+      const int rel = next / 16 - win.tile0;
+      n = kv4_chunk(win, rel, same);
+      nbits = (int)(win.ok >> rel & 3);
+    }
+    f32x4 st[NT][2];
+    kv4_scores<E, D, NT>(s, kr, st);
+    __builtin_amdgcn_sched_barrier(0);
+    if (MORE) kv4_load_k<D, NTL>(kr, lanes, n);
+    __builtin_amdgcn_sched_barrier(0);
+    if (tok0 + kChunk > seen || bits != 3) kv4_mask<D, NT>(s, vr, tok0, bits, data_end, st);
+    u32x4 pt[NT];
+    kv4_softmax<E, D, NT>(s, st, c, pt);
+    kv4_pv<E, D, NT>(s, vr, pt);
+    __builtin_amdgcn_sched_barrier(0);
+    if (MORE) kv4_load_v<D, NTL>(vr, lanes, n);
+    __builtin_amdgcn_sched_barrier(0);
+    tok0 = next;
+    bits = nbits;
+  };
+  while (tok0 + stride < tok_hi) step(std::true_type{});
+  step(std::false_type{});
+}
+
 // One workgroup's pass over chunks [c_lo, c_hi) of tile t of (seq, kvh): the whole tile
 // (written out) or a piece of it (partial in slot `slot` of the prefill partial arrays).
 //
@@ -2708,7 +2902,7 @@ static int resident_blocks(const void* kernel, int block_threads = 256, int* per
 
 // Sets the decode units (PAParams::NU, R1) of a launch of `kernel`, which holds `resident`
 // workgroups, `per_cu` on each CU; returns their workgroups.
-static int decode_units(PAParams& p, int resident, int per_cu, bool kv8) {
+static int decode_units(PAParams& p, int resident, int per_cu, bool packed, bool all) {
   int waves = resident * kWavesPerWG;
   if (waves > kMaxDecodeWaves) waves = kMaxDecodeWaves;
   int64_t units = waves / p.HGW;
@@ -2724,11 +2918,13 @@ static int decode_units(PAParams& p, int resident, int per_cu, bool kv8) {
   // SIMD (the two-tile verify rows, the 32-row cascade tiles) keeps both: C5 over E4M3 decode
   // 64.8 -> 58.1 us HBM-cold against two thirds of them. A kernel that fits one wave per SIMD
   // (the 64-row cascade tiles, 48 or 64 verify rows) keeps them all: halving would idle half
-  // the CUs.
+  // the CUs. MXFP4 caches of 64-wide heads (`all`) keep three as well: their loads are so short that more of them in
+  // flight outweigh the uneven ends (64 decodes of 1023-8191 keys 51.8 us, 59.8 with two thirds; at D = 128 two thirds
+  // are as fast with a head's rows together in a page, and 83-90 us against 99 with a token's).
   if (per_cu >= 2) {
-    if (!kv8)
+    if (!packed)
       units /= 2;
-    else if (per_cu >= 3)
+    else if (per_cu >= 3 && !all)
       units = units * 2 / 3;
   }
   if (p.CASC && units > kMaxCascadeWaves / p.HGW) units = kMaxCascadeWaves / p.HGW;  // prefix partial slots
@@ -2754,7 +2950,7 @@ template <class E, int D, int NT, int KV, int NX = 1, bool LINES = false>
 static int launch_decode_nt(PAParams& p, hipStream_t s) {
   int per_cu = 1;
   const int resident = resident_blocks((const void*)&pa_decode_kernel<E, D, NT, KV, NX, LINES>, 256, &per_cu);
-  const int wgs = decode_units(p, resident, per_cu, KV != kKv16);
+  const int wgs = decode_units(p, resident, per_cu, KV != kKv16, KV == kKv4 && D == 64);
   p.ND = p.NUP > 0 ? wgs : 0;  // NUP > 0: the workgroups behind the decode units plan the prefill launch
   hipLaunchKernelGGL((pa_decode_kernel<E, D, NT, KV, NX, LINES>), dim3(wgs + p.NUP), dim3(256), 0, s, p);
   return (int)hipGetLastError();
@@ -2798,7 +2994,7 @@ static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, Launc
   const int64_t dec_chunks = n_dec * (p.Hkv / p.HGW) * (((int64_t)p.W * p.BS + kChunk - 1) / kChunk);
   int err, per_cu = 1;
   const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV>, 256, &per_cu);
-  const int wgs = decode_units(p, resident, per_cu, KV != kKv16);
+  const int wgs = decode_units(p, resident, per_cu, KV != kKv16, KV == kKv4 && D == 64);
   if (NT > 1 || dec_chunks > kFusedUnitChunks * p.NU) {
     p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV>), cap) / 8 * 8);
     if ((err = launch_decode<E, D, KV>(p, NT, s))) return err;
