@@ -34,9 +34,10 @@ from typing import NamedTuple
 import torch
 import torch.nn.functional as F
 
-from kvserve_amd.attention import AttentionMetadata, HipAttention
+from kvserve_amd.attention import FP4, AttentionMetadata, HipAttention
 from kvserve_amd.engine import ops
 from kvserve_amd.engine.config import ModelConfig
+from kvserve_amd.logprobs import TokenLogprobs, token_logprobs
 
 # -- arithmetic ------------------------------------------------------------------------------
 
@@ -163,6 +164,10 @@ def load_hf_weights(path: Path, cfg: ModelConfig, device, dtype: torch.dtype) ->
 # -- the model -------------------------------------------------------------------------------
 
 
+# One layer of a KV pool: a tensor [2, blocks, BS, Hkv, D], or (keys, values, key scales, value scales) in MXFP4.
+KVLayer = torch.Tensor | tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+
+
 class StageOut(NamedTuple):
     """What a stage hands to the next attention step (or, after the last stage, the final
     hidden states in `resid`). Exactly one of `qkv` / `normed` is set before an attention step:
@@ -252,14 +257,19 @@ class PagedLlama:
         return StageOut(x, self._linear(h, self.w.layers[i].wqkv), None)
 
     # -- attention steps -----------------------------------------------------------------------
-    def attention(self, i: int, s: StageOut, positions: torch.Tensor, kv_layer: torch.Tensor, meta: AttentionMetadata,
+    def attention(self, i: int, s: StageOut, positions: torch.Tensor, kv_layer: KVLayer, meta: AttentionMetadata,
                   out: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:  # fmt: skip
-        """Layer i's attention over the pool slice kv_layer [2, blocks, BS, Hkv, D]: RoPE, this
+        """Layer i's attention over the pool slice kv_layer [2, blocks, BS, Hkv, D] (an MXFP4 pool's:
+        keys, values and the scales of each): RoPE, this
         step's K/V into the cache at meta.slot_mapping, then paged attention -> [T, H, D] (into
         `out` if given; `q_out` receives the rotated queries on the fused paths)."""
         lw = self.w.layers[i]
         k_cache, v_cache = kv_layer[0], kv_layer[1]
-        sc = {"k_scale": lw.k_scale, "v_scale": lw.v_scale} if k_cache.dtype == torch.float8_e4m3fn else {}
+        sc = {}
+        if k_cache.dtype == FP4:
+            sc = {"k_scale": kv_layer[2], "v_scale": kv_layer[3]}
+        elif k_cache.dtype == torch.float8_e4m3fn:
+            sc = {"k_scale": lw.k_scale, "v_scale": lw.v_scale}
         H = self.cfg.num_heads
         b = self.backend
         if s.normed is not None:
@@ -279,10 +289,11 @@ class PagedLlama:
 
     # -- whole passes ----------------------------------------------------------------------------
     @torch.inference_mode()
-    def hidden_states(self, input_ids: torch.Tensor, positions: torch.Tensor, kv_caches: torch.Tensor,
-                      meta: AttentionMetadata) -> torch.Tensor:  # fmt: skip
-        """Final hidden states [T, hidden] of one step; kv_caches [L, 2, blocks, BS, Hkv, D]."""
-        defer = self.defers_projection(input_ids.shape[0])
+    def hidden_states(self, input_ids: torch.Tensor, positions: torch.Tensor,
+                      kv_caches: torch.Tensor | list[KVLayer], meta: AttentionMetadata) -> torch.Tensor:  # fmt: skip
+        """Final hidden states [T, hidden] of one step; kv_caches [L, 2, blocks, BS, Hkv, D], or a
+        list of the layers' (the deferred projection writes no MXFP4 rows)."""
+        defer = self.defers_projection(input_ids.shape[0]) and kv_caches[0][0].dtype != FP4
         s = self.stage(0, input_ids, None, None, defer)
         for i in range(self.num_layers):
             a = self.attention(i, s, positions, kv_caches[i], meta)
@@ -295,6 +306,22 @@ class PagedLlama:
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         """fp32 logits [T, vocab]."""
         return self._linear(hidden, self.w.lm_head).float()
+
+    @torch.inference_mode()
+    def token_logprobs(self, hidden: torch.Tensor, tokens: torch.Tensor | None = None,
+                       top: int = 0) -> tuple[torch.Tensor, TokenLogprobs]:  # fmt: skip
+        """(tokens, their log probabilities after `hidden` [T, hidden] with `top` alternatives); tokens None: the
+        greedy ones. The logits stay in the weights' type: on the GPU one pass over them
+        (kvserve_amd.token_logprobs) widens them itself; on the CPU plain torch."""
+        logits = self._linear(hidden, self.w.lm_head)
+        if tokens is None:
+            tokens = logits.argmax(dim=-1)
+        if logits.is_cuda:
+            return tokens, token_logprobs(logits, tokens, top)
+        lp = logits.float().log_softmax(-1)
+        entropy = -torch.where(lp.exp() > 0, lp.exp() * lp, 0.0).sum(-1)
+        ids = lp.sort(dim=-1, descending=True, stable=True).indices[:, :top]
+        return tokens, TokenLogprobs(lp.gather(1, tokens[:, None])[:, 0], entropy, lp.gather(1, ids), ids)
 
 
 def build_model(cfg: ModelConfig, device, dtype: torch.dtype, max_positions: int, backend=HipAttention,

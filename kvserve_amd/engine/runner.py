@@ -27,8 +27,9 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from kvserve_amd.attention import AttentionMetadata, build_metadata
-from kvserve_amd.engine.model import PagedLlama, StageOut
+from kvserve_amd.attention import FP4, FP4_BLOCK, AttentionMetadata, build_metadata, fp4_caches
+from kvserve_amd.engine.model import KVLayer, PagedLlama, StageOut
+from kvserve_amd.logprobs import MAX_TOP, TokenLogprobs
 from kvserve_amd.metadata import DeviceMetadata, MetaBuffers
 
 
@@ -64,13 +65,17 @@ def _bucket(sizes: list[int], n: int) -> int | None:
 
 
 class KVPool:
-    """The paged KV cache of every layer, [L, 2, num_blocks + 1, BS, Hkv, D], and its free list.
+    """The paged KV cache of every layer, [L, 2, num_blocks + 1, BS, Hkv, D] (float4_e2m1fn_x2: a list of
+    the layers' `fp4_caches`), and its free list.
     Block `num_blocks` is scratch for graph padding rows and is never handed out."""
 
     def __init__(self, model: PagedLlama, num_blocks: int, block_size: int, dtype: torch.dtype):
         cfg = model.cfg
         shape = (cfg.num_layers, 2, num_blocks + 1, block_size, cfg.num_kv_heads, cfg.head_dim)
-        if dtype == torch.float8_e4m3fn:  # zero bytes viewed as E4M3 (+0)
+        self.tensor: torch.Tensor | list[KVLayer]
+        if dtype == FP4:
+            self.tensor = [fp4_caches(*shape[2:], model.device) for _ in range(cfg.num_layers)]
+        elif dtype == torch.float8_e4m3fn:  # zero bytes viewed as E4M3 (+0)
             self.tensor = torch.zeros(shape, dtype=torch.uint8, device=model.device).view(dtype)
         else:
             self.tensor = torch.zeros(shape, dtype=dtype, device=model.device)
@@ -83,7 +88,8 @@ class KVPool:
         """Blocks that fit `gib` GiB: K and V of every layer for `block_size` tokens each
         (the reference's sizing, model_runner.py:94-98)."""
         cfg = model.cfg
-        per_block = 2 * cfg.num_layers * block_size * cfg.num_kv_heads * cfg.head_dim * dtype.itemsize
+        row = cfg.head_dim // 2 + cfg.head_dim // FP4_BLOCK if dtype == FP4 else cfg.head_dim * dtype.itemsize
+        per_block = 2 * cfg.num_layers * block_size * cfg.num_kv_heads * row
         return max(1, int(gib * 2**30) // per_block)
 
     @property
@@ -108,6 +114,7 @@ class Sequence:
     table: list[int] = field(default_factory=list)  # physical block ids
     computed: int = 0  # tokens whose K/V are in the pool
     prompt_len: int = -1
+    logprobs: list[tuple[float, dict[int, float]]] = field(default_factory=list)  # of generated tokens, when asked for
 
     def __post_init__(self) -> None:
         if self.prompt_len < 0:
@@ -267,7 +274,8 @@ class PiecewiseGraphRunner:
                 self.graphs[(i, n)], _ = cap(lambda i=i, n=n: self._stage(i, n))
 
     @torch.inference_mode()
-    def run(self, n: int, positions: torch.Tensor, kv_caches: torch.Tensor, meta: AttentionMetadata) -> torch.Tensor:
+    def run(self, n: int, positions: torch.Tensor, kv_caches: torch.Tensor | list[KVLayer],
+            meta: AttentionMetadata) -> torch.Tensor:  # fmt: skip
         """Final hidden states [n, hidden] of a step whose token ids are in `self.ids[:n]`."""
         size = _bucket(self.sizes, n)
         L = self.model.num_layers
@@ -339,7 +347,7 @@ class ModelRunner:
                 self.decode_runner.capture(cap)
 
     @property
-    def kv_caches(self) -> torch.Tensor:
+    def kv_caches(self) -> torch.Tensor | list[KVLayer]:
         return self.pool.tensor
 
     def release(self, seq: Sequence) -> None:
@@ -357,13 +365,11 @@ class ModelRunner:
                 return "piecewise"
         return "eager"
 
-    @torch.inference_mode()
-    def execute(self, scheduled: list[tuple[Sequence, int]], eager: bool = False) -> dict[Sequence, int]:
-        """One forward over `scheduled`; every sequence whose whole context is computed after it
-        gets its greedy next token appended. Returns {sequence: token} for those."""
+    def _forward(self, scheduled: list[tuple[Sequence, int]], eager: bool) -> torch.Tensor:
+        """Final hidden states of one step over `scheduled`, its sequences' tokens in that order."""
         bs = self.block_size
         ids: list[int] = []
-        starts, qlens, last_rows, sampled = [], [], [], []
+        starts, qlens = [], []
         for seq, n in scheduled:
             start = seq.computed
             if n < 1 or start + n > len(seq.tokens):
@@ -376,9 +382,6 @@ class ModelRunner:
             ids += seq.tokens[start : start + n]
             starts.append(start)
             qlens.append(n)
-            if start + n == len(seq.tokens):
-                last_rows.append(len(ids) - 1)
-                sampled.append(seq)
         T = len(ids)
         path = self._route(qlens, T, eager)
         if self.dm is not None:
@@ -413,13 +416,72 @@ class ModelRunner:
         self.paths[path] += 1
         for seq, n in scheduled:
             seq.computed += n
+        return hidden
+
+    @torch.inference_mode()
+    def execute(self, scheduled: list[tuple[Sequence, int]], eager: bool = False,
+                logprobs: int | None = None) -> dict[Sequence, int]:  # fmt: skip
+        """One forward over `scheduled`; every sequence whose whole context is computed after it
+        gets its greedy next token appended. Returns {sequence: token} for those. With `logprobs`
+        (0 .. MAX_TOP) each such sequence's `logprobs` gets the token's log probability and
+        {id: log probability} of that many of the likeliest tokens."""
+        if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, self.model.cfg.vocab_size):
+            raise ValueError(f"logprobs must be 0 .. {min(MAX_TOP, self.model.cfg.vocab_size)} (got {logprobs})")
+        hidden = self._forward(scheduled, eager)
+        last_rows, sampled, row = [], [], -1
+        for seq, n in scheduled:
+            row += n
+            if seq.computed == len(seq.tokens):
+                last_rows.append(row)
+                sampled.append(seq)
         if not sampled:
             return {}
         rows = torch.tensor(last_rows, dtype=torch.long, device=self.device)
-        tokens = self.model.logits(hidden.index_select(0, rows)).argmax(dim=-1).tolist()
+        last = hidden.index_select(0, rows)
+        if logprobs is None:
+            tokens = self.model.logits(last).argmax(dim=-1).tolist()
+        else:
+            picked, lp = self.model.token_logprobs(last, None, logprobs)
+            tokens = picked.tolist()
+            for seq, own, ids, top in zip(sampled, lp.logprobs.tolist(), lp.top_ids.tolist(), lp.top_logprobs.tolist()):
+                seq.logprobs.append((own, dict(zip(ids, top))))
         for seq, tok in zip(sampled, tokens):
             seq.tokens.append(tok)
         return dict(zip(sampled, tokens))
+
+    @torch.inference_mode()
+    def score(self, prompts: list[list[int]], top: int = 0) -> list[TokenLogprobs]:
+        """Log probabilities of every prompt's tokens 1 .. after those before them (prompt log
+        probabilities, perplexity): TokenLogprobs of len(prompt) - 1 rows each. Steps of up to
+        `token_budget` tokens; the blocks go back to the pool as soon as a prompt is done."""
+        if not all(prompts):
+            raise ValueError("a prompt to score needs at least one token")
+        seqs = [Sequence(list(p)) for p in prompts]
+        parts: dict[Sequence, list[TokenLogprobs]] = {s: [] for s in seqs}
+        waiting = list(seqs)
+        try:
+            while waiting:
+                room, step = self.token_budget, []
+                for s in waiting:
+                    n = min(s.pending, room)
+                    if n > 0:
+                        step.append((s, n))
+                        room -= n
+                hidden = self._forward(step, eager=False)
+                # the token after each row; a prompt's last row has none and takes token 0, dropped below
+                after = [t for s, n in step for t in (s.tokens + [0])[s.computed - n + 1 : s.computed + 1]]
+                _, lp = self.model.token_logprobs(hidden, torch.tensor(after, device=self.device), top)
+                row = 0
+                for s, n in step:
+                    parts[s].append(TokenLogprobs(*(x[row : row + n] for x in lp)))
+                    row += n
+                for s in [s for s in waiting if s.pending == 0]:
+                    waiting.remove(s)
+                    self.release(s)
+        finally:
+            for s in waiting:
+                self.release(s)
+        return [TokenLogprobs(*(torch.cat(x)[:-1] for x in zip(*parts[s]))) for s in seqs]
 
     # convenience for benchmarks: whole batches in lockstep
     def prefill(self, seqs: list[Sequence]) -> None:
@@ -464,8 +526,8 @@ class Batcher:
     def busy(self) -> bool:
         return bool(self.admitted or self.queue)
 
-    def step(self, eager: bool = False) -> list[Sequence]:
-        """Run one step; returns the sequences it finished."""
+    def step(self, eager: bool = False, logprobs: int | None = None) -> list[Sequence]:
+        """Run one step (`logprobs`: see ModelRunner.execute); returns the sequences it finished."""
         room, plan = self.budget, []
         for seq in self.admitted:
             if room == 0:
@@ -481,7 +543,7 @@ class Batcher:
             room -= n
         if not plan:
             return []
-        self.runner.execute(plan, eager=eager)
+        self.runner.execute(plan, eager=eager, logprobs=logprobs)
         done = [s for s in self.admitted if s.finished]
         for s in done:
             self.admitted.remove(s)
