@@ -47,10 +47,12 @@ constexpr int kChunk = 32;  // tokens per wave iteration
 static_assert(kPlanChunk == kChunk, "the prefill plan counts the tiles' chunks");
 constexpr int kWavesPerWG = 4;
 // 16-row tiles per prefill wave: 3 over 16-bit caches (48 rows, 238 VGPRs at D = 128, 2 workgroups per
-// CU), 2 over the others (whose conversion registers leave no room for a third)
-template <int KV>
+// CU), 2 over E4M3 (whose conversion registers leave no room for a third). MXFP4 at D = 128 takes 3 with one
+// register set of chunks in flight (254 VGPRs): two chunks of 900-1024 tokens over 4000-10000 beside 24 decodes 272 us
+// with 2, 240 with 3; at D = 64 the third costs more than it saves (203 us, 210 with 3).
+template <int KV, int D>
 constexpr int prefill_nt() {
-  return KV == kKv16 ? 3 : 2;
+  return KV == kKv16 || (KV == kKv4 && D == 128) ? 3 : 2;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1780,8 +1782,8 @@ template <class E, int D, bool MIXED, bool BLK>
 static __global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
   constexpr int F = MIXED ? 4 : 1;
   constexpr int MR = merge_rows<D, F>();
-  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16>()) % MR == 0 &&
-                           (kWavesPerWG * 16 * prefill_nt<kKv8>()) % MR == 0),
+  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16, D>()) % MR == 0 &&
+                           (kWavesPerWG * 16 * prefill_nt<kKv8, D>()) % MR == 0),
                 "a prefill tile's rows split into whole merge chunks");
   const int CD = (p.HGW * p.RS + MR - 1) / MR;
   const int b = blockIdx.x;
@@ -2292,7 +2294,7 @@ template <class E, int D>
 __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                              int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                              int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<kKv16>();
+  constexpr int NT = prefill_nt<kKv16, D>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   c_lo = uni(c_lo);
@@ -2419,17 +2421,19 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
 // loads, as stored, the 8-element granules the DMA would have moved (8 bytes of E4M3; 4 of MXFP4
 // and their scale), converts them exactly to E's 16-bit type and writes them to the LDS
 // positions the DMA would have filled: the stage layout, the operand reads and the compute
-// are those of prefill_tile. Two register sets keep the loads two chunks ahead; chunk i is
+// are those of prefill_tile. Two register sets keep E4M3's loads two chunks ahead (MXFP4: one set, issued as soon as
+// the last chunk's bytes are converted, which a chunk's computation covers as well); chunk i is
 // converted and written right before the barrier that publishes it, so two LDS stages
 // suffice (stage i % 2 was last read by chunk i - 2, before the previous barrier).
 template <class E, int D, int KV>
 __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                                      int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                                      int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<KV>();
+  constexpr int NT = prefill_nt<KV, D>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   constexpr int KLW = L::kLoadsPerWave;
+  constexpr int kSets = KV == kKv4 ? 1 : 2;
   typedef __attribute__((address_space(3))) u32x4* lds_u32x4_ptr;
   c_lo = uni(c_lo);
   c_hi = uni(c_hi);
@@ -2466,7 +2470,7 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
   struct Raw {
     std::conditional_t<KV == kKv8, u32x2, uint32_t> g[KLW];
     uint32_t x[KLW];  // MXFP4: E8M0 bytes
-  } raw[2];
+  } raw[kSets];
   auto issue = [&](Raw& r, int ci) {
     const int rel = ci - win.c0;
     const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(win.off_hi, rel) << 32) |
@@ -2493,34 +2497,34 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
     }
   };
   issue(raw[0], c_lo);
-  if (n > 1) issue(raw[1], c_lo + 1);
+  if (kSets > 1 && n > 1) issue(raw[kSets - 1], c_lo + 1);
   const float c = pf_q_ready<E, D, NT>(s, p);
 
   PfPriority prio;  // wave priority as in prefill_tile
   prio.set(0, n, rest, total);
-  // step i: wait for chunk i's bytes, convert them into stage i % 2, publish, load chunk i + 2
+  // step i: wait for chunk i's bytes, convert them into stage i % 2, publish, load chunk i + kSets
   auto sync = [&](int i, auto set) {
     constexpr int S = decltype(set)::value;
     if (i >= prio.next_drop) prio.set(i, n, rest, total);
-    const int ci2 = c_lo + i + 2;
-    if (i + 2 < n && ci2 - win.c0 >= 64) {
+    const int ci2 = c_lo + i + kSets;
+    if (i + kSets < n && ci2 - win.c0 >= 64) {
       pf_window<KV>(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2, pl.xsb, pl.xss);
       // the unmasked run reaches as far as the new window allows (the old window's end
       // capped it; a missing page before this point has already ended the run)
       n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (i + 1 < n)
-      wait_vm<(KV == kKv4 ? 2 : 1) * KLW>();  // chunk i + 1 may stay in flight
+    if (kSets > 1 && i + 1 < n)
+      wait_vm<KLW>();  // chunk i + 1 may stay in flight
     else
       wait_vm<0>();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < KLW; ++k) {
-      const auto r = raw[S].g[k];
+      const auto r = raw[S % kSets].g[k];
       u32x4 o;
       if constexpr (KV == kKv4) {
-        const float f = fp4_scale(raw[S].x[k]);
+        const float f = fp4_scale(raw[S % kSets].x[k]);
         o = u32x4{E::template from_fp4x2<0>(r, f), E::template from_fp4x2<1>(r, f), E::template from_fp4x2<2>(r, f),
                   E::template from_fp4x2<3>(r, f)};
       } else {
@@ -2532,7 +2536,7 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
     }
     __syncthreads();  // the stage's writes are complete and visible; nothing else in flight
     __builtin_amdgcn_sched_barrier(0);
-    if (i + 2 < n) issue(raw[S], ci2);
+    if (i + kSets < n) issue(raw[S % kSets], ci2);
     __builtin_amdgcn_sched_barrier(0);
   };
   // chunk i from the stage at byte offset SOFF + stage (one masked instance with a runtime
@@ -2731,7 +2735,7 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
     if (p.ND > 0 && b >= p.ND) {
       __shared__ PreStart st;
       __shared__ int64_t wsum[kPlanThreads / 64];
-      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV>()>(p, b - p.ND, &st, wsum);
+      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV, D>()>(p, b - p.ND, &st, wsum);
       if (threadIdx.x == 0) {
         if (!work) st.u = -1;  // idle, rewritten on every call
         ((PreStart*)p.ws_plan)[b - p.ND] = st;
@@ -2837,7 +2841,7 @@ constexpr int prefill_lds_bytes() {
 template <class E, int D, int KV, bool PLANNED>
 __device__ __forceinline__ void prefill_unit(const PAParams& p, int block, char* lds) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  prefill_units<kWavesPerWG * 16 * prefill_nt<KV>(), PLANNED>(p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
+  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D>(), PLANNED>(p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
                                    int64_t slot, int rest, int total) {
     if constexpr (KV != kKv16)
       prefill_tile_convert<E, D, KV>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
@@ -2984,7 +2988,7 @@ constexpr int64_t kFusedUnitChunks = 4;
 // and 741). Apart as well when a decode row needs more than one 16-row tile (GQA groups above 16).
 template <class E, int D, int KV>
 static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
-  p.PR = kWavesPerWG * 16 * prefill_nt<KV>();
+  p.PR = kWavesPerWG * 16 * prefill_nt<KV, D>();
   // units x 2 partial slots x tile rows stay within the workspace's kMaxPrefillUnits x 2 x kPrefillRows
   const int cap = kMaxPrefillUnits * kPrefillRows / p.PR;
   // sequences that can be decode class: each of the others takes at most max_q of the T tokens
