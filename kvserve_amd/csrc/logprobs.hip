@@ -10,7 +10,7 @@
 // above kFar, delta would be no small number: there d_j = c (x_j - m).
 //
 // HBM-bound on the logits, with the vector units close behind (8 issue slots an element: widening, maximum, FMA,
-// exponential, two sums). A row is cut into S segments of whole 256-vector chunks, a workgroup each, so that few
+// exponential, two sums). A row is cut into S segments of 128 vectors or more, a workgroup each, so that few
 // rows fill the chip too; a second launch joins the segments (S = 1: none).
 //
 // The largest entries: the pass keeps the maxima of up to 16 x 64 cells, a cell being what four neighbouring threads read
@@ -37,7 +37,9 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kGroups = 64, kSpans = 16;  // quads of threads, parts of the pass
 constexpr int kCellsRead = 512;           // cells at or above thr, beyond which ties are taken in index order
-constexpr int kList = 1024, kJoinList = kMaxLogprobSplits * kMaxLogprobTop;
+// kList: a segment of fewer than 64 x 4 vectors leaves quads empty and may list all its entries
+constexpr int kList = 2048, kJoinList = kMaxLogprobSplits * kMaxLogprobTop;
+static_assert(kList >= kThreads * 8 && kJoinList <= kList, "rank_list holds an eighth of a list's 2048 in each thread");
 constexpr int kUnroll = 4;
 
 struct LogprobArgs {
@@ -138,9 +140,33 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return r;
 }
 
-// Ranks the n keys of `list` (distinct): emit(rank, key) for the first `top`.
+// Ranks the n keys of `list` (distinct, n <= kList; the list is used up): emit(rank, key) for the first `top`. Many are
+// thinned out first: the `top`-th largest of the threads' maxima is a lower bound, and few keys reach it.
 template <class F>
-__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int top, F&& emit) {
+__device__ __forceinline__ void rank_list(uint64_t* list, int n, int top, uint64_t* maxima, int* count, F&& emit) {
+  if (n > kThreads) {
+    uint64_t own[kList / kThreads], best = 0;
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) {
+      const int e = (int)threadIdx.x + i * kThreads;
+      own[i] = e < n ? list[e] : 0;
+      best = max64(best, own[i]);
+    }
+    maxima[threadIdx.x] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    int above = 0;
+    for (int i = 0; i < kThreads; ++i) above += maxima[i] > best;
+    __syncthreads();
+    if (above == top - 1) maxima[0] = best;
+    __syncthreads();
+    const uint64_t low = maxima[0];
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i)
+      if (own[i] >= low) list[atomicAdd(count, 1)] = own[i];
+    __syncthreads();
+    n = *count;
+  }
   for (int e = threadIdx.x; e < n; e += kThreads) {
     const uint64_t k = list[e];
     int r = 0;
@@ -154,7 +180,9 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
   using X = Vec<DT>;
   constexpr int N = X::N, EB = X::EB;
   __shared__ Sums s_sums[kWaves];
-  __shared__ float s_cell[kSpans][kGroups], s_group[kGroups], s_thr;
+  __shared__ alignas(8) float s_cell[kSpans][kGroups];  // (the keys' maxima of the threads once the entries are listed)
+  static_assert(sizeof(s_cell) >= kThreads * sizeof(uint64_t), "");
+  __shared__ float s_group[kGroups], s_thr;
   __shared__ uint64_t s_best[kWaves], s_list[kList];
   __shared__ uint16_t s_cand[kSpans * kGroups];
   __shared__ int s_n, s_nc, s_count[kWaves];
@@ -364,7 +392,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
   list_cells(true);
   int n = s_nc > kCellsRead ? kList + 1 : list_entries(true);
   if (n <= kList) {
-    rank_list(s_list, n, a.top, emit);
+    rank_list(s_list, n, a.top, (uint64_t*)s_cell, &s_nc, emit);
     if constexpr (!FINAL)
       for (int r = n + tid; r < a.top; r += kThreads) emit(r, 0);
     return;
@@ -375,7 +403,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
   list_cells(false);
   n = list_entries(false);
   if (n <= kList) {
-    rank_list(s_list, n, a.top, emit);
+    rank_list(s_list, n, a.top, (uint64_t*)s_cell, &s_nc, emit);
     // the rest: entries equal to thr (there are enough) in index order
     int found = n;
     auto take = [&](uint32_t hit, int first) INLINE {  // bit j: entry first + j is such a one
@@ -432,7 +460,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   __shared__ Sums s_sums;
   __shared__ uint64_t s_first[kMaxLogprobSplits], s_thr;
-  __shared__ uint64_t s_list[kJoinList];
+  __shared__ uint64_t s_list[kJoinList], s_maxima[kThreads];
   __shared__ int s_n;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
@@ -473,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   __syncthreads();
   const Sums v = s_sums;
   const float ln_s = logf(v.s);
-  rank_list(s_list, s_n, a.top, [&](int r, uint64_t k) {
+  rank_list(s_list, s_n, a.top, s_maxima, &s_n, [&](int r, uint64_t k) {
     a.top_logprobs[row * a.top + r] = key_value(k) - v.m - ln_s;
     a.top_ids[row * a.top + r] = key_index(k);
   });
@@ -483,7 +511,7 @@ int vec_elems(int32_t dtype) { return dtype == 0 ? 4 : 8; }
 
 }  // namespace
 
-// Segments of a row, whole chunks of 256 vectors each: up to kTarget workgroups in all, where a row to itself leaves the
+// Segments of a row, at least half of 256 vectors each: up to kTarget workgroups in all, where a row to itself leaves the
 // chip idle. A segment pays for its own alternatives and the joining launch, so no more (bf16, 128256 entries, 5
 // alternatives, us by segments: 512 rows 1: 28.8, 2: 34.1; 300 rows 27.1, 27.5; 128 rows 1: 20.1, 2: 18.4, 4: 17.8,
 // 8: 18.2; 64 rows 2: 17.7, 4: 15.1, 8: 14.5, 16: 15.0; 8 rows 8: 11.9, 32: 11.5, 63: 11.6).
@@ -510,8 +538,9 @@ int launch_token_logprobs(const void* logits, int64_t row_stride, const int64_t*
   a.V = V;
   a.top = top;
   a.S = logprob_splits(rows, V, dtype);
-  const int64_t chunks = (V / vec_elems(dtype) + kThreads - 1) / kThreads;
-  a.vps = (int32_t)((chunks + a.S - 1) / a.S) * kThreads;
+  // even shares of whole 128-byte lines
+  const int64_t nvec = V / vec_elems(dtype);
+  a.vps = (int32_t)((nvec + a.S - 1) / a.S + 7) / 8 * 8;
   a.part = (float4*)ws;
   a.keys = (uint64_t*)((char*)ws + rows * a.S * sizeof(float4));
   const dim3 block(kThreads);

@@ -62,6 +62,20 @@ def test_sizes(hip_device, T, V, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [300, 1030, 2007, 2065, 4200, 128256])
+def test_many_alternatives_of_short_segments(hip_device, V, dtype):
+    """64 alternatives where a segment has hardly as many groups of threads: hundreds to two thousand entries are listed
+    and thinned out. Rows at random, descending (ties in 16 bits), ascending and of one value; few and many rows."""
+    x, tok = _logits(4, V, dtype, hip_device, seed=V)
+    ramp = torch.arange(V, device=hip_device) * (20.0 / V)
+    x[1], x[2], x[3] = (-ramp).to(dtype), ramp.to(dtype), 0.5
+    _check(x, tok, 64)
+    few = token_logprobs(x[:3], tok[:3], 64)
+    many = token_logprobs(x.repeat(300, 1), tok.repeat(300), 64)
+    assert torch.equal(many.top_ids[:3], few.top_ids) and torch.equal(many.top_ids[1188:1191], few.top_ids)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("skip,stride", [(0, 4099), (1, 4099), (3, 5001), (5, 4112), (8, 4104)])
 def test_strides_and_alignments(hip_device, dtype, skip, stride):
     """Rows that begin at any element, more than a row apart: heads and tails of 0 .. 7 elements."""
