@@ -699,8 +699,7 @@ __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& 
 // scalar base and 32-bit lane offsets, chunks that every row sees whole take no masks, and a score costs one FMA and
 // one exponential. What bounds it now are the loads: with scores, softmax and values left out the walk still takes
 // 67-70 us, and 128 decodes of 8000-16000 keys (1.72 GB) 315 of 319 us, 5.4 TB/s. The window's offsets cost a short
-// walk 1.3 us (16 decodes 22.9 us, 21.6), and pages with a token's heads together, where a row of 64 bytes stands by
-// itself, are slower (89.6 us, 83.4): the documented layout keeps a head's rows together.
+// walk 1.3 us (16 decodes 22.9 us, 21.6).
 //
 // Byte offsets, from the cache's and the scales' first, of tiles tile0 .. tile0 + 63, one a lane; the values' are
 // apart only where their strides differ from the keys'. ok: the tiles that are there.
@@ -1380,10 +1379,12 @@ __device__ __forceinline__ void write_job_x(int32_t* job, int pieces, int64_t sl
 // Decode class: NU * HGW / 4 workgroups of 4 waves; wave w of workgroup `block` is head w % HGW
 // of unit (4 block + w) / HGW. KV: the caches' format. NX: 16-row tiles of a cascade prefix
 // group (XR = 16 NX rows; 1 outside the cascade).
-// LINES: whole-line K reads where the launch's mean unit asks for them (line_units).
+// LINES: whole-line K reads where the launch's mean unit asks for them (line_units); over MXFP4 caches non-temporal
+// loads (launch_decode_pages).
 template <class E, int D, int NT, int KV, int NX, bool LINES>
 __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool may_read_lines = true) {
-  static_assert(!LINES || (NT == 1 && NX == 1));
+  static_assert(!LINES || KV == kKv4 || (NT == 1 && NX == 1));
+  constexpr bool kLines = LINES && KV != kKv4;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gw = block * kWavesPerWG + wave;
@@ -1426,7 +1427,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
     scan_window(sw, p, blk0, Cs, Ns, L);
     Cs += sw.total;
     Ns += sw.ntotal;
-    if constexpr (LINES) wide |= __builtin_amdgcn_ballot_w64(sw.c > 0 && sw.ql * p.G > kLineRows);
+    if constexpr (kLines) wide |= __builtin_amdgcn_ballot_w64(sw.c > 0 && sw.ql * p.G > kLineRows);
   }
   const int64_t C = P + (int64_t)Cs * NHG;
   const int64_t NUa = active_units(C, p.NU);
@@ -1437,7 +1438,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
                         rounds ? kRound1Share : 1, rounds ? kRound2Share : 1);
   const int64_t a = split.begin(unit), b = split.begin(unit + 1);
   if (a >= b) return;
-  const bool lines = LINES && may_read_lines && wide == 0 && line_units(KV == kKv8, C, NUa);
+  const bool lines = kLines && may_read_lines && wide == 0 && line_units(KV == kKv8, C, NUa);
 
   int64_t pos = a;
   if constexpr (NT == 1) {
@@ -1497,7 +1498,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
     const int tok_hi = min(skip + (int)(y - seg_beg) * kChunk, sv.kv_total);
     WaveState<D, NT> st;
     const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
-    if constexpr (LINES) {
+    if constexpr (kLines) {
       if (lines) {
         load_q<D, NT, KV, true>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
         run_chunks<E, D, NT, KV, true, true>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
@@ -1505,7 +1506,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
     }
     if (!lines) {
       load_q<D, NT, KV>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-      run_chunks<E, D, NT, KV>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
+      run_chunks<E, D, NT, KV, KV != kKv4 || LINES>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
     }
     const bool whole = pos == seg_beg && y == seg_end && !member;
     const int64_t slot = (int64_t)seq * NHG + hg + unit;
@@ -2887,7 +2888,7 @@ static int resident_blocks(const void* kernel, int block_threads = 256, int* per
     const void* kernel;
     int blocks, per_cu;
   };
-  static thread_local Entry cache[64];  // every kernel of a dtype, head size and cache type, on several devices
+  static thread_local Entry cache[160];  // every kernel of a dtype, head size and cache type, on several devices
   static thread_local int cache_n = 0;
   for (int i = 0; i < cache_n; ++i)
     if (cache[i].dev == dev && cache[i].kernel == kernel) {
@@ -2899,7 +2900,7 @@ static int resident_blocks(const void* kernel, int block_threads = 256, int* per
   if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, block_threads, 0) != hipSuccess || per_cu <= 0)
     per_cu = 1;
   const int blocks = cus * per_cu;
-  if (cache_n < 64) cache[cache_n++] = Entry{dev, kernel, blocks, per_cu};
+  if (cache_n < 160) cache[cache_n++] = Entry{dev, kernel, blocks, per_cu};
   if (per_cu_out) *per_cu_out = per_cu;
   return blocks;
 }
@@ -2924,7 +2925,7 @@ static int decode_units(PAParams& p, int resident, int per_cu, bool packed, bool
   // (the 64-row cascade tiles, 48 or 64 verify rows) keeps them all: halving would idle half
   // the CUs. MXFP4 caches of 64-wide heads (`all`) keep three as well: their loads are so short that more of them in
   // flight outweigh the uneven ends (64 decodes of 1023-8191 keys 51.8 us, 59.8 with two thirds; at D = 128 two thirds
-  // are as fast with a head's rows together in a page, and 83-90 us against 99 with a token's).
+  // are as fast with a head's rows together in a page, and 90 us against 99 with a token's).
   if (per_cu >= 2) {
     if (!packed)
       units /= 2;
@@ -2960,6 +2961,17 @@ static int launch_decode_nt(PAParams& p, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+// Over MXFP4 caches non-temporal loads where a head's rows follow each other. Pages with a token's heads together share
+// each line among two or four heads' waves: ordinary loads keep it for the others (64 decodes of 1023-8191 keys 82.8 us
+// against 89.9, heads of 64 61.4 against 75.3; with a head's rows together 77.6 against 69.8). A kernel each: two loops
+// in one took 21 to 30 more registers and a wave per SIMD with them.
+template <class E, int D, int NT, int KV, int NX = 1>
+static int launch_decode_pages(PAParams& p, hipStream_t s) {
+  if constexpr (KV == kKv4)
+    if (p.k_ss == D / 2 && p.v_ss == D / 2) return launch_decode_nt<E, D, NT, KV, NX, true>(p, s);
+  return launch_decode_nt<E, D, NT, KV, NX>(p, s);
+}
+
 // The decode launch of a batch whose decode-class sequences take NT 16-row tiles (no cascade).
 template <class E, int D, int KV>
 static int launch_decode(PAParams& p, int NT, hipStream_t s) {
@@ -2968,10 +2980,10 @@ static int launch_decode(PAParams& p, int NT, hipStream_t s) {
       if constexpr (line_dim(D) && KV != kKv4)
         if (line_launch(D, p.NUP > 0 ? 0 : p.RS, p.k_ss * (KV == kKv8 ? 1 : 2)))
           return launch_decode_nt<E, D, 1, KV, 1, true>(p, s);
-      return launch_decode_nt<E, D, 1, KV>(p, s);
-    case 2: return launch_decode_nt<E, D, 2, KV>(p, s);
-    case 3: return launch_decode_nt<E, D, 3, KV>(p, s);
-    case 4: return launch_decode_nt<E, D, 4, KV>(p, s);
+      return launch_decode_pages<E, D, 1, KV>(p, s);
+    case 2: return launch_decode_pages<E, D, 2, KV>(p, s);
+    case 3: return launch_decode_pages<E, D, 3, KV>(p, s);
+    case 4: return launch_decode_pages<E, D, 4, KV>(p, s);
     default: return (int)hipErrorInvalidValue;
   }
 }
@@ -3040,7 +3052,7 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
     if ((err = launch_mixed<E, D, KV>(p, plan.NT, max_q, s, log))) return err;
   } else {
     constexpr int NX = KV == kKv16 ? 4 : 2;  // 64-row prefix groups (32 over E4M3 caches)
-    err = plan.cascade && p.XR == 16 * NX ? launch_decode_nt<E, D, 1, KV, NX>(p, s)
+    err = plan.cascade && p.XR == 16 * NX ? launch_decode_pages<E, D, 1, KV, NX>(p, s)
                                           : launch_decode<E, D, KV>(p, plan.NT, s);
     if (err) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
