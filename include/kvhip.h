@@ -118,7 +118,7 @@ KVH_API int kvh_reshape_and_cache_fp8(const void* k, int64_t k_tok_stride, int64
  * half a step), s at least 2; elements are x / 2^(s - 127) rounded to nearest even, at most 6. A block
  * with a NaN is stored under s = 255. head_dim a multiple of 32 up to 1024; k, v 16-byte aligned with
  * strides multiples of 16 bytes; caches 4-byte aligned with strides multiples of 4; a page's rows
- * within 2 GiB.
+ * within 2 GiB. A slot that several tokens name (graph padding) ends with a mixture of their rows.
  */
 KVH_API int kvh_reshape_and_cache_fp4(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
                               const void* v, int64_t v_tok_stride, int64_t v_head_stride,

@@ -853,32 +853,35 @@ __device__ __forceinline__ void kv4_mask(const WaveState<D, NT>& s, VRegs4<D>& v
     }
 }
 
-// Online-softmax update from (masked) raw scores, c > 0: pf_softmax with a shift that is always the row's maximum (in
-// thr as a raw score), so that the largest P is 1 and no rounding meets it: with the prefill's slack a softmax of few
-// large terms was off by 2.4e-3 instead of 1.7e-3 in bf16 (2-norm). A maximum moves some ten times in thousands of keys.
-template <class E, int D, int NT>
-__device__ __forceinline__ void kv4_softmax(WaveState<D, NT>& s, const f32x4 (&st)[NT][2], float c, u32x4 (&pt)[NT]) {
-  float mx[NT];
-  pf_lanemax<NT>(st, mx);
+// Online-softmax update from (masked) raw scores and per-lane maxima, c > 0. A row's shift is one of its scores (nsh; 0
+// while it has none), moved when a score passes thr. The difference is taken before the product: where scores pass
+// 2^24 one FMA would leave the rounding of the product, and P beyond fp16's range. Decode (SLACK = false) moves the shift
+// with every new maximum, some ten times in thousands of keys, so that the largest P is exactly 1: with pf_softmax's
+// slack a softmax of few large terms is off by 2.4e-3 instead of 1.7e-3 in bf16 (2-norm). The prefill's 16 rows a tile
+// move too often for that (240 -> 270 us) and keep the slack.
+template <class E, int D, int NT, bool SLACK>
+__device__ __forceinline__ void kv4_softmax(WaveState<D, NT>& s, const f32x4 (&st)[NT][2], const float (&mx)[NT], float c,
+                                            u32x4 (&pt)[NT]) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (__builtin_amdgcn_ballot_w64(mx[t] > s.thr[t])) {
-      const float top = fmaxf(s.thr[t], max_over_groups(mx[t]));
+      const bool first = s.thr[t] == -INFINITY;
+      const float top = fmaxf(first ? -INFINITY : s.nsh[t], max_over_groups(mx[t]));
       const bool empty = top == -INFINITY;  // the ballot is wave-wide
-      const float nsh = empty ? 0.f : -top * c;
-      const float alpha = s.thr[t] == -INFINITY ? 0.f : fast_exp2(nsh - s.nsh[t]);
+      const float ref = empty ? 0.f : top;
+      const float alpha = first ? 0.f : fast_exp2((s.nsh[t] - ref) * c);
       s.l[t] *= alpha;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) s.acc[t][i] *= alpha;
-      s.thr[t] = top;
-      s.nsh[t] = nsh;
-      s.m[t] = empty ? -INFINITY : -nsh;
+      s.thr[t] = SLACK ? top + kRescaleSlack / c : top;
+      s.nsh[t] = ref;
+      s.m[t] = top * c;
     }
     float pv[8];
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pv[4 * tile + e] = fast_exp2(__builtin_fmaf(st[t][tile][e], c, s.nsh[t]));
+      for (int e = 0; e < 4; ++e) pv[4 * tile + e] = fast_exp2((st[t][tile][e] - s.nsh[t]) * c);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       pt[t][w] = E::pack2(pv[2 * w], pv[2 * w + 1]);
@@ -2268,8 +2271,10 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
     if (MORE) kv4_load_k<D, NTL>(kr, lanes, n);
     __builtin_amdgcn_sched_barrier(0);
     if (tok0 + kChunk > seen || bits != 3) kv4_mask<D, NT>(s, vr, tok0, bits, data_end, st);
+    float mx[NT];
+    pf_lanemax<NT>(st, mx);
     u32x4 pt[NT];
-    kv4_softmax<E, D, NT>(s, st, c, pt);
+    kv4_softmax<E, D, NT, false>(s, st, mx, c, pt);
     kv4_pv<E, D, NT>(s, vr, pt);
     __builtin_amdgcn_sched_barrier(0);
     if (MORE) kv4_load_v<D, NTL>(vr, lanes, n);
@@ -2564,7 +2569,10 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
     pf_v_issue<D, SOFF + L::kKBytes, 0, kVLead>(vt, vb);
     __builtin_amdgcn_sched_barrier(0);
     u32x4 pt[NT];
-    pf_softmax<E, D, NT>(s, sc, mx, c, pt);
+    if constexpr (KV == kKv4)
+      kv4_softmax<E, D, NT, true>(s, sc, mx, c, pt);
+    else
+      pf_softmax<E, D, NT>(s, sc, mx, c, pt);
     pf_pv<E, D, NT, MASKED, SOFF + L::kKBytes>(s, vt, vb, cr, sv.kv_total, pt);
   };
   using I0 = std::integral_constant<int, 0>;

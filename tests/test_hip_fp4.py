@@ -142,6 +142,26 @@ def test_write_kv_many_tokens(hip_device, T):
     _check_rows(caches, before, slots.cpu(), fp4.quantize(k), fp4.quantize(v))
 
 
+def test_a_slot_named_twice(hip_device):
+    """Rows that share a slot (a graph's padding) touch that slot alone; where they are equal it holds them."""
+    dev = hip_device
+    g = torch.Generator(device=dev).manual_seed(3)
+    k, v = (torch.randn(40, 2, 64, generator=g, device=dev).bfloat16() for _ in range(2))
+    k[20:], v[20:] = k[19], v[19]
+    slots = torch.tensor([*range(32, 52), *[51] * 20], device=dev)
+    caches = _pool(5, 16, 2, 64, dev, "head", fill=0x5A)
+    before = [_bytes(c).cpu().clone() for c in caches]
+    HipAttention.write_kv(*caches[:2], k, v, slots, *caches[2:])
+    at = slots[:20].cpu()
+    _check_rows(caches, before, at, fp4.quantize(k[:20]), fp4.quantize(v[:20]))
+    k[30], v[30] = 1.0, -2.0  # not equal: that row is one of theirs or a mixture, the others stay
+    HipAttention.write_kv(*caches[:2], k, v, slots, *caches[2:])
+    for i, x in ((0, k), (1, v)):
+        code, s = fp4.quantize(x[:19])
+        assert torch.equal(_bytes(caches[i]).cpu().flatten(0, 1)[at[:19]], code)
+        assert torch.equal(_bytes(caches[i + 2]).cpu().flatten(0, 1)[at[:19]], s)
+
+
 def test_write_then_read_gives_what_the_format_keeps(hip_device):
     dev = hip_device
     g = torch.Generator(device=dev).manual_seed(8)
@@ -288,6 +308,59 @@ def test_verify_tiles(hip_device, head_dim, draft, dtype):
     assert _run(w, dtype, hip_device, seed=draft) == ["decode", "reduce"]
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("draft", [1, 2, 5, 12, 16])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_verify_tiles_of_token_pages(hip_device, head_dim, draft, dtype):
+    """The same where a page keeps a token's heads together (other loads), a single query among them."""
+    w = workloads.custom("verify", [draft] * 6, [40, 700, 1900, 3, 1200, 260], 32, 8, head_dim, 16, seed=draft)
+    assert _run(w, dtype, hip_device, "token", seed=draft) == ["decode", "reduce"]
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("scale", [-0.07, -0.0, 0.0])
+def test_scales_of_other_signs(hip_device, scale, head_dim):
+    """Decodes, drafts and prompt chunks under a negative scale (the smallest product weighs most) and none (a mean)."""
+    dev = hip_device
+    for q, c in (([1] * 5, [0, 5, 700, 1900, 31]), ([5] * 3, [1700, 2, 300]), ([200, 1, 60], [100, 900, 0]), ([1], [40])):
+        w = workloads.custom("scale", q, c, 16, 4, head_dim, 16, seed=3)
+        caches = _random_pool(w.num_blocks, 16, 4, head_dim, dev, "head", 8)
+        x = torch.randn(w.num_tokens, 16, head_dim, generator=torch.Generator(device=dev).manual_seed(4), device=dev).bfloat16()
+        meta = _meta(w, dev)
+        out = HipAttention.forward(x, *caches[:2], meta, scale, None, *caches[2:])
+        _within_bound(out, x, caches, meta, w.seq_lens, w.query_lens, scale)
+
+
+@pytest.mark.parametrize("scale", [4.0, 1e3, 3e5])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("q,c", [([1] * 4, [300, 900, 3000, 31]), ([5] * 3, [1700, 40, 300]), ([200, 60], [100, 900])])
+def test_large_scores(hip_device, q, c, dtype, scale):
+    """Scores to 10^10: where one key's leads by more than fp32 can blur (128 products: 2^-17 of the sum of their
+    magnitudes, here at most 128 * 6 * 200), that key's value comes out whole; no row is infinite or NaN."""
+    dev = hip_device
+    w = workloads.custom("large", q, c, 8, 2, 128, 16, seed=5)
+    caches = _random_pool(w.num_blocks, 16, 2, 128, dev, "head", 6)
+    x = torch.randn(w.num_tokens, 8, 128, generator=torch.Generator(device=dev).manual_seed(7), device=dev)
+    x = (50 * x).clamp(-200, 200).to(dtype)
+    meta = _meta(w, dev)
+    out = HipAttention.forward(x, *caches[:2], meta, scale, None, *caches[2:])
+    assert torch.isfinite(out).all()
+    k, v = (_values(caches[i], caches[i + 2]).flatten(0, 1) for i in range(2))
+    certain = t0 = 0
+    for table, n, total in zip(w.tables, w.query_lens, w.seq_lens):
+        at = torch.tensor(workloads.slots_for(table, 16, 0, total), device=dev)
+        for i in range(n):
+            see = at[: total - n + 1 + i]
+            for h in range(8):
+                best = (k[see, h // 4] @ x[t0 + i, h].double()).topk(2)
+                lead = (best.values[0] - best.values[1]).item() - 2 * 128 * 6 * 200 * 2.0**-17
+                if lead * scale > 200:
+                    certain += 1
+                    assert torch.equal(out[t0 + i, h].double(), v[see[best.indices[0]], h // 4])
+        t0 += n
+    assert certain > 0.8 * 8 * t0
+
+
 @pytest.mark.parametrize("heads", [(1, 1), (64, 1), (40, 10), (12, 12)], ids=str)
 def test_head_groups(hip_device, heads):
     w = workloads.custom("groups", [1, 3, 1, 20], [5000, 1200, 64, 300], *heads, 128, 16, seed=1)
@@ -330,6 +403,17 @@ def test_shared_prefix(hip_device):
         q, c, heads, D, BS, shared, width = SHARED[name]
         w = shared_workload(q, c, heads, D, BS, shared, width, seed=13)
         assert _run(w, torch.bfloat16, hip_device, seed=4)[0] == "share", name
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_shared_prefix_of_token_pages(hip_device, dtype):
+    from tests.test_hip_cascade import CASES as SHARED, shared_workload
+
+    for name in ("g4_b16", "d64_bs16_b9"):
+        q, c, heads, D, BS, shared, width = SHARED[name]
+        w = shared_workload(q, c, heads, D, BS, shared, width, seed=13)
+        assert _run(w, dtype, hip_device, "token", seed=4)[0] == "share", name
+        assert _run(w, dtype, hip_device, "head", seed=5)[0] == "share", name
 
 
 @pytest.mark.parametrize("idx", [2, 3, 5])
