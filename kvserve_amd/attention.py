@@ -130,8 +130,8 @@ def _kv_format(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float, v_s
 
 # MXFP4 KV caches (the *_fp4 entry points): float4_e2m1fn_x2 tensors, two elements to a byte, with a float8_e8m0fnu
 # tensor each that holds one power of two for every 32 elements of a row.
-FP4 = torch.float4_e2m1fn_x2
-E8M0 = torch.float8_e8m0fnu
+FP4 = getattr(torch, "float4_e2m1fn_x2", None)  # None: an older PyTorch, which has no such caches
+E8M0 = getattr(torch, "float8_e8m0fnu", None)
 FP4_BLOCK = 32
 
 
@@ -141,6 +141,7 @@ def fp4_caches(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: in
     kv_heads, D / 2] and float8_e8m0fnu tensors [.., D / 32]. A page holds each head's tokens together (the tensors
     are permuted views of [num_blocks, kv_heads, block_size, ..]), so that the attention reads whole lines: a token's
     row of one head is only 64 bytes at D = 128. Any other strides with a contiguous last dim are taken too."""
+    _require(FP4 is not None and E8M0 is not None, "this PyTorch has no float4_e2m1fn_x2")
     _require(head_dim > 0 and head_dim % FP4_BLOCK == 0, f"4-bit caches need head sizes in 32s, not {head_dim}")
 
     def pages(width: int, dtype: torch.dtype) -> torch.Tensor:

@@ -310,7 +310,7 @@ class ModelRunner:
         self.model = model
         self.device = model.device
         self.block_size, self.max_model_len = block_size, max_model_len
-        self.token_budget = token_budget
+        self.token_budget, self.max_seqs = token_budget, max_seqs
         kv_dtype = model.dtype if kv_cache_dtype is None else kv_cache_dtype
         if num_blocks is None:
             if kv_cache_gib is None:
@@ -461,12 +461,15 @@ class ModelRunner:
         waiting = list(seqs)
         try:
             while waiting:
-                room, step = self.token_budget, []
-                for s in waiting:
+                # oldest first, as many as the budget, the pool and the metadata hold: one prompt at most is left in parts
+                room, free, step = self.token_budget, self.pool.free_blocks, []
+                for s in waiting[: self.max_seqs]:
                     n = min(s.pending, room)
-                    if n > 0:
-                        step.append((s, n))
-                        room -= n
+                    free -= -(-(s.computed + n) // self.block_size) - len(s.table)
+                    if n == 0 or (free < 0 and step):
+                        break
+                    step.append((s, n))
+                    room -= n
                 hidden = self._forward(step, eager=False)
                 # the token after each row; a prompt's last row has none and takes token 0, dropped below
                 after = [t for s, n in step for t in (s.tokens + [0])[s.computed - n + 1 : s.computed + 1]]

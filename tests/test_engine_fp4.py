@@ -134,6 +134,28 @@ def test_generated_tokens_carry_their_log_probabilities():
             assert len(top) == 2 and top[tok] == own == max(top.values())
 
 
+@pytest.mark.parametrize("kw", [{"num_blocks": 3}, {"num_blocks": 40, "max_seqs": 4}, {"num_blocks": 40, "token_budget": 5}])
+def test_score_takes_what_the_pool_holds(kw):
+    """More prompts than blocks, sequences or tokens of a step: in turns, each as if alone."""
+    model = build_model(TINY, "cpu", torch.float32, 512, backend=TorchRefAttention, std=0.06)
+    prompts = [[(7 * i + j) % 300 for j in range(1 + 5 * i % 37)] for i in range(30)]
+    r = ModelRunner(model, block_size=16, max_model_len=512, **kw)
+    got = r.score(prompts)
+    assert r.pool.free_blocks == kw["num_blocks"]
+    big = ModelRunner(model, num_blocks=40, block_size=16, max_model_len=512)
+    for p, lp in zip(prompts, got):
+        torch.testing.assert_close(lp.logprobs, big.score([p])[0].logprobs, atol=1e-3, rtol=0)
+
+
+def test_score_of_a_prompt_past_the_pool():
+    model = build_model(TINY, "cpu", torch.float32, 512, backend=TorchRefAttention, std=0.06)
+    for budget in (2048, 7):
+        r = ModelRunner(model, num_blocks=3, block_size=16, max_model_len=512, token_budget=budget)
+        with pytest.raises(RuntimeError, match="exhausted"):
+            r.score([[3] * 20, [1] * 49, [2] * 5])
+        assert r.pool.free_blocks == 3
+
+
 def test_refusals_leave_the_pool_whole():
     r = _runner(TINY, "cpu", torch.float32, TorchRefAttention, kv_cache_dtype=None)
     with pytest.raises(ValueError, match="at least one token"):

@@ -5,6 +5,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -12,6 +15,8 @@ import torch
 from kvserve_amd import HipAttention, _lib, fp4_caches
 from kvserve_amd.attention import AttentionMetadata
 from oracle import fp4
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 # -- the oracle ------------------------------------------------------------------------------------
@@ -186,3 +191,12 @@ def test_methods_refuse_what_is_no_4bit_cache():
 def test_abi_takes_the_strides_as_they_are():
     a = _lib.i64x3(fp4_caches(4, 16, 2, 64, "cpu")[0].stride()[:3])
     assert isinstance(a, ctypes.Array) and list(a) == [1024, 32, 512]
+
+
+def test_a_pytorch_without_the_dtypes_still_imports():
+    code = ("import torch; del torch.float4_e2m1fn_x2, torch.float8_e8m0fnu\n"
+            "import kvserve_amd, kvserve_amd.engine\n"
+            "try: kvserve_amd.fp4_caches(1, 16, 1, 64, 'cpu')\n"
+            "except ValueError as e: print(e)")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and "no float4_e2m1fn_x2" in r.stdout, r.stderr
