@@ -367,6 +367,16 @@ def test_head_groups(hip_device, heads):
     _run(w, torch.bfloat16, hip_device, "token", seed=2)
 
 
+@pytest.mark.parametrize("layout", ["head", "token"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_wide_groups_beside_chunks(hip_device, dtype, head_dim, layout):
+    """GQA groups above 16: a decode row of several tiles in a mixed batch."""
+    for heads in ((64, 1), (40, 2)):
+        w = workloads.custom("wide", [1, 3, 1, 20], [5000, 1200, 64, 300], *heads, head_dim, 16, seed=1)
+        assert _run(w, dtype, hip_device, layout, seed=2) == ["decode", "prefill", "reduce"]
+
+
 @pytest.mark.parametrize("head_dim", [64, 128])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_short_tables(hip_device, head_dim, dtype):
