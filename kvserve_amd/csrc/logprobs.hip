@@ -118,13 +118,18 @@ __device__ __forceinline__ Sums wave_join(Sums v) {
   return v;
 }
 
-// The row's outputs but for the alternatives, from one thread.
+// The logit of the row's token, NaN for one outside the vocabulary: read ahead of the sums, two loads one after the other.
 template <int DT>
-__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const Sums& v, float ln_s) {
+__device__ __forceinline__ float token_logit(const LogprobArgs& a, int64_t row) {
   const int64_t tok = a.tokens[row];
   const bool in = tok >= 0 && tok < a.V;
   const float x = Vec<DT>::one(a.x + row * a.row_bytes + (in ? tok : 0) * Vec<DT>::EB);
-  a.logprobs[row] = in ? x - v.m - ln_s : __uint_as_float(0x7fc00000u);
+  return in ? x : __uint_as_float(0x7fc00000u);
+}
+
+// The row's outputs but for the alternatives, from one thread.
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, float x, const Sums& v, float ln_s) {
+  a.logprobs[row] = x - v.m - ln_s;
   a.entropy[row] = ln_s - kLn2 * (v.t / v.s);
 }
 
@@ -156,6 +161,7 @@ __device__ __forceinline__ void rank_list(uint64_t* list, int n, int top, uint64
     __syncthreads();
     if (threadIdx.x == 0) *count = 0;
     int above = 0;
+#pragma unroll 8
     for (int i = 0; i < kThreads; ++i) above += maxima[i] > best;
     __syncthreads();
     if (above == top - 1) maxima[0] = best;
@@ -170,6 +176,7 @@ __device__ __forceinline__ void rank_list(uint64_t* list, int n, int top, uint64
   for (int e = threadIdx.x; e < n; e += kThreads) {
     const uint64_t k = list[e];
     int r = 0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) r += list[i] > k;
     if (r < top) emit(r, k);
   }
@@ -279,6 +286,8 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
     if (--left == 0) end_span();
   };
   if (rounds > 0) load(even, 0);
+  float target = 0.f;
+  if constexpr (FINAL) target = token_logit<DT>(a, row);
   int round = 0;
   for (; round + 2 <= rounds; round += 2) {
     load(odd, round + 1);
@@ -287,7 +296,14 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
     sum(odd);
   }
   if (round < rounds) sum(even);
-  for (int i = v0 + rounds * (kThreads * kUnroll) + tid; i < v1; i += kThreads) vector(mid[i]);
+  if (const int i = v0 + rounds * (kThreads * kUnroll) + tid; v0 + rounds * (kThreads * kUnroll) < v1) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) odd[u] = mid[min(i + kThreads * u, v1 - 1)];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i + kThreads * u < v1) vector(odd[u]);
+  }
   if (has_tail) {
     const float v = X::one(x + (tail0 + tid) * EB);
     raise(v);
@@ -306,7 +322,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
   const float ln_s = logf(v.s);
   if (tid == 0) {
     if constexpr (FINAL)
-      write_row<DT>(a, row, v, ln_s);
+      write_row(a, row, target, v, ln_s);
     else
       a.part[row * a.S + seg] = float4{v.m, v.s, v.t, 0.f};
   }
@@ -318,6 +334,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
     if (lane == 0) s_thr = -INFINITY;
     __builtin_amdgcn_wave_barrier();
     int above = 0, reach = 0;
+#pragma unroll 16
     for (int k = 0; k < kGroups; ++k) {
       above += s_group[k] > g;
       reach += s_group[k] >= g;
@@ -469,6 +486,14 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     s_n = 0;
     s_thr = 1;
   }
+  const float target = token_logit<DT>(a, row);
+  // every load of the row's before the first is used
+  uint64_t own[kJoinList / kThreads];
+#pragma unroll
+  for (int i = 0; i < kJoinList / kThreads; ++i) {
+    const int k = tid + i * kThreads;
+    own[i] = k < a.S * a.top ? keys[k] : 0;
+  }
   // the segments' q-th largest keys: the (top / q)-th largest of them has `top` keys at or above it
   const int q = min(a.top, (2 * a.top + a.S - 1) / a.S);
   if (tid < 64) {
@@ -481,7 +506,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     v = wave_join(v);
     if (tid == 0) {
       s_sums = v;
-      write_row<DT>(a, row, v, logf(v.s));
+      write_row(a, row, target, v, logf(v.s));
     }
   }
   if (a.top == 0) return;
@@ -489,15 +514,15 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
   if (tid < kMaxLogprobSplits) {
     const uint64_t g = s_first[tid];
     int r = 0;
+#pragma unroll
     for (int k = 0; k < kMaxLogprobSplits; ++k) r += s_first[k] > g;
     if (r == (a.top + q - 1) / q - 1 && g != 0) s_thr = g;
   }
   __syncthreads();
   const uint64_t thr = s_thr;
-  for (int k = tid; k < a.S * a.top; k += kThreads) {
-    const uint64_t key = keys[k];
-    if (key >= thr) s_list[atomicAdd(&s_n, 1)] = key;
-  }
+#pragma unroll
+  for (int i = 0; i < kJoinList / kThreads; ++i)
+    if (own[i] >= thr) s_list[atomicAdd(&s_n, 1)] = own[i];
   __syncthreads();
   const Sums v = s_sums;
   const float ln_s = logf(v.s);

@@ -696,8 +696,7 @@ __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& 
 // MXFP4 caches. A chunk is a quarter of the 16-bit one's bytes, so run_chunks' own addresses and masks weigh four times
 // as much (254 of its 550 instructions a chunk were scalar: 64 decodes of 1023-8191 keys 75.6 us, here 70.2; 32
 // sequences of 6 queries 46.6, here 43.8). Here the page offsets of 64 tiles are computed one a lane, the loads take a
-// scalar base and 32-bit lane offsets, chunks that every row sees whole take no masks, and a score costs one FMA and
-// one exponential. What bounds it now are the loads: with scores, softmax and values left out the walk still takes
+// scalar base and 32-bit lane offsets, and chunks that every row sees whole take no masks. What bounds it now are the loads: with scores, softmax and values left out the walk still takes
 // 67-70 us, and 128 decodes of 8000-16000 keys (1.72 GB) 315 of 319 us, 5.4 TB/s. The window's offsets cost a short
 // walk 1.3 us (16 decodes 22.9 us, 21.6).
 //
