@@ -1,7 +1,7 @@
 """The MXFP4 KV-cache format from its definition, in 64 bits on the CPU. TEST INFRASTRUCTURE ONLY.
 
-The reference has no 4-bit cache, so the format is this build's: OCP microscaling with E2M1 elements (two to a byte,
-element 2i in the low nibble) and one E8M0 byte per 32 consecutive elements of a row. `quantize` works on float64
+The reference has no 4-bit cache; the format is OCP microscaling with E2M1 elements (two to a byte, element 2i in the
+low nibble) and one E8M0 byte per 32 consecutive elements of a row. `quantize` works on float64
 copies of the rows and compares every element with all eight magnitudes; `dequantize` decodes sign, exponent and
 mantissa bits. `attention` is softmax attention over values so decoded, sequence by sequence, with the sum of |p v| that
 rounding bounds are multiples of.
