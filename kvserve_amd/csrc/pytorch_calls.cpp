@@ -19,6 +19,7 @@
 
 #include <cmath>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -201,10 +202,15 @@ bool stream_of(const Caches& c, void** stream) {
   return !PyErr_Occurred();
 }
 
+// A new contiguous tensor on like's device: what at::empty comes to, without its dispatch.
+at::Tensor fresh(c10::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 // The output: the caller's tensor, checked, or a new contiguous one of q's dtype and device.
 bool output(PyObject* out, c10::IntArrayRef sizes, const at::Tensor& like, const Caches& c, at::Tensor* t) {
   if (out == Py_None) {
-    *t = at::empty(sizes, c10::TensorOptions().dtype(like.scalar_type()).device(like.device()));
+    *t = fresh(sizes, like.scalar_type(), like);
     return true;
   }
   const at::Tensor* o = gpu_tensor(out);
@@ -368,7 +374,7 @@ PyObject* forward_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (T == 0 || B == 0) return result(0, a[8], std::move(out));
     const size_t need = f_ws_size(T, B, H, c.kv_heads, c.head_dim, W, c.block_size, max_q, dtype);
     at::Tensor ws;
-    if (need) ws = at::empty({(int64_t)need}, c10::TensorOptions().dtype(c10::kByte).device(q->device()));
+    if (need) ws = fresh({(int64_t)need}, c10::kByte, *q);
     void* stream;
     if (!stream_of(c, &stream)) return nullptr;
     const int st = f_attention_fp4(
@@ -461,8 +467,7 @@ PyObject* read_kv_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (!slots || dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return nullptr;
     const auto type = dtype == KVH_DTYPE_F32 ? c10::kFloat : (dtype == KVH_DTYPE_F16 ? c10::kHalf : c10::kBFloat16);
     const int64_t T = slots->size(0), sizes[3] = {T, c.kv_heads, c.head_dim};
-    const auto options = c10::TensorOptions().dtype(type).device(c.k->device());
-    at::Tensor kv[2] = {at::empty(sizes, options), at::empty(sizes, options)};
+    at::Tensor kv[2] = {fresh(sizes, type, *c.k), fresh(sizes, type, *c.k)};
     void* stream;
     if (!stream_of(c, &stream)) return nullptr;
     const int st = f_read_fp4(FP4_ARGS(c), (const int64_t*)slots->data_ptr(), kv[0].data_ptr(), kv[0].stride(0),
@@ -484,12 +489,11 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int dtype = kvh_dtype(x->scalar_type());
     const int64_t T = x->size(0);
     if (dtype < 0 || T == 0) return nullptr;
-    const auto f32 = c10::TensorOptions().dtype(c10::kFloat).device(x->device());
-    at::Tensor t[4] = {at::empty({T}, f32), at::empty({T}, f32), at::empty({T, top}, f32),
-                       at::empty({T, top}, f32.dtype(c10::kLong))};
+    at::Tensor t[4] = {fresh({T}, c10::kFloat, *x), fresh({T}, c10::kFloat, *x), fresh({T, top}, c10::kFloat, *x),
+                       fresh({T, top}, c10::kLong, *x)};
     const size_t need = f_logprobs_ws(T, V, top, dtype);
     at::Tensor ws;
-    if (need) ws = at::empty({(int64_t)need}, f32.dtype(c10::kByte));
+    if (need) ws = fresh({(int64_t)need}, c10::kByte, *x);
     Caches where;
     where.k = x;
     void* stream;

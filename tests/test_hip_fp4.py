@@ -21,7 +21,7 @@ import random
 import pytest
 import torch
 
-from kvserve_amd import HipAttention, fp4_caches, last_launch_kernels, workloads
+from kvserve_amd import HipAttention, fp4_caches, last_launch_kernels, token_logprobs, workloads
 from kvserve_amd.attention import AttentionMetadata
 from oracle import fp4
 
@@ -555,6 +555,30 @@ def test_other_stream(hip_device):
         same = torch.equal(k, v)
     s.synchronize()
     assert same and torch.equal(k.cpu().double(), fp4.dequantize(*fp4.quantize((src * 2).cpu())))
+
+
+def test_new_tensors_are_plain_ones(hip_device):
+    """Outputs made by the calls: own storages, as any new tensor in and out of inference mode, empty ones too."""
+    dev = hip_device
+    caches = _random_pool(4, 16, 2, 64, dev, "head", 1)
+    meta = AttentionMetadata(torch.tensor([2], device=dev), torch.tensor([[1]], device=dev), torch.tensor([3], device=dev),
+                             torch.tensor([1], device=dev), torch.tensor([0, 1], device=dev), 3, 1)
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            q = torch.randn(1, 4, 64, device=dev).bfloat16()
+            slots = torch.arange(5, device=dev)
+            made = [*HipAttention.read_kv(*caches[:2], slots, torch.bfloat16, *caches[2:]),
+                    *HipAttention.read_kv(*caches[:2], slots[:0], torch.float32, *caches[2:]),
+                    HipAttention.forward(q, *caches[:2], meta, 0.1, None, *caches[2:]),
+                    *token_logprobs(torch.randn(3, 50, device=dev), slots[:3], 2)]
+        for t in made:
+            like = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=dev)
+            assert t.is_contiguous() and t.device == dev and t.is_inference() == inference and not t.requires_grad
+            assert t.storage_offset() == 0 and t.untyped_storage().nbytes() == like.untyped_storage().nbytes()
+        kept = made[0].clone()
+        del made[1:]
+        junk = [torch.full_like(kept, 9.0) for _ in range(8)]  # takes the freed blocks, not the one still held
+        assert torch.equal(made[0], kept) and len(junk) == 8
 
 
 def test_large_pool_offsets_pass_32_bits(hip_device):
