@@ -22,7 +22,9 @@
 // equal ones taken in index order; where more than kList are larger than thr (the largest entries all in few
 // cells), `top` rounds of a whole maximum take their place.
 //
-// NaN counts as -inf in the order and makes the row's s and t NaN; an infinite or all -inf row gives NaN as well.
+// NaN counts as -inf in the order and makes the row's s and t NaN; an infinite or all -inf row gives NaN as well. A
+// segment whose s is NaN takes its cells' maxima in a second pass, entry by entry: the first one's may lack what a signalling
+// NaN stood beside.
 #include <type_traits>
 
 #include "kvh_device.h"
@@ -133,7 +135,9 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, flo
   a.entropy[row] = ln_s - kLn2 * (v.t / v.s);
 }
 
-// max / min of three with no canonicalisation of the operands first (a NaN among them is dropped)
+// max / min of three with no canonicalisation of the operands first. A quiet NaN among them is dropped. A signalling one
+// comes out quieted where it meets another operand, and is dropped after that with what it met: logprob_kernel takes the
+// cells of a row with a NaN again.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -327,6 +331,25 @@ __global__ __launch_bounds__(kThreads, 6) void logprob_kernel(LogprobArgs a) {
       a.part[row * a.S + seg] = float4{v.m, v.s, v.t, 0.f};
   }
   if (a.top == 0) return;
+  if (v.s != v.s) {  // uniform: a NaN or a +inf. The cells again, entry by entry
+    span = 0, left = quads;
+    auto keep = [&](float e) INLINE { cell = e > cell ? e : cell; };  // no NaN is above
+    auto keep_vector = [&](int i) INLINE {
+      float f[N];
+      X::unpack(mid[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) keep(f[j]);
+    };
+    if (has_head) keep(X::one(x + tid * EB));
+    for (int i = v0 + tid, k = 0; k < rounds; ++k) {
+      for (int u = 0; u < kUnroll; ++u, i += kThreads) keep_vector(i);
+      if (--left == 0) end_span();
+    }
+    for (int i = v0 + rounds * (kThreads * kUnroll) + tid; i < v1; i += kThreads) keep_vector(i);
+    if (has_tail) keep(X::one(x + (tail0 + tid) * EB));
+    end_span();
+    __syncthreads();
+  }
   if (wave == 0) {
     float g = s_cell[0][lane];
     for (int k = 1; k < span; ++k) g = fmaxf(g, s_cell[k][lane]);

@@ -223,3 +223,26 @@ def test_step_by_step_path_gives_the_same_bits(hip_device, monkeypatch):
         m.setattr(_lib, "_calls", None)
         want = token_logprobs(x, tok, 5)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0x7F81), (torch.bfloat16, -0x7F), (torch.float16, 0x7C01),
+                                        (torch.float32, 0x7F800001), (torch.float32, -0x7FFFFF)], ids=str)  # fmt: skip
+@pytest.mark.parametrize("T,V,top", [(4, 5003, 9), (8, 128256, 20), (2100, 2061, 64)])
+def test_signalling_nans_hide_no_entry(hip_device, T, V, top, dtype, bits):
+    """NaN counts as -inf in the order, a signalling one too, wherever it stands beside larger entries: one in every
+    second place, one in each eight (the last of a vector), all but three places, and a single one beside the largest."""
+    x, tok = _logits(T, V, dtype, hip_device, seed=V)
+    raw = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    raw[0::4, 1::2] = bits
+    raw[1::4, 7::8] = bits
+    three = [3, V // 2, V - 2]
+    kept = raw[2::4, three]
+    raw[2::4] = bits
+    raw[2::4, three] = kept
+    single = raw[3::4]
+    best = x[3::4].float().argmax(1, keepdim=True)
+    single.scatter_(1, torch.where(best + 1 < V, best + 1, best - 1), bits)
+    r = token_logprobs(x, tok, top)
+    order = torch.sort(torch.where(x.isnan(), -math.inf, x.float()), dim=-1, descending=True, stable=True).indices
+    assert torch.equal(r.top_ids, order[:, :top])
+    assert r.logprobs.isnan().all() and r.entropy.isnan().all() and r.top_logprobs.isnan().all()
