@@ -132,8 +132,8 @@ def build_torch_calls(verbose: bool = False) -> Path:
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            f'-DKVH_TORCH_VERSION="{torch.__version__}"',
            f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", *[f"-isystem{d}" for d in include_paths()],
-           str(CSRC / "pytorch_calls.cpp"), *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_hip",
-           "-ltorch_cpu", "-lc10", "-ldl", "-o", str(tmp)]  # fmt: skip
+           str(CSRC / "pytorch_calls.cpp"), *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-ldl", "-o", str(tmp)]  # fmt: skip
     if verbose:
         print(" ".join(cmd))
     _run(cmd)

@@ -19,7 +19,6 @@
 
 #include <cmath>
 
-#include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -202,9 +201,10 @@ bool stream_of(const Caches& c, void** stream) {
   return !PyErr_Occurred();
 }
 
-// A new contiguous tensor on like's device: what at::empty comes to, without its dispatch.
+// A new contiguous tensor on like's device, by the operator: dispatch modes see it, and it is filled where
+// deterministic algorithms are asked for.
 at::Tensor fresh(c10::IntArrayRef sizes, c10::ScalarType type, const at::Tensor& like) {
-  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+  return at::empty(sizes, c10::TensorOptions().dtype(type).device(like.device()));
 }
 
 // The output: the caller's tensor, checked, or a new contiguous one of q's dtype and device.

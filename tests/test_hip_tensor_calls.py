@@ -6,8 +6,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
-from kvserve_amd import HipAttention, _lib, workloads
+from kvserve_amd import HipAttention, _lib, fp4_caches, token_logprobs, workloads
 from kvserve_amd.attention import FP8
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,55 @@ def test_status_errors_still_raise(batch):
     q = torch.cat([b.q.flatten(), b.q.flatten()])[1 : 1 + b.q.numel()].view(b.q.shape)  # 2 bytes off: KVH_E_ALIGN
     with pytest.raises(_lib.KvhError, match="kvh_paged_attention.*aligned"):
         HipAttention.forward(q, b.k_cache, b.v_cache, b.meta, 0.125)
+
+
+def _makers(b):
+    """Calls that make their outputs: attention, RoPE + write and read-back over 16-bit and MXFP4 caches, log probabilities."""
+    w, dev = b.workload, b.q.device
+    T, slots = b.q.shape[0], b.meta.slot_mapping
+    packed = fp4_caches(*b.k_cache.shape, dev)
+    qkv = torch.randn(T, 48 * 64, device=dev).to(b.q.dtype)
+    cos, sin = (torch.randn(600, 64, device=dev) for _ in range(2))
+    pos = torch.arange(T, device=dev)
+    kv = {"": (b.k_cache, b.v_cache, 1.0, 1.0), "_fp4": packed}
+    for name, (k, v, ks, vs) in kv.items():
+        yield "forward" + name, lambda k=k, v=v, ks=ks, vs=vs: HipAttention.forward(b.q, k, v, b.meta, w.scale, None, ks, vs)
+        yield "rope_and_cache" + name, lambda k=k, v=v, ks=ks, vs=vs: HipAttention.rope_and_cache(
+            qkv, pos, cos, sin, k, v, slots, 32, k_scale=ks, v_scale=vs)  # fmt: skip
+    k, v, ks, vs = packed
+    yield "read_kv", lambda: HipAttention.read_kv(k, v, slots, torch.bfloat16, ks, vs)
+    yield "token_logprobs", lambda: token_logprobs(qkv, pos, 3)
+
+
+def test_allocations_are_seen_by_a_dispatch_mode(batch):
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            got = func(*args, **(kwargs or {}))
+            if func is torch.ops.aten.empty.memory_format:
+                self.made.append(got.data_ptr())
+            return got
+
+    for name, call in _makers(batch):
+        with Seen() as seen:
+            seen.made = []
+            out = call()
+        for t in [out] if isinstance(out, torch.Tensor) else out:
+            assert t.data_ptr() in seen.made, name
+
+
+def test_new_outputs_are_filled_under_deterministic_algorithms(batch):
+    """As torch.empty's: rows behind the last sequence, which no call writes, are NaN then and not what memory held."""
+    b, dev = batch, batch.q.device
+    T = b.q.shape[0]
+    wide = torch.cat([b.q, torch.ones_like(b.q[:9])])
+    packed = fp4_caches(*b.k_cache.shape, dev)
+    for caches in ((b.k_cache, b.v_cache, 1.0, 1.0), packed):
+        k, v, ks, vs = caches
+        want = HipAttention.forward(wide, k, v, b.meta, 0.125, None, ks, vs)[:T].clone()
+        torch.full_like(wide, 7.0)  # freed: what the next allocation of this size finds
+        torch.use_deterministic_algorithms(True)
+        try:
+            out = HipAttention.forward(wide, k, v, b.meta, 0.125, None, ks, vs)
+        finally:
+            torch.use_deterministic_algorithms(False)
+        assert torch.equal(out[:T], want) and out[T:].isnan().all()
