@@ -37,7 +37,7 @@ import torch.nn.functional as F
 from kvserve_amd.attention import FP4, AttentionMetadata, HipAttention
 from kvserve_amd.engine import ops
 from kvserve_amd.engine.config import ModelConfig
-from kvserve_amd.logprobs import TokenLogprobs, token_logprobs
+from kvserve_amd.logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 
 # -- arithmetic ------------------------------------------------------------------------------
 
@@ -159,6 +159,21 @@ def load_hf_weights(path: Path, cfg: ModelConfig, device, dtype: torch.dtype) ->
     w.final_norm = get("norm.weight")
     w.lm_head = w.embed if cfg.tie_word_embeddings else get("lm_head.weight")
     return w
+
+
+def _torch_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
+    """kvserve_amd.token_logprobs in plain torch, its special rows and refusals included."""
+    vocab = logits.shape[1]
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 .. {min(MAX_TOP, vocab)} (got {top})")
+    x = logits.float()
+    lp = x.log_softmax(-1)
+    entropy = -(lp.exp() * lp).masked_fill(lp == -math.inf, 0.0).sum(-1)
+    own = lp.gather(1, tokens.clamp(0, vocab - 1)[:, None])[:, 0]
+    own = own.masked_fill((tokens < 0) | (tokens >= vocab), math.nan)
+    # by the logits themselves, NaN as -inf: rounded log probabilities have ties that logits have not
+    ids = x.masked_fill(x.isnan(), -math.inf).sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    return TokenLogprobs(own, entropy, lp.gather(1, ids), ids)
 
 
 # -- the model -------------------------------------------------------------------------------
@@ -318,10 +333,7 @@ class PagedLlama:
             tokens = logits.argmax(dim=-1)
         if logits.is_cuda:
             return tokens, token_logprobs(logits, tokens, top)
-        lp = logits.float().log_softmax(-1)
-        entropy = -torch.where(lp.exp() > 0, lp.exp() * lp, 0.0).sum(-1)
-        ids = lp.sort(dim=-1, descending=True, stable=True).indices[:, :top]
-        return tokens, TokenLogprobs(lp.gather(1, tokens[:, None])[:, 0], entropy, lp.gather(1, ids), ids)
+        return tokens, _torch_token_logprobs(logits, tokens, top)
 
 
 def build_model(cfg: ModelConfig, device, dtype: torch.dtype, max_positions: int, backend=HipAttention,

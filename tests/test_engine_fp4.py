@@ -263,3 +263,46 @@ def test_score_is_the_pass_over_the_heads_logits(hip_device):
     want = token_logprobs(logits, torch.tensor(p[1:] + [0], device=hip_device), 5)
     for a, b in zip(got, want):
         assert torch.equal(a, b[:-1])
+
+
+# -- the model's pass over the head's logits without a GPU ------------------------------------------
+
+
+def _cpu_token_logprobs(logits, tokens, top):
+    """PagedLlama.token_logprobs where the head gives these logits."""
+    model = build_model(TINY, "cpu", torch.float32, 512, backend=TorchRefAttention)
+    model._linear = lambda x, w: logits
+    return model.token_logprobs(torch.zeros(len(logits), TINY.hidden_size), tokens, top)[1]
+
+
+def test_cpu_log_probabilities_of_special_rows():
+    """As kvserve_amd.token_logprobs has them: NaN for a row with a NaN or a +inf or of -inf alone, and for a token
+    outside the vocabulary; a logit of -inf adds nothing to the entropy; NaN counts as -inf in the order."""
+    inf, nan = math.inf, math.nan
+    x = torch.tensor([[0.0, nan, 2.0, 1.0], [0.0, inf, 2.0, 1.0], [-inf] * 4, [-inf, 0.0, -inf, 0.0], [0.0] * 4, [0.0] * 4])
+    lp = _cpu_token_logprobs(x, torch.tensor([0, 1, 2, 0, 4, -1]), 4)
+    for row in range(3):
+        assert lp.logprobs[row].isnan() and lp.entropy[row].isnan() and lp.top_logprobs[row].isnan().all()
+    assert lp.top_ids[:4].tolist() == [[2, 3, 0, 1], [1, 2, 3, 0], [0, 1, 2, 3], [1, 3, 0, 2]]
+    # log 2 and log 4 in fp32: two roundings of exponentials and a logarithm
+    assert lp.logprobs[3] == -inf and abs(lp.entropy[3].item() - math.log(2)) <= 2.0**-22
+    assert lp.top_logprobs[3, 2:].tolist() == [-inf, -inf]
+    assert lp.logprobs[4:].isnan().all() and (lp.entropy[4:] - math.log(4)).abs().max() <= 2.0**-21
+
+
+def test_cpu_alternatives_are_ordered_by_their_logits():
+    """Log probabilities of neighbouring logits round to one value beside a far larger one; the order is the logits'."""
+    x = torch.zeros(2, 40)
+    x[:, 7] = 100.0
+    x[0, 20], x[0, 30] = 1.0, 1.0 + 2.0**-23
+    lp = _cpu_token_logprobs(x, torch.tensor([7, 7]), 5)
+    assert lp.top_logprobs[0, 1] == lp.top_logprobs[0, 2]
+    assert lp.top_ids.tolist() == [[7, 30, 20, 0, 1], [7, 0, 1, 2, 3]]
+
+
+@pytest.mark.parametrize("top", [-1, 65, 301])
+def test_cpu_refuses_other_numbers_of_alternatives(top):
+    r = _runner(TINY, "cpu", torch.float32, TorchRefAttention, kv_cache_dtype=None)
+    with pytest.raises(ValueError, match="top must be 0 .. 64"):
+        r.score([[1, 2, 3]], top=top)
+    assert r.pool.free_blocks == 96
