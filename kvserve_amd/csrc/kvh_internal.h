@@ -185,7 +185,7 @@ int launch_gemv_silu_mul(const void* x, int64_t x_rs, const void* w, int64_t w_r
                          int32_t inter, int32_t k, int32_t dtype, hipStream_t s);
 
 // Log probabilities (logprobs.hip): segments of a row and alternatives at most.
-constexpr int kMaxLogprobSplits = 32, kMaxLogprobTop = 64;
+constexpr int kMaxLogprobSplits = 32, kMaxLogprobTop = KVH_LOGPROBS_MAX_TOP;
 int32_t logprob_splits(int64_t rows, int32_t V, int32_t dtype);
 int launch_token_logprobs(const void* logits, int64_t row_stride, const int64_t* tokens, float* logprobs,
                           float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int32_t V, int32_t top,

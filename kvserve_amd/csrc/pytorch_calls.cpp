@@ -484,8 +484,9 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     int32_t top, V;
     if (!x || !tok || !integer(a[2], &top) || !current_device(*x) || tok->get_device() != x->get_device()) return nullptr;
     if (x->dim() != 2 || x->stride(1) != 1 || tok->dim() != 1 || tok->stride(0) != 1 || tok->size(0) != x->size(0) ||
-        tok->scalar_type() != c10::kLong || !same_int32(x->size(1), &V) || top < 0)
-      return nullptr;
+        tok->scalar_type() != c10::kLong || !same_int32(x->size(1), &V) || top < 0 ||
+        top > KVH_LOGPROBS_MAX_TOP || top > V)
+      return nullptr;  // nothing allocated for a mistaken top
     const int dtype = kvh_dtype(x->scalar_type());
     const int64_t T = x->size(0);
     if (dtype < 0 || T == 0) return nullptr;

@@ -246,3 +246,13 @@ def test_signalling_nans_hide_no_entry(hip_device, T, V, top, dtype, bits):
     order = torch.sort(torch.where(x.isnan(), -math.inf, x.float()), dim=-1, descending=True, stable=True).indices
     assert torch.equal(r.top_ids, order[:, :top])
     assert r.logprobs.isnan().all() and r.entropy.isnan().all() and r.top_logprobs.isnan().all()
+
+
+@pytest.mark.parametrize("top", [65, 101, 10**6])
+def test_a_refused_number_of_alternatives_allocates_nothing(hip_device, top):
+    x, tok = _logits(4, 100, torch.float32, hip_device)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="top"):
+        token_logprobs(x, tok, top)
+    assert torch.cuda.max_memory_allocated() == before

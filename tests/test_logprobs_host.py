@@ -3,10 +3,13 @@ workspace's size."""
 
 from __future__ import annotations
 
+from pathlib import Path
+
 import pytest
 import torch
 
 from kvserve_amd import _lib, token_logprobs
+from kvserve_amd.logprobs import MAX_TOP
 
 P = 0x10000
 NULL, SHAPE, DTYPE, ALIGN, UNSUP, WS = -1, -2, -3, -4, -5, -6
@@ -49,3 +52,9 @@ def test_method_refusals():
         token_logprobs(x.t(), torch.zeros(3, dtype=torch.long))
     with pytest.raises(ValueError, match="contiguous last dim"):
         token_logprobs(x[0], torch.zeros(3, dtype=torch.long))
+
+
+def test_the_method_and_the_header_agree_on_the_alternatives():
+    header = (Path(__file__).resolve().parents[1] / "include" / "kvhip.h").read_text()
+    assert f"#define KVH_LOGPROBS_MAX_TOP {MAX_TOP}\n" in header
+    assert _call(V=1000, top=MAX_TOP + 1) == UNSUP
