@@ -461,9 +461,11 @@ class ModelRunner:
         waiting = list(seqs)
         try:
             while waiting:
-                # oldest first, as many as the budget, the pool and the metadata hold: one prompt at most is left in parts
+                # oldest first, as many as the budget, the pool and the metadata hold beside the sequences that live there
+                # already: one prompt at most is left in parts, and has its row
                 room, free, step = self.token_budget, self.pool.free_blocks, []
-                for s in waiting[: self.max_seqs]:
+                rows = self.max_seqs if self.dm is None else self.dm.free_rows + (waiting[0].computed > 0)
+                for s in waiting[: max(rows, 1)]:
                     n = min(s.pending, room)
                     free -= -(-(s.computed + n) // self.block_size) - len(s.table)
                     if n == 0 or (free < 0 and step):

@@ -94,6 +94,11 @@ class DeviceMetadata:
         if ent is not None:
             self._free.append(ent[0])
 
+    @property
+    def free_rows(self) -> int:
+        """Sequences that can still be added."""
+        return len(self._free)
+
     def _entry(self, key: Hashable, table: list[int]) -> list:
         ent = self._rows.get(key)
         if ent is None:

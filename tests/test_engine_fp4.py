@@ -265,6 +265,26 @@ def test_score_is_the_pass_over_the_heads_logits(hip_device):
         assert torch.equal(a, b[:-1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("live", [1, 3])
+def test_score_beside_live_sequences(hip_device, live):
+    """Sequences being generated keep their rows of the resident tables: prompts to score take turns on the others."""
+    r = _runner(SMALL, hip_device, torch.bfloat16, HipAttention, decode_graphs=False, piecewise_graphs=False, max_seqs=4)
+    seqs = [Sequence(list(p)) for p in PROMPTS[:live]]
+    r.execute([(s, s.pending) for s in seqs])
+    free = r.pool.free_blocks
+    prompts = [PROMPTS[i % len(PROMPTS)][i:] + [7, 8] for i in range(10)]
+    got = r.score(prompts, top=2)
+    assert r.pool.free_blocks == free
+    alone = _runner(SMALL, hip_device, torch.bfloat16, HipAttention, decode_graphs=False, piecewise_graphs=False)
+    for p, lp in zip(prompts, got):
+        # logits of two batches, bounded as the graphs are: 3% of their scale, twice (the token's and the normaliser)
+        top = _all_logits(alone, p).abs().max().item()
+        assert (lp.logprobs - alone.score([p])[0].logprobs).abs().max().item() <= 0.06 * top
+    r.execute([(s, s.pending) for s in seqs])
+    assert all(len(s.generated) == 2 for s in seqs)
+
+
 # -- the model's pass over the head's logits without a GPU ------------------------------------------
 
 
