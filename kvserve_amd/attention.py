@@ -417,6 +417,16 @@ class HipAttention:
         _lib.check(st, "kvh_read_cache_fp4")
         return k, v
 
+    @staticmethod
+    def check_fp4_model(num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, dtype: torch.dtype) -> None:
+        """Raises ValueError for a model whose steps `forward` refuses over float4_e2m1fn_x2 caches
+        (kvh_paged_attention_fp4)."""
+        _require(dtype in (torch.bfloat16, torch.float16), f"float4_e2m1fn_x2 caches need a bf16 or fp16 model, not {dtype}")
+        _require(head_dim in MFMA_HEAD_DIMS, f"float4_e2m1fn_x2 caches need head sizes {MFMA_HEAD_DIMS}, not {head_dim}")
+        _require(block_size >= 16 and block_size % 16 == 0, f"float4_e2m1fn_x2 caches need blocks in 16s, not {block_size}")
+        _require(num_heads % num_kv_heads == 0 and num_heads // num_kv_heads <= 64,
+                 f"float4_e2m1fn_x2 caches need 1 to 64 query heads per kv head, not {num_heads} over {num_kv_heads}")  # fmt: skip
+
     # Extension beyond the reference's interface: RoPE + QKV split + write_kv in one kernel.
     fused_rope_cache = True
 

@@ -74,6 +74,8 @@ class KVPool:
         shape = (cfg.num_layers, 2, num_blocks + 1, block_size, cfg.num_kv_heads, cfg.head_dim)
         self.tensor: torch.Tensor | list[KVLayer]
         if dtype == FP4:
+            if (check := getattr(model.backend, "check_fp4_model", None)) is not None:  # here, not at the first step
+                check(cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, block_size, model.dtype)
             self.tensor = [fp4_caches(*shape[2:], model.device) for _ in range(cfg.num_layers)]
         elif dtype == torch.float8_e4m3fn:  # zero bytes viewed as E4M3 (+0)
             self.tensor = torch.zeros(shape, dtype=torch.uint8, device=model.device).view(dtype)

@@ -168,6 +168,30 @@ def test_refusals_leave_the_pool_whole():
     assert r.pool.free_blocks == 96
 
 
+@pytest.mark.parametrize("over,dtype,block,match", [
+    ({}, torch.float32, 16, "bf16 or fp16"), ({"head_dim": 96}, torch.bfloat16, 16, "head sizes"),
+    ({"head_dim": 32}, torch.float16, 16, "head sizes"), ({}, torch.bfloat16, 24, "blocks in 16s"),
+    ({"num_heads": 65, "num_kv_heads": 1}, torch.bfloat16, 16, "query heads"),
+])  # fmt: skip
+def test_pools_that_the_backend_cannot_attend_over_are_refused(over, dtype, block, match):
+    """At construction, not at the first step; the same model's 16-bit pool is as before."""
+    cfg = ModelConfig(**{"vocab_size": 64, "hidden_size": 64, "intermediate_size": 32, "num_layers": 1, "num_heads": 4,
+                         "num_kv_heads": 2, "head_dim": 64, "tie_word_embeddings": True, **over})  # fmt: skip
+    model = build_model(cfg, "cpu", dtype, 64, backend=HipAttention)
+    with pytest.raises(ValueError, match=match):
+        ModelRunner(model, num_blocks=4, block_size=block, max_model_len=64, kv_cache_dtype=FP4)
+    ModelRunner(model, num_blocks=4, block_size=block, max_model_len=64)
+
+
+@pytest.mark.parametrize("group,head_dim,dtype", [(1, 64, torch.float16), (8, 128, torch.bfloat16), (64, 64, torch.bfloat16)])
+def test_pools_that_the_backend_takes(group, head_dim, dtype):
+    cfg = ModelConfig(vocab_size=64, hidden_size=64, intermediate_size=32, num_layers=1, num_heads=group, num_kv_heads=1,
+                      head_dim=head_dim, tie_word_embeddings=True)  # fmt: skip
+    model = build_model(cfg, "cpu", dtype, 64, backend=HipAttention)
+    r = ModelRunner(model, num_blocks=4, block_size=32, max_model_len=64, kv_cache_dtype=FP4)
+    assert r.kv_caches[0][0].shape == (5, 32, 1, head_dim // 2)
+
+
 # -- on the GPU --------------------------------------------------------------------------------
 
 
