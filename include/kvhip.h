@@ -415,8 +415,8 @@ KVH_API int kvh_gemv_silu_mul(const void* x, int64_t x_row_stride, const void* w
  * and the `top` largest logits in descending order, equal ones by ascending id, as top_ids [num_rows,
  * top] with their log probabilities in top_logprobs [num_rows, top] (both may be NULL when top = 0).
  * Statistics in fp32; one pass over the logits. A row with a NaN or a +inf, or of -inf alone, gives NaN
- * (its ids are still distinct and in range). top at most KVH_LOGPROBS_MAX_TOP and at most vocab; rows may have any stride
- * and alignment of whole elements. workspace: kvh_token_logprobs_workspace_size bytes, 16-byte aligned,
+ * (its ids are still distinct and in range). num_rows below 2^24; top at most KVH_LOGPROBS_MAX_TOP and at
+ * most vocab; rows may have any stride and alignment of whole elements. workspace: kvh_token_logprobs_workspace_size bytes, 16-byte aligned,
  * which may be 0; it needs no clearing, and calls that overlap on one device need one each.
  * Serves the engine's sampling and prompt scoring; kvserve samples without log probabilities.
  */

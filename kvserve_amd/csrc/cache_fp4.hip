@@ -115,7 +115,7 @@ __device__ __forceinline__ void store_granule(const Fp4Cache& k, const SlotAt& a
   if ((g & 3) == 0) k.x[at.x + (int64_t)h * k.xsh + g / 4] = (uint8_t)e8m0;
 }
 
-constexpr int kMaxTokens = 4;  // of a workgroup
+constexpr int kMaxTokens = kFp4TokensPerWg;
 
 // Thread r of a workgroup takes granules r, r + 256, ... of each of its nt tokens' K|V rows (K heads, then V heads):
 // the tokens' loads are issued together, the conversions and stores follow.

@@ -227,11 +227,12 @@ static int fp4_caches(int32_t head_dim, int32_t block_size, void* k_cache, const
   return KVH_OK;
 }
 
-static int check_fp4_rows(int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim,
-                          int32_t block_size, int32_t dtype) {
+// per_wg: tokens of a workgroup where there are many.
+static int check_fp4_rows(int per_wg, int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t block_size, int32_t dtype) {
   if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
   if (num_tokens < 0 || num_blocks < 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0) return KVH_E_SHAPE;
-  if (num_tokens > 0x7fffffffLL || num_blocks > INT64_MAX / block_size) return KVH_E_SHAPE;
+  if (num_tokens > per_wg * kMaxWorkgroups256 || num_blocks > INT64_MAX / block_size) return KVH_E_SHAPE;
   if (head_dim % kFp4Block != 0 || head_dim > 1024 || num_kv_heads > 65535) return KVH_E_UNSUPPORTED;
   return KVH_OK;
 }
@@ -253,7 +254,7 @@ int kvh_reshape_and_cache_fp4(const void* k, int64_t k_tok_stride, int64_t k_hea
                               const int64_t v_scale_strides[3], const int64_t* slot_mapping, int64_t num_tokens,
                               int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                               int32_t dtype, void* stream) {
-  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  int st = check_fp4_rows(kFp4TokensPerWg, num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
   if (st != KVH_OK || num_tokens == 0) return st;
   if ((st = check_fp4_tensor(k, k_tok_stride, k_head_stride, dtype)) != KVH_OK) return st;
   if ((st = check_fp4_tensor(v, v_tok_stride, v_head_stride, dtype)) != KVH_OK) return st;
@@ -274,7 +275,7 @@ int kvh_rope_and_cache_fp4(const void* qkv, int64_t qkv_tok_stride, const int64_
                            void* v_scale, const int64_t v_scale_strides[3], const int64_t* slot_mapping,
                            int64_t num_tokens, int64_t num_blocks, int32_t num_heads, int32_t num_kv_heads,
                            int32_t head_dim, int32_t block_size, int32_t dtype, void* stream) {
-  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  int st = check_fp4_rows(1, num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
   if (st != KVH_OK) return st;
   if (num_heads <= 0 || max_positions <= 0) return KVH_E_SHAPE;
   if (head_dim % (2 * kFp4Block) != 0 || num_heads > 65535) return KVH_E_UNSUPPORTED;  // half a row is whole blocks
@@ -299,7 +300,7 @@ int kvh_read_cache_fp4(const void* k_cache, const int64_t k_cache_strides[3], co
                        int64_t k_tok_stride, int64_t k_head_stride, void* v, int64_t v_tok_stride,
                        int64_t v_head_stride, int64_t num_tokens, int64_t num_blocks, int32_t num_kv_heads,
                        int32_t head_dim, int32_t block_size, int32_t dtype, void* stream) {
-  int st = check_fp4_rows(num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
+  int st = check_fp4_rows(kFp4TokensPerWg, num_tokens, num_blocks, num_kv_heads, head_dim, block_size, dtype);
   if (st != KVH_OK || num_tokens == 0) return st;
   if ((st = check_fp4_tensor(k, k_tok_stride, k_head_stride, dtype)) != KVH_OK) return st;
   if ((st = check_fp4_tensor(v, v_tok_stride, v_head_stride, dtype)) != KVH_OK) return st;
@@ -834,8 +835,8 @@ int kvh_gemm_skinny_silu_mul(const void* x, int64_t x_row_stride, const void* w_
 static int check_logprobs(int64_t rows, int32_t vocab, int32_t top, int32_t dtype) {
   if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
   if (rows < 0 || vocab <= 0 || top < 0 || top > vocab) return KVH_E_SHAPE;
-  // workgroups of a launch, and a row's bytes, within 32 bits
-  if (top > kMaxLogprobTop || rows > 0x7fffffffLL / kMaxLogprobSplits || vocab > 0x1fffffff) return KVH_E_UNSUPPORTED;
+  // a workgroup a row (several only where rows are few); a row's bytes within 32 bits
+  if (top > kMaxLogprobTop || rows > kMaxWorkgroups256 || vocab > 0x1fffffff) return KVH_E_UNSUPPORTED;
   return KVH_OK;
 }
 

@@ -184,6 +184,9 @@ int launch_gemm_skinny(const void* x, int64_t x_rs, const void* w, int64_t w_rs,
 int launch_gemv_silu_mul(const void* x, int64_t x_rs, const void* w, int64_t w_rs, void* y, int64_t y_rs, int32_t m,
                          int32_t inter, int32_t k, int32_t dtype, hipStream_t s);
 
+// Workgroups of 256 threads of a launch: its threads are counted in 32 bits.
+constexpr int64_t kMaxWorkgroups256 = 0xffffffffLL / 256;
+
 // Log probabilities (logprobs.hip): segments of a row and alternatives at most.
 constexpr int kMaxLogprobSplits = 32, kMaxLogprobTop = KVH_LOGPROBS_MAX_TOP;
 int32_t logprob_splits(int64_t rows, int32_t V, int32_t dtype);
@@ -202,6 +205,7 @@ int launch_gemv_rope_and_cache(const void* x, int64_t x_rs, const void* w, int64
                                const int64_t* vcs, const int64_t* slots, int64_t num_blocks, int32_t H, int32_t Hkv,
                                int32_t D, int32_t BS, int32_t dtype, bool kv8, float k_scale, float v_scale,
                                hipStream_t s);
+constexpr int kFp4TokensPerWg = 4;  // of a write or read, where tokens are many
 // MXFP4 caches (cache_fp4.hip). kcs / vcs and kxs / vxs: {block, slot, head} byte strides of the packed rows and of
 // their E8M0 bytes.
 struct Fp4Cache {

@@ -167,6 +167,13 @@ def test_attention_refusals(over, want):
     assert _attend(**dict(over)) == want
 
 
+def test_more_tokens_than_a_launch_has_threads_for():
+    """A launch holds fewer than 2^32 threads: a workgroup of 256 takes 4 tokens of a write or read, 1 of a rotation."""
+    most = (2**32 - 1) // 256
+    assert _write(T=4 * most + 1) == SHAPE and _read(T=4 * most + 1) == SHAPE and _rope(T=most + 1) == SHAPE
+    assert _write(T=4 * most, k=None) == NULL and _rope(T=most, pos=None) == NULL
+
+
 # -- refusals of the methods (CPU tensors never reach a kernel) -------------------------------------
 def test_methods_refuse_what_is_no_4bit_cache():
     k, v, ks, vs = fp4_caches(4, 16, 2, 64, "cpu")

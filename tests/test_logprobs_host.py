@@ -34,6 +34,12 @@ def test_refusals(over, want):
     assert _call(**over) == want
 
 
+def test_more_rows_than_a_launch_has_threads_for():
+    """A launch holds fewer than 2^32 threads, a workgroup of 256 for each row."""
+    most = (2**32 - 1) // 256
+    assert _call(rows=most + 1) == UNSUP and _call(rows=most, x=None) == NULL
+
+
 def test_workspace_size():
     f = _lib.load().kvh_token_logprobs_workspace_size
     assert f(4, 1000, 5, 2) == 0 and f(300, 128256, 5, 2) == 0  # one segment a row
