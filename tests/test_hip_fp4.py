@@ -673,3 +673,33 @@ def test_step_by_step_path_gives_the_same_bits(hip_device, monkeypatch):
         m.setattr(_lib, "_calls", None)
         want = everything()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("layout", ["head", "token"])
+@pytest.mark.parametrize("scale", [4.0, 1e3, 3e5])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("q,c", [([1] * 4, [300, 900, 3000, 31]), ([5] * 3, [1700, 40, 300]), ([200, 60], [100, 900])])
+def test_large_scores_of_heads_of_64(hip_device, q, c, dtype, scale, layout):
+    """As test_large_scores: 64 products blur by 2^-18 of at most 64 * 6 * 200. The scores' standard deviation is about
+    600, a leader's mean distance some 600 / sqrt(2 ln n) = 180, and e^(-50 / 180) = 3 of 4 lead by the 50 of scale 4."""
+    dev = hip_device
+    w = workloads.custom("large", q, c, 8, 2, 64, 16, seed=5)
+    caches = _random_pool(w.num_blocks, 16, 2, 64, dev, layout, 6)
+    x = torch.randn(w.num_tokens, 8, 64, generator=torch.Generator(device=dev).manual_seed(7), device=dev)
+    x = (50 * x).clamp(-200, 200).to(dtype)
+    out = HipAttention.forward(x, *caches[:2], _meta(w, dev), scale, None, *caches[2:])
+    assert torch.isfinite(out).all()
+    k, v = (_values(caches[i], caches[i + 2]).flatten(0, 1) for i in range(2))
+    certain = t0 = 0
+    for table, n, total in zip(w.tables, w.query_lens, w.seq_lens):
+        at = torch.tensor(workloads.slots_for(table, 16, 0, total), device=dev)
+        for i in range(n):
+            see = at[: total - n + 1 + i]
+            for h in range(8):
+                best = (k[see, h // 4] @ x[t0 + i, h].double()).topk(2)
+                lead = (best.values[0] - best.values[1]).item() - 2 * 64 * 6 * 200 * 2.0**-18
+                if lead * scale > 200:
+                    certain += 1
+                    assert torch.equal(out[t0 + i, h].double(), v[see[best.indices[0]], h // 4])
+        t0 += n
+    assert certain > 0.5 * 8 * t0

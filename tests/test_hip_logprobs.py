@@ -158,7 +158,7 @@ def test_largest_in_few_threads(hip_device, dtype, per, top):
     r = token_logprobs(x, tok, top)
     assert (r.top_ids == r.top_ids[0]).all() and (r.top_logprobs == r.top_logprobs[0]).all()
     _check(x[-2:], tok[-2:], top, type(r)(*(f[-2:] for f in r)))
-    _check(x[:1], tok[:1], top)  # in 63 segments
+    _check(x[:1], tok[:1], top)  # in 32 segments, none of which lists as many
 
 
 def test_tokens_outside_the_vocabulary(hip_device):
@@ -256,3 +256,18 @@ def test_a_refused_number_of_alternatives_allocates_nothing(hip_device, top):
     with pytest.raises(ValueError, match="top"):
         token_logprobs(x, tok, top)
     assert torch.cuda.max_memory_allocated() == before
+
+
+@pytest.mark.parametrize("top", [9, 64])
+def test_largest_in_few_threads_of_two_segments(hip_device, top):
+    """As above in segments of a row: the 4096 largest entries of each lie in the strides of sixteen threads, past
+    the list of candidates, and the rounds' keys go through the join. 200 rows of 128256 make two segments of 8016 vectors."""
+    V, T, per = 128256, 200, 8
+    at = torch.arange(V, device=hip_device)
+    within = at % (8016 * per)
+    own = within % (256 * per) < 16 * per
+    row = torch.where(own, 1.0 + at / 1024, at % 7 / 8).to(torch.bfloat16)[None]
+    x, tok = row.expand(T, -1), at[-T:]
+    r = token_logprobs(x, tok, top)
+    assert (r.top_ids == r.top_ids[0]).all() and (r.top_logprobs == r.top_logprobs[0]).all()
+    _check(x[-2:], tok[-2:], top, type(r)(*(f[-2:] for f in r)))
