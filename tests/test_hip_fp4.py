@@ -703,3 +703,65 @@ def test_large_scores_of_heads_of_64(hip_device, q, c, dtype, scale, layout):
                     assert torch.equal(out[t0 + i, h].double(), v[see[best.indices[0]], h // 4])
         t0 += n
     assert certain > 0.5 * 8 * t0
+
+
+@pytest.mark.parametrize("rows,scales", [(("head", "token"), ("head", "token")), (("token", "head"), ("token", "head")),
+                                         (("apart", "head"), ("head", "apart")), (("head", "head"), ("token", "token")),
+                                         (("apart", "apart"), ("apart", "apart"))], ids=str)  # fmt: skip
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_keys_values_and_scales_in_pages_of_their_own(hip_device, head_dim, rows, scales):
+    """Each of the four tensors has strides of its own: decodes over long and short tables, drafts, prompt chunks, a batch
+    of both and a shared prefix."""
+    dev = hip_device
+    batches = [workloads.custom("own", q, c, 16, 4, head_dim, 16, seed=3) for q, c in (
+        ([1] * 6, [0, 5, 700, 1900, 31, 5000]), ([1, 1], [40, 63]), ([5] * 3, [1700, 2, 300]), ([200, 60], [100, 900]),
+        ([1, 1, 90], [700, 3000, 400]))]  # fmt: skip
+    for w in batches:
+        made = {name: _random_pool(w.num_blocks, 16, 4, head_dim, dev, name, 8) for name in {*rows, *scales}}
+        caches = [made[rows[0]][0], made[rows[1]][1], made[scales[0]][2], made[scales[1]][3]]
+        x = torch.randn(w.num_tokens, 16, head_dim, generator=torch.Generator(device=dev).manual_seed(4), device=dev).bfloat16()
+        meta = _meta(w, dev)
+        out = HipAttention.forward(x, *caches[:2], meta, w.scale, None, *caches[2:])
+        _within_bound(out, x, caches, meta, w.seq_lens, w.query_lens, w.scale)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_value_scales_over_their_range(hip_device, head_dim, n):
+    """Sequences of n tokens whose key is the same for each and whose value too: the output is that value, for every scale
+    under which n of them add up in fp32 (40 * 6 * 2^120 do), the subnormal ones of bf16 too."""
+    dev, hkv, BS = hip_device, 2, 64
+    at = list(range(248))  # E8M0 bytes
+    caches = _random_pool(len(at), BS, hkv, head_dim, dev, "head", seed=1)
+    for c in (*caches[:2], caches[2]):  # every token's rows as the first's
+        _bytes(c).copy_(_bytes(c)[:, :1].expand(-1, BS, -1, -1).clone())
+    _bytes(caches[3]).copy_(torch.tensor(at, dtype=torch.uint8, device=dev).view(-1, 1, 1, 1).expand(caches[3].shape))
+    B = len(at)
+    meta = AttentionMetadata(torch.empty(0, dtype=torch.long, device=dev), torch.arange(B, device=dev).view(B, 1),
+                             torch.full((B,), n, device=dev), torch.full((B,), n, device=dev),
+                             torch.arange(B + 1, device=dev) * n, n, n)  # fmt: skip
+    q = torch.randn(B * n, hkv, head_dim, device=dev).bfloat16()
+    out = HipAttention.forward(q, *caches[:2], meta, head_dim**-0.5, k_scale=caches[2], v_scale=caches[3])
+    want = _values(caches[1], caches[3])[:, 0].repeat_interleave(n, 0)
+    # equal scores give P = 1 and exact sums; their quotient is off by two roundings to fp32, and bf16 holds the value
+    # itself (2^-128 at least; its subnormals lie 2^-133 apart)
+    assert torch.equal(out.double(), want)
+
+
+@pytest.mark.parametrize("layout", ["head", "token"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("lens", [[96], [1500, 40], [7000] * 40])
+def test_chunks_of_nan_keys_make_their_rows_nan(hip_device, head_dim, layout, lens):
+    """Whole runs of NaN keys, as a diverged prompt leaves them: a piece of a split that sees nothing else included."""
+    dev = hip_device
+    w = workloads.custom("nan", [1] * len(lens), [n - 1 for n in lens], 8, 2, head_dim, 16, seed=4)
+    caches = _random_pool(w.num_blocks, 16, 2, head_dim, dev, layout, seed=4)
+    meta = _meta(w, dev)
+    q = torch.randn(w.num_tokens, 8, head_dim, device=dev).to(torch.bfloat16)
+    clean = HipAttention.forward(q, *caches[:2], meta, w.scale, None, *caches[2:])
+    run = torch.tensor(w.tables[0][: lens[0] // 16 // 2], device=dev)
+    _bytes(caches[2])[run, :, 1] = 255
+    out = HipAttention.forward(q, *caches[:2], meta, w.scale, None, *caches[2:])
+    assert out[0, 4:].isnan().all()
+    out[0, 4:] = clean[0, 4:]
+    assert torch.equal(out, clean)
