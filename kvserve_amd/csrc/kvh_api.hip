@@ -198,9 +198,9 @@ int kvh_reshape_and_cache_fp8(const void* k, int64_t k_tok_stride, int64_t k_hea
 
 // The caches of the *_fp4 entry points: packed rows of head_dim / 2 bytes in 4-byte granules (`wide`: the
 // attention's loads of an eighth of head_dim bytes), E8M0 rows of head_dim / 32 bytes.
-static int fp4_caches(int32_t head_dim, int32_t block_size, void* k_cache, const int64_t k_cache_strides[3], void* k_scale, const int64_t k_scale_strides[3], void* v_cache,
-                      const int64_t v_cache_strides[3], void* v_scale, const int64_t v_scale_strides[3], bool wide,
-                      Fp4Cache* kc, Fp4Cache* vc) {
+static int fp4_caches(int32_t head_dim, int32_t block_size, void* k_cache, const int64_t k_cache_strides[3],
+                      void* k_scale, const int64_t k_scale_strides[3], void* v_cache, const int64_t v_cache_strides[3],
+                      void* v_scale, const int64_t v_scale_strides[3], bool wide, Fp4Cache* kc, Fp4Cache* vc) {
   if (!k_cache || !k_cache_strides || !k_scale || !k_scale_strides || !v_cache || !v_cache_strides || !v_scale ||
       !v_scale_strides)
     return KVH_E_NULL;

@@ -10,8 +10,8 @@
 // above kFar, delta would be no small number: there d_j = c (x_j - m).
 //
 // HBM-bound on the logits, with the vector units close behind (8 issue slots an element: widening, maximum, FMA,
-// exponential, two sums). A row is cut into S segments of 128 vectors or more, a workgroup each, so that few
-// rows fill the chip too; a second launch joins the segments (S = 1: none).
+// exponential, two sums). A row is cut into S segments of 128 vectors or more (the last has what is left, down to
+// none), a workgroup each, so that few rows fill the chip too; a second launch joins the segments (S = 1: none).
 //
 // The largest entries: the pass keeps the maxima of up to 16 x 64 cells, a cell being what four neighbouring threads read
 // in a sixteenth of it (one more maximum a vector). The `top`-th largest of the 64 maxima over a quad of threads each
@@ -559,10 +559,10 @@ int vec_elems(int32_t dtype) { return dtype == 0 ? 4 : 8; }
 
 }  // namespace
 
-// Segments of a row, at least half of 256 vectors each: up to kTarget workgroups in all, where a row to itself leaves the
+// Segments of a row, one for every 256 vectors at most: up to kTarget workgroups in all, where a row to itself leaves the
 // chip idle. A segment pays for its own alternatives and the joining launch, so no more (bf16, 128256 entries, 5
 // alternatives, us by segments: 512 rows 1: 28.8, 2: 34.1; 300 rows 27.1, 27.5; 128 rows 1: 20.1, 2: 18.4, 4: 17.8,
-// 8: 18.2; 64 rows 2: 17.7, 4: 15.1, 8: 14.5, 16: 15.0; 8 rows 8: 11.9, 32: 11.5, 63: 11.6).
+// 8: 18.2; 64 rows 2: 17.7, 4: 15.1, 8: 14.5, 16: 15.0; 8 rows 8: 11.9, 32: 11.5).
 int32_t logprob_splits(int64_t rows, int32_t V, int32_t dtype) {
   constexpr int64_t kTarget = 512;
   const int64_t chunks = (V / vec_elems(dtype) + kThreads - 1) / kThreads;
@@ -586,7 +586,7 @@ int launch_token_logprobs(const void* logits, int64_t row_stride, const int64_t*
   a.V = V;
   a.top = top;
   a.S = logprob_splits(rows, V, dtype);
-  // even shares of whole 128-byte lines
+  // shares in 8 vectors, whole 128-byte lines of rows that begin on one; the last segment takes the rest
   const int64_t nvec = V / vec_elems(dtype);
   a.vps = (int32_t)((nvec + a.S - 1) / a.S + 7) / 8 * 8;
   a.part = (float4*)ws;

@@ -49,7 +49,8 @@ constexpr int kWavesPerWG = 4;
 // 16-row tiles per prefill wave: 3 over 16-bit caches (48 rows, 238 VGPRs at D = 128, 2 workgroups per
 // CU), 2 over E4M3 (whose conversion registers leave no room for a third). MXFP4 at D = 128 takes 3 with one
 // register set of chunks in flight (254 VGPRs): two chunks of 900-1024 tokens over 4000-10000 beside 24 decodes 272 us
-// with 2, 240 with 3; at D = 64 the third costs more than it saves (203 us, 210 with 3).
+// with 2, 240 with 3, two prompts of 2000 tokens 126 and 118; a lone chunk of 500 tokens, which fills few workgroups, 47.1
+// and 49.1. At D = 64 the third costs more than it saves (203 us, 210 with 3).
 template <int KV, int D>
 constexpr int prefill_nt() {
   return KV == kKv16 || (KV == kKv4 && D == 128) ? 3 : 2;
@@ -696,9 +697,9 @@ __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& 
 // MXFP4 caches. A chunk is a quarter of the 16-bit one's bytes, so run_chunks' own addresses and masks weigh four times
 // as much (254 of its 550 instructions a chunk were scalar: 64 decodes of 1023-8191 keys 75.6 us, here 70.2; 32
 // sequences of 6 queries 46.6, here 43.8). Here the page offsets of 64 tiles are computed one a lane, the loads take a
-// scalar base and 32-bit lane offsets, and chunks that every row sees whole take no masks. What bounds it now are the loads: with scores, softmax and values left out the walk still takes
-// 67-70 us, and 128 decodes of 8000-16000 keys (1.72 GB) 315 of 319 us, 5.4 TB/s. The window's offsets cost a short
-// walk 1.3 us (16 decodes 22.9 us, 21.6).
+// scalar base and 32-bit lane offsets, and chunks that every row sees whole take no masks. What bounds it now are the
+// loads: with scores, softmax and values left out the walk still takes 67-70 us, and 128 decodes of 8000-16000 keys
+// (1.72 GB) 315 of 319 us, 5.4 TB/s. The window's offsets cost a short walk 1.3 us (16 decodes 22.9 us, 21.6).
 //
 // Byte offsets, from the cache's and the scales' first, of tiles tile0 .. tile0 + 63, one a lane; the values' are
 // apart only where their strides differ from the keys'. ok: the tiles that are there.
@@ -1786,7 +1787,8 @@ static __global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
   constexpr int F = MIXED ? 4 : 1;
   constexpr int MR = merge_rows<D, F>();
   static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16, D>()) % MR == 0 &&
-                           (kWavesPerWG * 16 * prefill_nt<kKv8, D>()) % MR == 0),
+                           (kWavesPerWG * 16 * prefill_nt<kKv8, D>()) % MR == 0 &&
+                           (kWavesPerWG * 16 * prefill_nt<kKv4, D>()) % MR == 0),
                 "a prefill tile's rows split into whole merge chunks");
   const int CD = (p.HGW * p.RS + MR - 1) / MR;
   const int b = blockIdx.x;
@@ -1818,8 +1820,8 @@ static __global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
 
 // ---------------------------------------------------------------------------------------
 // Prefill class (q_len > QS): a workgroup of 4 waves computes 64 NT query rows of one
-// (sequence, kv head) (PAParams::PR: 192 over 16-bit caches, 128 over E4M3 caches), wave w
-// holding rows 16 NT w .. 16 NT (w + 1) - 1 of the tile.
+// (sequence, kv head) (PAParams::PR: 192 over 16-bit caches and MXFP4 ones of D = 128, 128 over
+// E4M3 caches and MXFP4 ones of D = 64), wave w holding rows 16 NT w .. 16 NT (w + 1) - 1 of the tile.
 //
 // The 4 waves share every 32-key K/V chunk through a 3-stage LDS ring filled by direct
 // global->LDS loads (no VGPR staging): chunk c + 2 is in flight while chunk c is computed.
@@ -2840,7 +2842,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   }
 }
 
-// LDS of a prefill workgroup: the ring's stages (3 over 16-bit caches, 2 over E4M3 caches).
+// LDS of a prefill workgroup: the ring's stages (3 over 16-bit caches, 2 over E4M3 and MXFP4 caches).
 template <int D, int KV>
 constexpr int prefill_lds_bytes() {
   return (KV == kKv16 ? PrefillLds<D>::kStages : 2) * PrefillLds<D>::kStageBytes;
@@ -2849,8 +2851,9 @@ constexpr int prefill_lds_bytes() {
 template <class E, int D, int KV, bool PLANNED>
 __device__ __forceinline__ void prefill_unit(const PAParams& p, int block, char* lds) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D>(), PLANNED>(p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
-                                   int64_t slot, int rest, int total) {
+  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D>(), PLANNED>(
+      p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
+                         int64_t slot, int rest, int total) {
     if constexpr (KV != kKv16)
       prefill_tile_convert<E, D, KV>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
     else
@@ -2968,7 +2971,8 @@ static int launch_decode_nt(PAParams& p, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-// Over MXFP4 caches non-temporal loads where a head's rows follow each other. Pages with a token's heads together share
+// Over MXFP4 caches this launch takes non-temporal loads where a head's rows follow each other (the short decode and the
+// decode part of a mixed launch always take ordinary ones). Pages with a token's heads together share
 // each line among two or four heads' waves: ordinary loads keep it for the others (64 decodes of 1023-8191 keys 82.8 us
 // against 89.9, heads of 64 61.4 against 75.3; with a head's rows together 77.6 against 69.8). A kernel each: two loops
 // in one took 21 to 30 more registers and a wave per SIMD with them.

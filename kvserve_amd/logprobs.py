@@ -25,7 +25,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     top: alternatives per row, 0 .. MAX_TOP.
 
     Statistics in fp32 whatever the logits' type. A logit of -inf is a token that cannot be; a row with a NaN or a +inf,
-    or of -inf alone, gives NaN, as does a token outside the vocabulary (its row's other outputs are unaffected)."""
+    or of -inf alone, gives NaN, as does a token outside the vocabulary (its row's other outputs are unaffected). NaN counts
+    as -inf in the order of the alternatives. Forward only: the outputs carry no gradient, whatever the logits require."""
     calls = _calls()
     if calls is not None:
         r = calls.token_logprobs(logits, tokens, top)
