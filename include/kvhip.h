@@ -46,6 +46,13 @@ enum kvh_dtype {
   KVH_DTYPE_BF16 = 2,
 };
 
+/* Storage formats of a KV cache, where one entry point takes them all. */
+enum kvh_cache_format {
+  KVH_CACHE_DTYPE = 0, /* elements of the call's dtype */
+  KVH_CACHE_E4M3 = 1,  /* kvh_reshape_and_cache_fp8 */
+  KVH_CACHE_MXFP4 = 2, /* kvh_reshape_and_cache_fp4 */
+};
+
 enum kvh_status {
   KVH_OK = 0,
   KVH_E_NULL = -1,        /* a required pointer is NULL */
@@ -339,6 +346,32 @@ KVH_API int kvh_paged_attention_fp4(const void* q, int64_t q_tok_stride, int64_t
                             int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                             int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale,
                             int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * paged_attention_window: kvh_paged_attention with a sliding window and sinks, over any cache format. A query token at
+ * position p sees the last `window` tokens, itself among them, and the first `sinks`:
+ *   out[t, h] = softmax_j(scale * q[t, h] . K[j]) V[j],  j <= p and (p - j < window or j < sinks)
+ * window >= 1, sinks >= 0. Pages that hold nothing a sequence's tokens of this step see are not read: their table
+ * entries, and the bytes of tokens that none of them sees, may be anything. Where window + sinks reaches the tables'
+ * capacity (max_blocks_per_seq * block_size) this is the call without a window, shared prefixes included.
+ * cache_format (KVH_CACHE_*) says what the caches hold: k_scale / v_scale count for E4M3 ones, k_scales / v_scales
+ * (the E8M0 bytes with their strides) for MXFP4 ones, and are ignored otherwise. Shapes, alignments and workspace
+ * (kvh_paged_attention_workspace_size) as the entry point of that format. The reference has no windowed attention.
+ */
+KVH_API int kvh_paged_attention_window(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                               const void* k_cache, const int64_t k_cache_strides[3],
+                               const void* k_scales, const int64_t k_scales_strides[3],
+                               const void* v_cache, const int64_t v_cache_strides[3],
+                               const void* v_scales, const int64_t v_scales_strides[3],
+                               int64_t num_blocks,
+                               void* out, int64_t o_tok_stride, int64_t o_head_stride,
+                               const int64_t* block_tables, int64_t bt_row_stride, int32_t max_blocks_per_seq,
+                               const int64_t* seq_lens, const int64_t* query_start_loc,
+                               int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                               int32_t head_dim, int32_t block_size, int32_t max_query_len,
+                               int32_t window, int32_t sinks, float scale, int32_t cache_format,
+                               float k_scale, float v_scale, int32_t dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Engine-harness kernels (no counterpart in the attention path; they serve the Llama layer

@@ -153,6 +153,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _vp, _sz, _vp,  # workspace, stream
         ],  # fmt: skip
     ),
+    "kvh_paged_attention_window": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _i64,  # q
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _i64,  # caches, each with its scales, num_blocks
+            _vp, _i64, _i64,  # out
+            _vp, _i64, _i32,  # block tables
+            _vp, _vp,  # seq_lens, query_start_loc
+            _i64, _i32, _i32, _i32, _i32, _i32, _i32,  # sizes
+            _i32, _i32, _f32, _i32, _f32, _f32, _i32,  # window, sinks, scale, cache format and scales, dtype
+            _vp, _sz, _vp,  # workspace, stream
+        ],  # fmt: skip
+    ),
     "kvh_add_rmsnorm": (
         ctypes.c_int,
         [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _f32, _i32, _vp],

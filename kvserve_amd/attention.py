@@ -264,6 +264,55 @@ def _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale) -> tor
     return out
 
 
+# KVH_CACHE_*: what the caches of an entry point for every format hold
+_CACHE_DTYPE, _CACHE_E4M3, _CACHE_MXFP4 = range(3)
+
+
+def _cache_args(k_cache, v_cache, k_scale, v_scale) -> tuple:
+    """(num_blocks, block_size, kv_heads, head_dim, device index, KVH_CACHE_*, k_scale, v_scale, address and strides of the
+    keys, their scales, the values and theirs) of caches of any format, checked."""
+    if FP4 is not None and k_cache.dtype == FP4:
+        layout = _fp4_layout(k_cache, v_cache, k_scale, v_scale)
+        return (*layout, _CACHE_MXFP4, 1.0, 1.0, _fp4_args(k_cache, k_scale, v_cache, v_scale))
+    num_blocks, block_size, num_kv_heads, head_dim, kcs, vcs, dev = _cache_layout(k_cache, v_cache)
+    fp8 = _kv_format(k_cache, v_cache, k_scale, v_scale)
+    args = [k_cache.data_ptr(), _lib.i64x3(kcs), None, None, v_cache.data_ptr(), _lib.i64x3(vcs), None, None]
+    return (num_blocks, block_size, num_kv_heads, head_dim, dev, _CACHE_E4M3 if fp8 else _CACHE_DTYPE, float(k_scale),
+            float(v_scale), args)  # fmt: skip
+
+
+def _check_window(window, sinks) -> tuple[int, int]:
+    _require(isinstance(window, int) and window >= 1, f"window must be a positive integer (got {window!r})")
+    _require(isinstance(sinks, int) and sinks >= 0, f"sinks must be a non-negative integer (got {sinks!r})")
+    return min(window, 2**31 - 1), min(sinks, 2**31 - 1)
+
+
+def _forward_window(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale, window, sinks) -> torch.Tensor:
+    window, sinks = _check_window(window, sinks)
+    num_blocks, block_size, num_kv_heads, head_dim, dev, fmt, ks, vs, caches = _cache_args(k_cache, v_cache, k_scale, v_scale)
+    out, tables, seq_lens, qsl = _check_attention(q, meta, num_kv_heads, head_dim, dev, out)
+    dtype = _dtype_code(q, k_cache, v_cache, out) if fmt == _CACHE_DTYPE else _dtype_code(q, out)
+    _require(fmt == _CACHE_DTYPE or q.dtype != torch.float32, f"{k_cache.dtype} caches need bf16 or fp16 queries")
+    num_tokens, num_heads, _ = q.shape
+    num_seqs, width = tables.shape
+    if num_tokens == 0 or num_seqs == 0:
+        return out
+    lib = _lib.load()
+    max_q = int(meta.max_query_len)
+    ws_bytes = _workspace_size(lib, num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, width, block_size, max_q,
+                               dtype)  # fmt: skip
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _current(dev):
+        st = lib.kvh_paged_attention_window(
+            q.data_ptr(), q.stride(0), q.stride(1), *caches, num_blocks, out.data_ptr(), out.stride(0), out.stride(1),
+            tables.data_ptr(), tables.stride(0), width, seq_lens.data_ptr(), qsl.data_ptr(), num_tokens, num_seqs,
+            num_heads, num_kv_heads, head_dim, block_size, max_q, window, sinks, float(scale), fmt, ks, vs, dtype,
+            ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(q.device),
+        )  # fmt: skip
+    _lib.check(st, "kvh_paged_attention_window")
+    return out
+
+
 def _check_index(t: torch.Tensor, name: str, dim: int) -> None:
     _require(t.dtype == torch.int64, f"{name} must be int64 (got {t.dtype})")
     _require(t.dim() == dim and t.stride(-1) == 1, f"{name} must be {dim}-d with a contiguous last dim")
@@ -544,10 +593,19 @@ class HipAttention:
         out: torch.Tensor | None = None,
         k_scale: float = 1.0,
         v_scale: float = 1.0,
+        window: int | None = None,
+        sinks: int = 0,
     ) -> torch.Tensor:
         """q: [T, H, D]; caches: [num_blocks, block_size, H_kv, D]. Returns [T, H, D] (in `out` if given).
         float8_e4m3fn caches hold keys / values as e4m3 * k_scale / v_scale (q and out bf16 or fp16);
-        float4_e2m1fn_x2 caches as MXFP4, k_scale and v_scale their float8_e8m0fnu tensors (see write_kv)."""
+        float4_e2m1fn_x2 caches as MXFP4, k_scale and v_scale their float8_e8m0fnu tensors (see write_kv).
+
+        window: every token sees the last `window` tokens, itself among them, and the first `sinks` of its sequence
+        (kvh_paged_attention_window); what lies between is not read, and its pages' table entries may be anything.
+        None: every token before it."""
+        if window is not None:
+            return _forward_window(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale, window, sinks)
+        _require(sinks == 0, "sinks belong to a window")
         if k_cache.dtype == FP4:
             return _forward_fp4(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale)
         calls = _calls()

@@ -40,6 +40,8 @@ SOURCES = [
     "paged_attention.hip",
     "paged_attention_f32.hip",
     "paged_attention_kv4.hip",
+    "paged_attention_kv4_window.hip",
+    "paged_attention_window.hip",
     "probes.hip",
     "reshape_and_cache.hip",
     "rope_and_cache.hip",
@@ -52,6 +54,8 @@ SOURCES = [
 SOURCE_FLAGS = {
     "paged_attention.hip": ["-fno-honor-nans"],
     "paged_attention_kv4.hip": ["-fno-honor-nans"],
+    "paged_attention_kv4_window.hip": ["-fno-honor-nans"],
+    "paged_attention_window.hip": ["-fno-honor-nans"],
     "rope_and_cache.hip": ["-ffp-contract=off"],
     "cache_fp4.hip": ["-ffp-contract=off"],
 }

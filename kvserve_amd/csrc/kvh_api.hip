@@ -40,7 +40,7 @@ void LaunchLog::after_launch(int kind, hipStream_t s) {
 }
 
 Plan make_plan(int64_t T, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t W, int32_t BS, int32_t max_q,
-               int32_t dtype) {
+               int32_t dtype, int32_t window, int32_t sinks) {
   Plan pl{};
   pl.G = H / Hkv;
   if (max_q < 1) max_q = 1;
@@ -58,7 +58,7 @@ Plan make_plan(int64_t T, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t 
   pl.RS = pl.QS * G;
   pl.HGW = Hkv % 8 == 0 ? 8 : (Hkv % 4 == 0 ? 4 : (Hkv % 2 == 0 ? 2 : 1));
   pl.slots = (int64_t)B * Hkv / pl.HGW + kMaxDecodeWaves / pl.HGW;
-  pl.short_decode = !pl.launch_prefill && pl.NT == 1 && (int64_t)W * BS <= kShortTokens;
+  pl.short_decode = !pl.launch_prefill && pl.NT == 1 && seq_keys(W, BS, window, sinks, pl.QS) <= kShortTokens;
   if (dtype == KVH_DTYPE_F32 || !mfma_shape(D, BS, G) || pl.short_decode) {
     pl.ws_acc_bytes = pl.ws_ml_bytes = pl.ws_job_bytes = pl.ws_pacc_bytes = pl.ws_pml_bytes = pl.ws_plan_bytes =
         pl.ws_bytes = 0;
@@ -79,7 +79,8 @@ Plan make_plan(int64_t T, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t 
                                                align_up((size_t)kMaxPrefillUnits * kPreStartBytes)
                                          : 0;
     // cascade over a shared prefix: share header, decode list, prefix partials, merge jobs
-    pl.cascade = !pl.launch_prefill && pl.NT == 1 && B >= 2 && (int64_t)W * BS > kCascadeMinTokens;
+    // (not under a window: what sequences share lies behind most of their windows)
+    pl.cascade = !pl.launch_prefill && pl.NT == 1 && B >= 2 && (int64_t)W * BS > kCascadeMinTokens && window <= 0;
     // A prefix group stacks the query rows of SG = XR / RS members into NX 16-row tiles
     // (XR = 16 NX rows). When the batch holds more than one tile's worth: over 16-bit caches
     // four tiles (64 rows), so up to 64 / RS members read the shared K/V once; over E4M3
@@ -452,7 +453,7 @@ size_t kvh_paged_attention_workspace_size(int64_t num_tokens, int32_t num_seqs, 
 }  // extern "C"
 
 // kvh_paged_attention (kv: kKv16), kvh_paged_attention_fp8 (kKv8: E4M3 caches with scales k_scale, v_scale) and
-// kvh_paged_attention_fp4 (kKv4: MXFP4 caches, whose E8M0 bytes are kx, vx).
+// kvh_paged_attention_fp4 (kKv4: MXFP4 caches, whose E8M0 bytes are kx, vx); window > 0: kvh_paged_attention_window.
 static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
                                 const int64_t k_cache_strides[3], const void* v_cache,
                                 const int64_t v_cache_strides[3], int64_t num_blocks, void* out, int64_t o_tok_stride,
@@ -462,7 +463,8 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
                                 int32_t head_dim, int32_t block_size, int32_t max_query_len, float scale,
                                 int32_t dtype, int32_t kv, float k_scale, float v_scale, const void* kx,
                                 const int64_t kx_strides[3], const void* vx, const int64_t vx_strides[3],
-                                void* workspace, size_t workspace_bytes, void* stream) {
+                                void* workspace, size_t workspace_bytes, void* stream, int32_t window = 0,
+                                int32_t sinks = 0) {
   // the timing hook covers exactly one call, whatever its outcome
   LaunchLog log;
   void* armed[8];
@@ -508,7 +510,7 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   }
 
   const Plan plan = make_plan(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, max_blocks_per_seq, block_size,
-                              max_query_len, dtype);
+                              max_query_len, dtype, window, sinks);
   if (plan.ws_bytes > 0 && (!workspace || workspace_bytes < plan.ws_bytes || !aligned16(workspace)))
     return KVH_E_WORKSPACE;
 
@@ -550,6 +552,8 @@ static int paged_attention_impl(const void* q, int64_t q_tok_stride, int64_t q_h
   p.vx_sb = vc.xsb;
   p.vx_ss = vc.xss;
   p.vx_sh = vc.xsh;
+  p.WND = window;
+  p.SNK = sinks;
   p.QS = plan.QS;
   p.RS = plan.RS;
   p.HGW = plan.HGW;
@@ -713,6 +717,37 @@ int kvh_paged_attention_fp4(const void* q, int64_t q_tok_stride, int64_t q_head_
                               max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
                               num_kv_heads, head_dim, block_size, max_query_len, scale, dtype, kKv4, 1.f, 1.f, k_scale,
                               k_scale_strides, v_scale, v_scale_strides, workspace, workspace_bytes, stream);
+}
+
+int kvh_paged_attention_window(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k_cache,
+                               const int64_t k_cache_strides[3], const void* k_scales,
+                               const int64_t k_scales_strides[3], const void* v_cache,
+                               const int64_t v_cache_strides[3], const void* v_scales,
+                               const int64_t v_scales_strides[3], int64_t num_blocks, void* out, int64_t o_tok_stride,
+                               int64_t o_head_stride, const int64_t* block_tables, int64_t bt_row_stride,
+                               int32_t max_blocks_per_seq, const int64_t* seq_lens, const int64_t* query_start_loc,
+                               int64_t num_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                               int32_t head_dim, int32_t block_size, int32_t max_query_len, int32_t window,
+                               int32_t sinks, float scale, int32_t cache_format, float k_scale, float v_scale,
+                               int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (window < 1 || sinks < 0) return KVH_E_SHAPE;
+  if (cache_format < KVH_CACHE_DTYPE || cache_format > KVH_CACHE_MXFP4) return KVH_E_DTYPE;
+  if (max_blocks_per_seq > 0 && block_size > 0) {
+    const int64_t keys = (int64_t)max_blocks_per_seq * block_size;
+    // a window that no sequence outgrows is none
+    if ((int64_t)window + sinks >= keys)
+      window = sinks = 0;
+    else if (keys > 0x7fffff00LL)  // a walk's positions, rounded up to chunks
+      return KVH_E_UNSUPPORTED;
+  }
+  const bool fp8 = cache_format == KVH_CACHE_E4M3;
+  return paged_attention_impl(q, q_tok_stride, q_head_stride, k_cache, k_cache_strides, v_cache, v_cache_strides,
+                              num_blocks, out, o_tok_stride, o_head_stride, block_tables, bt_row_stride,
+                              max_blocks_per_seq, seq_lens, query_start_loc, num_tokens, num_seqs, num_heads,
+                              num_kv_heads, head_dim, block_size, max_query_len, scale, dtype,
+                              fp8 ? kKv8 : (cache_format == KVH_CACHE_MXFP4 ? kKv4 : kKv16), fp8 ? k_scale : 1.f,
+                              fp8 ? v_scale : 1.f, k_scales, k_scales_strides, v_scales, v_scales_strides, workspace,
+                              workspace_bytes, stream, window, sinks);
 }
 
 static bool a16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

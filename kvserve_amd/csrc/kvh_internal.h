@@ -94,7 +94,18 @@ struct PAParams {
   int64_t kx_sb, kx_ss, kx_sh;
   const uint8_t* vx;
   int64_t vx_sb, vx_ss, vx_sh;
+  // sliding window (0: none): a query token sees the last WND tokens, itself among them, and the first SNK (WND + SNK
+  // below W BS)
+  int32_t WND, SNK;
 };
+
+// Keys of a decode-class sequence at most that its rows read (the table's capacity, or the chunks of a window's walk).
+inline int64_t seq_keys(int32_t W, int32_t BS, int32_t window, int32_t sinks, int32_t QS) {
+  const int64_t all = (int64_t)W * BS;
+  if (window <= 0) return all;
+  const int64_t seen = ((int64_t)sinks + 31) / 32 * 32 + (int64_t)window + QS - 1 + 31;
+  return seen < all ? seen : all;
+}
 
 // Launch plan: a pure function of static shapes (graph-capture safe).
 struct Plan {
@@ -116,7 +127,7 @@ inline int32_t cascade_group(int32_t RS, int32_t nx) { return RS >= 16 * nx ? 1 
 inline int32_t cascade_tiles(int32_t NX, bool packed) { return packed && NX > 2 ? 2 : NX; }
 
 Plan make_plan(int64_t T, int32_t B, int32_t H, int32_t Hkv, int32_t D, int32_t W, int32_t BS, int32_t max_q,
-               int32_t dtype);
+               int32_t dtype, int32_t window = 0, int32_t sinks = 0);
 
 // Kernel launchers (return hipError_t as int). `kinds` collects launched kernel kinds.
 struct LaunchLog {
@@ -131,6 +142,10 @@ int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_
                                 hipStream_t s, LaunchLog& log);
 int launch_paged_attention_kv4(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
                                LaunchLog& log);
+int launch_paged_attention_window(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t kv, int32_t max_q,
+                                  hipStream_t s, LaunchLog& log);
+int launch_paged_attention_kv4_window(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q,
+                                      hipStream_t s, LaunchLog& log);
 // Whether a 16-bit launch takes the MFMA kernels: head sizes 64 and 128, pages a whole number
 // of 16-token tiles, GQA groups of at most 64 rows per token (four 16-row tiles). Every other
 // 16-bit shape, and fp32, takes the vector-ALU kernel (no workspace).

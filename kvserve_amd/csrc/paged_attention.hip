@@ -51,9 +51,10 @@ constexpr int kWavesPerWG = 4;
 // register set of chunks in flight (254 VGPRs): two chunks of 900-1024 tokens over 4000-10000 beside 24 decodes 272 us
 // with 2, 240 with 3, two prompts of 2000 tokens 126 and 118; a lone chunk of 500 tokens, which fills few workgroups, 47.1
 // and 49.1. At D = 64 the third costs more than it saves (203 us, 210 with 3).
-template <int KV, int D>
+// Under a window, whose masked loop ahead takes registers of its own, MXFP4 keeps 2 (3 spill 11 registers).
+template <int KV, int D, bool WIN>
 constexpr int prefill_nt() {
-  return KV == kKv16 || (KV == kKv4 && D == 128) ? 3 : 2;
+  return KV == kKv16 || (KV == kKv4 && D == 128 && !WIN) ? 3 : 2;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -140,6 +141,44 @@ struct VRegs4 {
 };
 
 __device__ __forceinline__ int kv4_token(int j, int e) { return 4 * e + j; }
+
+// A sliding window with sinks (the kernels of WIN; PAParams::WND, SNK): a row of limit l sees keys l - WND .. l - 1 and
+// those below SNK. What a run of rows reads is walked as one range of 32-token chunks: walk position v is token v in the
+// sinks' chunks and token v + skip behind them, the first row's window starting in the first chunk there.
+struct Window {
+  int sink;   // tokens of the sinks' chunks
+  int skip;   // tokens left out behind them, whole chunks
+  int lo;     // tokens below it that are no sinks are seen by none of the rows
+  int hi;     // tokens from it on are in the window of every row that does not end before them
+  int sinks;
+  __device__ __forceinline__ int token(int v) const { return v < sink ? v : v + skip; }
+  // walk position (in chunks) of the first of the walk's chunks that are chunk c of the cache or a later one
+  __device__ __forceinline__ int walk(int c) const { return c <= sink / 32 ? c : max(sink / 32, c - skip / 32); }
+};
+struct NoWindow {};
+template <bool WIN>
+using WindowOf = std::conditional_t<WIN, Window, NoWindow>;
+
+// The window of rows whose limits run from `first` to `last`.
+template <bool WIN>
+__device__ __forceinline__ WindowOf<WIN> make_window(const PAParams& p, int first, int last) {
+  if constexpr (WIN) {
+    Window w;
+    w.sink = (p.SNK + 31) / 32 * 32;
+    w.lo = first - p.WND;
+    w.hi = last - p.WND;
+    w.skip = max(0, w.lo / 32 * 32 - w.sink);
+    w.sinks = p.SNK;
+    return w;
+  } else {
+    return {};
+  }
+}
+__device__ __forceinline__ int walk_token(const Window& w, int v) { return w.token(v); }
+__device__ __forceinline__ int walk_token(const NoWindow&, int v) { return v; }
+__device__ __forceinline__ int walk_chunk(const Window& w, int c) { return w.walk(c); }
+__device__ __forceinline__ int walk_chunk(const NoWindow&, int c) { return c; }
+
 // Uniform description of a chunk: first token and the block of each 16-token tile.
 struct ChunkRef {
   int tok0;
@@ -415,9 +454,10 @@ __device__ __forceinline__ f32x4 line_scores(const WaveState<D, 1>& s, const KR&
 // LAZY: skip the accumulator rescale when no row max moved (a uniform branch; exact, and a
 // win for decode where the max settles early); otherwise the body is straight-line so the
 // row tiles' dependency chains interleave.
-template <class E, int D, int NT, bool MASKED, bool LINES, bool LAZY = true, class KR>
+// A window's lower edge is masked in the chunks that some row sees in part (a uniform branch with no load in it).
+template <class E, int D, int NT, bool MASKED, bool LINES, bool LAZY = true, class KR, class WN = NoWindow>
 __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, const PAParams& p,
-                                             const ChunkRef& c, u32x4 pt[NT]) {
+                                             const ChunkRef& c, u32x4 pt[NT], const WN& w = WN{}) {
   const int j = (threadIdx.x & 63) >> 4;
   f32x4 st[NT][2];
   if constexpr (LINES) {
@@ -462,6 +502,20 @@ __device__ __forceinline__ void chunk_scores(WaveState<D, NT>& s, const KR& kr, 
         }
         st[t][tile][e] = x;
         mx = fmaxf(mx, x);
+      }
+    }
+    if constexpr (std::is_same_v<WN, Window>) {
+      if (c.tok0 < w.hi) {
+        mx = -INFINITY;
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = c.tok0 + 16 * tile + 4 * j + e;
+            const float x = tok >= s.limit[t] - p.WND || tok < w.sinks ? st[t][tile][e] : -INFINITY;
+            st[t][tile][e] = x;
+            mx = fmaxf(mx, x);
+          }
       }
     }
     mx = max_over_groups(mx);
@@ -514,8 +568,9 @@ __device__ __forceinline__ void pf_scores(const WaveState<D, NT>& s, const KRegs
 }
 
 // Causal / absent-page mask of one chunk's scores (-inf where the key is not visible).
-template <int NT>
-__device__ __forceinline__ void pf_mask(f32x4 st[NT][2], const int limit[NT], const ChunkRef& ch) {
+template <int NT, class WN>
+__device__ __forceinline__ void pf_mask(f32x4 st[NT][2], const int limit[NT], const ChunkRef& ch, const PAParams& p,
+                                        const WN& w) {
   const int j = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -525,6 +580,12 @@ __device__ __forceinline__ void pf_mask(f32x4 st[NT][2], const int limit[NT], co
       const int lim = ch.blk[tile] >= 0 ? limit[t] - (ch.tok0 + 16 * tile + 4 * j) : INT32_MIN;
 #pragma unroll
       for (int e = 0; e < 4; ++e) st[t][tile][e] = e < lim ? st[t][tile][e] : -INFINITY;
+      if constexpr (std::is_same_v<WN, Window>) {
+        // and of a window those from its first key on, or below the sinks
+        const int tok = ch.tok0 + 16 * tile + 4 * j, from = limit[t] - p.WND - tok, sinks = w.sinks - tok;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[t][tile][e] = e >= from || e < sinks ? st[t][tile][e] : -INFINITY;
+      }
     }
 }
 
@@ -575,12 +636,27 @@ __device__ __forceinline__ void pf_softmax(WaveState<D, NT>& s, const f32x4 st[N
   }
 }
 
+// Values of a chunk's tokens that no row's window holds: their pages may be given away already, and hold anything.
+template <int DW, class VR>
+__device__ __forceinline__ void win_values(VR& vr, const ChunkRef& c, int j, const Window& w) {
+  if (c.tok0 < w.lo) {
+#pragma unroll
+    for (int t8 = 0; t8 < 8; ++t8) {
+      const int tok = c.tok0 + 16 * (t8 >> 2) + 4 * j + (t8 & 3);
+#pragma unroll
+      for (int x = 0; x < DW; ++x) vr.v[t8][x] = tok >= w.lo || tok < w.sinks ? vr.v[t8][x] : 0u;
+    }
+  }
+}
+template <int DW, class VR>
+__device__ __forceinline__ void win_values(VR&, const ChunkRef&, int, const NoWindow&) {}
+
 // O^T += V^T P^T for one chunk. In the masked case, slots at or past seq_len may hold any
 // bits (stale or never written cache slots): P is 0 there but 0 * NaN is NaN, so V is
 // zeroed like the reference's masked loads (other=0.0).
-template <class E, int D, int NT, bool MASKED>
+template <class E, int D, int NT, bool MASKED, class WN = NoWindow>
 __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs<D>& vr, const ChunkRef& c, int data_end,
-                                         const u32x4 pt[NT]) {
+                                         const u32x4 pt[NT], const WN& w = WN{}) {
   constexpr int VW = D / 16;
   const int j = (threadIdx.x & 63) >> 4;
   if (MASKED) {
@@ -592,6 +668,7 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs<D>& vr, cons
       for (int x = 0; x < VW / 2; ++x) vr.v[t8][x] = keep ? vr.v[t8][x] : 0u;  // select, no branch
     }
   }
+  win_values<VW / 2>(vr, c, j, w);
   // V^T A operand i: element 4*tile + e of lane (j, m) = V[token 16*tile + 4j + e][VW*m + i]
 #pragma unroll
   for (int i = 0; i < VW; ++i) {
@@ -610,9 +687,9 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs<D>& vr, cons
 // w, element i of tokens t8 = 2w and 2w + 1; one byte permute gathers that pair for two
 // neighbouring i (bytes b0, b1 of the dwords), and the two halves of the result convert to
 // the two operands' dwords. Masked tokens are zeroed in the raw bytes (E4M3 0x00 is +0).
-template <class E, int D, int NT, bool MASKED>
+template <class E, int D, int NT, bool MASKED, class WN = NoWindow>
 __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs8<D>& vr, const ChunkRef& c, int data_end,
-                                         const u32x4 pt[NT]) {
+                                         const u32x4 pt[NT], const WN& w = WN{}) {
   constexpr int VW = D / 16;
   const int j = (threadIdx.x & 63) >> 4;
   if (MASKED) {
@@ -624,6 +701,7 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs8<D>& vr, con
       for (int x = 0; x < VW / 4; ++x) vr.v[t8][x] = keep ? vr.v[t8][x] : 0u;
     }
   }
+  win_values<VW / 4>(vr, c, j, w);
 #pragma unroll
   for (int x = 0; x < VW / 4; ++x)
 #pragma unroll
@@ -646,22 +724,62 @@ __device__ __forceinline__ void chunk_pv(WaveState<D, NT>& s, VRegs8<D>& vr, con
     }
 }
 
-template <class E, int D, int NT, bool NTL>
+template <class E, int D, int NT, bool NTL, class WN>
 __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
-                                               int tok_begin, int stride, int tok_hi, int data_end);
+                                               int tok_begin, int stride, int tok_hi, int data_end, const WN& w);
+
+// run_chunks under a window: the same loop over walk positions.
+template <class E, int D, int NT, int KV, bool NTL, bool LINES>
+__device__ __forceinline__ void run_chunks_win(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
+                                               int v_begin, int stride, int v_hi, int data_end, const Window& w) {
+  const int tok_hi = w.token(v_hi - 1) + 1, page_end = (tok_hi + p.BS - 1) / p.BS;
+  const LaneOffsets lo = lane_offsets<D, KV, LINES>(p);
+  PageWindow pw;
+  load_window(pw, p, btrow, w.token(v_begin) / p.BS, page_end);
+  ChunkRef c = chunk_ref(pw, p, btrow, w.token(v_begin), tok_hi, page_end);
+  std::conditional_t<KV == kKv8, KRegs8<D>, KRegs<D>> kr;
+  std::conditional_t<KV == kKv8, VRegs8<D>, VRegs<D>> vr;
+  load_k<D, NTL, LINES>(kr, p, c, kvh, lo.k);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v<D, NTL>(vr, p, c, kvh, lo.v);
+  __builtin_amdgcn_sched_barrier(0);
+  int v = v_begin;
+  while (v + stride < v_hi) {
+    v += stride;
+    const ChunkRef cn = chunk_ref(pw, p, btrow, w.token(v), tok_hi, page_end);
+    u32x4 pt[NT];
+    chunk_scores<E, D, NT, true, LINES>(s, kr, p, c, pt, w);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k<D, NTL, LINES>(kr, p, cn, kvh, lo.k);
+    __builtin_amdgcn_sched_barrier(0);
+    chunk_pv<E, D, NT, true>(s, vr, c, data_end, pt, w);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v<D, NTL>(vr, p, cn, kvh, lo.v);
+    __builtin_amdgcn_sched_barrier(0);
+    c = cn;
+  }
+  u32x4 pt[NT];
+  chunk_scores<E, D, NT, true, LINES>(s, kr, p, c, pt, w);
+  chunk_pv<E, D, NT, true>(s, vr, c, data_end, pt, w);
+}
 
 // Chunk loop of one wave over tokens tok_begin, tok_begin + stride, ... < tok_hi.
 // The body is straight-line (masks always applied, loads unconditional) and the loads are
 // pinned in the order K(c+1), V(c+1) with scheduling barriers, so each s_waitcnt waits for
-// exactly the operand it guards while the other half of the next chunk stays in flight.
-template <class E, int D, int NT, int KV = kKv16, bool NTL = true, bool LINES = false>
+// exactly the operand it guards while the other half of the next chunk stays in flight. Under a window tok_begin,
+// stride and tok_hi are walk positions (Window).
+template <class E, int D, int NT, int KV = kKv16, bool NTL = true, bool LINES = false, class WN = NoWindow>
 __device__ __forceinline__ void run_chunks(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
-                                           int tok_begin, int stride, int tok_hi, int data_end) {
+                                           int tok_begin, int stride, int tok_hi, int data_end, const WN& w = WN{}) {
   if constexpr (KV == kKv4) {
-    run_chunks_kv4<E, D, NT, NTL>(s, p, btrow, kvh, tok_begin, stride, tok_hi, data_end);
+    run_chunks_kv4<E, D, NT, NTL>(s, p, btrow, kvh, tok_begin, stride, tok_hi, data_end, w);
     return;
   }
   if (tok_begin >= tok_hi) return;
+  if constexpr (std::is_same_v<WN, Window>) {
+    run_chunks_win<E, D, NT, KV, NTL, LINES>(s, p, btrow, kvh, tok_begin, stride, tok_hi, data_end, w);
+    return;
+  }
   const int page_end = (tok_hi + p.BS - 1) / p.BS;
   const LaneOffsets lo = lane_offsets<D, KV, LINES>(p);
   PageWindow pw;
@@ -713,10 +831,11 @@ __device__ __forceinline__ bool kv4_same_strides(const PAParams& p) {
   return p.k_sb == p.v_sb && p.k_ss == p.v_ss && p.kx_sb == p.vx_sb && p.kx_ss == p.vx_ss;
 }
 
+template <class WN>
 __device__ __forceinline__ void kv4_window(Kv4Window& w, const PAParams& p, const int64_t* btrow, int tile0,
-                                           int tile_end, bool same) {
-  const int tile = tile0 + (threadIdx.x & 63), r = p.BS / 16, page = tile / r;
-  const bool in = tile < tile_end;
+                                           int tile_end, bool same, const WN& wn) {
+  const int at = tile0 + (threadIdx.x & 63), tile = walk_token(wn, 16 * at) / 16, r = p.BS / 16, page = tile / r;
+  const bool in = at < tile_end;
   const int64_t raw = btrow[in ? page : 0];  // every lane loads: no divergent branch
   const bool ok = in && raw >= 0 && raw < p.num_blocks;
   const uint64_t b = ok ? (uint64_t)raw : 0, slot = (uint64_t)((tile - page * r) * 16);
@@ -834,13 +953,15 @@ __device__ __forceinline__ void kv4_scores(const WaveState<D, NT>& s, const KReg
 
 // -inf where row and key do not meet (bits: the tiles that are there). The values of a token that is not there take the
 // scale 2^-127: finite whatever their bytes (an E2M1 code has no NaN), for its P of 0.
-template <int D, int NT>
+template <int D, int NT, class WN>
 __device__ __forceinline__ void kv4_mask(const WaveState<D, NT>& s, VRegs4<D>& vr, int tok0, int bits, int data_end,
-                                         f32x4 (&st)[NT][2]) {
+                                         f32x4 (&st)[NT][2], const PAParams& p, const WN& w) {
   const int lane = threadIdx.x & 63, j = lane >> 4;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const bool in = ((bits >> t) & 1) && tok0 + 16 * t + kv4_token(j, lane & 3) < data_end;
+    const int tok = tok0 + 16 * t + kv4_token(j, lane & 3);
+    bool in = ((bits >> t) & 1) && tok < data_end;
+    if constexpr (std::is_same_v<WN, Window>) in = in && (tok >= w.lo || tok < w.sinks);
     vr.x[t] = in ? vr.x[t] : 0u;
   }
 #pragma unroll
@@ -850,6 +971,11 @@ __device__ __forceinline__ void kv4_mask(const WaveState<D, NT>& s, VRegs4<D>& v
       const int lim = (bits >> tile) & 1 ? s.limit[t] - (tok0 + 16 * tile + j) : INT32_MIN;
 #pragma unroll
       for (int e = 0; e < 4; ++e) st[t][tile][e] = 4 * e < lim ? st[t][tile][e] : -INFINITY;
+      if constexpr (std::is_same_v<WN, Window>) {
+        const int tok = tok0 + 16 * tile + j, from = s.limit[t] - p.WND - tok, sinks = w.sinks - tok;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[t][tile][e] = 4 * e >= from || 4 * e < sinks ? st[t][tile][e] : -INFINITY;
+      }
     }
 }
 
@@ -1088,11 +1214,20 @@ __device__ __forceinline__ bool cascade_member(const PAParams& p, const SeqView&
   return v.q_len > 0 && v.q_len <= p.QS && clamp64(v.ctx, 0, v.kv_total) >= kCascadeMinChunks * kChunk;
 }
 
+// The window of all of a sequence's rows.
+template <bool WIN>
+__device__ __forceinline__ WindowOf<WIN> seq_window(const PAParams& p, const SeqView& v) {
+  return make_window<WIN>(p, (int)clamp64(v.ctx + 1, 0, v.kv_total), (int)clamp64(v.ctx + v.q_len, 0, v.kv_total));
+}
+
 // skip: keys [0, skip) of every cascade member are computed by the prefix segments
 // (skip <= its context then), so its own segments cover [skip, kv_total).
+// WIN: those of the window's walk.
+template <bool WIN>
 __device__ __forceinline__ int seq_chunks(const PAParams& p, const SeqView& v, int skip) {
   if (v.q_len == 0 || v.q_len > p.QS) return 0;
-  const int sk = skip > 0 && cascade_member(p, v) ? skip : 0;
+  int sk = skip > 0 && cascade_member(p, v) ? skip : 0;
+  if constexpr (WIN) sk = seq_window<true>(p, v).skip;
   return max(1, (v.kv_total - sk + kChunk - 1) / kChunk);
 }
 
@@ -1110,6 +1245,7 @@ struct SeqWindow {
   int qs, ql, ctx, kvt;  // this lane's SeqView (ctx clamped to [-q_len, kv_total])
 };
 
+template <bool WIN>
 __device__ __forceinline__ void scan_window(SeqWindow& sw, const PAParams& p, int blk0, int base, int nbase,
                                             int skip) {
   const int lane = threadIdx.x & 63;
@@ -1117,7 +1253,7 @@ __device__ __forceinline__ void scan_window(SeqWindow& sw, const PAParams& p, in
   int c = 0, mem = 0, qs = 0, ql = 0, cx = 0, kt = 0;
   if (s < p.B) {
     const SeqView v = seq_view(p, s);
-    c = seq_chunks(p, v, skip);
+    c = seq_chunks<WIN>(p, v, skip);
     mem = cascade_member(p, v) ? 1 : 0;
     // 32-bit copies for the segment walk: qs <= T < 2^31 and kv_total < 2^31 (checked on the
     // host); ctx is only read as clamp(ctx + qi + 1, 0, kv_total) for 0 <= qi < q_len and as
@@ -1384,7 +1520,7 @@ __device__ __forceinline__ void write_job_x(int32_t* job, int pieces, int64_t sl
 // group (XR = 16 NX rows; 1 outside the cascade).
 // LINES: whole-line K reads where the launch's mean unit asks for them (line_units); over MXFP4 caches non-temporal
 // loads (launch_decode_pages).
-template <class E, int D, int NT, int KV, int NX, bool LINES>
+template <class E, int D, int NT, int KV, int NX, bool LINES, bool WIN>
 __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool may_read_lines = true) {
   static_assert(!LINES || KV == kKv4 || (NT == 1 && NX == 1));
   constexpr bool kLines = LINES && KV != kKv4;
@@ -1411,7 +1547,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
   // Cascade: keys [0, L) of every decode-class sequence come from the prefix segments, which
   // take the first P = groups * NHG * L / 32 positions of the flat space.
   int L = 0, ngrp = 0, r0 = 0, nd = 0;
-  if constexpr (NT == 1) {
+  if constexpr (NT == 1 && !WIN) {
     if (p.CASC) {
       L = (int)uni64(p.ws_share[0]);
       ngrp = (int)uni64(p.ws_share[1]);
@@ -1427,7 +1563,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
   uint64_t wide = 0;  // sequences past the rows that whole-line reads serve
   for (int blk0 = 0; blk0 < p.B; blk0 += 64) {
     SeqWindow sw;
-    scan_window(sw, p, blk0, Cs, Ns, L);
+    scan_window<WIN>(sw, p, blk0, Cs, Ns, L);
     Cs += sw.total;
     Ns += sw.ntotal;
     if constexpr (kLines) wide |= __builtin_amdgcn_ballot_w64(sw.c > 0 && sw.ql * p.G > kLineRows);
@@ -1444,7 +1580,7 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
   const bool lines = kLines && may_read_lines && wide == 0 && line_units(KV == kKv8, C, NUa);
 
   int64_t pos = a;
-  if constexpr (NT == 1) {
+  if constexpr (NT == 1 && !WIN) {
     // prefix segments (g, hg): the XR-row tiles of group g against keys [0, L) of head group
     // hg, read through the first sequence's table (the shared blocks); always partial
     while (pos < b && pos < P) {
@@ -1470,10 +1606,10 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
 
   // walk the segments overlapping [a, b) (positions past the prefix region)
   SeqWindow sw;
-  scan_window(sw, p, 0, 0, 0, L);
+  scan_window<WIN>(sw, p, 0, 0, 0, L);
   while (pos < b) {
     while (P + (int64_t)(sw.base + sw.total) * NHG <= pos)
-      scan_window(sw, p, sw.blk0 + 64, sw.base + sw.total, sw.nbase + sw.ntotal, L);
+      scan_window<WIN>(sw, p, sw.blk0 + 64, sw.base + sw.total, sw.nbase + sw.ntotal, L);
     const int64_t start = P + (int64_t)(sw.base + sw.excl) * NHG;  // first chunk of this lane's sequence
     const uint64_t hit = __builtin_amdgcn_ballot_w64(sw.c > 0 && start <= pos && pos < start + (int64_t)sw.c * NHG);
     if (hit == 0) break;  // cannot happen for consistent metadata; never index lane 64
@@ -1497,19 +1633,22 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
     const int R = sv.q_len * p.G;
     const bool member = L > 0 && __builtin_amdgcn_readlane(sw.mem, l);
     const int skip = member ? L : 0;
+    const auto win = seq_window<WIN>(p, sv);
+    int walk_end = sv.kv_total;  // in walk positions under a window
+    if constexpr (WIN) walk_end -= win.skip;
     const int tok_lo = skip + (int)(pos - seg_beg) * kChunk;
-    const int tok_hi = min(skip + (int)(y - seg_beg) * kChunk, sv.kv_total);
+    const int tok_hi = min(skip + (int)(y - seg_beg) * kChunk, walk_end);
     WaveState<D, NT> st;
     const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
     if constexpr (kLines) {
       if (lines) {
         load_q<D, NT, KV, true>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-        run_chunks<E, D, NT, KV, true, true>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
+        run_chunks<E, D, NT, KV, true, true>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total, win);
       }
     }
     if (!lines) {
       load_q<D, NT, KV>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-      run_chunks<E, D, NT, KV, KV != kKv4 || LINES>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total);
+      run_chunks<E, D, NT, KV, KV != kKv4 || LINES>(st, p, btrow, kvh, tok_lo, kChunk, tok_hi, sv.kv_total, win);
     }
     const bool whole = pos == seg_beg && y == seg_end && !member;
     const int64_t slot = (int64_t)seq * NHG + hg + unit;
@@ -1554,7 +1693,8 @@ __device__ __forceinline__ void decode_unit(const PAParams& p, int block, bool m
 // workspace and no merge launch follows: a batch this small is bound by latency, and the
 // merge launch was a third of it.
 // LINES: whole-line, non-temporal K/V loads for up to 8 rows (launch_mfma_typed).
-template <class E, int D, int KV, bool LINES>
+// WIN: the chunks of the window's walk.
+template <class E, int D, int KV, bool LINES, bool WIN>
 __global__ __launch_bounds__(256) void pa_decode_short_kernel(PAParams p) {
   constexpr int NI = D / 16;
   __shared__ f32x4 x_acc[kWavesPerWG - 1][NI][64];
@@ -1567,12 +1707,15 @@ __global__ __launch_bounds__(256) void pa_decode_short_kernel(PAParams p) {
   const int R = sv.q_len * p.G;
   WaveState<D, 1> st;
   const int64_t* btrow = p.bt + (int64_t)seq * p.bt_rs;
+  const auto win = seq_window<WIN>(p, sv);
+  int walk_end = sv.kv_total;
+  if constexpr (WIN) walk_end -= win.skip;
   if (LINES && R <= kLineRows) {
     load_q<D, 1, KV, LINES>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-    run_chunks<E, D, 1, KV, true, LINES>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
+    run_chunks<E, D, 1, KV, true, LINES>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, walk_end, sv.kv_total, win);
   } else {
     load_q<D, 1, KV>(st, p, sv.qs, R, 0, kvh, sv.ctx, sv.kv_total);
-    run_chunks<E, D, 1, KV, false>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, sv.kv_total, sv.kv_total);
+    run_chunks<E, D, 1, KV, false>(st, p, btrow, kvh, w * kChunk, kWavesPerWG * kChunk, walk_end, sv.kv_total, win);
   }
   if (w > 0) {
 #pragma unroll
@@ -1786,9 +1929,9 @@ template <class E, int D, bool MIXED, bool BLK>
 static __global__ __launch_bounds__(256) void pa_merge_kernel(PAParams p) {
   constexpr int F = MIXED ? 4 : 1;
   constexpr int MR = merge_rows<D, F>();
-  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16, D>()) % MR == 0 &&
-                           (kWavesPerWG * 16 * prefill_nt<kKv8, D>()) % MR == 0 &&
-                           (kWavesPerWG * 16 * prefill_nt<kKv4, D>()) % MR == 0),
+  static_assert(!MIXED || ((kWavesPerWG * 16 * prefill_nt<kKv16, D, false>()) % MR == 0 &&
+                           (kWavesPerWG * 16 * prefill_nt<kKv8, D, false>()) % MR == 0 &&
+                           (kWavesPerWG * 16 * prefill_nt<kKv4, D, false>()) % MR == 0),
                 "a prefill tile's rows split into whole merge chunks");
   const int CD = (p.HGW * p.RS + MR - 1) / MR;
   const int b = blockIdx.x;
@@ -1940,10 +2083,11 @@ struct PfWindow {
   int first_bad;            // first chunk >= c0 with a missing half (c0 + 64 when none)
 };
 
-template <int KV = kKv16>
+// Under a window (wn) the chunks are those of its walk, and a missing half below chunk `masked` counts as none.
+template <int KV, class WN>
 __device__ __forceinline__ void pf_window(PfWindow& win, const PAParams& p, const int64_t* btrow, int c0, int c_end,
-                                          int page_end, int hmine, int64_t sb2, int64_t ss2, int64_t xsb = 0,
-                                          int64_t xss = 0) {
+                                          int page_end, int hmine, int64_t sb2, int64_t ss2, const WN& wn, int masked,
+                                          int64_t xsb = 0, int64_t xss = 0) {
   const int lane = threadIdx.x & 63;
   const int c = c0 + lane;
   const int r = p.BS / 16;  // 16-token halves per page (BS % 16 == 0)
@@ -1956,7 +2100,7 @@ __device__ __forceinline__ void pf_window(PfWindow& win, const PAParams& p, cons
   // branch whose join could hold a spill store ahead of the exec restore.
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int hh = 2 * c + h;
+    const int hh = 2 * (walk_token(wn, kChunk * c) / kChunk) + h;
     const int pg = hh / r;
     off[h] = (hh - pg * r) * 16;
     in[h] = c < c_end && pg < page_end;
@@ -1970,7 +2114,9 @@ __device__ __forceinline__ void pf_window(PfWindow& win, const PAParams& p, cons
   }
   win.ok0 = __builtin_amdgcn_ballot_w64(ok[0]);
   win.ok1 = __builtin_amdgcn_ballot_w64(ok[1]);
-  const uint64_t bad = ~(win.ok0 & win.ok1);
+  uint64_t bad = ~(win.ok0 & win.ok1);
+  if constexpr (std::is_same_v<WN, Window>)
+    if (masked > c0) bad &= masked - c0 < 64 ? ~0ull << (masked - c0) : 0ull;
   win.first_bad = c0 + (bad ? (int)__builtin_ctzll(bad) : 64);
   const int idm = hmine ? id[1] : id[0];
   const int offm = hmine ? off[1] : off[0];
@@ -2111,9 +2257,9 @@ __device__ __forceinline__ void lgkm_wait_tied(u32x2& a, u32x2& b) {
 // may still be in flight.
 constexpr int kVLead = 2;
 
-template <class E, int D, int NT, bool MASKED, int VOFF>
+template <class E, int D, int NT, bool MASKED, int VOFF, class WN>
 __device__ __forceinline__ void pf_pv(WaveState<D, NT>& s, VTr<D>& v, uint32_t vbase, const ChunkRef& c,
-                                      int data_end, const u32x4 pt[NT]) {
+                                      int data_end, const u32x4 pt[NT], const WN& wn) {
   constexpr int NI = D / 16;
   const int lane = threadIdx.x & 63;
   const int j = lane >> 4;
@@ -2125,6 +2271,9 @@ __device__ __forceinline__ void pf_pv(WaveState<D, NT>& s, VTr<D>& v, uint32_t v
       const int tok = c.tok0 + 16 * h + 4 * j + 2 * (w & 1);
       const bool ok = c.blk[h] >= 0;
       keep[w] = (ok && tok < data_end ? 0x0000ffffu : 0u) | (ok && tok + 1 < data_end ? 0xffff0000u : 0u);
+      if constexpr (std::is_same_v<WN, Window>)  // as win_values
+        keep[w] &= (tok >= wn.lo || tok < wn.sinks ? 0x0000ffffu : 0u) |
+                   (tok + 1 >= wn.lo || tok + 1 < wn.sinks ? 0xffff0000u : 0u);
     }
   }
   StaticFor<NI>::run([&](auto I) {
@@ -2227,14 +2376,14 @@ __device__ __forceinline__ float pf_q_ready(WaveState<D, NT>& s, const PAParams&
 }
 
 // run_chunks over an MXFP4 cache: the next chunk's K and V are in flight while this one is computed.
-template <class E, int D, int NT, bool NTL>
+template <class E, int D, int NT, bool NTL, class WN>
 __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAParams& p, const int64_t* btrow, int kvh,
-                                               int tok_begin, int stride, int tok_hi, int data_end) {
+                                               int tok_begin, int stride, int tok_hi, int data_end, const WN& w) {
   if (tok_begin >= tok_hi) return;
   const bool same = kv4_same_strides(p);
   const int tile_end = (tok_hi + 15) / 16;
   Kv4Window win;
-  kv4_window(win, p, btrow, tok_begin / 16, tile_end, same);
+  kv4_window(win, p, btrow, tok_begin / 16, tile_end, same, w);
   Kv4Lanes<D> lanes(p, kvh);
   KRegs4<D> kr;
   VRegs4<D> vr;
@@ -2249,7 +2398,7 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
   }
   const float c = pf_q_ready<E, D, NT>(s, p);
   // keys that every row sees
-  int seen = min(tok_hi, data_end);
+  int seen = min(walk_token(w, tok_hi - 1) + 1, data_end);
 #pragma unroll
   for (int t = 0; t < NT; ++t) seen = min(seen, s.limit[t]);
 #pragma unroll
@@ -2261,7 +2410,7 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
     Kv4Chunk n;
     int nbits = 0;
     if (MORE) {
-      if (next / 16 + 2 - win.tile0 > 64) kv4_window(win, p, btrow, next / 16, tile_end, same);
+      if (next / 16 + 2 - win.tile0 > 64) kv4_window(win, p, btrow, next / 16, tile_end, same, w);
       const int rel = next / 16 - win.tile0;
       n = kv4_chunk(win, rel, same);
       nbits = (int)(win.ok >> rel & 3);
@@ -2271,7 +2420,10 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
     __builtin_amdgcn_sched_barrier(0);
     if (MORE) kv4_load_k<D, NTL>(kr, lanes, n);
     __builtin_amdgcn_sched_barrier(0);
-    if (tok0 + kChunk > seen || bits != 3) kv4_mask<D, NT>(s, vr, tok0, bits, data_end, st);
+    const int tok = walk_token(w, tok0);
+    bool edge = tok + kChunk > seen || bits != 3;
+    if constexpr (std::is_same_v<WN, Window>) edge = edge || tok < w.hi;
+    if (edge) kv4_mask<D, NT>(s, vr, tok, bits, data_end, st, p, w);
     float mx[NT];
     pf_lanemax<NT>(st, mx);
     u32x4 pt[NT];
@@ -2297,11 +2449,13 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
 // ring stage of each step known at compile time, so every LDS address is an immediate
 // offset), the chunks on the causal diagonal or with a missing page (masked), then the
 // chunks past the wave's rows (loads and barriers only).
-template <class E, int D>
+// Under a window the chunks are those of its walk, and a masked loop goes ahead: the sinks' chunks and those in which
+// some row's window starts, to a whole turn of the ring.
+template <class E, int D, bool WIN>
 __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                              int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                              int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<kKv16, D>();
+  constexpr int NT = prefill_nt<kKv16, D, WIN>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   c_lo = uni(c_lo);
@@ -2315,6 +2469,11 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
 
   // keys below every valid row's causal limit (that of the wave's first row)
   const int lim_all = row0 < R ? (int)clamp64(sv.ctx + row0 / p.G + 1, 0, sv.kv_total) : 0;
+  const auto wn = make_window<WIN>(p, (int)clamp64(sv.ctx + wg_row0 / p.G + 1, 0, sv.kv_total), kv_lim);
+  // chunks from c_lo on in which a row of this wave may have its window start
+  int n_edge = 0;
+  if constexpr (WIN)
+    n_edge = max(0, walk_chunk(wn, (max(my_lim - p.WND, 0) + kChunk - 1) / kChunk) - c_lo);
 
   // the page window first: the first chunks' loads wait for it, the query tile is not
   // needed before they are in flight
@@ -2323,7 +2482,7 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
   PfLoads<D> pl;
   pf_loads_init<D>(pl, p, w, kvh);
   PfWindow win;
-  pf_window(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2);
+  pf_window<kKv16>(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2, wn, c_lo + n_edge);
   WaveState<D, NT> s;
   load_q<D, NT>(s, p, sv.qs, R, row0, kvh, sv.ctx, sv.kv_total);
   uint32_t ka[D / 32];
@@ -2337,8 +2496,8 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
   const int n = c_hi - c_lo;
   // this wave's rows see chunks c_lo .. c_lo + n_my - 1 only; it keeps taking part in the
   // loads and barriers of the rest
-  const int n_my = max(0, min(n, (my_lim + kChunk - 1) / kChunk - c_lo));
-  int n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
+  const int n_my = max(0, min(n, walk_chunk(wn, (my_lim + kChunk - 1) / kChunk) - c_lo));
+  int n_int = max(0, min(n_my, min(walk_chunk(wn, lim_all / kChunk), win.first_bad) - c_lo));
   pf_issue<D>(lds, 0, pl, win, c_lo);
   if (n > 1) pf_issue<D>(lds, L::kStageBytes, pl, win, c_lo + 1);
   // Q and the page window were loaded together, Q is transformed while the first chunks load
@@ -2351,10 +2510,10 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
     if (i >= prio.next_drop) prio.set(i, n, rest, total);
     const int ci2 = c_lo + i + 2;
     if (i + 2 < n && ci2 - win.c0 >= 64) {  // the window moves on (every 62 chunks)
-      pf_window(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2);
+      pf_window<kKv16>(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2, wn, c_lo + n_edge);
       // the unmasked run reaches as far as the new window allows (the old window's end
       // capped it; a missing page before this point has already ended the run)
-      n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
+      n_int = max(0, min(n_my, min(walk_chunk(wn, lim_all / kChunk), win.first_bad) - c_lo));
     }
     __builtin_amdgcn_sched_barrier(0);
     if (i + 1 < n)
@@ -2373,13 +2532,13 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
     f32x4 sc[NT][2];
     pf_scores_lds<E, D, NT>(s, ka, SOFF + stage, sc);
     ChunkRef cr;
-    cr.tok0 = (c_lo + i) * kChunk;
+    cr.tok0 = walk_token(wn, (c_lo + i) * kChunk);
     cr.blk[0] = cr.blk[1] = 0;
     if (MASKED) {
       const int rel = c_lo + i - win.c0;
       cr.blk[0] = (win.ok0 >> rel) & 1 ? 0 : -1;
       cr.blk[1] = (win.ok1 >> rel) & 1 ? 0 : -1;
-      pf_mask<NT>(sc, s.limit, cr);
+      pf_mask<NT>(sc, s.limit, cr, p, wn);
     }
     float mx[NT];
     pf_lanemax<NT>(sc, mx);
@@ -2392,12 +2551,22 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
     __builtin_amdgcn_sched_barrier(0);
     u32x4 pt[NT];
     pf_softmax<E, D, NT>(s, sc, mx, c, pt);
-    pf_pv<E, D, NT, MASKED, SOFF + L::kKBytes>(s, vt, vb, cr, sv.kv_total, pt);
+    pf_pv<E, D, NT, MASKED, SOFF + L::kKBytes>(s, vt, vb, cr, sv.kv_total, pt, wn);
   };
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, L::kStageBytes>;
   using S2 = std::integral_constant<int, 2 * L::kStageBytes>;
   int i = 0;
+  if constexpr (WIN) {
+    const int ahead = min((n_edge + 2) / 3 * 3, n_my);
+    int st = 0;
+    for (; i < ahead; ++i) {
+      sync(i, (st == 0 ? 2 : st - 1) * L::kStageBytes);
+      compute(i, st * L::kStageBytes, S0{}, std::true_type{});
+      st = st == 2 ? 0 : st + 1;
+    }
+    if (st != 0) n_int = 0;  // the wave's rows end inside a turn
+  }
   while (i < n_int) {  // unmasked, unrolled by the ring's 3 stages
     sync(i, 2 * L::kStageBytes);
     compute(i, 0, S0{}, std::false_type{});
@@ -2432,11 +2601,11 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
 // the last chunk's bytes are converted, which a chunk's computation covers as well); chunk i is
 // converted and written right before the barrier that publishes it, so two LDS stages
 // suffice (stage i % 2 was last read by chunk i - 2, before the previous barrier).
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                                      int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                                      int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<KV, D>();
+  constexpr int NT = prefill_nt<KV, D, WIN>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   constexpr int KLW = L::kLoadsPerWave;
@@ -2452,6 +2621,11 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
   const int my_last = min(row0 + 16 * NT - 1, R - 1);
   const int my_lim = row0 < R ? (int)clamp64(sv.ctx + my_last / p.G + 1, 0, sv.kv_total) : 0;
   const int lim_all = row0 < R ? (int)clamp64(sv.ctx + row0 / p.G + 1, 0, sv.kv_total) : 0;
+  const auto wn = make_window<WIN>(p, (int)clamp64(sv.ctx + wg_row0 / p.G + 1, 0, sv.kv_total), kv_lim);
+  // chunks from c_lo on in which a row of this wave may have its window start
+  int n_edge = 0;
+  if constexpr (WIN)
+    n_edge = max(0, walk_chunk(wn, (max(my_lim - p.WND, 0) + kChunk - 1) / kChunk) - c_lo);
 
   // the page window first: the first chunks' loads wait for it, the query tile is not
   // needed before they are in flight
@@ -2460,7 +2634,7 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
   PfLoads<D> pl;
   pf_loads_init<D, KV>(pl, p, w, kvh);
   PfWindow win;
-  pf_window<KV>(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2, pl.xsb, pl.xss);
+  pf_window<KV>(win, p, btrow, c_lo, c_hi, page_end, pl.h, pl.sb2, pl.ss2, wn, c_lo + n_edge, pl.xsb, pl.xss);
   WaveState<D, NT> s;
   load_q<D, NT>(s, p, sv.qs, R, row0, kvh, sv.ctx, sv.kv_total);
   uint32_t ka[D / 32];
@@ -2471,8 +2645,8 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
   __builtin_amdgcn_s_barrier();  // every wave has finished reading the stages (previous tile)
   __builtin_amdgcn_sched_barrier(0);
   const int n = c_hi - c_lo;
-  const int n_my = max(0, min(n, (my_lim + kChunk - 1) / kChunk - c_lo));
-  int n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
+  const int n_my = max(0, min(n, walk_chunk(wn, (my_lim + kChunk - 1) / kChunk) - c_lo));
+  int n_int = max(0, min(n_my, min(walk_chunk(wn, lim_all / kChunk), win.first_bad) - c_lo));
 
   struct Raw {
     std::conditional_t<KV == kKv8, u32x2, uint32_t> g[KLW];
@@ -2515,10 +2689,10 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
     if (i >= prio.next_drop) prio.set(i, n, rest, total);
     const int ci2 = c_lo + i + kSets;
     if (i + kSets < n && ci2 - win.c0 >= 64) {
-      pf_window<KV>(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2, pl.xsb, pl.xss);
+      pf_window<KV>(win, p, btrow, c_lo + i, c_hi, page_end, pl.h, pl.sb2, pl.ss2, wn, c_lo + n_edge, pl.xsb, pl.xss);
       // the unmasked run reaches as far as the new window allows (the old window's end
       // capped it; a missing page before this point has already ended the run)
-      n_int = max(0, min(n_my, min(lim_all / kChunk, win.first_bad) - c_lo));
+      n_int = max(0, min(n_my, min(walk_chunk(wn, lim_all / kChunk), win.first_bad) - c_lo));
     }
     __builtin_amdgcn_sched_barrier(0);
     if (kSets > 1 && i + 1 < n)
@@ -2554,13 +2728,13 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
     f32x4 sc[NT][2];
     pf_scores_lds<E, D, NT>(s, ka, SOFF + stage, sc);
     ChunkRef cr;
-    cr.tok0 = (c_lo + i) * kChunk;
+    cr.tok0 = walk_token(wn, (c_lo + i) * kChunk);
     cr.blk[0] = cr.blk[1] = 0;
     if (MASKED) {
       const int rel = c_lo + i - win.c0;
       cr.blk[0] = (win.ok0 >> rel) & 1 ? 0 : -1;
       cr.blk[1] = (win.ok1 >> rel) & 1 ? 0 : -1;
-      pf_mask<NT>(sc, s.limit, cr);
+      pf_mask<NT>(sc, s.limit, cr, p, wn);
     }
     float mx[NT];
     pf_lanemax<NT>(sc, mx);
@@ -2574,13 +2748,24 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
       kv4_softmax<E, D, NT, true>(s, sc, mx, c, pt);
     else
       pf_softmax<E, D, NT>(s, sc, mx, c, pt);
-    pf_pv<E, D, NT, MASKED, SOFF + L::kKBytes>(s, vt, vb, cr, sv.kv_total, pt);
+    pf_pv<E, D, NT, MASKED, SOFF + L::kKBytes>(s, vt, vb, cr, sv.kv_total, pt, wn);
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, L::kStageBytes>;
   int i = 0;
+  if constexpr (WIN) {
+    const int ahead = min((n_edge + 1) / 2 * 2, n_my);
+    for (; i < ahead; ++i) {
+      if (i & 1)
+        sync(i, I1{});
+      else
+        sync(i, I0{});
+      compute(i, (i & 1) * L::kStageBytes, S0{}, std::true_type{});
+    }
+    if (i & 1) n_int = 0;
+  }
   while (i < n_int) {  // unmasked, unrolled by the two stages
     sync(i, I0{});
     compute(i, 0, S0{}, std::false_type{});
@@ -2603,16 +2788,27 @@ __device__ __forceinline__ PreSeq pre_seq(const PAParams& p, const SeqView& sv) 
   return PreSeq{sv.q_len * p.G, sv.q_len, sv.kv_total, sv.ctx};
 }
 
+template <bool WIN>
 __device__ __forceinline__ int pre_tile_chunks(const PAParams& p, const SeqView& sv, int R, int t) {
-  return pre_tile_chunks(PreSeq{R, sv.q_len, sv.kv_total, sv.ctx}, p.G, p.PR, t);
+  const PreSeq s{R, sv.q_len, sv.kv_total, sv.ctx};
+  int c = pre_tile_chunks(s, p.G, p.PR, t);
+  if constexpr (WIN) c -= pre_tile_skip(s, p.G, p.PR, p.WND, p.SNK, t);
+  return c;
+}
+
+template <int PR, bool WIN>
+__device__ __forceinline__ int64_t pre_positions(const PAParams& p, const PreSeq& s, int step, int t) {
+  int64_t n = pre_prefix(s, p.G, PR, step, t);
+  if constexpr (WIN) n -= pre_skips(s, p.G, PR, p.WND, p.SNK, t);
+  return n;
 }
 
 // Flat positions of all tiles of one kv head of a prefill-class sequence; 0 for others.
-template <int PR>
+template <int PR, bool WIN>
 __device__ __forceinline__ int64_t pre_seq_positions(const PAParams& p, const SeqView& sv, int step) {
   if (sv.q_len <= p.QS) return 0;
   const PreSeq s = pre_seq(p, sv);
-  return pre_prefix(s, p.G, PR, step, (s.R + PR - 1) / PR);
+  return pre_positions<PR, WIN>(p, s, step, (s.R + PR - 1) / PR);
 }
 
 // x / y of non-negative wave-uniform values, in 32 bits where they fit.
@@ -2648,7 +2844,7 @@ static_assert(sizeof(PreStart) == kPreStartBytes, "the workspace holds one per p
 
 // DIVIDES: whether the group divides PR, known here so that either form of pre_prefix has code of its own (one code
 // for both: 8 decodes of 1000 keys and a 200-token chunk over E4M3 caches 33.0 us, so 32.7).
-template <int PR, bool DIVIDES>
+template <int PR, bool DIVIDES, bool WIN>
 __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreStart* st, int64_t* wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int per = (p.B + kPlanThreads - 1) / kPlanThreads;
@@ -2659,7 +2855,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
   int64_t pos = 0;
   for (int sq = s0; sq < s1; ++sq) {
     sv = seq_view(p, sq);
-    pos += (int64_t)p.Hkv * pre_seq_positions<PR>(p, sv, step);
+    pos += (int64_t)p.Hkv * pre_seq_positions<PR, WIN>(p, sv, step);
   }
   int64_t incl = pos;
 #pragma unroll
@@ -2700,7 +2896,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
       const int end = __builtin_amdgcn_readlane(s1, l);
       for (;; ++sq) {
         v = seq_view_uniform(p, sq);
-        per_kvh = uni64(pre_seq_positions<PR>(p, v, step));
+        per_kvh = uni64(pre_seq_positions<PR, WIN>(p, v, step));
         if (off < p.Hkv * per_kvh || sq + 1 >= end) break;
         off -= p.Hkv * per_kvh;
       }
@@ -2713,7 +2909,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
     int t = 0;
     int64_t t_beg = 0;
     for (int t0 = 0; t0 < tiles; t0 += 64) {
-      const int64_t x = pre_prefix(s, p.G, PR, step, min(t0 + lane, tiles));
+      const int64_t x = pre_positions<PR, WIN>(p, s, step, min(t0 + lane, tiles));
       const uint64_t le = __builtin_amdgcn_ballot_w64(t0 + lane < tiles && x <= off);
       if (le == 0) break;
       const int k = 63 - __builtin_clzll(le);
@@ -2729,23 +2925,24 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
   return true;
 }
 
-template <int PR>
+template <int PR, bool WIN>
 __device__ __forceinline__ bool prefill_start(const PAParams& p, int b, PreStart* st, int64_t* wsum) {
-  return PR % p.G == 0 ? prefill_start_as<PR, true>(p, b, st, wsum) : prefill_start_as<PR, false>(p, b, st, wsum);
+  return PR % p.G == 0 ? prefill_start_as<PR, true, WIN>(p, b, st, wsum)
+                       : prefill_start_as<PR, false, WIN>(p, b, st, wsum);
 }
 
 // In a mixed batch's own decode launch NUP more workgroups follow the decode units (grid (NU HGW
 // / 4) + NUP): each writes where a prefill unit starts, under the decode work, and the prefill
 // launch behind it begins with one load. (Computed by the prefill workgroups themselves it was
 // on that launch's path: 512 decodes and four 384-token chunks over E4M3 caches 483 -> 492 us.)
-template <class E, int D, int NT, int KV, int NX, bool LINES>
+template <class E, int D, int NT, int KV, int NX, bool LINES, bool WIN>
 __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
   const int b = blockIdx.x;
   if constexpr (NX == 1) {
     if (p.ND > 0 && b >= p.ND) {
       __shared__ PreStart st;
       __shared__ int64_t wsum[kPlanThreads / 64];
-      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV, D>()>(p, b - p.ND, &st, wsum);
+      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV, D, WIN>(), WIN>(p, b - p.ND, &st, wsum);
       if (threadIdx.x == 0) {
         if (!work) st.u = -1;  // idle, rewritten on every call
         ((PreStart*)p.ws_plan)[b - p.ND] = st;
@@ -2753,7 +2950,7 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
       return;
     }
   }
-  decode_unit<E, D, NT, KV, NX, LINES>(p, b);
+  decode_unit<E, D, NT, KV, NX, LINES, WIN>(p, b);
 }
 
 // Stream-K over the prefill-class work: a flat space of (sequence, kv head, tile, chunk),
@@ -2772,7 +2969,7 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
 // R, seq, kvh, t, c_lo, c_hi, partial, slot, rest, total)` computes chunks [c_lo, c_hi) of tile t.
 // PLANNED: the start is in the workspace (pa_decode_kernel); else it is computed here, in lds,
 // which is free again when the first tile is computed.
-template <int PR, bool PLANNED, class TileFn>
+template <int PR, bool PLANNED, bool WIN, class TileFn>
 __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* lds, TileFn&& tile) {
   int32_t* job = p.ws_job + (int64_t)(kMaxDecodeWaves + b) * kJobInts;
   if (threadIdx.x == 0) job[0] = kJobNone;
@@ -2781,7 +2978,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
     st = (const PreStart*)p.ws_plan + b;
     if (uni(st->u) < 0) return;
   } else {
-    if (!prefill_start<PR>(p, b, (PreStart*)lds, (int64_t*)(lds + sizeof(PreStart)))) return;
+    if (!prefill_start<PR, WIN>(p, b, (PreStart*)lds, (int64_t*)(lds + sizeof(PreStart)))) return;
   }
   const int64_t C = uni64(st->C);
   const int NUa = (int)active_units(C, p.NUP);
@@ -2799,7 +2996,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   const int total = (int)(x1 - x);  // positions of this unit: < 2^31 (C / NUa + 1)
   int R = sv.q_len * p.G;
   int tiles = (R + p.PR - 1) / p.PR;
-  int n_t = pre_tile_chunks(p, sv, R, t);
+  int n_t = pre_tile_chunks<WIN>(p, sv, R, t);
   // a: this unit's first position within the tile. Positions a .. b - 1 of a tile are its
   // chunks max(0, a - kTileCost) .. max(0, b - kTileCost) - 1, the same map at both ends
   // of every unit, so the pieces partition the chunks; a range inside the virtual prefix is
@@ -2838,7 +3035,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
         tiles = (R + p.PR - 1) / p.PR;
       }
     }
-    n_t = pre_tile_chunks(p, sv, R, t);
+    n_t = pre_tile_chunks<WIN>(p, sv, R, t);
   }
 }
 
@@ -2848,24 +3045,24 @@ constexpr int prefill_lds_bytes() {
   return (KV == kKv16 ? PrefillLds<D>::kStages : 2) * PrefillLds<D>::kStageBytes;
 }
 
-template <class E, int D, int KV, bool PLANNED>
+template <class E, int D, int KV, bool PLANNED, bool WIN>
 __device__ __forceinline__ void prefill_unit(const PAParams& p, int block, char* lds) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D>(), PLANNED>(
+  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D, WIN>(), PLANNED, WIN>(
       p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
                          int64_t slot, int rest, int total) {
     if constexpr (KV != kKv16)
-      prefill_tile_convert<E, D, KV>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
+      prefill_tile_convert<E, D, KV, WIN>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
     else
-      prefill_tile<E, D>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
+      prefill_tile<E, D, WIN>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
   });
 }
 
 // 4-wave workgroups of 64 NT rows (PAParams::PR), 2 per CU.
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
-  prefill_unit<E, D, KV, true>(p, blockIdx.x, lds);
+  prefill_unit<E, D, KV, true, WIN>(p, blockIdx.x, lds);
 }
 
 // A mixed batch in one launch: the first ND workgroups are its decode units, the next NUP its
@@ -2873,14 +3070,14 @@ __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
 // (launch_mixed): its workgroups leave their places at once, and no launch runs ahead of the
 // prefill work. Four prompts of 300-2500 tokens (D = 128, bf16): step 201 -> 176 us; two chunks
 // of 900-1024 tokens over 4000-10000 cached ones, E4M3: 328 -> 310 us.
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 __global__ __launch_bounds__(256, 2) void pa_mixed_kernel(PAParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
   const int b = blockIdx.x;
   if (b < p.ND)
-    decode_unit<E, D, 1, KV, 1, line_dim(D) && KV == kKv16>(p, b, p.LINES);  // (E4M3: its units are too short for lines)
+    decode_unit<E, D, 1, KV, 1, line_dim(D) && KV == kKv16, WIN>(p, b, p.LINES);  // (E4M3: its units are too short for lines)
   else
-    prefill_unit<E, D, KV, false>(p, b - p.ND, lds);
+    prefill_unit<E, D, KV, false, WIN>(p, b - p.ND, lds);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -2946,7 +3143,7 @@ static int decode_units(PAParams& p, int resident, int per_cu, bool packed, bool
   // No launch takes more units than its static shape can give work (kMinUnitChunks chunks of
   // at most W BS keys per segment): a small batch dispatches a grid of its own size, and the
   // merge launch scans that many job records, not one per wave the device could hold.
-  const int64_t seg_chunks = ((int64_t)p.W * p.BS + kChunk - 1) / kChunk;
+  const int64_t seg_chunks = (seq_keys(p.W, p.BS, p.WND, p.SNK, p.QS) + kChunk - 1) / kChunk;
   const int64_t max_chunks = (int64_t)(p.Hkv / p.HGW) * p.B * (seg_chunks > 1 ? seg_chunks : 1);
   const int64_t cap = (max_chunks + kMinUnitChunks - 1) / kMinUnitChunks;
   if (units > cap) units = cap;
@@ -2961,13 +3158,13 @@ static int decode_units(PAParams& p, int resident, int per_cu, bool packed, bool
   return wgs;
 }
 
-template <class E, int D, int NT, int KV, int NX = 1, bool LINES = false>
+template <class E, int D, int NT, int KV, bool WIN, int NX = 1, bool LINES = false>
 static int launch_decode_nt(PAParams& p, hipStream_t s) {
   int per_cu = 1;
-  const int resident = resident_blocks((const void*)&pa_decode_kernel<E, D, NT, KV, NX, LINES>, 256, &per_cu);
+  const int resident = resident_blocks((const void*)&pa_decode_kernel<E, D, NT, KV, NX, LINES, WIN>, 256, &per_cu);
   const int wgs = decode_units(p, resident, per_cu, KV != kKv16, KV == kKv4 && D == 64);
   p.ND = p.NUP > 0 ? wgs : 0;  // NUP > 0: the workgroups behind the decode units plan the prefill launch
-  hipLaunchKernelGGL((pa_decode_kernel<E, D, NT, KV, NX, LINES>), dim3(wgs + p.NUP), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pa_decode_kernel<E, D, NT, KV, NX, LINES, WIN>), dim3(wgs + p.NUP), dim3(256), 0, s, p);
   return (int)hipGetLastError();
 }
 
@@ -2976,25 +3173,25 @@ static int launch_decode_nt(PAParams& p, hipStream_t s) {
 // each line among two or four heads' waves: ordinary loads keep it for the others (64 decodes of 1023-8191 keys 82.8 us
 // against 89.9, heads of 64 61.4 against 75.3; with a head's rows together 77.6 against 69.8). A kernel each: two loops
 // in one took 21 to 30 more registers and a wave per SIMD with them.
-template <class E, int D, int NT, int KV, int NX = 1>
+template <class E, int D, int NT, int KV, bool WIN, int NX = 1>
 static int launch_decode_pages(PAParams& p, hipStream_t s) {
   if constexpr (KV == kKv4)
-    if (p.k_ss == D / 2 && p.v_ss == D / 2) return launch_decode_nt<E, D, NT, KV, NX, true>(p, s);
-  return launch_decode_nt<E, D, NT, KV, NX>(p, s);
+    if (p.k_ss == D / 2 && p.v_ss == D / 2) return launch_decode_nt<E, D, NT, KV, WIN, NX, true>(p, s);
+  return launch_decode_nt<E, D, NT, KV, WIN, NX>(p, s);
 }
 
 // The decode launch of a batch whose decode-class sequences take NT 16-row tiles (no cascade).
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 static int launch_decode(PAParams& p, int NT, hipStream_t s) {
   switch (NT) {
     case 1:
       if constexpr (line_dim(D) && KV != kKv4)
         if (line_launch(D, p.NUP > 0 ? 0 : p.RS, p.k_ss * (KV == kKv8 ? 1 : 2)))
-          return launch_decode_nt<E, D, 1, KV, 1, true>(p, s);
-      return launch_decode_pages<E, D, 1, KV>(p, s);
-    case 2: return launch_decode_pages<E, D, 2, KV>(p, s);
-    case 3: return launch_decode_pages<E, D, 3, KV>(p, s);
-    case 4: return launch_decode_pages<E, D, 4, KV>(p, s);
+          return launch_decode_nt<E, D, 1, KV, WIN, 1, true>(p, s);
+      return launch_decode_pages<E, D, 1, KV, WIN>(p, s);
+    case 2: return launch_decode_pages<E, D, 2, KV, WIN>(p, s);
+    case 3: return launch_decode_pages<E, D, 3, KV, WIN>(p, s);
+    case 4: return launch_decode_pages<E, D, 4, KV, WIN>(p, s);
     default: return (int)hipErrorInvalidValue;
   }
 }
@@ -3009,24 +3206,25 @@ constexpr int64_t kFusedUnitChunks = 4;
 // of 255-4095 keys beside four 384-token chunks 851 us in one launch, 816 apart; 100 decodes of
 // 255-2000 keys beside the same chunks 216 and 188; 512 decodes beside one 17-token chunk 721
 // and 741). Apart as well when a decode row needs more than one 16-row tile (GQA groups above 16).
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
-  p.PR = kWavesPerWG * 16 * prefill_nt<KV, D>();
+  p.PR = kWavesPerWG * 16 * prefill_nt<KV, D, WIN>();
   // units x 2 partial slots x tile rows stay within the workspace's kMaxPrefillUnits x 2 x kPrefillRows
   const int cap = kMaxPrefillUnits * kPrefillRows / p.PR;
   // sequences that can be decode class: each of the others takes at most max_q of the T tokens
   const int64_t over = p.T - (int64_t)p.B * p.QS;
   const int64_t n_pre = over > 0 ? (over + max_q - p.QS - 1) / (max_q - p.QS) : 0;
   const int64_t n_dec = p.B > n_pre ? p.B - n_pre : 0;
-  const int64_t dec_chunks = n_dec * (p.Hkv / p.HGW) * (((int64_t)p.W * p.BS + kChunk - 1) / kChunk);
+  const int64_t dec_chunks =
+      n_dec * (p.Hkv / p.HGW) * ((seq_keys(p.W, p.BS, p.WND, p.SNK, p.QS) + kChunk - 1) / kChunk);
   int err, per_cu = 1;
-  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV>, 256, &per_cu);
+  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV, WIN>, 256, &per_cu);
   const int wgs = decode_units(p, resident, per_cu, KV != kKv16, KV == kKv4 && D == 64);
   if (NT > 1 || dec_chunks > kFusedUnitChunks * p.NU) {
-    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV>), cap) / 8 * 8);
-    if ((err = launch_decode<E, D, KV>(p, NT, s))) return err;
+    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV, WIN>), cap) / 8 * 8);
+    if ((err = launch_decode<E, D, KV, WIN>(p, NT, s))) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
-    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV>), dim3(p.NUP), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV, WIN>), dim3(p.NUP), dim3(256), 0, s, p);
     if ((err = (int)hipGetLastError())) return err;
     log.after_launch(KVH_KERNEL_PREFILL, s);
     return 0;
@@ -3034,21 +3232,22 @@ static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, Launc
   p.NUP = std::max(8, std::min(resident, cap) / 8 * 8);
   p.LINES = KV == kKv16 && line_launch(D, 0, p.k_ss * 2);
   p.ND = (wgs + 7) / 8 * 8;  // prefill workgroup b keeps XCD b % 8
-  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV, WIN>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
   if ((err = (int)hipGetLastError())) return err;
   log.after_launch(KVH_KERNEL_MIXED, s);
   return 0;
 }
 
-template <class E, int D, int KV>
+template <class E, int D, int KV, bool WIN>
 static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipStream_t s, LaunchLog& log) {
   int err = 0;
   if (plan.short_decode) {
-    if (KV != kKv4 && line_short(D, KV == kKv8, (int64_t)p.B * p.Hkv * D, (int64_t)p.W * p.BS))
-      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, KV != kKv4 && can_read_lines(D, KV == kKv8)>),
+    if (KV != kKv4 && line_short(D, KV == kKv8, (int64_t)p.B * p.Hkv * D,
+                                seq_keys(p.W, p.BS, p.WND, p.SNK, p.QS)))
+      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, KV != kKv4 && can_read_lines(D, KV == kKv8), WIN>),
                          dim3(p.Hkv, p.B), dim3(256), 0, s, p);
     else
-      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, false>), dim3(p.Hkv, p.B), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((pa_decode_short_kernel<E, D, KV, false, WIN>), dim3(p.Hkv, p.B), dim3(256), 0, s, p);
     if ((err = (int)hipGetLastError())) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
     return 0;
@@ -3060,11 +3259,14 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
     log.after_launch(KVH_KERNEL_SHARE, s);
   }
   if (plan.launch_prefill) {
-    if ((err = launch_mixed<E, D, KV>(p, plan.NT, max_q, s, log))) return err;
+    if ((err = launch_mixed<E, D, KV, WIN>(p, plan.NT, max_q, s, log))) return err;
   } else {
     constexpr int NX = KV == kKv16 ? 4 : 2;  // 64-row prefix groups (32 over E4M3 caches)
-    err = plan.cascade && p.XR == 16 * NX ? launch_decode_pages<E, D, 1, KV, NX>(p, s)
-                                          : launch_decode<E, D, KV>(p, plan.NT, s);
+    if constexpr (WIN)
+      err = launch_decode<E, D, KV, WIN>(p, plan.NT, s);
+    else
+      err = plan.cascade && p.XR == 16 * NX ? launch_decode_pages<E, D, 1, KV, WIN, NX>(p, s)
+                                            : launch_decode<E, D, KV, WIN>(p, plan.NT, s);
     if (err) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
   }
@@ -3088,30 +3290,45 @@ static int launch_mfma_typed(PAParams& p, const Plan& plan, int32_t max_q, hipSt
   return 0;
 }
 
-template <int KV>
+template <int KV, bool WIN>
 static int launch_mfma_kv(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
                           LaunchLog& log) {
   const bool bf = dtype == 2;
   if (D == 128)
-    return bf ? launch_mfma_typed<BF16, 128, KV>(p, plan, max_q, s, log)
-              : launch_mfma_typed<F16, 128, KV>(p, plan, max_q, s, log);
+    return bf ? launch_mfma_typed<BF16, 128, KV, WIN>(p, plan, max_q, s, log)
+              : launch_mfma_typed<F16, 128, KV, WIN>(p, plan, max_q, s, log);
   if (D == 64)
-    return bf ? launch_mfma_typed<BF16, 64, KV>(p, plan, max_q, s, log)
-              : launch_mfma_typed<F16, 64, KV>(p, plan, max_q, s, log);
+    return bf ? launch_mfma_typed<BF16, 64, KV, WIN>(p, plan, max_q, s, log)
+              : launch_mfma_typed<F16, 64, KV, WIN>(p, plan, max_q, s, log);
   return (int)hipErrorInvalidValue;
 }
 
-#ifdef KVH_KV4_OBJECT
+// The instances are compiled in four objects, at once: by the caches' format (KVH_KV4_OBJECT) and with a window or
+// without (KVH_WINDOW_OBJECT).
+#if defined(KVH_KV4_OBJECT) && defined(KVH_WINDOW_OBJECT)
+int launch_paged_attention_kv4_window(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q,
+                                      hipStream_t s, LaunchLog& log) {
+  return launch_mfma_kv<kKv4, true>(p, plan, D, dtype, max_q, s, log);
+}
+#elif defined(KVH_KV4_OBJECT)
 int launch_paged_attention_kv4(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
                                LaunchLog& log) {
-  return launch_mfma_kv<kKv4>(p, plan, D, dtype, max_q, s, log);
+  return launch_mfma_kv<kKv4, false>(p, plan, D, dtype, max_q, s, log);
+}
+#elif defined(KVH_WINDOW_OBJECT)
+int launch_paged_attention_window(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t kv, int32_t max_q,
+                                  hipStream_t s, LaunchLog& log) {
+  if (kv == kKv4) return launch_paged_attention_kv4_window(p, plan, D, dtype, max_q, s, log);
+  return kv == kKv8 ? launch_mfma_kv<kKv8, true>(p, plan, D, dtype, max_q, s, log)
+                    : launch_mfma_kv<kKv16, true>(p, plan, D, dtype, max_q, s, log);
 }
 #else
 int launch_paged_attention_mfma(PAParams& p, const Plan& plan, int32_t D, int32_t dtype, int32_t kv, int32_t max_q,
                                 hipStream_t s, LaunchLog& log) {
+  if (p.WND > 0) return launch_paged_attention_window(p, plan, D, dtype, kv, max_q, s, log);
   if (kv == kKv4) return launch_paged_attention_kv4(p, plan, D, dtype, max_q, s, log);
-  return kv == kKv8 ? launch_mfma_kv<kKv8>(p, plan, D, dtype, max_q, s, log)
-                    : launch_mfma_kv<kKv16>(p, plan, D, dtype, max_q, s, log);
+  return kv == kKv8 ? launch_mfma_kv<kKv8, false>(p, plan, D, dtype, max_q, s, log)
+                    : launch_mfma_kv<kKv16, false>(p, plan, D, dtype, max_q, s, log);
 }
 #endif
 

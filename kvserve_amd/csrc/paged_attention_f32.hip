@@ -42,7 +42,8 @@ struct Half16 {
   }
 };
 
-template <class S, int DPL>  // d columns per lane: d = lane + 64 * x, x < DPL
+// WIN: a sliding window with sinks (PAParams::WND, SNK): tiles between the two are passed over.
+template <class S, int DPL, bool WIN>  // d columns per lane: d = lane + 64 * x, x < DPL
 __global__ __launch_bounds__(64) void pa_valu_kernel(PAParams p, int D) {
   const int seq = blockIdx.x, head = blockIdx.y;
   const int lane = threadIdx.x;
@@ -69,11 +70,13 @@ __global__ __launch_bounds__(64) void pa_valu_kernel(PAParams p, int D) {
 #pragma unroll
     for (int x = 0; x < DPL; ++x) acc[x] = 0.f;
 
+    const int from = WIN ? limit - p.WND : 0;  // the window's first key
     for (int k0 = 0; k0 < limit; k0 += 64) {
+      if (WIN && k0 >= p.SNK && k0 < from / 64 * 64) k0 = from / 64 * 64;
       const int key = k0 + lane;
       float s = -INFINITY;
       int64_t vbase = -1;
-      if (key < limit) {
+      if (key < limit && (!WIN || key >= from || key < p.SNK)) {
         const int64_t blk = btrow[key / p.BS];
         if (blk >= 0 && blk < p.num_blocks) {
           const int64_t slot = key % p.BS;
@@ -126,27 +129,28 @@ __global__ __launch_bounds__(64) void pa_valu_kernel(PAParams p, int D) {
   }
 }
 
-template <class S>
+template <class S, bool WIN>
 static int launch_valu(const PAParams& p, int32_t D, int32_t max_q, hipStream_t s) {
   dim3 grid(p.B, p.H, (max_q + kRowsPerWG - 1) / kRowsPerWG);
   if (D <= 64)
-    hipLaunchKernelGGL((pa_valu_kernel<S, 1>), grid, dim3(64), 0, s, p, D);
+    hipLaunchKernelGGL((pa_valu_kernel<S, 1, WIN>), grid, dim3(64), 0, s, p, D);
   else if (D <= 128)
-    hipLaunchKernelGGL((pa_valu_kernel<S, 2>), grid, dim3(64), 0, s, p, D);
+    hipLaunchKernelGGL((pa_valu_kernel<S, 2, WIN>), grid, dim3(64), 0, s, p, D);
   else
-    hipLaunchKernelGGL((pa_valu_kernel<S, 4>), grid, dim3(64), 0, s, p, D);
+    hipLaunchKernelGGL((pa_valu_kernel<S, 4, WIN>), grid, dim3(64), 0, s, p, D);
   return (int)hipGetLastError();
 }
 
 int launch_paged_attention_valu(const PAParams& p, int32_t D, int32_t dtype, int32_t max_q, hipStream_t s,
                                 LaunchLog& log) {
   int err;
+  const bool win = p.WND > 0;
   if (dtype == 0)
-    err = launch_valu<F32>(p, D, max_q, s);
+    err = win ? launch_valu<F32, true>(p, D, max_q, s) : launch_valu<F32, false>(p, D, max_q, s);
   else if (dtype == 1)
-    err = launch_valu<Half16<kvh::F16>>(p, D, max_q, s);
+    err = win ? launch_valu<Half16<kvh::F16>, true>(p, D, max_q, s) : launch_valu<Half16<kvh::F16>, false>(p, D, max_q, s);
   else
-    err = launch_valu<Half16<BF16>>(p, D, max_q, s);
+    err = win ? launch_valu<Half16<BF16>, true>(p, D, max_q, s) : launch_valu<Half16<BF16>, false>(p, D, max_q, s);
   if (!err) log.after_launch(dtype == 0 ? KVH_KERNEL_F32 : KVH_KERNEL_VALU16, s);
   return err;
 }

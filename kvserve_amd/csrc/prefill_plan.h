@@ -102,4 +102,43 @@ KVH_PLAN_FN int64_t pre_prefix(const PreSeq& s, int G, int PR, int step, int t) 
   return n;
 }
 
+// A sliding window of WND keys with SNK sinks leaves out, behind the sinks' chunks, the chunks of tile t that end
+// before its first row's window. (A tile's last row sees more than its first row's window skips: it keeps a chunk.)
+KVH_PLAN_FN int pre_tile_skip(const PreSeq& s, int G, int PR, int WND, int SNK, int t) {
+  int64_t lim = s.ctx + (int64_t)PR * t / G + 1;
+  lim = lim < 0 ? 0 : (lim > s.kv_total ? s.kv_total : lim);
+  const int64_t from = lim - WND, c = from / kPlanChunk - (SNK + kPlanChunk - 1) / kPlanChunk;
+  return from > 0 && c > 0 ? (int)c : 0;
+}
+
+// The chunks that tiles 0 .. t - 1 leave out. With no clamped length tile i's are floor((A G + PR i) / (32 G)) where
+// that is positive, A = ctx + 1 - WND - 32 ceil(SNK / 32): from the first tile i0 that leaves one out, the quotients of
+// tiles a period apart (at most G tiles, as in pre_prefix) differ by a constant.
+KVH_PLAN_FN int64_t pre_skips(const PreSeq& s, int G, int PR, int WND, int SNK, int t) {
+  int64_t n = 0;
+  if (s.ctx < 0 || s.ctx + s.q_len != s.kv_total) {
+    for (int i = 0; i < t; ++i) n += pre_tile_skip(s, G, PR, WND, SNK, i);
+    return n;
+  }
+  const int M = kPlanChunk * G;
+  int64_t b = (s.ctx + 1 - WND - (int64_t)(SNK + kPlanChunk - 1) / kPlanChunk * kPlanChunk) * G;
+  const int64_t i0 = b >= M ? 0 : (M - b + PR - 1) / PR;
+  if (i0 >= t) return 0;
+  b += PR * i0;
+  const int tiles = t - (int)i0, g = pre_gcd(PR, M), period = M / g, per = PR / g;
+  int64_t q = b / M;
+  int rem = (int)(b % M);
+  for (int r = 0; r < period && r < tiles; ++r) {  // tiles i0 + r, i0 + r + period, ...
+    const int64_t m = (tiles - r + period - 1) / period;
+    n += m * q + per * (m * (m - 1) / 2);
+    q += PR / M;
+    rem += PR % M;
+    if (rem >= M) {
+      rem -= M;
+      ++q;
+    }
+  }
+  return n;
+}
+
 }  // namespace kvh
