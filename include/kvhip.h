@@ -203,6 +203,32 @@ KVH_API int kvh_rope_and_cache_fp4(const void* qkv, int64_t qkv_tok_stride, cons
                            int32_t dtype, void* stream);
 
 /*
+ * norm_rope_and_cache: rope_and_cache for models whose query and key heads are normed, or rotated in part or in
+ * neighbouring pairs, into a cache of any format. For every query and key head x of token t, p = positions[t] (clamped
+ * to the tables),
+ *   y = x * rsqrt(mean(x^2) + eps) * w          w = q_norm or k_norm [head_dim], of dtype; NULL: y = x
+ *   y_a' = y_a cos[p, i] - y_b sin[p, i],  y_b' = y_b cos[p, i] + y_a sin[p, i]    i < rotary_dim / 2
+ * with (a, b) = (i, i + rotary_dim / 2), or (2i, 2i + 1) where `interleaved`; elements from rotary_dim on are not rotated.
+ * cos_table / sin_table: fp32 [max_positions, rotary_dim / 2], one entry for each pair (frequencies and factors of
+ * stretched contexts are the tables'); unused with rotary_dim = 0. The queries are written to q_out, the keys and the
+ * (untouched) values to the pool at slot_mapping[t] (slots outside the pool are skipped). Computed in fp32 and rounded
+ * once: the queries to dtype, the keys to the cache's format.
+ * cache_format and scales as in kvh_paged_attention_window. head_dim a multiple of 8 (MXFP4: of 32) up to 256, rotary_dim
+ * a multiple of 16 up to head_dim; pointers 16-byte aligned (E4M3 caches 8, MXFP4 ones 4) and rows' strides likewise.
+ */
+KVH_API int kvh_norm_rope_and_cache(const void* qkv, int64_t qkv_tok_stride, const int64_t* positions,
+                            const float* cos_table, const float* sin_table, int64_t max_positions,
+                            int32_t rotary_dim, int32_t interleaved, const void* q_norm, const void* k_norm,
+                            float eps, void* q_out, int64_t q_tok_stride, int64_t q_head_stride,
+                            void* k_cache, const int64_t k_cache_strides[3],
+                            void* k_scales, const int64_t k_scales_strides[3],
+                            void* v_cache, const int64_t v_cache_strides[3],
+                            void* v_scales, const int64_t v_scales_strides[3],
+                            const int64_t* slot_mapping, int64_t num_tokens, int64_t num_blocks,
+                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                            int32_t cache_format, float k_scale, float v_scale, int32_t dtype, void* stream);
+
+/*
  * prepare_metadata: one step's attention metadata, built on the device from block tables that
  * stay resident in HBM. table_pool int64 [pool_rows, pool_row_stride] holds one row per live
  * sequence (its block table, first pool_width entries usable) and persists across calls; the

@@ -84,6 +84,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp,  # slots, sizes, dtype, stream
         ],  # fmt: skip
     ),
+    "kvh_norm_rope_and_cache": (
+        ctypes.c_int,
+        [
+            _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32,  # qkv, positions, cos/sin tables, rotary dim, interleaved
+            _vp, _vp, _f32,  # norms
+            _vp, _i64, _i64,  # q_out
+            _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p,  # caches, each with its scales
+            _vp, _i64, _i64, _i32, _i32, _i32, _i32,  # slots, sizes
+            _i32, _f32, _f32, _i32, _vp,  # cache format and scales, dtype, stream
+        ],  # fmt: skip
+    ),
     "kvh_gemv_rope_and_cache": (
         ctypes.c_int,
         [

@@ -530,6 +530,68 @@ class HipAttention:
         _lib.check(st, "kvh_rope_and_cache_fp8" if fp8 else "kvh_rope_and_cache")
         return out
 
+    @staticmethod
+    def norm_rope_and_cache(
+        qkv: torch.Tensor,
+        positions: torch.Tensor,
+        cos: torch.Tensor,
+        sin: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        slots: torch.Tensor,
+        num_heads: int,
+        q_norm: torch.Tensor | None = None,
+        k_norm: torch.Tensor | None = None,
+        eps: float = 1e-6,
+        interleaved: bool = False,
+        out: torch.Tensor | None = None,
+        k_scale: float = 1.0,
+        v_scale: float = 1.0,
+    ) -> torch.Tensor:
+        """rope_and_cache for models whose heads are normed, or rotated in part or in neighbouring pairs, into a cache of
+        any format (kvh_norm_rope_and_cache).
+
+        qkv: [T, (num_heads + 2 kv_heads) head_dim]; q_norm, k_norm: the RMS norms' weights [head_dim] of qkv's dtype
+        (None: no norm); cos, sin: fp32 [max_positions, rotary_dim / 2], one entry for each pair of the first rotary_dim
+        elements of a head: (i, i + rotary_dim / 2), or (2i, 2i + 1) where `interleaved`. Norm, rotation and their
+        products are fp32, rounded once: the queries, returned as [T, num_heads, head_dim] (in `out` if given), to qkv's
+        dtype, the keys to the cache's format. Scales and slots as write_kv."""
+        num_blocks, block_size, num_kv_heads, head_dim, dev, fmt, ks, vs, caches = _cache_args(k_cache, v_cache, k_scale,
+                                                                                               v_scale)  # fmt: skip
+        _on_device(dev, qkv=qkv, positions=positions, cos=cos, sin=sin, slot_mapping=slots)
+        _require(qkv.dim() == 2 and qkv.stride(-1) == 1, "qkv must be [T, (H + 2 Hkv) D] with a contiguous last dim")
+        _require(num_heads > 0 and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim, "qkv width != (H + 2 Hkv) D")
+        _require(cos.dtype == torch.float32 and sin.dtype == torch.float32, "cos/sin tables must be fp32")
+        _require(cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous(),
+                 "cos/sin must be contiguous [P, rotary_dim / 2]")  # fmt: skip
+        _require(2 * cos.shape[1] <= head_dim and cos.shape[1] % 8 == 0, f"rotary_dim must be a multiple of 16 up to {head_dim}")
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                _on_device(dev, **{name: w})
+                _require(w.shape == (head_dim,) and w.is_contiguous() and w.dtype == qkv.dtype,
+                         f"{name} must be [head_dim] of qkv's dtype")  # fmt: skip
+        _check_index(positions, "positions", 1)
+        _check_index(slots, "slot_mapping", 1)
+        num_tokens = qkv.shape[0]
+        _require(positions.shape[0] == num_tokens and slots.shape[0] == num_tokens, "one position and slot per token")
+        if out is None:
+            out = torch.empty((num_tokens, num_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+        _on_device(dev, out=out)
+        _require(out.shape == (num_tokens, num_heads, head_dim) and out.stride(-1) == 1, "out must be [T, H, D]")
+        dtype = _dtype_code(qkv, k_cache, v_cache, out) if fmt == _CACHE_DTYPE else _dtype_code(qkv, out)
+        if num_tokens == 0:
+            return out
+        with _current(dev):
+            st = _lib.load().kvh_norm_rope_and_cache(
+                qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                2 * cos.shape[1], int(interleaved), q_norm.data_ptr() if q_norm is not None else None,
+                k_norm.data_ptr() if k_norm is not None else None, float(eps), out.data_ptr(), out.stride(0), out.stride(1),
+                *caches, slots.data_ptr(), num_tokens, num_blocks, num_heads, num_kv_heads, head_dim, block_size, fmt, ks, vs,
+                dtype, _stream_handle(qkv.device),
+            )  # fmt: skip
+        _lib.check(st, "kvh_norm_rope_and_cache")
+        return out
+
     # rows up to which gemv_rope_and_cache applies (up to 4 on the GEMV, then on the MFMA units)
     GEMV_ROPE_MAX_ROWS = 64
 

@@ -37,6 +37,7 @@ SOURCES = [
     "kvh_api.hip",
     "logprobs.hip",
     "metadata.hip",
+    "norm_rope.hip",
     "paged_attention.hip",
     "paged_attention_f32.hip",
     "paged_attention_kv4.hip",

@@ -378,6 +378,76 @@ int kvh_rope_and_cache_fp8(const void* qkv, int64_t qkv_tok_stride, const int64_
                              dtype, true, k_scale, v_scale, stream);
 }
 
+int kvh_norm_rope_and_cache(const void* qkv, int64_t qkv_tok_stride, const int64_t* positions, const float* cos_table,
+                            const float* sin_table, int64_t max_positions, int32_t rotary_dim, int32_t interleaved,
+                            const void* q_norm, const void* k_norm, float eps, void* q_out, int64_t q_tok_stride,
+                            int64_t q_head_stride, void* k_cache, const int64_t k_cache_strides[3], void* k_scales,
+                            const int64_t k_scales_strides[3], void* v_cache, const int64_t v_cache_strides[3],
+                            void* v_scales, const int64_t v_scales_strides[3], const int64_t* slot_mapping,
+                            int64_t num_tokens, int64_t num_blocks, int32_t num_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t cache_format, float k_scale, float v_scale,
+                            int32_t dtype, void* stream) {
+  if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
+  if (cache_format < KVH_CACHE_DTYPE || cache_format > KVH_CACHE_MXFP4) return KVH_E_DTYPE;
+  const bool fp8 = cache_format == KVH_CACHE_E4M3, fp4 = cache_format == KVH_CACHE_MXFP4;
+  if (fp8 && !(k_scale > 0.f && k_scale < INFINITY && v_scale > 0.f && v_scale < INFINITY)) return KVH_E_SHAPE;
+  if (num_tokens < 0 || num_blocks < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
+      max_positions <= 0 || rotary_dim < 0 || rotary_dim > head_dim || !(eps >= 0.f))
+    return KVH_E_SHAPE;
+  if (num_tokens > kMaxWorkgroups256 || num_blocks > INT64_MAX / block_size) return KVH_E_SHAPE;
+  if (num_heads > 65535 || num_kv_heads > 65535 || head_dim > 256 || head_dim % (fp4 ? kFp4Block : 8) != 0 ||
+      rotary_dim % 16 != 0)
+    return KVH_E_UNSUPPORTED;
+  if (num_tokens == 0) return KVH_OK;
+  if (!positions || !slot_mapping || (rotary_dim > 0 && (!cos_table || !sin_table)) || !k_cache || !v_cache ||
+      !k_cache_strides || !v_cache_strides)
+    return KVH_E_NULL;
+  int st = check_fp4_tensor(qkv, qkv_tok_stride, 0, dtype);
+  if (st == KVH_OK) st = check_fp4_tensor(q_out, q_tok_stride, q_head_stride, dtype);
+  if (st != KVH_OK) return st;
+  if (qkv_tok_stride < ((int64_t)num_heads + 2 * (int64_t)num_kv_heads) * head_dim) return KVH_E_SHAPE;
+  if (((uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)q_norm | (uintptr_t)k_norm) & 15u) return KVH_E_ALIGN;
+  NormRopeArgs a{};
+  if (fp4) {
+    st = fp4_caches(head_dim, block_size, k_cache, k_cache_strides, k_scales, k_scales_strides, v_cache,
+                    v_cache_strides, v_scales, v_scales_strides, false, &a.kc, &a.vc);
+    if (st != KVH_OK) return st;
+  } else {
+    // granules of 8 elements: 8 bytes of an E4M3 row, else 16-byte vectors
+    const int vec = fp8 ? 8 : 16 / elem_bytes(dtype);
+    for (const int64_t* strides : {k_cache_strides, v_cache_strides})
+      for (int i = 0; i < 3; ++i) {
+        if (strides[i] < 0) return KVH_E_SHAPE;
+        if (strides[i] % vec) return KVH_E_ALIGN;
+      }
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache) & (uintptr_t)(fp8 ? 7 : 15)) return KVH_E_ALIGN;
+    a.kc = Fp4Cache{(uint8_t*)k_cache, k_cache_strides[0], k_cache_strides[1], k_cache_strides[2], nullptr, 0, 0, 0};
+    a.vc = Fp4Cache{(uint8_t*)v_cache, v_cache_strides[0], v_cache_strides[1], v_cache_strides[2], nullptr, 0, 0, 0};
+  }
+  a.qkv = (const uint8_t*)qkv;
+  a.qkv_ts = qkv_tok_stride;
+  a.positions = positions;
+  a.cos_t = cos_table;
+  a.sin_t = sin_table;
+  a.max_pos = max_positions;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.q_out = (uint8_t*)q_out;
+  a.q_ts = q_tok_stride;
+  a.q_hs = q_head_stride;
+  a.slots = slot_mapping;
+  a.num_slots = num_blocks * block_size;
+  a.H = num_heads;
+  a.Hkv = num_kv_heads;
+  a.D = head_dim;
+  a.R = rotary_dim;
+  a.BS = block_size;
+  a.eps = eps;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  return launch_norm_rope(a, num_tokens, cache_format, interleaved != 0, dtype, (hipStream_t)stream);
+}
+
 int kvh_prepare_metadata(const int32_t* packed, int32_t num_seqs, int32_t num_pad_seqs, int32_t num_updates,
                          int64_t num_tokens, int64_t* table_pool, int32_t pool_rows, int64_t pool_row_stride,
                          int32_t pool_width, int64_t* block_tables, int64_t bt_row_stride, int32_t bt_width,

@@ -229,6 +229,24 @@ struct Fp4Cache {
   uint8_t* x;
   int64_t xsb, xss, xsh;
 };
+// norm_rope_and_cache (norm_rope.hip). Strides in elements, the caches' as in Fp4Cache (x: MXFP4 alone).
+struct NormRopeArgs {
+  const uint8_t* qkv;
+  int64_t qkv_ts;
+  const int64_t* positions;
+  const float *cos_t, *sin_t;  // [max_pos, R / 2]
+  int64_t max_pos;
+  const void *q_norm, *k_norm;  // [D] or null
+  uint8_t* q_out;
+  int64_t q_ts, q_hs;
+  Fp4Cache kc, vc;
+  const int64_t* slots;
+  int64_t num_slots;
+  int32_t H, Hkv, D, R, BS;
+  int32_t hpw;  // heads of a workgroup (set by the launcher)
+  float eps, k_scale, v_scale;
+};
+int launch_norm_rope(const NormRopeArgs& a, int64_t T, int32_t cache, bool pairs, int32_t dtype, hipStream_t s);
 int launch_reshape_and_cache_fp4(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
                                  const Fp4Cache& kc, const Fp4Cache& vc, const int64_t* slots, int64_t T,
                                  int64_t num_blocks, int32_t Hkv, int32_t D, int32_t BS, int32_t dtype, hipStream_t s);
