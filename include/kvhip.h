@@ -467,6 +467,22 @@ KVH_API int kvh_gemv_silu_mul(const void* x, int64_t x_row_stride, const void* w
                               void* stream);
 
 /*
+ * linear4: y = x W^T with a weight held in 4 bits, W[r][c] = s[r][c / group] (q[r][c] - z[r][c / group]), codes q and zero points
+ * z in 0 .. 15; x [m, k] and y [m, n] fp16 or bf16 (dtype), the scales of that type, sums in fp32, rounded once. Any m;
+ * group 32, 64 or 128, k a multiple of it. silu_mul: the rows of W are n / 2 gate rows, then as many up rows (n % 32 == 0), and
+ *   y[i][j] = silu(g) * u, g and u the products with rows j and n / 2 + j, rounded once; y is [m, n / 2].
+ * The weight is packed once (all sizes rounded up, little endian):
+ *   codes  [n / 16][k / 128][4 j][16 r][4 u] dwords: row r of the tile, elements 32 u + 8 j + i of the block, i = 2 p in
+ *          bits 4 p .. + 3 and i = 2 p + 1 in bits 16 + 4 p .. + 3
+ *   scales [n / 16][k / 128][128 / group][16 r] dwords: s in the low half and 16 + z in the high half, both as dtype; 0 past k
+ * x, codes and scales 16-byte aligned, x_row_stride a multiple of 8. An infinity in a row of x makes that row of y NaN. The
+ * reference has no 4-bit weights.
+ */
+KVH_API int kvh_linear4(const void* x, int64_t x_row_stride, const void* codes, const void* scales, void* y,
+                        int64_t y_row_stride, int64_t m, int32_t n, int32_t k, int32_t group, int32_t silu_mul,
+                        int32_t dtype, void* stream);
+
+/*
  * token_logprobs: for each of num_rows rows of logits [num_rows, vocab] (fp32, fp16 or bf16, row stride
  * in elements) and its given token,
  *   logprobs[r] = log softmax(logits[r])[tokens[r]]     NaN for a token outside [0, vocab)

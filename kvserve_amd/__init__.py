@@ -22,12 +22,14 @@ from kvserve_amd.attention import (
     last_launch_kernels,
     last_launches,
 )
+from kvserve_amd.linear4 import Weight4, linear4, linear4_silu_mul, quantize_weight4
 from kvserve_amd.logprobs import TokenLogprobs, token_logprobs
 
 __all__ = [
     "AttentionMetadata",
     "HipAttention",
     "TokenLogprobs",
+    "Weight4",
     "build_metadata",
     "fp4_caches",
     "get_backend",
@@ -35,5 +37,8 @@ __all__ = [
     "hip_eligible",
     "last_launch_kernels",
     "last_launches",
+    "linear4",
+    "linear4_silu_mul",
+    "quantize_weight4",
     "token_logprobs",
 ]

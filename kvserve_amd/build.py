@@ -35,6 +35,7 @@ SOURCES = [
     "cache_fp4.hip",
     "engine_ops.hip",
     "kvh_api.hip",
+    "linear4.hip",
     "logprobs.hip",
     "metadata.hip",
     "norm_rope.hip",

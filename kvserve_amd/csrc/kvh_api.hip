@@ -937,6 +937,36 @@ int kvh_gemm_skinny_silu_mul(const void* x, int64_t x_row_stride, const void* w_
                             (hipStream_t)stream);
 }
 
+int kvh_linear4(const void* x, int64_t x_row_stride, const void* codes, const void* scales, void* y,
+                int64_t y_row_stride, int64_t m, int32_t n, int32_t k, int32_t group, int32_t silu_mul, int32_t dtype,
+                void* stream) {
+  if (dtype != KVH_DTYPE_F16 && dtype != KVH_DTYPE_BF16) return KVH_E_DTYPE;
+  if (m < 0 || n < 0 || k <= 0) return KVH_E_SHAPE;
+  if (group != 32 && group != 64 && group != 128) return KVH_E_UNSUPPORTED;
+  // rows of x in 31 bits and 65535 workgroups; rows of the weight in tiles of 16 (each half of a gated one)
+  if (k % group != 0 || m > 16 * 65535 || n > 0x7fffff00 || k > 0x7fffff00 || (silu_mul && n % 32 != 0))
+    return KVH_E_UNSUPPORTED;
+  if (m == 0 || n == 0) return KVH_OK;
+  if (!x || !codes || !scales || !y) return KVH_E_NULL;
+  const int32_t cols = silu_mul ? n / 2 : n;
+  if (x_row_stride < k || y_row_stride < cols) return KVH_E_SHAPE;
+  if (x_row_stride % 8 || !a16(x) || !a16(codes) || !a16(scales) || ((uintptr_t)y & 1u)) return KVH_E_ALIGN;
+  Linear4Args a{};
+  a.x = (const uint16_t*)x;
+  a.x_rs = x_row_stride;
+  a.codes = (const uint8_t*)codes;
+  a.scales = (const uint32_t*)scales;
+  a.y = (uint16_t*)y;
+  a.y_rs = y_row_stride;
+  a.m = (int32_t)m;
+  a.n = cols;
+  a.k = k;
+  a.tiles = (n + 15) / 16;
+  a.blocks = (k + 127) / 128;
+  a.vec = y_row_stride % 4 == 0 && ((uintptr_t)y & 7u) == 0;
+  return launch_linear4(a, group, silu_mul != 0, dtype, (hipStream_t)stream);
+}
+
 static int check_logprobs(int64_t rows, int32_t vocab, int32_t top, int32_t dtype) {
   if (dtype < KVH_DTYPE_F32 || dtype > KVH_DTYPE_BF16) return KVH_E_DTYPE;
   if (rows < 0 || vocab <= 0 || top < 0 || top > vocab) return KVH_E_SHAPE;

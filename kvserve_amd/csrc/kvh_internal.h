@@ -199,6 +199,20 @@ int launch_gemm_skinny(const void* x, int64_t x_rs, const void* w, int64_t w_rs,
 int launch_gemv_silu_mul(const void* x, int64_t x_rs, const void* w, int64_t w_rs, void* y, int64_t y_rs, int32_t m,
                          int32_t inter, int32_t k, int32_t dtype, hipStream_t s);
 
+// Products with 4-bit weights (linear4.hip): rows of y are n wide, the weight has `tiles` tiles of 16 rows (GLU: half of them
+// gate rows, then up rows) of `blocks` blocks of 128 k.
+struct Linear4Args {
+  const uint16_t* x;
+  int64_t x_rs;
+  const uint8_t* codes;
+  const uint32_t* scales;
+  uint16_t* y;
+  int64_t y_rs;
+  int32_t m, n, k, tiles, blocks;
+  bool vec;  // rows of y 8-byte aligned
+};
+int launch_linear4(const Linear4Args& a, int32_t group, bool glu, int32_t dtype, hipStream_t s);
+
 // Workgroups of 256 threads of a launch: its threads are counted in 32 bits.
 constexpr int64_t kMaxWorkgroups256 = 0xffffffffLL / 256;
 
