@@ -186,9 +186,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kvh_gemm_skinny": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
     "kvh_gemm_skinny_silu_mul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
     "kvh_gemv_silu_mul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "kvh_linear4_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
     "kvh_linear4": (
         ctypes.c_int,
-        [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp],
+        [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp],
     ),
     "kvh_token_logprobs_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
     "kvh_token_logprobs": (

@@ -937,20 +937,34 @@ int kvh_gemm_skinny_silu_mul(const void* x, int64_t x_row_stride, const void* w_
                             (hipStream_t)stream);
 }
 
-int kvh_linear4(const void* x, int64_t x_row_stride, const void* codes, const void* scales, void* y,
-                int64_t y_row_stride, int64_t m, int32_t n, int32_t k, int32_t group, int32_t silu_mul, int32_t dtype,
-                void* stream) {
+static int check_linear4(int64_t m, int32_t n, int32_t k, int32_t group, int32_t silu_mul, int32_t dtype) {
   if (dtype != KVH_DTYPE_F16 && dtype != KVH_DTYPE_BF16) return KVH_E_DTYPE;
   if (m < 0 || n < 0 || k <= 0) return KVH_E_SHAPE;
   if (group != 32 && group != 64 && group != 128) return KVH_E_UNSUPPORTED;
-  // rows of x in 31 bits and 65535 workgroups; rows of the weight in tiles of 16 (each half of a gated one)
-  if (k % group != 0 || m > 16 * 65535 || n > 0x7fffff00 || k > 0x7fffff00 || (silu_mul && n % 32 != 0))
+  // rows of x in 65535 workgroups of 16 or more; rows of the weight in tiles of 16 (each half of a gated one); columns,
+  // rounded up to a few blocks, in 31 bits
+  if (k % group != 0 || m > 16 * 65535 || n > 0x7fffff00 || k > 0x3fffff00 || (silu_mul && n % 32 != 0))
     return KVH_E_UNSUPPORTED;
+  return KVH_OK;
+}
+
+size_t kvh_linear4_workspace_size(int64_t m, int32_t n, int32_t k, int32_t silu_mul) {
+  if (check_linear4(m, n, 32, 32, silu_mul, KVH_DTYPE_BF16) != KVH_OK || k <= 0 || k > 0x3fffff00 || m == 0 || n == 0) return 0;
+  return linear4_workspace(m, (n + 15) / 16, (k + 127) / 128, silu_mul != 0);
+}
+
+int kvh_linear4(const void* x, int64_t x_row_stride, const void* codes, const void* scales, void* y,
+                int64_t y_row_stride, int64_t m, int32_t n, int32_t k, int32_t group, int32_t silu_mul, int32_t dtype,
+                void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_linear4(m, n, k, group, silu_mul, dtype);
+  if (st != KVH_OK) return st;
   if (m == 0 || n == 0) return KVH_OK;
   if (!x || !codes || !scales || !y) return KVH_E_NULL;
   const int32_t cols = silu_mul ? n / 2 : n;
   if (x_row_stride < k || y_row_stride < cols) return KVH_E_SHAPE;
   if (x_row_stride % 8 || !a16(x) || !a16(codes) || !a16(scales) || ((uintptr_t)y & 1u)) return KVH_E_ALIGN;
+  const size_t need = kvh_linear4_workspace_size(m, n, k, silu_mul);
+  if (need > 0 && (!workspace || workspace_bytes < need || !a16(workspace))) return KVH_E_WORKSPACE;
   Linear4Args a{};
   a.x = (const uint16_t*)x;
   a.x_rs = x_row_stride;
@@ -964,6 +978,7 @@ int kvh_linear4(const void* x, int64_t x_row_stride, const void* codes, const vo
   a.tiles = (n + 15) / 16;
   a.blocks = (k + 127) / 128;
   a.vec = y_row_stride % 4 == 0 && ((uintptr_t)y & 7u) == 0;
+  a.ws = (float*)workspace;
   return launch_linear4(a, group, silu_mul != 0, dtype, (hipStream_t)stream);
 }
 

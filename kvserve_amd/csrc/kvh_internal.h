@@ -210,7 +210,10 @@ struct Linear4Args {
   int64_t y_rs;
   int32_t m, n, k, tiles, blocks;
   bool vec;  // rows of y 8-byte aligned
+  float* ws;  // [splits, m, tiles, 16] sums of splits of k
+  int32_t splits;  // set by the launcher
 };
+size_t linear4_workspace(int64_t m, int32_t tiles, int32_t blocks, bool glu);
 int launch_linear4(const Linear4Args& a, int32_t group, bool glu, int32_t dtype, hipStream_t s);
 
 // Workgroups of 256 threads of a launch: its threads are counted in 32 bits.

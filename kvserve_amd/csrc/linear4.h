@@ -1,21 +1,66 @@
-// How a product with a 4-bit weight is cut (linear4.hip): plain functions of its shape, also compiled for the host.
+// How a product with a 4-bit weight is cut (linear4.hip): plain functions of its shape, also compiled for the host by the
+// test that holds them to their limits.
 #pragma once
 #include <stdint.h>
 
 namespace kvh {
 
-constexpr int kW4Rows = 16, kW4Block = 128;  // weight rows and k of a packed block
+constexpr int kW4Block = 128;  // k of a packed block
 
-// Rows of x (in 16s) and weight tiles a wave holds, and the waves that share a tile's k.
+// A workgroup multiplies `rows` rows of x with wr groups of rt weight tiles; wk waves share a group's k, each s blocks of
+// every chunk of wk s blocks; `splits` workgroups share the chunks.
 struct Linear4Form {
-  int mt, rt, wk;
+  int rows, rt, wr, wk, s;
+  int splits;
 };
 
-inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m) {
+constexpr int linear4_chunk(const Linear4Form& f) { return f.wk * f.s; }
+// LDS of a workgroup: two chunks of x, or the waves' sums
+constexpr int linear4_lds(const Linear4Form& f) {
+  const int x = 2 * f.wk * f.s * f.rows * 2 * kW4Block, sums = f.wr * f.wk * f.rt * ((f.rows + 15) / 16) * 1024;
+  return x > sums ? x : sums;
+}
+
+// Times in us of (m rows of x; rows x columns of the weight), bf16, groups of 128, weights not in the caches; g: gated.
+//  * Up to 16 rows of x: one tile a group as long as the tiles fit the CUs once ((1; 4096 x 4096) 5.2, with two tiles a wave
+//    6.4), in sixteen slices of a long k ((8; 4096 x 14336) 10.9, in eight 11.8); two tiles behind that ((16; 6144 x 4096)
+//    7.1, one 10.5), and two groups, which share x ((16; 9216 x 4096) 8.6; (8; 12288 x 4096) 8.6, one group 11.9), or four
+//    where two would load the CUs unevenly ((g 8; 28672 x 4096) 14.4 and 15.1; but (8; 32768 x 4096) 17.9 and 15.5).
+//  * Up to 32 rows likewise ((20; 4096 x 4096) 8.1, in four splits 8.9; (32; 6144 x 4096) 9.6, 10.7; (g 24; 16384 x 2048)
+//    8.6, four groups 11.5), then eight tiles in two groups for one round of workgroups, in four for more ((g 32; 28672 x
+//    4096) 19.6 and 21.4; (32; 128256 x 2048) 46.6 and 39.9).
+//  * More rows: x is as many bytes as the weight, so groups of 128 weight rows share it, and what that leaves of the CUs is
+//    filled by splitting k, four chunks at least each: (33; 2048 x 8192) 13.2 in eight splits, 14.1 in sixteen;
+//    (64; 4096 x 14336) 23.3 in eight, 25.6 in six; (100; 4096 x 4096) 16.5 in four, 19.7 in two.
+//  * Past 64 rows of x the MFMAs and the codes' conversion bound it, which add up on this GPU: 256 weight rows and 64 of x
+//    a workgroup where they fill it ((500; 6144 x 4096) 41.7, 128 rows 58.8; but (g 100; 16384 x 2048) 23.3 and 18.8).
+inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m, bool glu) {
+  if (m <= 16) {
+    if (tiles <= 256 && !glu) {
+      if (m > 8) return {16, 1, 1, 8, 2, 1};
+      return blocks < 48 ? Linear4Form{8, 1, 1, 8, 2, 1} : Linear4Form{8, 1, 1, 16, 2, 1};
+    }
+    if (tiles < 768 && !glu) return {16, 2, 1, 8, 2, 1};
+    return tiles > 1024 && tiles <= 1792 ? Linear4Form{16, 2, 4, 4, 2, 1} : Linear4Form{16, 2, 2, 4, 2, 1};
+  }
   Linear4Form f;
-  f.mt = m > 48 ? 4 : (int)((m + 15) / 16);
-  f.rt = f.mt >= 3 || tiles >= 1024 ? 2 : 1;
-  f.wk = blocks >= 16 && tiles / f.rt < 1024 ? 8 : 4;
+  if (m <= 32) {
+    if (tiles < 512 && blocks < 48 && !glu)
+      return tiles <= 256 ? Linear4Form{32, 1, 1, 8, 1, 1} : Linear4Form{32, 1, 2, 8, 1, 1};
+    if (tiles >= 512 && tiles < 1536) return {32, 2, 2, 4, 2, 1};
+    if (tiles >= 1536 && tiles <= 2048) return {32, 4, 2, 4, 1, 1};
+    f = {32, 2, 4, 2, 1, 1};
+  } else if (m <= 48) {
+    if (tiles >= 1536) return {48, 4, 2, 4, 1, 1};
+    f = {48, 2, 4, 2, 1, 1};
+  } else if (m > 64 && (tiles + 15) / 16 * ((m + 63) / 64) >= 150) {
+    return {64, 4, 4, 2, 1, 1};
+  } else {
+    f = {64, 2, 4, 2, 1, 1};
+  }
+  const int64_t groups = (tiles + 7) / 8 * ((m + 63) / 64), most = (blocks + f.wk - 1) / f.wk / 4;
+  const int64_t z = 256 / groups < most ? 256 / groups : most;
+  f.splits = z > 1 ? (int)z : 1;
   return f;
 }
 

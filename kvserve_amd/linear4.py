@@ -110,10 +110,13 @@ def _product(x: torch.Tensor, weight: Weight4, silu_mul: bool, out: torch.Tensor
         out = torch.empty((m, cols), dtype=x.dtype, device=x.device)
     _require(out.shape == (m, cols) and out.dtype == x.dtype and out.stride(-1) == 1 and out.device == x.device,
              f"out must be [{m}, {cols}] of x's dtype and device with a contiguous last dim")  # fmt: skip
+    lib = _lib.load()
+    need = lib.kvh_linear4_workspace_size(m, n, k, int(silu_mul))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with _current(x.get_device()):
-        st = _lib.load().kvh_linear4(x.data_ptr(), x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                     out.data_ptr(), out.stride(0), m, n, k, weight.group, int(silu_mul),
-                                     _lib.KVH_DTYPE[x.dtype], _stream_handle(x.device))  # fmt: skip
+        st = lib.kvh_linear4(x.data_ptr(), x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
+                             out.stride(0), m, n, k, weight.group, int(silu_mul), _lib.KVH_DTYPE[x.dtype],
+                             ws.data_ptr() if ws is not None else None, need, _stream_handle(x.device))  # fmt: skip
     _lib.check(st, "kvh_linear4")
     return out
 

@@ -2,6 +2,13 @@
 
 from __future__ import annotations
 
+import ctypes
+import random
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -67,11 +74,11 @@ def test_refusals():
 
 
 def _call(m=1, n=16, k=128, group=128, silu=0, dtype=2, xs=128, ys=16, x=None, y=None):
-    return _lib.load().kvh_linear4(x, xs, x, x, y, ys, m, n, k, group, silu, dtype, None)
+    return _lib.load().kvh_linear4(x, xs, x, x, y, ys, m, n, k, group, silu, dtype, None, 0, None)
 
 
 def test_refusals_of_the_c_abi():
-    null, shape, dtype, align, unsupported = -1, -2, -3, -4, -5
+    null, shape, dtype, align, unsupported, workspace = -1, -2, -3, -4, -5, -6
     assert _call() == null
     assert _call(m=0) == 0 and _call(n=0) == 0
     assert _call(dtype=0) == dtype and _call(dtype=3) == dtype
@@ -80,4 +87,69 @@ def test_refusals_of_the_c_abi():
     assert _call(silu=1) == unsupported and _call(n=0x7FFFFFFF) == unsupported
     # refused before anything is launched: addresses that are never read
     assert _call(x=16, y=16, xs=127) == shape and _call(x=16, y=16, ys=15) == shape
+    assert _call(x=16, y=16, m=64, n=1024, k=8192, xs=8192, ys=1024) == workspace
     assert _call(x=16, y=16, xs=132) == align and _call(x=24, y=16) == align and _call(x=16, y=17) == align
+
+
+CSRC = Path(__file__).resolve().parent.parent / "kvserve_amd/csrc"
+
+SOURCE = """
+#include "linear4.h"
+using namespace kvh;
+extern "C" int lds(int rows, int rt, int wr, int wk, int s) { return linear4_lds(Linear4Form{rows, rt, wr, wk, s, 1}); }
+extern "C" void form(int64_t tiles, int64_t blocks, int64_t m, int glu, int* o) {
+  const Linear4Form f = linear4_form(tiles, blocks, m, glu);
+  o[0] = f.rows, o[1] = f.rt, o[2] = f.wr, o[3] = f.wk, o[4] = f.s, o[5] = f.splits;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def forms(tmp_path_factory):
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no host C++ compiler")
+    d = tmp_path_factory.mktemp("forms")
+    (d / "forms.cpp").write_text(SOURCE)
+    subprocess.run([cxx, "-std=c++17", "-O1", "-shared", "-fPIC", f"-I{CSRC}", str(d / "forms.cpp"), "-o", str(d / "forms.so")],
+                   check=True)  # fmt: skip
+    lib = ctypes.CDLL(str(d / "forms.so"))
+    lib.form.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+    lib.form.restype = None
+
+    def form(tiles, blocks, m, glu=0):
+        o = (ctypes.c_int * 6)()
+        lib.form(tiles, blocks, m, glu, o)
+        return tuple(o)
+
+    form.lds = lib.lds
+    return form
+
+
+def test_every_form_is_built_and_reached(forms):
+    """The forms that the rule gives are those that the launcher has kernels of, within a workgroup's limits; a split has
+    four chunks at least, and the workspace covers them."""
+    src = (CSRC / "linear4.hip").read_text()
+    plain, both = re.search(r"if constexpr \(!GLU\) \{(.*?)\}(.*?)#undef", src, re.S).groups()
+    find = lambda t: {tuple(map(int, m)) for m in re.findall(r"KVH_FORM\((\d+), (\d+), (\d+), (\d+), (\d+)\)", t)}  # noqa: E731
+    built = {0: find(plain) | find(both), 1: find(both)}
+    assert built[1] and all(f[1] % 2 == 0 for f in built[1])
+    rng = random.Random(3)
+    span = lambda top: min(top, int(2 ** rng.uniform(0, top.bit_length())))  # noqa: E731
+    seen = {0: set(), 1: set()}
+    for _ in range(40000):
+        tiles, blocks, m, glu = span(10000), span(300), span(4000), rng.randint(0, 1)
+        if glu:
+            tiles += tiles % 2
+        *f, z = forms(tiles, blocks, m, glu)
+        f = tuple(f)
+        assert f in built[glu], (tiles, blocks, m, glu, f)
+        seen[glu].add(f)
+        rows, rt, wr, wk, s = f
+        assert rows >= min(m, 64) and 64 * wr * wk <= 1024 and forms.lds(*f) <= 160 * 1024
+        chunks = -(-blocks // (wk * s))
+        assert z == 1 or 4 * z <= chunks
+        assert -(-m // (16 * -(-rows // 16))) <= 65535 and z <= 65535
+        n, k = 16 * tiles, 128 * blocks
+        assert _lib.load().kvh_linear4_workspace_size(m, n, k, glu) == (z * m * tiles * 64 if z > 1 else 0)
+    assert seen == built
