@@ -468,8 +468,9 @@ KVH_API int kvh_gemv_silu_mul(const void* x, int64_t x_row_stride, const void* w
 
 /*
  * linear4: y = x W^T with a weight held in 4 bits, W[r][c] = s[r][c / group] (q[r][c] - z[r][c / group]), codes q and zero points
- * z in 0 .. 15; x [m, k] and y [m, n] fp16 or bf16 (dtype), the scales of that type, sums in fp32, rounded once. Any m;
- * group 32, 64 or 128, k a multiple of it. silu_mul: the rows of W are n / 2 gate rows, then as many up rows (n % 32 == 0), and
+ * z in 0 .. 15; x [m, k] and y [m, n] fp16 or bf16 (dtype), the scales of that type, sums in fp32, rounded once. m below 2^20,
+ * n up to 2^28; group 32, 64 or 128, k a multiple of it. silu_mul: the rows of W are n / 2 gate rows, then as many up rows
+ * (n % 32 == 0), and
  *   y[i][j] = silu(g) * u, g and u the products with rows j and n / 2 + j, rounded once; y is [m, n / 2].
  * The weight is packed once (all sizes rounded up, little endian):
  *   codes  [n / 16][k / 128][4 j][16 r][4 u] dwords: row r of the tile, elements 32 u + 8 j + i of the block, i = 2 p in

@@ -288,6 +288,14 @@ def _check_window(window, sinks) -> tuple[int, int]:
 
 
 def _forward_window(q, k_cache, v_cache, meta, scale, out, k_scale, v_scale, window, sinks) -> torch.Tensor:
+    calls = _calls()
+    if calls is not None:
+        r = calls.forward_window(q, k_cache, v_cache, meta.block_tables, meta.seq_lens, meta.query_start_loc,
+                                 meta.max_query_len, scale, out, k_scale, v_scale, window, sinks)  # fmt: skip
+        if type(r) is int:
+            _lib.check(r, "kvh_paged_attention_window")
+        if r is not None:
+            return r
     window, sinks = _check_window(window, sinks)
     num_blocks, block_size, num_kv_heads, head_dim, dev, fmt, ks, vs, caches = _cache_args(k_cache, v_cache, k_scale, v_scale)
     out, tables, seq_lens, qsl = _check_attention(q, meta, num_kv_heads, head_dim, dev, out)
@@ -556,6 +564,14 @@ class HipAttention:
         elements of a head: (i, i + rotary_dim / 2), or (2i, 2i + 1) where `interleaved`. Norm, rotation and their
         products are fp32, rounded once: the queries, returned as [T, num_heads, head_dim] (in `out` if given), to qkv's
         dtype, the keys to the cache's format. Scales and slots as write_kv."""
+        calls = _calls()
+        if calls is not None:
+            r = calls.norm_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, q_norm, k_norm, eps,
+                                          interleaved, out, k_scale, v_scale)  # fmt: skip
+            if type(r) is int:
+                _lib.check(r, "kvh_norm_rope_and_cache")
+            if r is not None:
+                return r
         num_blocks, block_size, num_kv_heads, head_dim, dev, fmt, ks, vs, caches = _cache_args(k_cache, v_cache, k_scale,
                                                                                                v_scale)  # fmt: skip
         _on_device(dev, qkv=qkv, positions=positions, cos=cos, sin=sin, slot_mapping=slots)

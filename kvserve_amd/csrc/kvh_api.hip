@@ -941,9 +941,9 @@ static int check_linear4(int64_t m, int32_t n, int32_t k, int32_t group, int32_t
   if (dtype != KVH_DTYPE_F16 && dtype != KVH_DTYPE_BF16) return KVH_E_DTYPE;
   if (m < 0 || n < 0 || k <= 0) return KVH_E_SHAPE;
   if (group != 32 && group != 64 && group != 128) return KVH_E_UNSUPPORTED;
-  // rows of x in 65535 workgroups of 16 or more; rows of the weight in tiles of 16 (each half of a gated one); columns,
-  // rounded up to a few blocks, in 31 bits
-  if (k % group != 0 || m > 16 * 65535 || n > 0x7fffff00 || k > 0x3fffff00 || (silu_mul && n % 32 != 0))
+  // rows of x in 65535 workgroups of 16 or more; rows of the weight in tiles of 16 (each half of a gated one), 128 threads
+  // at most each and fewer than 2^32 in all; columns, rounded up to a few blocks, in 31 bits
+  if (k % group != 0 || m > 16 * 65535 || n > 0x10000000 || k > 0x3fffff00 || (silu_mul && n % 32 != 0))
     return KVH_E_UNSUPPORTED;
   return KVH_OK;
 }

@@ -3,8 +3,8 @@
 // A decode step of a small model is two calls whose kernels take about 10 us together; reading
 // some fifty tensor attributes through Python, allocating the output and converting arguments
 // took twice that (a step of 8 sequences of 64-512 keys: 20 us of host time against 10 us of
-// kernels). forward(), write_kv(), rope_and_cache(), their *_fp4 forms, read_kv_fp4() and
-// token_logprobs() here check what the Python methods check, on the tensors themselves, allocate the
+// kernels). forward(), write_kv(), rope_and_cache(), their *_fp4 forms, read_kv_fp4(), forward_window(),
+// norm_rope_and_cache(), linear4() and token_logprobs() here check what the Python methods check, on the tensors themselves, allocate the
 // output and the workspace and call the C ABI.
 //
 // A call is taken only when every check passes on plain torch.Tensor arguments; otherwise (a wrong
@@ -40,6 +40,10 @@ decltype(&kvh_rope_and_cache_fp4) f_rope_fp4;
 decltype(&kvh_read_cache_fp4) f_read_fp4;
 decltype(&kvh_token_logprobs_workspace_size) f_logprobs_ws;
 decltype(&kvh_token_logprobs) f_logprobs;
+decltype(&kvh_paged_attention_window) f_window;
+decltype(&kvh_norm_rope_and_cache) f_norm_rope;
+decltype(&kvh_linear4_workspace_size) f_linear4_ws;
+decltype(&kvh_linear4) f_linear4;
 PyObject* g_raw_stream;  // callable: device index -> the current stream's handle
 
 // bind(handle, raw_stream): the dlopen handle of the loaded libkvhip
@@ -72,6 +76,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   SYM(f_read_fp4, "kvh_read_cache_fp4")
   SYM(f_logprobs_ws, "kvh_token_logprobs_workspace_size")
   SYM(f_logprobs, "kvh_token_logprobs")
+  SYM(f_window, "kvh_paged_attention_window")
+  SYM(f_norm_rope, "kvh_norm_rope_and_cache")
+  SYM(f_linear4_ws, "kvh_linear4_workspace_size")
+  SYM(f_linear4, "kvh_linear4")
 #undef SYM
   PyObject* old = g_raw_stream;
   Py_INCREF(args[1]);
@@ -180,6 +188,35 @@ bool fp4_caches(PyObject* k, PyObject* v, PyObject* k_scale, PyObject* v_scale, 
 
 #define FP4_ARGS(c)                                                                                               \
   (c).k->data_ptr(), (c).ks, (c).kx->data_ptr(), (c).kxs, (c).v->data_ptr(), (c).vs, (c).vx->data_ptr(), (c).vxs
+
+// Caches of any format, on the current device.
+struct AnyCaches : Fp4Caches {
+  int32_t format;
+};
+
+bool any_caches(PyObject* k, PyObject* v, PyObject* k_scale, PyObject* v_scale, AnyCaches* c) {
+  const at::Tensor* t = gpu_tensor(k);
+  if (!t) return false;
+  if (t->scalar_type() == c10::ScalarType::Float4_e2m1fn_x2) {
+    c->format = KVH_CACHE_MXFP4;
+    return fp4_caches(k, v, k_scale, v_scale, c);
+  }
+  if (!current_device(*t) || !caches(k, v, k_scale, v_scale, c)) return false;
+  c->format = c->fp8 ? KVH_CACHE_E4M3 : KVH_CACHE_DTYPE;
+  c->kx = c->vx = nullptr;
+  return true;
+}
+
+#define ANY_ARGS(c)                                                                                            \
+  (c).k->data_ptr(), (c).ks, (c).kx ? (c).kx->data_ptr() : nullptr, (c).kx ? (c).kxs : nullptr, (c).v->data_ptr(), \
+      (c).vs, (c).vx ? (c).vx->data_ptr() : nullptr, (c).vx ? (c).vxs : nullptr
+
+// KVH_DTYPE_* of an operand over them, or -1.
+int any_dtype(const at::Tensor& t, const AnyCaches& c) {
+  const int dtype = kvh_dtype(t.scalar_type());
+  if (c.format == KVH_CACHE_DTYPE && t.scalar_type() != c.k->scalar_type()) return -1;
+  return dtype;
+}
 
 // An int64 index tensor of `dim` dimensions with a contiguous last one, on the caches' device.
 const at::Tensor* index_tensor(PyObject* o, int64_t dim, const Caches& c) {
@@ -443,6 +480,131 @@ PyObject* rope_and_cache_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
+// forward_window(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, max_query_len, scale, out, k_scale, v_scale,
+// window, sinks)
+PyObject* forward_window(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return attempt(nargs, 13, [&]() -> PyObject* {
+    AnyCaches c;
+    if (!any_caches(a[1], a[2], a[9], a[10], &c)) return nullptr;
+    const at::Tensor* q = gpu_tensor(a[0]);
+    const at::Tensor *bt = index_tensor(a[3], 2, c), *sl = index_tensor(a[4], 1, c), *qsl = index_tensor(a[5], 1, c);
+    int32_t max_q, B, H, W, window, sinks;
+    double scale;
+    if (!q || !bt || !sl || !qsl || !integer(a[6], &max_q) || !number(a[7], &scale)) return nullptr;
+    if (!integer(a[11], &window) || !integer(a[12], &sinks) || window < 1 || sinks < 0) return nullptr;
+    if (q->get_device() != c.k->get_device() || q->dim() != 3 || q->size(2) != c.head_dim || q->stride(2) != 1)
+      return nullptr;
+    const int dtype = any_dtype(*q, c);
+    if (dtype < 0 || (c.format != KVH_CACHE_DTYPE && dtype == KVH_DTYPE_F32)) return nullptr;
+    const int64_t T = q->size(0);
+    if (!same_int32(bt->size(0), &B) || !same_int32(bt->size(1), &W) || !same_int32(q->size(1), &H)) return nullptr;
+    if (c.kv_heads <= 0 || H % c.kv_heads != 0 || sl->size(0) != B || qsl->size(0) != (int64_t)B + 1) return nullptr;
+    at::Tensor out;
+    if (!output(a[8], q->sizes(), *q, c, &out)) return nullptr;
+    if (T == 0 || B == 0) return result(0, a[8], std::move(out));
+    const size_t need = f_ws_size(T, B, H, c.kv_heads, c.head_dim, W, c.block_size, max_q, dtype);
+    at::Tensor ws;
+    if (need) ws = fresh({(int64_t)need}, c10::kByte, *q);
+    void* stream;
+    if (!stream_of(c, &stream)) return nullptr;
+    const int st = f_window(q->data_ptr(), q->stride(0), q->stride(1), ANY_ARGS(c), c.k->size(0), out.data_ptr(),
+                            out.stride(0), out.stride(1), (const int64_t*)bt->data_ptr(), bt->stride(0), W,
+                            (const int64_t*)sl->data_ptr(), (const int64_t*)qsl->data_ptr(), T, B, H, c.kv_heads,
+                            c.head_dim, c.block_size, max_q, window, sinks, (float)scale, c.format, c.k_scale, c.v_scale,
+                            dtype, need ? ws.data_ptr() : nullptr, need, stream);
+    return result(st, a[8], std::move(out));
+  });
+}
+
+// norm_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slots, num_heads, q_norm, k_norm, eps, interleaved, out,
+// k_scale, v_scale)
+PyObject* norm_rope_and_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return attempt(nargs, 15, [&]() -> PyObject* {
+    AnyCaches c;
+    if (!any_caches(a[4], a[5], a[13], a[14], &c)) return nullptr;
+    const at::Tensor *qkv = gpu_tensor(a[0]), *cos = gpu_tensor(a[2]), *sin = gpu_tensor(a[3]);
+    const at::Tensor *pos = index_tensor(a[1], 1, c), *slots = index_tensor(a[6], 1, c);
+    int32_t H, rotary;
+    double eps;
+    if (!qkv || !cos || !sin || !pos || !slots || !integer(a[7], &H) || H <= 0 || !number(a[10], &eps)) return nullptr;
+    if (!PyBool_Check(a[11])) return nullptr;
+    const auto dev = c.k->get_device();
+    if (qkv->get_device() != dev || cos->get_device() != dev || sin->get_device() != dev) return nullptr;
+    const int64_t T = qkv->dim() == 2 ? qkv->size(0) : 0;
+    if (T == 0 || qkv->stride(1) != 1 || qkv->size(1) != ((int64_t)H + 2 * (int64_t)c.kv_heads) * c.head_dim)
+      return nullptr;
+    if (cos->scalar_type() != c10::kFloat || sin->scalar_type() != c10::kFloat || cos->dim() != 2 ||
+        cos->sizes() != sin->sizes() || !cos->is_contiguous() || !sin->is_contiguous() || cos->size(1) % 8 != 0 ||
+        2 * cos->size(1) > c.head_dim || !same_int32(2 * cos->size(1), &rotary))
+      return nullptr;
+    if (pos->size(0) != T || slots->size(0) != T) return nullptr;
+    const void* norm[2] = {};
+    for (int i = 0; i < 2; ++i) {
+      if (a[8 + i] == Py_None) continue;
+      const at::Tensor* w = gpu_tensor(a[8 + i]);
+      if (!w || w->get_device() != dev || w->dim() != 1 || w->size(0) != c.head_dim || !w->is_contiguous() ||
+          w->scalar_type() != qkv->scalar_type())
+        return nullptr;
+      norm[i] = w->data_ptr();
+    }
+    const int dtype = any_dtype(*qkv, c);
+    if (dtype < 0) return nullptr;
+    at::Tensor out;
+    const int64_t sizes[3] = {T, H, c.head_dim};
+    if (!output(a[12], sizes, *qkv, c, &out)) return nullptr;
+    void* stream;
+    if (!stream_of(c, &stream)) return nullptr;
+    const int st = f_norm_rope(qkv->data_ptr(), qkv->stride(0), (const int64_t*)pos->data_ptr(),
+                               (const float*)cos->data_ptr(), (const float*)sin->data_ptr(), cos->size(0), rotary,
+                               a[11] == Py_True, norm[0], norm[1], (float)eps, out.data_ptr(), out.stride(0),
+                               out.stride(1), ANY_ARGS(c), (const int64_t*)slots->data_ptr(), T, c.k->size(0), H,
+                               c.kv_heads, c.head_dim, c.block_size, c.format, c.k_scale, c.v_scale, dtype, stream);
+    return result(st, a[12], std::move(out));
+  });
+}
+
+// linear4(x, codes, scales, n, k, group, KVH_DTYPE_* of the scales, silu_mul, out)
+PyObject* linear4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return attempt(nargs, 9, [&]() -> PyObject* {
+    const at::Tensor *x = gpu_tensor(a[0]), *codes = gpu_tensor(a[1]), *scales = gpu_tensor(a[2]);
+    int32_t n, k, group, type;
+    if (!x || !codes || !scales || !integer(a[3], &n) || !integer(a[4], &k) || !integer(a[5], &group) ||
+        !integer(a[6], &type) || !PyBool_Check(a[7]) || !current_device(*x))
+      return nullptr;
+    const bool gated = a[7] == Py_True;
+    const auto dev = x->get_device();
+    if (codes->get_device() != dev || scales->get_device() != dev || n < 0 || k <= 0 || (gated && n % 32 != 0) ||
+        (group != 32 && group != 64 && group != 128))
+      return nullptr;
+    const int64_t tiles = ((int64_t)n + 15) / 16, blocks = ((int64_t)k + 127) / 128;
+    for (const at::Tensor* t : {codes, scales})
+      if (t->scalar_type() != c10::kInt || !t->is_contiguous()) return nullptr;
+    if (codes->numel() != tiles * blocks * 256 || scales->numel() != tiles * blocks * (128 / group) * 16) return nullptr;
+    if (x->dim() != 2 || x->size(1) != k || x->stride(1) != 1 || kvh_dtype(x->scalar_type()) != type) return nullptr;
+    const int64_t m = x->size(0), cols = gated ? n / 2 : n;
+    at::Tensor out;
+    if (a[8] == Py_None) {
+      out = fresh({m, cols}, x->scalar_type(), *x);
+    } else {
+      const at::Tensor* o = gpu_tensor(a[8]);
+      if (!o || o->get_device() != dev || o->dim() != 2 || o->size(0) != m || o->size(1) != cols || o->stride(1) != 1 ||
+          o->scalar_type() != x->scalar_type())
+        return nullptr;
+      out = *o;
+    }
+    const size_t need = f_linear4_ws(m, n, k, gated);
+    at::Tensor ws;
+    if (need) ws = fresh({(int64_t)need}, c10::kByte, *x);
+    Caches where;
+    where.k = x;
+    void* stream;
+    if (!stream_of(where, &stream)) return nullptr;
+    const int st = f_linear4(x->data_ptr(), x->stride(0), codes->data_ptr(), scales->data_ptr(), out.data_ptr(),
+                             out.stride(0), m, n, k, group, gated, type, need ? ws.data_ptr() : nullptr, need, stream);
+    return result(st, a[8], std::move(out));
+  });
+}
+
 // The tensors as a tuple, or null with a Python error.
 template <int N>
 PyObject* tuple(at::Tensor (&t)[N]) {
@@ -517,6 +679,9 @@ PyMethodDef methods[] = {
     {"write_kv_fp4", FAST(write_kv_fp4), "HipAttention.write_kv into MXFP4 caches, or None"},
     {"rope_and_cache_fp4", FAST(rope_and_cache_fp4), "HipAttention.rope_and_cache into MXFP4 caches, or None"},
     {"read_kv_fp4", FAST(read_kv_fp4), "HipAttention.read_kv, or None"},
+    {"forward_window", FAST(forward_window), "HipAttention.forward with a window over any cache, or None"},
+    {"norm_rope_and_cache", FAST(norm_rope_and_cache), "HipAttention.norm_rope_and_cache on plain tensors, or None"},
+    {"linear4", FAST(linear4), "linear4 and linear4_silu_mul on plain tensors, or None"},
     {"token_logprobs", FAST(token_logprobs), "token_logprobs on plain tensors, or None"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -8,7 +8,7 @@ from dataclasses import dataclass
 import torch
 
 from kvserve_amd import _lib
-from kvserve_amd.attention import _current, _require, _stream_handle
+from kvserve_amd.attention import _calls, _current, _require, _stream_handle
 
 GROUPS = (32, 64, 128)
 
@@ -23,6 +23,14 @@ class Weight4:
     shape: tuple[int, int]  # (n, k)
     group: int
     dtype: torch.dtype  # of the scales, and of x and y
+
+    def __post_init__(self):
+        n, k = self.shape
+        _require(self.group in GROUPS and n >= 0 and k > 0 and k % self.group == 0, f"no groups of {self.group} in {self.shape}")
+        tiles, blocks = -(-n // 16), -(-k // 128)
+        for name, t, want in (("codes", self.codes, (tiles, blocks, 256)),
+                              ("scales", self.scales, (tiles, blocks * (128 // self.group), 16))):  # fmt: skip
+            _require(t.dtype == torch.int32 and t.shape == want and t.is_contiguous(), f"{name} must be contiguous int32 {want}")
 
     @property
     def device(self) -> torch.device:
@@ -99,6 +107,13 @@ def quantize_weight4(weight: torch.Tensor, group: int = 128) -> Weight4:
 
 def _product(x: torch.Tensor, weight: Weight4, silu_mul: bool, out: torch.Tensor | None) -> torch.Tensor:
     n, k = weight.shape
+    calls = _calls()
+    if calls is not None:
+        r = calls.linear4(x, weight.codes, weight.scales, n, k, weight.group, _lib.KVH_DTYPE.get(weight.dtype), silu_mul, out)
+        if type(r) is int:
+            _lib.check(r, "kvh_linear4")
+        if r is not None:
+            return r
     _require(x.dim() == 2 and x.shape[1] == k and x.stride(-1) == 1, f"x must be [m, {k}] with a contiguous last dim")
     _require(x.dtype == weight.dtype, f"x is {x.dtype}, the weight's scales are {weight.dtype}")
     _require(x.is_cuda, "x must be on a HIP device")

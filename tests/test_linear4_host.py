@@ -69,6 +69,11 @@ def test_refusals():
     for W, group in ((torch.zeros(4, 96), 32), (torch.zeros(4, 96).half(), 64), (torch.zeros(4, 96).half(), 48), (torch.zeros(96).half(), 32)):
         with pytest.raises(ValueError):
             quantize_weight4(W, group)
+    w = Weight4.pack(codes, s, z)
+    for bad in ((w.codes[:1], w.scales, w.shape, 64), (w.codes, w.scales, w.shape, 32), (w.codes.long(), w.scales, w.shape, 64),
+                (w.codes, w.scales.transpose(0, 1), w.shape, 64), (w.codes, w.scales, (20, 190), 64)):  # fmt: skip
+        with pytest.raises(ValueError):
+            Weight4(*bad, torch.bfloat16)
     with pytest.raises(ValueError):  # no CPU form
         linear4(torch.zeros(2, 192).bfloat16(), Weight4.pack(codes, s, z))
 
@@ -84,7 +89,7 @@ def test_refusals_of_the_c_abi():
     assert _call(dtype=0) == dtype and _call(dtype=3) == dtype
     assert _call(m=-1) == shape and _call(n=-1) == shape and _call(k=0) == shape
     assert _call(group=48) == unsupported and _call(k=192) == unsupported and _call(m=16 * 65535 + 1) == unsupported
-    assert _call(silu=1) == unsupported and _call(n=0x7FFFFFFF) == unsupported
+    assert _call(silu=1) == unsupported and _call(n=0x7FFFFFFF) == unsupported and _call(n=2**28 + 1) == unsupported
     # refused before anything is launched: addresses that are never read
     assert _call(x=16, y=16, xs=127) == shape and _call(x=16, y=16, ys=15) == shape
     assert _call(x=16, y=16, m=64, n=1024, k=8192, xs=8192, ys=1024) == workspace
