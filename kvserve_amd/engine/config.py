@@ -21,6 +21,16 @@ class ModelConfig:
     rope_scaling: dict | None = None
     max_position_embeddings: int = 131072
     tie_word_embeddings: bool = False
+    # Of models that are no Llama:
+    qk_norm: bool = False  # RMS norms of the query and key heads, ahead of RoPE
+    rotary_dim: int | None = None  # leading elements of a head that RoPE turns (None: all)
+    rope_interleaved: bool = False  # RoPE over neighbouring elements, not over halves
+    sliding_window: int | None = None  # tokens a token sees, itself among them (None: all before it)
+    attention_sinks: int = 0  # first tokens of a sequence that it sees as well
+    full_layers: tuple[int, ...] = ()  # layers without the window
+
+    def window(self, layer: int) -> int | None:
+        return None if layer in self.full_layers else self.sliding_window
 
     @classmethod
     def from_dir(cls, path: Path) -> ModelConfig:
@@ -51,7 +61,9 @@ class ModelConfig:
         )
 
     def to_hf_dict(self) -> dict:
-        """A Hugging Face style config.json for this shape."""
+        """A Hugging Face style config.json for this shape (a Llama's)."""
+        if self.qk_norm or self.rotary_dim is not None or self.rope_interleaved or self.sliding_window is not None:
+            raise ValueError("a Llama config has no head norms, other rotations or windows")
         d = {
             "model_type": "llama",
             "architectures": ["LlamaForCausalLM"],

@@ -22,12 +22,16 @@ reference fuses them (q|k|v rows, gate|up rows). The arithmetic is Hugging Face 
 (RMSNorm with fp32 statistics, rotate-half RoPE with Llama 3 frequency scaling, SiLU MLP),
 which the CPU tests pin against transformers' own model. On the GPU with 16-bit weights the
 row-wise work runs on libkvhip's layer kernels (`engine.ops`).
+
+A config may also ask for normed query and key heads, RoPE over a part of a head or over
+neighbouring elements (on the HIP backend `norm_rope_and_cache`) and a sliding window with
+sinks; projections held in 4 bits (`quantize_projections4`) run on `linear4`.
 """
 
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from pathlib import Path
 from typing import NamedTuple
 
@@ -37,6 +41,7 @@ import torch.nn.functional as F
 from kvserve_amd.attention import FP4, AttentionMetadata, HipAttention
 from kvserve_amd.engine import ops
 from kvserve_amd.engine.config import ModelConfig
+from kvserve_amd.linear4 import Weight4, linear4, linear4_silu_mul, quantize_weight4
 from kvserve_amd.logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 
 # -- arithmetic ------------------------------------------------------------------------------
@@ -51,13 +56,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
 
 
 def rope_inv_freq(cfg: ModelConfig) -> torch.Tensor:
-    """RoPE inverse frequencies theta^(-2i/D), i < D/2, with Llama 3's long-context rescaling
+    """RoPE inverse frequencies theta^(-2i/D), i < D/2 (D: the rotated elements of a head), with Llama 3's long-context rescaling
     when the config carries it (reference model.py:35-52): a component whose wavelength
     2 pi / f exceeds original_ctx / low_freq_factor is slowed by `factor`, one below
     original_ctx / high_freq_factor is kept, and in between the two are blended linearly in
     original_ctx / wavelength."""
-    half = torch.arange(0, cfg.head_dim, 2, dtype=torch.int64).float()
-    base = 1.0 / (cfg.rope_theta ** (half / cfg.head_dim))
+    dim = cfg.head_dim if cfg.rotary_dim is None else cfg.rotary_dim
+    half = torch.arange(0, dim, 2, dtype=torch.int64).float()
+    base = 1.0 / (cfg.rope_theta ** (half / dim))
     sc = cfg.rope_scaling or {}
     if sc.get("rope_type", sc.get("type")) != "llama3":
         return base
@@ -77,6 +83,12 @@ def rope_tables(cfg: ModelConfig, max_positions: int, device=None) -> tuple[torc
     return angles.cos().to(device), angles.sin().to(device)
 
 
+def half_rope_tables(cfg: ModelConfig, max_positions: int, device=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 cos / sin tables [max_positions, D / 2] of the angles p * f_i, one for each pair of rotated elements."""
+    angles = torch.arange(max_positions, dtype=torch.float32)[:, None] * rope_inv_freq(cfg)[None, :]
+    return angles.cos().to(device), angles.sin().to(device)
+
+
 def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """x [T, heads, D] rotated by per-token cos / sin rows [T, D] (already in x's dtype):
     x * cos + (-x2, x1) * sin with x1, x2 the two halves of the last dim."""
@@ -85,19 +97,36 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return x * cos[:, None, :] + turned * sin[:, None, :]
 
 
+def norm_and_rope(x: torch.Tensor, weight: torch.Tensor | None, eps: float, cos: torch.Tensor, sin: torch.Tensor,
+                  interleaved: bool) -> torch.Tensor:  # fmt: skip
+    """HipAttention.norm_rope_and_cache's norm and rotation of x [T, heads, D] in plain torch: fp32, rounded once.
+    cos, sin: fp32 rows [T, pairs] of the tokens."""
+    y = x.float()
+    if weight is not None:
+        y = y * torch.rsqrt(y.square().mean(dim=-1, keepdim=True) + eps) * weight.float()
+    turn, rest = y.split([2 * cos.shape[1], y.shape[2] - 2 * cos.shape[1]], dim=-1)
+    a, b = turn.unflatten(-1, (-1, 2)).unbind(-1) if interleaved else turn.chunk(2, dim=-1)
+    c, s = cos[:, None, :], sin[:, None, :]
+    a, b = a * c - b * s, b * c + a * s
+    turn = torch.stack((a, b), dim=-1).flatten(-2) if interleaved else torch.cat((a, b), dim=-1)
+    return torch.cat((turn, rest), dim=-1).to(x.dtype)
+
+
 # -- weights ---------------------------------------------------------------------------------
 
 
 @dataclass
 class LayerWeights:
     attn_norm: torch.Tensor  # [hidden]
-    wqkv: torch.Tensor  # [(H + 2 Hkv) D, hidden]: query heads, then key heads, then value heads
-    wo: torch.Tensor  # [hidden, H D]
+    wqkv: torch.Tensor | Weight4  # [(H + 2 Hkv) D, hidden]: query heads, then key heads, then value heads
+    wo: torch.Tensor | Weight4  # [hidden, H D]
     mlp_norm: torch.Tensor  # [hidden]
-    w_gate_up: torch.Tensor  # [2 I, hidden]: gate rows, then up rows
-    w_down: torch.Tensor  # [hidden, I]
+    w_gate_up: torch.Tensor | Weight4  # [2 I, hidden]: gate rows, then up rows
+    w_down: torch.Tensor | Weight4  # [hidden, I]
     k_scale: float = 1.0  # per-layer scales of a float8_e4m3fn KV cache
     v_scale: float = 1.0
+    q_norm: torch.Tensor | None = None  # [D], of a config with qk_norm
+    k_norm: torch.Tensor | None = None
 
 
 @dataclass
@@ -116,14 +145,16 @@ def random_weights(cfg: ModelConfig, device, dtype: torch.dtype, seed: int = 0, 
     def normal(*shape: int) -> torch.Tensor:
         return (torch.randn(shape, generator=gen, device=device, dtype=torch.float32) * std).to(dtype)
 
-    def ones() -> torch.Tensor:
-        return torch.ones(cfg.hidden_size, device=device, dtype=dtype)
+    def ones(width: int = cfg.hidden_size) -> torch.Tensor:
+        return torch.ones(width, device=device, dtype=dtype)
 
     H, Hkv, D, hid, inter = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.hidden_size, cfg.intermediate_size
     w = Weights(embed=normal(cfg.vocab_size, hid))
     for _ in range(cfg.num_layers):
         w.layers.append(LayerWeights(ones(), normal((H + 2 * Hkv) * D, hid), normal(hid, H * D), ones(),
                                      normal(2 * inter, hid), normal(hid, inter)))  # fmt: skip
+        if cfg.qk_norm:
+            w.layers[-1].q_norm, w.layers[-1].k_norm = ones(D), ones(D)
     w.final_norm = ones()
     w.lm_head = w.embed if cfg.tie_word_embeddings else normal(cfg.vocab_size, hid)
     return w
@@ -156,9 +187,21 @@ def load_hf_weights(path: Path, cfg: ModelConfig, device, dtype: torch.dtype) ->
         w.layers.append(LayerWeights(get(p + "input_layernorm.weight"), qkv, get(p + "self_attn.o_proj.weight"),
                                      get(p + "post_attention_layernorm.weight"), gate_up,
                                      get(p + "mlp.down_proj.weight")))  # fmt: skip
+        if cfg.qk_norm:
+            w.layers[-1].q_norm, w.layers[-1].k_norm = (get(p + f"self_attn.{x}_norm.weight") for x in "qk")
     w.final_norm = get("norm.weight")
     w.lm_head = w.embed if cfg.tie_word_embeddings else get("lm_head.weight")
     return w
+
+
+def quantize_projections4(w: Weights, group: int = 128) -> Weights:
+    """The weights with every layer's projections held in 4 bits (quantize_weight4); embedding, head and norms as they
+    are."""
+    layers = []
+    for lw in w.layers:
+        packed = {name: quantize_weight4(getattr(lw, name), group) for name in ("wqkv", "wo", "w_gate_up", "w_down")}
+        layers.append(replace(lw, **packed))
+    return replace(w, layers=layers)
 
 
 def _torch_token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
@@ -199,23 +242,32 @@ class PagedLlama:
 
     def __init__(self, cfg: ModelConfig, weights: Weights, backend=HipAttention, max_positions: int = 4096,
                  fused_ops: bool | None = None, fused_rope: bool | None = None):  # fmt: skip
+        if cfg.attention_sinks < 0 or (cfg.sliding_window is None and cfg.attention_sinks) or (
+                cfg.sliding_window is not None and cfg.sliding_window < 1):  # fmt: skip
+            raise ValueError(f"window {cfg.sliding_window} with {cfg.attention_sinks} sinks")
         self.cfg = cfg
         self.w = weights
         self.backend = backend
         self.device, self.dtype = weights.embed.device, weights.embed.dtype
         self.max_positions = max_positions
-        self.cos, self.sin = rope_tables(cfg, max_positions, self.device)
+        # norms of heads and rotations that rope_and_cache has not
+        self.head_rope = cfg.qk_norm or cfg.rotary_dim is not None or cfg.rope_interleaved
+        tables = half_rope_tables if self.head_rope else rope_tables
+        self.cos, self.sin = tables(cfg, max_positions, self.device)
         self.scale = cfg.head_dim**-0.5
         self.q_width = cfg.num_heads * cfg.head_dim
         self.kv_width = cfg.num_kv_heads * cfg.head_dim
         # What the backend offers beyond write_kv / forward. fused_rope=False drives it exactly
         # as kvserve's Attention.attend does (src/kvserve/model.py:84-108): split + RoPE in
         # torch, write_kv with v a strided view of the fused QKV output, then forward(out=...).
-        offered = callable(getattr(backend, "rope_and_cache", None))
+        fused = "norm_rope_and_cache" if self.head_rope else "rope_and_cache"
+        offered = callable(getattr(backend, fused, None))
         if fused_rope and not offered:
-            raise ValueError("the backend has no fused RoPE + cache write (rope_and_cache)")
+            raise ValueError(f"the backend has no fused RoPE + cache write ({fused})")
         self.fused_rope = offered if fused_rope is None else bool(fused_rope)
-        self.fused_projection = self.fused_rope and callable(getattr(backend, "gemv_rope_and_cache", None))
+        self.fused_projection = (self.fused_rope and not self.head_rope
+                                 and callable(getattr(backend, "gemv_rope_and_cache", None))
+                                 and not any(isinstance(lw.wqkv, Weight4) for lw in weights.layers))  # fmt: skip
         probe = torch.empty(0, dtype=self.dtype, device=self.device)
         self.fused_ops = ops.enabled(probe) if fused_ops is None else bool(fused_ops)
         if self.fused_ops and not ops.enabled(probe):
@@ -226,7 +278,9 @@ class PagedLlama:
         return len(self.w.layers)
 
     # -- row-wise stages ------------------------------------------------------------------------
-    def _linear(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    def _linear(self, x: torch.Tensor, w: torch.Tensor | Weight4) -> torch.Tensor:
+        if isinstance(w, Weight4):
+            return linear4(x, w) if x.is_cuda else F.linear(x, w.dequantize(x.dtype))
         return ops.linear(x, w) if self.fused_ops else F.linear(x, w)
 
     def _add_norm(self, x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor):
@@ -239,10 +293,12 @@ class PagedLlama:
         return x, rms_norm(x, weight, eps)
 
     def _mlp(self, h: torch.Tensor, lw: LayerWeights) -> torch.Tensor:
+        if isinstance(lw.w_gate_up, Weight4) and h.is_cuda:
+            return self._linear(linear4_silu_mul(h, lw.w_gate_up), lw.w_down)
         if self.fused_ops:
-            return ops.linear(ops.mlp_act(h, lw.w_gate_up), lw.w_down)
-        gate, up = F.linear(h, lw.w_gate_up).chunk(2, dim=-1)
-        return F.linear(F.silu(gate) * up, lw.w_down)
+            return self._linear(ops.mlp_act(h, lw.w_gate_up), lw.w_down)
+        gate, up = self._linear(h, lw.w_gate_up).chunk(2, dim=-1)
+        return self._linear(F.silu(gate) * up, lw.w_down)
 
     def defers_projection(self, rows: int) -> bool:
         """Whether a layer's QKV projection over `rows` rows moves into the attention step
@@ -290,16 +346,27 @@ class PagedLlama:
         if s.normed is not None:
             q = b.gemv_rope_and_cache(s.normed, lw.wqkv, positions, self.cos, self.sin, k_cache, v_cache,
                                       meta.slot_mapping, H, out=q_out, **sc)  # fmt: skip
+        elif self.fused_rope and self.head_rope:
+            q = b.norm_rope_and_cache(s.qkv, positions, self.cos, self.sin, k_cache, v_cache, meta.slot_mapping, H, lw.q_norm,
+                                      lw.k_norm, self.cfg.rms_norm_eps, self.cfg.rope_interleaved, q_out, **sc)  # fmt: skip
         elif self.fused_rope:
             q = b.rope_and_cache(s.qkv, positions, self.cos, self.sin, k_cache, v_cache, meta.slot_mapping, H,
                                  out=q_out, **sc)  # fmt: skip
         else:
             n, D = s.qkv.shape[0], self.cfg.head_dim
             q, k, v = s.qkv.split([self.q_width, self.kv_width, self.kv_width], dim=-1)
-            cos, sin = self.cos[positions].to(q.dtype), self.sin[positions].to(q.dtype)
-            q = apply_rope(q.view(n, H, D), cos, sin)
-            k = apply_rope(k.view(n, -1, D), cos, sin)
+            q, k = q.view(n, H, D), k.view(n, -1, D)
+            cos, sin = self.cos[positions], self.sin[positions]
+            if self.head_rope:
+                eps, pairs = self.cfg.rms_norm_eps, self.cfg.rope_interleaved
+                q = norm_and_rope(q, lw.q_norm, eps, cos, sin, pairs)
+                k = norm_and_rope(k, lw.k_norm, eps, cos, sin, pairs)
+            else:
+                cos, sin = cos.to(q.dtype), sin.to(q.dtype)
+                q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
             b.write_kv(k_cache, v_cache, k, v.view(n, -1, D), meta.slot_mapping, **sc)
+        if (window := self.cfg.window(i)) is not None:
+            sc |= {"window": window, "sinks": self.cfg.attention_sinks}
         return b.forward(q, k_cache, v_cache, meta, self.scale, out=out, **sc)
 
     # -- whole passes ----------------------------------------------------------------------------
@@ -338,12 +405,16 @@ class PagedLlama:
 
 def build_model(cfg: ModelConfig, device, dtype: torch.dtype, max_positions: int, backend=HipAttention,
                 weights: Path | None = None, seed: int = 0, std: float = 0.02,
-                fused_ops: bool | None = None, fused_rope: bool | None = None) -> PagedLlama:  # fmt: skip
+                fused_ops: bool | None = None, fused_rope: bool | None = None,
+                weight4_group: int | None = None) -> PagedLlama:  # fmt: skip
     """A PagedLlama on `device` in `dtype`: weights from a Hugging Face safetensors directory,
     else synthetic (`random_weights`). fused_ops (default: on a GPU with 16-bit weights) selects
     libkvhip's layer kernels for the row-wise work; fused_rope=False keeps the backend to
-    kvserve's write_kv + forward calls (default: its fused RoPE + cache write when offered)."""
+    kvserve's write_kv + forward calls (default: its fused RoPE + cache write when offered).
+    weight4_group: hold the projections in 4 bits, in groups of that many columns (None: in `dtype`)."""
     device = torch.device(device)
     w = load_hf_weights(weights, cfg, device, dtype) if weights is not None else random_weights(cfg, device, dtype,
                                                                                                  seed, std)  # fmt: skip
+    if weight4_group is not None:
+        w = quantize_projections4(w, weight4_group)
     return PagedLlama(cfg, w, backend, max_positions, fused_ops, fused_rope)
