@@ -51,10 +51,15 @@ constexpr int kWavesPerWG = 4;
 // register set of chunks in flight (254 VGPRs): two chunks of 900-1024 tokens over 4000-10000 beside 24 decodes 272 us
 // with 2, 240 with 3, two prompts of 2000 tokens 126 and 118; a lone chunk of 500 tokens, which fills few workgroups, 47.1
 // and 49.1. At D = 64 the third costs more than it saves (203 us, 210 with 3).
-// Under a window, whose masked loop ahead takes registers of its own, MXFP4 keeps 2 (3 spill 11 registers).
+// Under a window, whose masked loop ahead takes registers of its own, MXFP4 keeps 2 (3 spill 11 registers); 16-bit caches
+// of 128-wide heads take 2 as well where these tiles suit the launch better (pre_window_nt).
 template <int KV, int D, bool WIN>
 constexpr int prefill_nt() {
   return KV == kKv16 || (KV == kKv4 && D == 128 && !WIN) ? 3 : 2;
+}
+template <int KV, int D, bool WIN>
+constexpr bool prefill_two_tiles() {
+  return WIN && KV == kKv16 && D == 128;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -2451,11 +2456,10 @@ __device__ __forceinline__ void run_chunks_kv4(WaveState<D, NT>& s, const PAPara
 // chunks past the wave's rows (loads and barriers only).
 // Under a window the chunks are those of its walk, and a masked loop goes ahead: the sinks' chunks and those in which
 // some row's window starts, to a whole turn of the ring.
-template <class E, int D, bool WIN>
+template <class E, int D, bool WIN, int NT>
 __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const SeqView& sv, int R, int seq,
                                              int kvh, int t, int c_lo, int c_hi, int w, bool partial,
                                              int64_t slot, int rest, int total) {
-  constexpr int NT = prefill_nt<kKv16, D, WIN>();
   constexpr int PRW = kWavesPerWG * 16 * NT;  // rows of a tile
   using L = PrefillLds<D>;
   c_lo = uni(c_lo);
@@ -2474,6 +2478,14 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
   int n_edge = 0;
   if constexpr (WIN)
     n_edge = max(0, walk_chunk(wn, (max(my_lim - p.WND, 0) + kChunk - 1) / kChunk) - c_lo);
+  // of them, those that none of its rows sees (a later wave's window starts up to three waves' rows on)
+  auto unseen = [&](int i) {
+    if constexpr (WIN) {
+      const int tok = walk_token(wn, (c_lo + i) * kChunk);
+      return tok >= p.SNK && tok + kChunk <= lim_all - p.WND;
+    }
+    return false;
+  };
 
   // the page window first: the first chunks' loads wait for it, the query tile is not
   // needed before they are in flight
@@ -2562,7 +2574,7 @@ __device__ __forceinline__ void prefill_tile(char* lds, const PAParams& p, const
     int st = 0;
     for (; i < ahead; ++i) {
       sync(i, (st == 0 ? 2 : st - 1) * L::kStageBytes);
-      compute(i, st * L::kStageBytes, S0{}, std::true_type{});
+      if (!unseen(i)) compute(i, st * L::kStageBytes, S0{}, std::true_type{});
       st = st == 2 ? 0 : st + 1;
     }
     if (st != 0) n_int = 0;  // the wave's rows end inside a turn
@@ -2626,6 +2638,14 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
   int n_edge = 0;
   if constexpr (WIN)
     n_edge = max(0, walk_chunk(wn, (max(my_lim - p.WND, 0) + kChunk - 1) / kChunk) - c_lo);
+  // of them, those that none of its rows sees (a later wave's window starts up to three waves' rows on)
+  auto unseen = [&](int i) {
+    if constexpr (WIN) {
+      const int tok = walk_token(wn, (c_lo + i) * kChunk);
+      return tok >= p.SNK && tok + kChunk <= lim_all - p.WND;
+    }
+    return false;
+  };
 
   // the page window first: the first chunks' loads wait for it, the query tile is not
   // needed before they are in flight
@@ -2762,7 +2782,7 @@ __device__ __forceinline__ void prefill_tile_convert(char* lds, const PAParams& 
         sync(i, I1{});
       else
         sync(i, I0{});
-      compute(i, (i & 1) * L::kStageBytes, S0{}, std::true_type{});
+      if (!unseen(i)) compute(i, (i & 1) * L::kStageBytes, S0{}, std::true_type{});
     }
     if (i & 1) n_int = 0;
   }
@@ -2942,7 +2962,11 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
     if (p.ND > 0 && b >= p.ND) {
       __shared__ PreStart st;
       __shared__ int64_t wsum[kPlanThreads / 64];
-      const bool work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV, D, WIN>(), WIN>(p, b - p.ND, &st, wsum);
+      bool work;
+      if (prefill_two_tiles<KV, D, WIN>() && p.PR == kWavesPerWG * 32)
+        work = prefill_start<kWavesPerWG * 32, WIN>(p, b - p.ND, &st, wsum);
+      else
+        work = prefill_start<kWavesPerWG * 16 * prefill_nt<KV, D, WIN>(), WIN>(p, b - p.ND, &st, wsum);
       if (threadIdx.x == 0) {
         if (!work) st.u = -1;  // idle, rewritten on every call
         ((PreStart*)p.ws_plan)[b - p.ND] = st;
@@ -2961,7 +2985,8 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
 // same amount of work whatever the mix of prompt lengths. A tile split between units leaves
 // partials: unit u keeps the piece of its first non-empty tile in slot 2u and of its last in
 // slot 2u + 1 (tiles in between are whole and written out), and the unit holding a split
-// tile's first piece records its merge job (in the record of its workgroup). Workgroups are
+// tile's first piece records its merge job (in the record of its workgroup). Under a window, where tiles are short and
+// alike, the units take whole tiles where that is cheaper (pre_whole_tiles). Workgroups are
 // dealt to the 8 XCDs round-robin, so the units are numbered XCD by XCD: the units of one
 // XCD are contiguous in the flat space and read the same sequence's K/V through that
 // XCD's L2.
@@ -3003,12 +3028,19 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   // empty and skipped.
   int64_t a = uni(st->rem);
   if constexpr (!PLANNED) __syncthreads();  // every wave has read the start before the tile's loads overwrite it
-  bool first = true;
+  bool first = true, whole_tiles = false;
+  if constexpr (WIN) whole_tiles = pre_whole_tiles(C, NUa, pre_full_tile(p.G, PR, p.WND, p.SNK));
   for (;;) {
     const int64_t tw = kTileCost + n_t;
-    const int64_t e = min(tw, a + (x1 - x));
+    if (whole_tiles) {
+      const int64_t mid = x - a + tw / 2;
+      if (mid >= x1) break;
+      const int rest = (int)max((int64_t)0, x1 - (x - a + tw));
+      if (mid >= x) tile(sv, R, seq, kvh, t, 0, n_t, false, 0, rest, total);
+    }
+    const int64_t e = whole_tiles ? tw : min(tw, a + (x1 - x));
     const int c_lo = (int)max((int64_t)0, a - kTileCost), c_hi = (int)max((int64_t)0, e - kTileCost);
-    if (c_hi > c_lo) {
+    if (!whole_tiles && c_hi > c_lo) {
       const bool whole = c_lo == 0 && c_hi == n_t;
       const int64_t slot = 2 * (int64_t)u + (first ? 0 : 1);
       const int rest = (int)(x1 - (x + (e - a)));
@@ -3045,24 +3077,24 @@ constexpr int prefill_lds_bytes() {
   return (KV == kKv16 ? PrefillLds<D>::kStages : 2) * PrefillLds<D>::kStageBytes;
 }
 
-template <class E, int D, int KV, bool PLANNED, bool WIN>
+template <class E, int D, int KV, bool PLANNED, bool WIN, int NT>
 __device__ __forceinline__ void prefill_unit(const PAParams& p, int block, char* lds) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  prefill_units<kWavesPerWG * 16 * prefill_nt<KV, D, WIN>(), PLANNED, WIN>(
+  prefill_units<kWavesPerWG * 16 * NT, PLANNED, WIN>(
       p, block, lds, [&](const SeqView& sv, int R, int seq, int kvh, int t, int c_lo, int c_hi, bool partial,
                          int64_t slot, int rest, int total) {
     if constexpr (KV != kKv16)
       prefill_tile_convert<E, D, KV, WIN>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
     else
-      prefill_tile<E, D, WIN>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
+      prefill_tile<E, D, WIN, NT>(lds, p, sv, R, seq, kvh, t, c_lo, c_hi, w, partial, slot, rest, total);
   });
 }
 
 // 4-wave workgroups of 64 NT rows (PAParams::PR), 2 per CU.
-template <class E, int D, int KV, bool WIN>
+template <class E, int D, int KV, bool WIN, int NT = prefill_nt<KV, D, WIN>()>
 __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
-  prefill_unit<E, D, KV, true, WIN>(p, blockIdx.x, lds);
+  prefill_unit<E, D, KV, true, WIN, NT>(p, blockIdx.x, lds);
 }
 
 // A mixed batch in one launch: the first ND workgroups are its decode units, the next NUP its
@@ -3070,14 +3102,14 @@ __global__ __launch_bounds__(256, 2) void pa_prefill_kernel(PAParams p) {
 // (launch_mixed): its workgroups leave their places at once, and no launch runs ahead of the
 // prefill work. Four prompts of 300-2500 tokens (D = 128, bf16): step 201 -> 176 us; two chunks
 // of 900-1024 tokens over 4000-10000 cached ones, E4M3: 328 -> 310 us.
-template <class E, int D, int KV, bool WIN>
+template <class E, int D, int KV, bool WIN, int NT = prefill_nt<KV, D, WIN>()>
 __global__ __launch_bounds__(256, 2) void pa_mixed_kernel(PAParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[prefill_lds_bytes<D, KV>()];
   const int b = blockIdx.x;
   if (b < p.ND)
     decode_unit<E, D, 1, KV, 1, line_dim(D) && KV == kKv16, WIN>(p, b, p.LINES);  // (E4M3: its units are too short for lines)
   else
-    prefill_unit<E, D, KV, false, WIN>(p, b - p.ND, lds);
+    prefill_unit<E, D, KV, false, WIN, NT>(p, b - p.ND, lds);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -3199,6 +3231,12 @@ static int launch_decode(PAParams& p, int NT, hipStream_t s) {
 // Decode chunks per unit up to which a mixed batch takes one launch (launch_mixed).
 constexpr int64_t kFusedUnitChunks = 4;
 
+// Sequences that are prefill class at least: each takes at most max_q of the T tokens.
+static int64_t prefill_seqs(const PAParams& p, int32_t max_q) {
+  const int64_t over = p.T - (int64_t)p.B * p.QS;
+  return over > 0 ? (over + max_q - p.QS - 1) / (max_q - p.QS) : 0;
+}
+
 // A batch with prefill-class sequences. Where the static shape leaves the decode part at most
 // kFusedUnitChunks chunks per unit (prompts alone, or with a few short decodes), decode and
 // prefill units share one launch. A larger decode part goes ahead in a launch of its own: the
@@ -3206,25 +3244,22 @@ constexpr int64_t kFusedUnitChunks = 4;
 // of 255-4095 keys beside four 384-token chunks 851 us in one launch, 816 apart; 100 decodes of
 // 255-2000 keys beside the same chunks 216 and 188; 512 decodes beside one 17-token chunk 721
 // and 741). Apart as well when a decode row needs more than one 16-row tile (GQA groups above 16).
-template <class E, int D, int KV, bool WIN>
-static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
-  p.PR = kWavesPerWG * 16 * prefill_nt<KV, D, WIN>();
+template <class E, int D, int KV, bool WIN, int PNT>
+static int launch_mixed_tiles(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
+  p.PR = kWavesPerWG * 16 * PNT;
   // units x 2 partial slots x tile rows stay within the workspace's kMaxPrefillUnits x 2 x kPrefillRows
   const int cap = kMaxPrefillUnits * kPrefillRows / p.PR;
-  // sequences that can be decode class: each of the others takes at most max_q of the T tokens
-  const int64_t over = p.T - (int64_t)p.B * p.QS;
-  const int64_t n_pre = over > 0 ? (over + max_q - p.QS - 1) / (max_q - p.QS) : 0;
-  const int64_t n_dec = p.B > n_pre ? p.B - n_pre : 0;
+  const int64_t n_pre = prefill_seqs(p, max_q), n_dec = p.B > n_pre ? p.B - n_pre : 0;
   const int64_t dec_chunks =
       n_dec * (p.Hkv / p.HGW) * ((seq_keys(p.W, p.BS, p.WND, p.SNK, p.QS) + kChunk - 1) / kChunk);
   int err, per_cu = 1;
-  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV, WIN>, 256, &per_cu);
+  const int resident = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV, WIN, PNT>, 256, &per_cu);
   const int wgs = decode_units(p, resident, per_cu, KV != kKv16, KV == kKv4 && D == 64);
   if (NT > 1 || dec_chunks > kFusedUnitChunks * p.NU) {
-    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV, WIN>), cap) / 8 * 8);
+    p.NUP = std::max(8, std::min(resident_blocks((const void*)&pa_prefill_kernel<E, D, KV, WIN, PNT>), cap) / 8 * 8);
     if ((err = launch_decode<E, D, KV, WIN>(p, NT, s))) return err;
     log.after_launch(KVH_KERNEL_DECODE, s);
-    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV, WIN>), dim3(p.NUP), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pa_prefill_kernel<E, D, KV, WIN, PNT>), dim3(p.NUP), dim3(256), 0, s, p);
     if ((err = (int)hipGetLastError())) return err;
     log.after_launch(KVH_KERNEL_PREFILL, s);
     return 0;
@@ -3232,10 +3267,21 @@ static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, Launc
   p.NUP = std::max(8, std::min(resident, cap) / 8 * 8);
   p.LINES = KV == kKv16 && line_launch(D, 0, p.k_ss * 2);
   p.ND = (wgs + 7) / 8 * 8;  // prefill workgroup b keeps XCD b % 8
-  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV, WIN>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pa_mixed_kernel<E, D, KV, WIN, PNT>), dim3(p.ND + p.NUP), dim3(256), 0, s, p);
   if ((err = (int)hipGetLastError())) return err;
   log.after_launch(KVH_KERNEL_MIXED, s);
   return 0;
+}
+
+template <class E, int D, int KV, bool WIN>
+static int launch_mixed(PAParams& p, int NT, int32_t max_q, hipStream_t s, LaunchLog& log) {
+  if constexpr (prefill_two_tiles<KV, D, WIN>()) {
+    const int64_t n_pre = prefill_seqs(p, max_q), n_dec = p.B > n_pre ? p.B - n_pre : 0;
+    const int units = resident_blocks((const void*)&pa_mixed_kernel<E, D, KV, WIN>);
+    if (pre_window_nt(std::max((int64_t)0, p.T - n_dec * p.QS) * p.G, n_pre, p.Hkv, p.G, p.WND, p.SNK, units) == 2)
+      return launch_mixed_tiles<E, D, KV, WIN, 2>(p, NT, max_q, s, log);
+  }
+  return launch_mixed_tiles<E, D, KV, WIN, prefill_nt<KV, D, WIN>()>(p, NT, max_q, s, log);
 }
 
 template <class E, int D, int KV, bool WIN>

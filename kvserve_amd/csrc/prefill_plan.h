@@ -141,4 +141,41 @@ KVH_PLAN_FN int64_t pre_skips(const PreSeq& s, int G, int PR, int WND, int SNK, 
   return n;
 }
 
+// Whether the units of a windowed launch take whole tiles, each those whose middle (its first position + half of its
+// positions) lies in the unit's range, instead of splitting tiles where ranges meet. A split tile's pieces are written in
+// fp32 and read back by the merge, as long as kSplitCost chunk steps a unit; whole tiles leave the last of a unit's
+// rounds of `tile` positions (a tile's where its rows see a whole window) part empty. Us split and whole, by the steps
+// left empty (32 heads over 8 of 128, bf16; prompt and window): 2 (3000, 512) 76 and 57, 13 (12000, 1024) 260 and 238,
+// 22 (8191, 1024) 194 and 182, 32 (4096, 1024) 108.9 and 110.4, 48 (8191, 2048) 275 and 293.
+constexpr int kSplitCost = 26;
+
+constexpr int pre_full_tile(int G, int PR, int WND, int SNK) {
+  return kTileCost + (int)(((int64_t)WND + (PR + G - 1) / G + kPlanChunk - 1) / kPlanChunk + 1 +
+                           ((int64_t)SNK + kPlanChunk - 1) / kPlanChunk);
+}
+
+KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t units, int tile) {
+  const int64_t per = C / units, left = per % tile;
+  return left == 0 || tile - left <= kSplitCost;
+}
+
+// 16-row tiles a wave takes under a window, 3 or 2, for `rows` query rows per kv head in `seqs` sequences: the cheaper by
+// the above, with steps of 40 and 31 (a long prompt, window 4096: 936 us and 1060). Tiles of 2 fill a launch better that
+// has few, or whose last round is part empty: (2000, 512) 49 us and 41, (4096, 1024) 109 and 94.5, chunks of 1000 and 900
+// tokens over thousands, window 2048, 107 and 89, of 200 tokens, window 1024, 41 and 37; but (3000, 512) 57 and 63,
+// (12000, 1024) 238 and 256.
+inline int64_t pre_window_cost(int nt, int64_t rows, int64_t seqs, int Hkv, int G, int WND, int SNK, int64_t units) {
+  const int64_t PR = 64 * nt, step = nt == 3 ? 40 : 31;
+  const int64_t tiles = Hkv * ((rows + PR - 1) / PR + (seqs > 1 ? (seqs - 1) / 2 : 0));
+  const int64_t tile = pre_full_tile(G, (int)PR, WND, SNK);
+  const int64_t whole = (tiles + units - 1) / units * tile * step;
+  const int64_t split = tiles * tile * step / units + kSplitCost * (nt == 3 ? 40 : 27);  // (the pieces' rows)
+  return whole < split ? whole : split;
+}
+
+inline int pre_window_nt(int64_t rows, int64_t seqs, int Hkv, int G, int WND, int SNK, int64_t units) {
+  return pre_window_cost(2, rows, seqs, Hkv, G, WND, SNK, units) < pre_window_cost(3, rows, seqs, Hkv, G, WND, SNK, units)
+             ? 2 : 3;
+}
+
 }  // namespace kvh

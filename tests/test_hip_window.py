@@ -287,3 +287,14 @@ def test_no_sequences_and_refusals(hip_device):
         HipAttention.forward(b.q.cpu(), b.k, b.v, b.meta, b.scale, window=8)
     with pytest.raises(ValueError):
         HipAttention.forward(b.q.float(), b.k, b.v, b.meta, b.scale, window=8)
+
+
+@pytest.mark.parametrize("kv", ["own", "e4m3", "fp4"])
+@pytest.mark.parametrize("q_lens,ctx,H,D,window,sinks", [
+    ([3000], [0], 32, 128, 512, 0), ([2000], [0], 32, 128, 500, 4), ([5000], [0], 32, 128, 2048, 0), ([512], [3001], 32, 128, 1000, 70),
+    ([2900, 900, 1], [100, 3000, 2000], 32, 64, 300, 33), ([1000, 900] + [1] * 12, [2000, 3000] + [1700] * 12, 40, 128, 1024, 64),
+])  # fmt: skip
+def test_prompts_that_fill_the_launch(hip_device, kv, q_lens, ctx, H, D, window, sinks):
+    """Tiles of two and of three to a wave, whole to a unit and split between units."""
+    b = Batch(hip_device, q_lens, ctx, H, 8, D, 16, window, sinks, torch.bfloat16, kv, seed=len(q_lens) + window)
+    b.check(b.forward())

@@ -22,6 +22,14 @@ using namespace kvh;
 extern "C" {
 int skip(int R, int q, int kv, int64_t ctx, int G, int PR, int W, int S, int t) { return pre_tile_skip({R, q, kv, ctx}, G, PR, W, S, t); }
 int64_t skips(int R, int q, int kv, int64_t ctx, int G, int PR, int W, int S, int t) { return pre_skips({R, q, kv, ctx}, G, PR, W, S, t); }
+int chunks(int R, int q, int kv, int64_t ctx, int G, int PR, int W, int S, int t) {
+  return kTileCost + pre_tile_chunks({R, q, kv, ctx}, G, PR, t) - pre_tile_skip({R, q, kv, ctx}, G, PR, W, S, t);
+}
+int full_tile(int G, int PR, int W, int S) { return pre_full_tile(G, PR, W, S); }
+int whole_tiles(int64_t C, int64_t units, int tile) { return pre_whole_tiles(C, units, tile); }
+int window_nt(int64_t rows, int64_t seqs, int Hkv, int G, int W, int S, int64_t units) {
+  return pre_window_nt(rows, seqs, Hkv, G, W, S, units);
+}
 }
 """
 
@@ -40,7 +48,49 @@ def plan(tmp_path_factory):
     i, l = ctypes.c_int, ctypes.c_int64
     lib.skip.argtypes = lib.skips.argtypes = [i, i, i, l, i, i, i, i, i]
     lib.skips.restype = l
+    lib.chunks.argtypes = lib.skip.argtypes
+    lib.whole_tiles.argtypes = [l, l, i]
+    lib.window_nt.argtypes = [l, l, i, i, i, i, l]
     return lib
+
+
+@pytest.mark.parametrize("PR,G", [(128, 4), (192, 4), (192, 1), (128, 7), (192, 64)])
+def test_whole_tiles_are_shared_out_once(plan, PR, G):
+    """Units that take the tiles whose middle lies in their range take every tile once, none more than a round above the
+    mean; and no tile is longer than the one the rule counts with."""
+    rng = random.Random(PR + G)
+    for _ in range(40):
+        W, S = rng.randint(1, 3000), rng.choice([0, 0, 1, 33, 200])
+        full = plan.full_tile(G, PR, W, S)
+        sizes = []
+        for _ in range(rng.randint(1, 5)):
+            q, ctx = rng.randint(1, 3000), rng.choice([0, rng.randint(0, 9000)])
+            R = q * G
+            sizes += [plan.chunks(R, q, q + ctx, ctx, G, PR, W, S, t) for t in range(-(-R // PR))] * rng.randint(1, 8)
+        assert max(sizes) <= full
+        C, units = sum(sizes), rng.randint(1, 512)
+        units = min(units, -(-C // 2))
+        owner, x = [], 0
+        for tw in sizes:
+            mid = x + tw // 2
+            owner.append(((mid + 1) * units - 1) // C)  # the unit u with u C / units <= mid < (u + 1) C / units
+            assert owner[-1] * C // units <= mid < (owner[-1] + 1) * C // units
+            x += tw
+        load = [0] * units
+        for u, tw in zip(owner, sizes):
+            load[u] += tw
+        assert max(load) <= C // units + 1 + full
+        left = C // units % full
+        assert bool(plan.whole_tiles(C, units, full)) == (left == 0 or full - left <= 26)
+
+
+def test_tiles_a_wave(plan):
+    """Two where that fills the launch better: the measured cases of 32 heads over 8 on 512 units."""
+    for q, seqs, W, S, want in ((8191, 1, 1024, 0, 3), (8191, 1, 4096, 0, 3), (4096, 1, 1024, 0, 2), (2000, 1, 512, 0, 2),
+                                (3000, 1, 512, 0, 3), (12000, 1, 1024, 0, 3), (1900, 2, 2048, 64, 2), (200, 1, 1024, 0, 2)):  # fmt: skip
+        assert plan.window_nt(4 * q, seqs, 8, 4, W, S, 512) == want
+    for args in ((0, 0, 1, 1, 1, 0, 8), (1, 1, 1, 64, 2**31 - 1, 0, 512), (2**40, 65535, 128, 64, 2**30, 2**30, 512)):
+        assert plan.window_nt(*args) in (2, 3)
 
 
 @pytest.mark.parametrize("PR", [128, 192])
