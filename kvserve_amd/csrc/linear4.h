@@ -15,9 +15,14 @@ struct Linear4Form {
 };
 
 constexpr int linear4_chunk(const Linear4Form& f) { return f.wk * f.s; }
-// LDS of a workgroup: two chunks of x, or the waves' sums
+// Whether the waves that read the same x take turns at its groups' sums, four of them a group of weight rows (gated 64;
+// 28672 x 4096: 33.5 us, so 30.7; two of them 8.6, 8.9 at (24; 16384 x 2048))
+constexpr bool linear4_shares(const Linear4Form& f) { return f.wr >= 4 && f.rows > 16; }
+constexpr int linear4_x(const Linear4Form& f) { return 2 * f.wk * f.s * f.rows * 2 * kW4Block; }
+// LDS of a workgroup: two chunks of x with its sums over up to four groups a block, or the waves' sums
 constexpr int linear4_lds(const Linear4Form& f) {
-  const int x = 2 * f.wk * f.s * f.rows * 2 * kW4Block, sums = f.wr * f.wk * f.rt * ((f.rows + 15) / 16) * 1024;
+  const int x = linear4_x(f) + (linear4_shares(f) ? 2 * f.wk * f.s * 4 * f.rows * 4 : 0);
+  const int sums = f.wr * f.wk * f.rt * ((f.rows + 15) / 16) * 1024;
   return x > sums ? x : sums;
 }
 
@@ -28,12 +33,12 @@ constexpr int linear4_lds(const Linear4Form& f) {
 //    where two would load the CUs unevenly ((g 8; 28672 x 4096) 14.4 and 15.1; but (8; 32768 x 4096) 17.9 and 15.5).
 //  * Up to 32 rows likewise ((20; 4096 x 4096) 8.1, in four splits 8.9; (32; 6144 x 4096) 9.6, 10.7; (g 24; 16384 x 2048)
 //    8.6, four groups 11.5), then eight tiles in two groups for one round of workgroups, in four for more ((g 32; 28672 x
-//    4096) 19.6 and 21.4; (32; 128256 x 2048) 46.6 and 39.9).
+//    4096) 19.6 and 21.4; (32; 128256 x 2048) 48.3 and 38.5).
 //  * More rows: x is as many bytes as the weight, so groups of 128 weight rows share it, and what that leaves of the CUs is
-//    filled by splitting k, four chunks at least each: (33; 2048 x 8192) 13.2 in eight splits, 14.1 in sixteen;
-//    (64; 4096 x 14336) 23.3 in eight, 25.6 in six; (100; 4096 x 4096) 16.5 in four, 19.7 in two.
+//    filled by splitting k, four chunks at least each: (33; 2048 x 8192) 13.1 in eight splits, 13.8 in twelve;
+//    (64; 4096 x 14336) 22.6 in eight, 24.7 in six; (100; 4096 x 4096) 16.3 in four, 19.1 in two.
 //  * Past 64 rows of x the MFMAs and the codes' conversion bound it, which add up on this GPU: 256 weight rows and 64 of x
-//    a workgroup where they fill it ((500; 6144 x 4096) 41.7, 128 rows 58.8; but (g 100; 16384 x 2048) 23.3 and 18.8).
+//    a workgroup where they fill it ((500; 6144 x 4096) 39.7, 128 rows 54.5; but (g 100; 16384 x 2048) 23.3 and 18.8).
 inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m, bool glu) {
   if (m <= 16) {
     if (tiles <= 256 && !glu) {

@@ -72,7 +72,10 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
   constexpr int TOTAL = KB * ROWS * 16, PIECES = (TOTAL + 64 * W - 1) / (64 * W);  // of 16 bytes, in a chunk, a thread
   static_assert(!GLU || RT % 2 == 0);
   static_assert(S % PD == 0 || PD % S == 0);
-  __shared__ __attribute__((aligned(16))) char lds[linear4_lds(Linear4Form{ROWS, RT, WR, WK, S, 1})];
+  constexpr Linear4Form kForm{ROWS, RT, WR, WK, S, 1};
+  constexpr bool SHARE = linear4_shares(kForm);
+  static_assert(!SHARE || ROWS % 16 == 0);
+  __shared__ __attribute__((aligned(16))) char lds[linear4_lds(kForm)];
   const int lane = threadIdx.x & 63, j = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave % WR, wk = wave / WR;
@@ -132,7 +135,42 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
   };
   uint32_t k16 = Code<E>::k16;
   asm("" : "+v"(k16));  // in a register: an instruction takes one constant
-  auto step = [&](const Codes& d, const char* xb) __attribute__((always_inline)) {
+  // SHARE: X of block i of a chunk in buffer `buf`, [group][row], written by the waves of a slice in turn and read a
+  // chunk later, behind the barrier that is there; minus s z of the blocks that it is for meanwhile in sz.
+  float sz[SHARE ? S : 1][RT][NG];
+  auto sums_of = [&](int buf, int i) __attribute__((always_inline)) {
+    return (float*)(lds + linear4_x(kForm)) + (buf * KB + wk * S + i) * NG * ROWS;
+  };
+  auto write_sums = [&](const char* xb, float* X) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < (MT + WR - 1) / WR; ++q) {
+      const int t = q * WR + wr;
+      if (t >= MT) break;
+      const char* row = xb + (16 * t + n) * 2 * kW4Block;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = g * SPG; u < (g + 1) * SPG; ++u)
+          v = E::mfma(*(const u32x4*)(row + 16 * ((4 * u + j) ^ n)),
+                      u32x4{Code<E>::kOne, Code<E>::kOne, Code<E>::kOne, Code<E>::kOne}, v);
+        if (n == 0) *(f32x4*)(X + g * ROWS + 16 * t + 4 * j) = v;
+      }
+    }
+  };
+  auto subtract = [&](int i, const float* X) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const f32x4 v = *(const f32x4*)(X + g * ROWS + 16 * t + 4 * j);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(sz[i][r][g], v[e], acc[r][t][e]);
+      }
+  };
+  auto step = [&](const Codes& d, const char* xb, int i) __attribute__((always_inline)) {
     u32x4 x[kSteps][MT];
 #pragma unroll
     for (int u = 0; u < kSteps; ++u)
@@ -145,7 +183,7 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
     for (int g = 0; g < NG; ++g) {
       f32x4 X[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int t = 0; t < MT && !SHARE; ++t) {
         X[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = g * SPG; u < (g + 1) * SPG; ++u)
@@ -163,10 +201,12 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
           for (int t = 0; t < MT; ++t) ag[t] = E::mfma(x[u][t], q, ag[t]);
         }
         const float s = E::to_f32((uint16_t)(d.s[r][g] & 0xffffu)), z = E::to_f32((uint16_t)(d.s[r][g] >> 16));
+        if constexpr (SHARE) sz[i][r][g] = -s * z;  // exact
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(s, __builtin_fmaf(-z, X[t][e], ag[t][e]), acc[r][t][e]);
+          for (int e = 0; e < 4; ++e)
+            acc[r][t][e] = __builtin_fmaf(s, SHARE ? ag[t][e] : __builtin_fmaf(-z, X[t][e], ag[t][e]), acc[r][t][e]);
       }
     }
   };
@@ -188,11 +228,19 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
       const bool more = c + 1 < c_hi;
       if (more) stage_load(c + 1);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (SHARE)
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+          if (c > c_lo) subtract(i, sums_of((c - 1 - c_lo) & 1, i));  // (an earlier chunk is whole)
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         const int b = c * KB + wk * S + i;
         Codes& wi = w[(cc * S + i) % PD];
-        if (b < a.blocks) step(wi, lds + (((c - c_lo) & 1) * KB + wk * S + i) * XB);
+        if (b < a.blocks) {
+          const char* xb = lds + (((c - c_lo) & 1) * KB + wk * S + i) * XB;
+          if constexpr (SHARE) write_sums(xb, sums_of((c - c_lo) & 1, i));
+          step(wi, xb, i);
+        }
         __builtin_amdgcn_sched_barrier(0);
         load_codes(wi, (c + (i + PD) / S) * KB + wk * S + (i + PD) % S);  // the block PD steps on
         __builtin_amdgcn_sched_barrier(0);
@@ -204,6 +252,12 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
   // the slices' sums in order: lane l of a wave takes row l / 4 and columns 4 (l % 4) .. of an output tile
   float* red = (float*)lds;
   __syncthreads();
+  if constexpr (SHARE) {
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+      if ((c_hi - 1) * KB + wk * S + i < a.blocks) subtract(i, sums_of((c_hi - 1 - c_lo) & 1, i));
+    __syncthreads();
+  }
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
