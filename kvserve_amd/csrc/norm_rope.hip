@@ -9,7 +9,9 @@
 // A lane holds a granule of 8 elements, a group of L = 8, 16 or 32 lanes a head (the power of two from D / 8 up): the sum
 // of squares takes log2 L DPP steps, no LDS. The other half's elements of a pair (i, i + R/2) are loaded as a granule
 // of their own, which the caches hold already, instead of moved between lanes. A thread keeps its place in the head over
-// all of a token's heads, so that the table row and the weights are read once.
+// all of a token's heads, so that the table row and the weights are read once, and loads a pass ahead of what it computes
+// (2048 tokens of 32 + 2 * 8 heads of 128, bf16, HBM-cold: 19.0 us, so 15.4; a copy of the projection takes 11.6). Bound by
+// HBM (8192: 44.6 us, 4.5 TB/s) or, at a decode step's few tokens, by one launch.
 #include "cache_rows.h"
 #include "kvh_device.h"
 #include "kvh_internal.h"
@@ -46,6 +48,27 @@ __device__ __forceinline__ void store_e4m3(uint8_t* dst, const float (&x)[8], fl
   *(u32x2*)dst = u32x2{fp8_pack4(y[0], y[1], y[2], y[3]), fp8_pack4(y[4], y[5], y[6], y[7])};
 }
 
+// 8 elements as they lie in memory.
+template <int DT>
+struct Granule {
+  u32x4 w[DT == 0 ? 2 : 1];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    w[0] = *(const u32x4*)p;
+    if constexpr (DT == 0) w[1] = *(const u32x4*)(p + 16);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (DT == 0) {
+        x[i] = __uint_as_float(w[i / 4][i % 4]);
+      } else {
+        const uint16_t h = (uint16_t)(w[0][i / 2] >> (16 * (i & 1)));
+        x[i] = DT == 2 ? BF16::to_f32(h) : F16::to_f32(h);
+      }
+    }
+  }
+};
+
 // Workgroup (t, part) takes heads part * hpw .. of token t: query heads, then key heads, then value heads.
 template <int DT, int CACHE, int L, bool PAIRS>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a) {
@@ -56,11 +79,29 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a) {
   const int d = in ? 8 * g : 0;
   const bool rot = d < a.R, low = d < half;
   const int d2 = rot && !PAIRS ? (low ? d + half : d - half) : d;  // the granule of the pairs' other elements
+  const uint8_t* row = a.qkv + t * a.qkv_ts * EB;
+  const int NH = a.H + 2 * a.Hkv, h0 = blockIdx.y * a.hpw, h1 = min(h0 + a.hpw, NH);
+  // one pass ahead: this granule and the pairs' other one of the next head
+  Granule<DT> xn, yn;
+  auto load_head = [&](int hb) __attribute__((always_inline)) {
+    const uint8_t* src = row + (int64_t)min(hb + (int)(threadIdx.x / L), h1 - 1) * D * EB;
+    xn.load(src + d * EB);
+    if (!PAIRS) yn.load(src + d2 * EB);
+  };
+  load_head(h0);
+  Granule<DT> wq[2], wk[2];
+  if (a.q_norm) {
+    wq[0].load((const uint8_t*)a.q_norm + d * EB);
+    wq[1].load((const uint8_t*)a.q_norm + d2 * EB);
+  }
+  if (a.k_norm) {
+    wk[0].load((const uint8_t*)a.k_norm + d * EB);
+    wk[1].load((const uint8_t*)a.k_norm + d2 * EB);
+  }
   const int64_t pos = clamp64(a.positions[t], 0, a.max_pos - 1);
   const int64_t slot = a.slots[t];
   const bool in_pool = slot >= 0 && slot < a.num_slots;
   const int64_t blk = in_pool ? slot / a.BS : 0, off = in_pool ? slot % a.BS : 0;
-  const uint8_t* row = a.qkv + t * a.qkv_ts * EB;
   // the factors of this granule's own and other elements
   float c[8], s[8];
 #pragma unroll
@@ -80,26 +121,24 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a) {
       for (int i = 0; i < 8; ++i) s[i] = low ? -s[i] : s[i];
     }
   }
-  const int NH = a.H + 2 * a.Hkv, h0 = blockIdx.y * a.hpw, h1 = min(h0 + a.hpw, NH);
   for (int hb = h0; hb < h1; hb += HEADS) {
     const int hw = hb + threadIdx.x / L;
     const int h = min(hw, h1 - 1);  // a group past the last head repeats it and stores nothing
     const bool is_q = h < a.H, is_v = h >= a.H + a.Hkv;
-    const uint8_t* src = row + (int64_t)h * D * EB;
     float x[8], y[8];
-    Rows<DT>::load8(src + d * EB, x);
-    if (!PAIRS) Rows<DT>::load8(src + d2 * EB, y);
-    const uint8_t* w = (const uint8_t*)(is_q ? a.q_norm : a.k_norm);
+    xn.get(x);
+    if (!PAIRS) yn.get(y);
+    if (hb + HEADS < h1) load_head(hb + HEADS);
     if (!is_v) {
-      if (w) {
+      if (is_q ? a.q_norm : a.k_norm) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
         ss = group_sum<L>(in ? ss : 0.f);
         const float r = rsqrtf(ss / (float)D + a.eps);
         float wx[8], wy[8];
-        Rows<DT>::load8(w + d * EB, wx);
-        if (!PAIRS) Rows<DT>::load8(w + d2 * EB, wy);
+        (is_q ? wq : wk)[0].get(wx);
+        if (!PAIRS) (is_q ? wq : wk)[1].get(wy);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] = x[i] * r * wx[i];
@@ -139,7 +178,10 @@ template <int DT, int CACHE, int L>
 int launch(NormRopeArgs a, bool pairs, int64_t T, hipStream_t s) {
   constexpr int heads = kThreads / L;
   const int NH = a.H + 2 * a.Hkv;
-  // few tokens: a workgroup for each pass over `heads` heads, so that a step of a few sequences is one round of loads
+  // few tokens: a workgroup for each pass over `heads` heads, so that a step of a few sequences is one round of loads;
+  // many: one for a token, whose table row and weights are read once (32 + 2 * 8 heads of 128, HBM-cold, us: 8 tokens 3.0
+  // and 4.0, 256 4.4 and 5.0, 512 6.5 and 6.0, 2048 19.1 and 15.4, 8192 64.6 and 44.6; of 64: 256 3.7 and 4.1, 2048 12.8
+  // and 11.0)
   a.hpw = T >= 512 ? NH : heads;
   const dim3 grid((unsigned)T, (NH + a.hpw - 1) / a.hpw);
   if (pairs)
