@@ -3029,7 +3029,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   int64_t a = uni(st->rem);
   if constexpr (!PLANNED) __syncthreads();  // every wave has read the start before the tile's loads overwrite it
   bool first = true, whole_tiles = false;
-  if constexpr (WIN) whole_tiles = pre_whole_tiles(C, NUa, pre_full_tile(p.G, PR, p.WND, p.SNK));
+  if constexpr (WIN) whole_tiles = pre_whole_tiles(C, NUa, p.NUP, pre_full_tile(p.G, PR, p.WND, p.SNK));
   for (;;) {
     const int64_t tw = kTileCost + n_t;
     if (whole_tiles) {

@@ -143,10 +143,11 @@ KVH_PLAN_FN int64_t pre_skips(const PreSeq& s, int G, int PR, int WND, int SNK, 
 
 // Whether the units of a windowed launch take whole tiles, each those whose middle (its first position + half of its
 // positions) lies in the unit's range, instead of splitting tiles where ranges meet. A split tile's pieces are written in
-// fp32 and read back by the merge, as long as kSplitCost chunk steps a unit; whole tiles leave the last of a unit's
-// rounds of `tile` positions (a tile's where its rows see a whole window) part empty. Us split and whole, by the steps
-// left empty (32 heads over 8 of 128, bf16; prompt and window): 2 (3000, 512) 76 and 57, 13 (12000, 1024) 260 and 238,
-// 22 (8191, 1024) 194 and 182, 32 (4096, 1024) 108.9 and 110.4, 48 (8191, 2048) 275 and 293.
+// fp32 and read back by the merge, as long as kSplitCost chunk steps where all units hold pieces; whole tiles leave the
+// last of a unit's rounds of `tile` positions (a tile's where its rows see a whole window) part empty. Us split and whole,
+// by the steps left empty (32 heads over 8 of 128, bf16; prompt and window): 2 (3000, 512) 76 and 57, 13 (12000, 1024) 260
+// and 238, 22 (8191, 1024) 194 and 182, 32 (4096, 1024) 108.9 and 110.4, 48 (8191, 2048) 275 and 293. Chunks over 4000
+// tokens: 20 (400, 512) 42 and 31, 29 (512, 1024) 41 and 50; on a third of the units: 21 (40, 512) 26 and 30.
 constexpr int kSplitCost = 26;
 
 constexpr int pre_full_tile(int G, int PR, int WND, int SNK) {
@@ -154,9 +155,10 @@ constexpr int pre_full_tile(int G, int PR, int WND, int SNK) {
                            ((int64_t)SNK + kPlanChunk - 1) / kPlanChunk);
 }
 
-KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t units, int tile) {
+// C positions over `units` of the launch's `all` units.
+KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t units, int64_t all, int tile) {
   const int64_t per = C / units, left = per % tile;
-  return left == 0 || tile - left <= kSplitCost;
+  return left == 0 || (tile - left) * all <= kSplitCost * units;
 }
 
 // 16-row tiles a wave takes under a window, 3 or 2, for `rows` query rows per kv head in `seqs` sequences: the cheaper by
@@ -169,7 +171,8 @@ inline int64_t pre_window_cost(int nt, int64_t rows, int64_t seqs, int Hkv, int 
   const int64_t tiles = Hkv * ((rows + PR - 1) / PR + (seqs > 1 ? (seqs - 1) / 2 : 0));
   const int64_t tile = pre_full_tile(G, (int)PR, WND, SNK);
   const int64_t whole = (tiles + units - 1) / units * tile * step;
-  const int64_t split = tiles * tile * step / units + kSplitCost * (nt == 3 ? 40 : 27);  // (the pieces' rows)
+  const int64_t used = tiles * tile / 2 < units ? tiles * tile / 2 : units;
+  const int64_t split = tiles * tile * step / units + kSplitCost * (nt == 3 ? 40 : 27) * used / units;  // (the pieces' rows)
   return whole < split ? whole : split;
 }
 

@@ -26,7 +26,7 @@ int chunks(int R, int q, int kv, int64_t ctx, int G, int PR, int W, int S, int t
   return kTileCost + pre_tile_chunks({R, q, kv, ctx}, G, PR, t) - pre_tile_skip({R, q, kv, ctx}, G, PR, W, S, t);
 }
 int full_tile(int G, int PR, int W, int S) { return pre_full_tile(G, PR, W, S); }
-int whole_tiles(int64_t C, int64_t units, int tile) { return pre_whole_tiles(C, units, tile); }
+int whole_tiles(int64_t C, int64_t units, int64_t all, int tile) { return pre_whole_tiles(C, units, all, tile); }
 int window_nt(int64_t rows, int64_t seqs, int Hkv, int G, int W, int S, int64_t units) {
   return pre_window_nt(rows, seqs, Hkv, G, W, S, units);
 }
@@ -49,7 +49,7 @@ def plan(tmp_path_factory):
     lib.skip.argtypes = lib.skips.argtypes = [i, i, i, l, i, i, i, i, i]
     lib.skips.restype = l
     lib.chunks.argtypes = lib.skip.argtypes
-    lib.whole_tiles.argtypes = [l, l, i]
+    lib.whole_tiles.argtypes = [l, l, l, i]
     lib.window_nt.argtypes = [l, l, i, i, i, i, l]
     return lib
 
@@ -81,7 +81,7 @@ def test_whole_tiles_are_shared_out_once(plan, PR, G):
             load[u] += tw
         assert max(load) <= C // units + 1 + full
         left = C // units % full
-        assert bool(plan.whole_tiles(C, units, full)) == (left == 0 or full - left <= 26)
+        assert bool(plan.whole_tiles(C, units, 512, full)) == (left == 0 or (full - left) * 512 <= 26 * units)
 
 
 def test_tiles_a_wave(plan):
