@@ -31,14 +31,17 @@ constexpr int linear4_lds(const Linear4Form& f) {
 //    6.4), in sixteen slices of a long k ((8; 4096 x 14336) 10.9, in eight 11.8); two tiles behind that ((16; 6144 x 4096)
 //    7.1, one 10.5), and two groups, which share x ((16; 9216 x 4096) 8.6; (8; 12288 x 4096) 8.6, one group 11.9), or four
 //    where two would load the CUs unevenly ((g 8; 28672 x 4096) 14.4 and 15.1; but (8; 32768 x 4096) 17.9 and 15.5).
-//  * Up to 32 rows likewise ((20; 4096 x 4096) 8.1, in four splits 8.9; (32; 6144 x 4096) 9.6, 10.7; (g 24; 16384 x 2048)
-//    8.6, four groups 11.5), then eight tiles in two groups for one round of workgroups, in four for more ((g 32; 28672 x
-//    4096) 19.6 and 21.4; (32; 128256 x 2048) 48.3 and 38.5).
-//  * More rows: x is as many bytes as the weight, so groups of 128 weight rows share it, and what that leaves of the CUs is
-//    filled by splitting k, four chunks at least each: (33; 2048 x 8192) 13.1 in eight splits, 13.8 in twelve;
-//    (64; 4096 x 14336) 22.6 in eight, 24.7 in six; (100; 4096 x 4096) 16.3 in four, 19.1 in two.
+//  * More rows: workgroups of 32, 64, 128 or 256 weight rows, the fewest whose number fits the CUs once, in four slices of
+//    k up to 64: (500; 2048 x 2048) 11.7 with 64, 16.0 with 128; (64; 12288 x 4096) 18.7, 22.1; (64; 6144 x 4096) 14.5 with
+//    32, 15.3 with 64, 16.5 with 128. Each reads all of x: where that is more than 128 MB in all, wider ones ((250; 2048 x
+//    8192) 21.1 with 128, 22.8 with 64), or 80 MB where they would be split besides ((48; 4096 x 8192) 14.8 with 64, 15.4
+//    with 32). What they leave of the CUs is filled by splitting k, four chunks at least each: (33; 2048 x 8192) 10.9 in four.
+//  * Up to 32 rows eight slices in workgroups of 16 or 32 weight rows, as long as k is short ((20; 4096 x 4096) 8.1, 32 rows
+//    8.9; (20; 6144 x 4096) 9.1, four slices 9.6).
+//  * Where workgroups of 64 weight rows are too many, up to 48 rows of x take four tiles a wave in two groups for one round,
+//    two in four groups for more ((g 32; 28672 x 4096) 19.6 and 21.4; (32; 128256 x 2048) 48.3 and 38.5).
 //  * Past 64 rows of x the MFMAs and the codes' conversion bound it, which add up on this GPU: 256 weight rows and 64 of x
-//    a workgroup where they fill it ((500; 6144 x 4096) 39.7, 128 rows 54.5; but (g 100; 16384 x 2048) 23.3 and 18.8).
+//    a workgroup where they fill it ((500; 6144 x 4096) 39.7, 128 rows 54.5; but (g 100; 16384 x 2048) 22.7 and 18.0).
 inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m, bool glu) {
   if (m <= 16) {
     if (tiles <= 256 && !glu) {
@@ -48,22 +51,25 @@ inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m, bool g
     if (tiles < 768 && !glu) return {16, 2, 1, 8, 2, 1};
     return tiles > 1024 && tiles <= 1792 ? Linear4Form{16, 2, 4, 4, 2, 1} : Linear4Form{16, 2, 2, 4, 2, 1};
   }
-  Linear4Form f;
-  if (m <= 32) {
-    if (tiles < 512 && blocks < 48 && !glu)
-      return tiles <= 256 ? Linear4Form{32, 1, 1, 8, 1, 1} : Linear4Form{32, 1, 2, 8, 1, 1};
-    if (tiles >= 512 && tiles < 1536) return {32, 2, 2, 4, 2, 1};
-    if (tiles >= 1536 && tiles <= 2048) return {32, 4, 2, 4, 1, 1};
-    f = {32, 2, 4, 2, 1, 1};
-  } else if (m <= 48) {
-    if (tiles >= 1536) return {48, 4, 2, 4, 1, 1};
-    f = {48, 2, 4, 2, 1, 1};
-  } else if (m > 64 && (tiles + 15) / 16 * ((m + 63) / 64) >= 150) {
-    return {64, 4, 4, 2, 1, 1};
-  } else {
-    f = {64, 2, 4, 2, 1, 1};
+  if (m <= 32 && blocks < 48 && !glu) {
+    if (tiles <= 256) return {32, 1, 1, 8, 1, 1};
+    if (tiles < 512) return {32, 1, 2, 8, 1, 1};
   }
-  const int64_t groups = (tiles + 7) / 8 * ((m + 63) / 64), most = (blocks + f.wk - 1) / f.wk / 4;
+  const int rows = m <= 32 ? 32 : (m <= 48 ? 48 : 64);
+  const int64_t mb = (m + 63) / 64;
+  auto fits = [&](int64_t groups) {
+    return groups <= 256 && groups * rows * blocks * 2 * kW4Block <= (groups > 128 ? 128 : 80) * (int64_t)(1 << 20);
+  };
+  Linear4Form f{rows, 2, 4, 2, 1, 1};
+  if (!glu && fits((tiles + 1) / 2 * mb))
+    f = {rows, 1, 2, 4, 1, 1};
+  else if (fits((tiles + 3) / 4 * mb))
+    f = {rows, 2, 2, 4, 1, 1};
+  else if (m <= 48 && tiles > 1024 && tiles <= 2048)
+    return {rows, 4, 2, 4, 1, 1};
+  else if (m > 64 && (tiles + 15) / 16 * mb >= 150)
+    return {64, 4, 4, 2, 1, 1};
+  const int64_t groups = (tiles + f.rt * f.wr - 1) / (f.rt * f.wr) * mb, most = (blocks + f.wk - 1) / f.wk / 4;
   const int64_t z = 256 / groups < most ? 256 / groups : most;
   f.splits = z > 1 ? (int)z : 1;
   return f;

@@ -340,15 +340,20 @@ int launch_form(const Linear4Args& a, const Linear4Form& f, hipStream_t s) {
     KVH_FORM(16, 2, 1, 8, 2)
     KVH_FORM(32, 1, 1, 8, 1)
     KVH_FORM(32, 1, 2, 8, 1)
+    KVH_FORM(32, 1, 2, 4, 1)
+    KVH_FORM(48, 1, 2, 4, 1)
+    KVH_FORM(64, 1, 2, 4, 1)
   }
   KVH_FORM(16, 2, 2, 4, 2)
   KVH_FORM(16, 2, 4, 4, 2)
-  KVH_FORM(32, 2, 2, 4, 2)
+  KVH_FORM(32, 2, 2, 4, 1)
+  KVH_FORM(48, 2, 2, 4, 1)
+  KVH_FORM(64, 2, 2, 4, 1)
   KVH_FORM(32, 2, 4, 2, 1)
-  KVH_FORM(32, 4, 2, 4, 1)
   KVH_FORM(48, 2, 4, 2, 1)
-  KVH_FORM(48, 4, 2, 4, 1)
   KVH_FORM(64, 2, 4, 2, 1)
+  KVH_FORM(32, 4, 2, 4, 1)
+  KVH_FORM(48, 4, 2, 4, 1)
   KVH_FORM(64, 4, 4, 2, 1)
 #undef KVH_FORM
   return (int)hipErrorInvalidValue;

@@ -201,3 +201,30 @@ def test_refusals(hip_device):
             linear4(x, w, out=out)
     with pytest.raises(RuntimeError):
         linear4(torch.empty((3, 260), dtype=x.dtype, device=dev)[:, 2:258], w)  # rows that are not 16-byte aligned
+
+
+@pytest.mark.parametrize("dtype,group", [(torch.bfloat16, 128), (torch.float16, 32), (torch.bfloat16, 64)], ids=str)
+@pytest.mark.parametrize("m,n", [(40, 1040), (64, 1040), (200, 2064), (24, 12320), (40, 12320), (64, 12320), (500, 2080), (20, 20000),
+                                 (40, 20000), (64, 20000), (24, 40032), (33, 40032), (200, 16448), (100, 33024)])  # fmt: skip
+def test_wide_products(hip_device, dtype, group, m, n):
+    """Workgroups of 32 to 256 weight rows, plain and gated, k of an odd number of blocks."""
+    k = 1056 if group == 32 else 1088 if group == 64 else 1152
+    w, W, mag = _weight(n, k, group, dtype, hip_device, seed=m)
+    x = _x(m, k, dtype, hip_device, n)
+    y, err = _bounds(x, W, mag)
+    _check(linear4(x, w), y, err, dtype)
+    if n % 32 == 0:
+        x = x / float(y.std())  # gates of a spread of 1
+        y, err = _bounds(x, W, mag)
+        (g, u), (eg, eu) = y.chunk(2, -1), err.chunk(2, -1)
+        silu = g * torch.sigmoid(g)
+        es = 1.1 * eg + 2.0**-20 * silu.abs()
+        _check(linear4_silu_mul(x, w), silu * u, es * u.abs() + (silu.abs() + es) * eu, dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(24, 1024, 12288), (40, 512, 8320), (64, 4096, 14336), (100, 1000, 4224), (300, 1024, 8192)])
+def test_split_products(hip_device, m, n, k):
+    """k over several workgroups."""
+    w, W, mag = _weight(n, k, 64, torch.bfloat16, hip_device, seed=m)
+    x = _x(m, k, torch.bfloat16, hip_device, n)
+    _check(linear4(x, w), *_bounds(x, W, mag), torch.bfloat16)
