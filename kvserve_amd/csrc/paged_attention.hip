@@ -52,10 +52,13 @@ constexpr int kWavesPerWG = 4;
 // with 2, 240 with 3, two prompts of 2000 tokens 126 and 118; a lone chunk of 500 tokens, which fills few workgroups, 47.1
 // and 49.1. At D = 64 the third costs more than it saves (203 us, 210 with 3).
 // Under a window, whose masked loop ahead takes registers of its own, MXFP4 keeps 2 (3 spill 11 registers); 16-bit caches
-// of 128-wide heads take 2 as well where these tiles suit the launch better (pre_window_nt).
+// of 128-wide heads take 2 as well where these tiles suit the launch better (pre_window_nt), and those of 64-wide heads
+// always, whose third workgroup per CU then fits (130 VGPRs, 170 with 3; 32 heads over 8: a prompt of 8192 tokens, window
+// 1024, 120 us and 132, of 16000, window 4096, 561 and 631, chunks of 1000 and 900 tokens, window 2048, 73 and 79; a chunk
+// of 200, window 1024, 37 and 35).
 template <int KV, int D, bool WIN>
 constexpr int prefill_nt() {
-  return KV == kKv16 || (KV == kKv4 && D == 128 && !WIN) ? 3 : 2;
+  return (KV == kKv16 && !(WIN && D == 64)) || (KV == kKv4 && D == 128 && !WIN) ? 3 : 2;
 }
 template <int KV, int D, bool WIN>
 constexpr bool prefill_two_tiles() {

@@ -137,7 +137,7 @@ def _product(x: torch.Tensor, weight: Weight4, silu_mul: bool, out: torch.Tensor
 
 
 def linear4(x: torch.Tensor, weight: Weight4, out: torch.Tensor | None = None) -> torch.Tensor:
-    """x [m, k] @ weight.T as [m, n] (in `out` if given): bf16 or fp16, sums in fp32, rounded once. Any m."""
+    """x [m, k] @ weight.T as [m, n] (in `out` if given, which must not overlap x): bf16 or fp16, sums in fp32, rounded once. Any m."""
     return _product(x, weight, False, out)
 
 

@@ -298,3 +298,9 @@ def test_prompts_that_fill_the_launch(hip_device, kv, q_lens, ctx, H, D, window,
     """Tiles of two and of three to a wave, whole to a unit and split between units."""
     b = Batch(hip_device, q_lens, ctx, H, 8, D, 16, window, sinks, torch.bfloat16, kv, seed=len(q_lens) + window)
     b.check(b.forward())
+
+
+@pytest.mark.parametrize("q_lens,ctx,H,window,sinks", [([4000], [0], 32, 300, 0), ([3001], [500], 32, 2000, 4), ([300, 900], [0, 3000], 56, 700, 70)])
+def test_prompts_over_heads_of_64(hip_device, q_lens, ctx, H, window, sinks):
+    b = Batch(hip_device, q_lens, ctx, H, 8, 64, 16, window, sinks, torch.float16, seed=window)
+    b.check(b.forward())
