@@ -33,9 +33,10 @@ constexpr int linear4_lds(const Linear4Form& f) {
 //    where two would load the CUs unevenly ((g 8; 28672 x 4096) 14.4 and 15.1; but (8; 32768 x 4096) 17.9 and 15.5).
 //  * More rows: workgroups of 32, 64, 128 or 256 weight rows, the fewest whose number fits the CUs once, in four slices of
 //    k up to 64: (500; 2048 x 2048) 11.7 with 64, 16.0 with 128; (64; 12288 x 4096) 18.7, 22.1; (64; 6144 x 4096) 14.5 with
-//    32, 15.3 with 64, 16.5 with 128. Each reads all of x: where that is more than 128 MB in all, wider ones ((250; 2048 x
-//    8192) 21.1 with 128, 22.8 with 64), or 80 MB where they would be split besides ((48; 4096 x 8192) 14.8 with 64, 15.4
-//    with 32). What they leave of the CUs is filled by splitting k, four chunks at least each: (33; 2048 x 8192) 10.9 in four.
+//    32, 15.3 with 64, 16.5 with 128. Each reads all of x: wider ones where that is more than 128 MB in all (at 128,
+//    (64; 8192 x 4096), 16.1 with 32, 16.8 with 64), or 80 MB where they would be split besides ((250; 2048 x 8192) 21.1 with
+//    128, 22.8 with 64; (48; 4096 x 8192) 14.8 with 64, 15.4 with 32). What they leave of the CUs is filled by splitting k,
+//    four chunks at least each: (33; 2048 x 8192) 10.9 in four.
 //  * Up to 32 rows eight slices in workgroups of 16 or 32 weight rows, as long as k is short ((20; 4096 x 4096) 8.1, 32 rows
 //    8.9; (20; 6144 x 4096) 9.1, four slices 9.6).
 //  * Where workgroups of 64 weight rows are too many, up to 48 rows of x take four tiles a wave in two groups for one round,

@@ -14,9 +14,9 @@
 // the type. Rows past the last and c past k are padded; there s = 0, and x is read again from its row's end.
 //
 // x goes through LDS a chunk at a time, one chunk ahead, for all waves of a workgroup: read by each wave from the caches it
-// took the loads' path from the weight (8 rows against (28672, 4096), gated: 18.9 us, so 13.7; 64 rows 83 and 30). Where the
+// took the loads' path from the weight (8 rows against (28672, 4096), gated: 18.9 us, so 14.0; 64 rows 83 and 30.5). Where the
 // weight has few rows its k is split over workgroups as well, whose sums a second launch adds in order: every further
-// workgroup of rows reads all of x. Few rows are bound by the codes (those 8: 4.5 TB/s),
+// workgroup of rows reads all of x. Few rows are bound by the codes (those 8: 4.4 TB/s),
 // many by MFMAs and conversion, which add up: 1000 rows against (8192, 4096) 0.8 PFLOP/s.
 #include "kvh_device.h"
 #include "kvh_internal.h"

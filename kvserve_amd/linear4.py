@@ -13,7 +13,7 @@ from kvserve_amd.attention import _calls, _current, _require, _stream_handle
 GROUPS = (32, 64, 128)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Weight4:
     """A weight [n, k] in 4 bits, laid out for `linear4` (kvh_linear4): W[r][c] = scale (code - zero), with a scale and
     a zero point for every row and `group` consecutive columns. Made by `pack` or `quantize_weight4`."""
