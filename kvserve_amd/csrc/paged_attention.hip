@@ -2834,11 +2834,6 @@ __device__ __forceinline__ int64_t pre_seq_positions(const PAParams& p, const Se
   return pre_positions<PR, WIN>(p, s, step, (s.R + PR - 1) / PR);
 }
 
-// x / y of non-negative wave-uniform values, in 32 bits where they fit.
-__device__ __forceinline__ int64_t div_uniform(int64_t x, int64_t y) {
-  return ((uint64_t)x | (uint64_t)y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
-}
-
 __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   return ((int64_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
 }
@@ -2855,15 +2850,29 @@ __device__ __forceinline__ int next_prefill_seq(const PAParams& p, int from) {
 }
 
 // Where a prefill workgroup's unit starts, computed by the workgroup itself (LDS: PreStart
-// and one word per wave): its 256 threads each add up the flat positions of B / 256 sequences, a
+// and kPlanWords): its 256 threads each add up the flat positions of B / 256 sequences, a
 // block scan gives the size C of the flat space, and the wave whose range holds the unit's
 // first position finds the sequence, kv head and tile there, trying 64 tiles at a time.
 struct alignas(16) PreStart {
   int64_t C, x0, x1, qs, ctx;
-  int32_t u, t, rem, q_len, kv_total;
+  int32_t u;  // under a window + kWholeTiles where the units take whole tiles
+  int32_t t, rem, q_len, kv_total;
   uint16_t seq, kvh;  // at most 65535 of each (checked on the host)
 };
 static_assert(sizeof(PreStart) == kPreStartBytes, "the workspace holds one per prefill unit");
+constexpr int kWholeTiles = 1 << 16;
+static_assert(kMaxPrefillUnits * kPrefillRows / (kWavesPerWG * 32) <= kWholeTiles);
+// LDS words of prefill_start: the positions of each wave's sequences, and under a window their tiles (fp32).
+constexpr int kPlanWords = kPlanThreads / 64 * 3 / 2;
+
+// The sum over the wave's lanes, in each of them.
+template <int CTRL>
+__device__ __forceinline__ float add_row_ror(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return sum_over_groups(add_row_ror<0x121>(add_row_ror<0x122>(add_row_ror<0x124>(add_row_ror<0x128>(x)))));
+}
 
 // DIVIDES: whether the group divides PR, known here so that either form of pre_prefix has code of its own (one code
 // for both: 8 decodes of 1000 keys and a 200-token chunk over E4M3 caches 33.0 us, so 32.7).
@@ -2876,9 +2885,12 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
   __builtin_assume(DIVIDES == (step > 0));
   SeqView sv{};  // this thread's last sequence: the only one in batches of up to 256
   int64_t pos = 0;
+  float tiles_in = 0.f;  // under a window: tiles, for a rule that compares their mean alone
   for (int sq = s0; sq < s1; ++sq) {
     sv = seq_view(p, sq);
     pos += (int64_t)p.Hkv * pre_seq_positions<PR, WIN>(p, sv, step);
+    if constexpr (WIN)
+      if (sv.q_len > p.QS) tiles_in += (float)((sv.q_len * p.G + PR - 1) / PR);
   }
   int64_t incl = pos;
 #pragma unroll
@@ -2886,7 +2898,11 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
     const int64_t y = __shfl_up(incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 63) wsum[wv] = incl;
+  if constexpr (WIN) tiles_in = wave_sum(tiles_in);
+  if (lane == 63) {
+    wsum[wv] = incl;
+    if constexpr (WIN) ((float*)(wsum + kPlanThreads / 64))[wv] = tiles_in;
+  }
   __syncthreads();
   int64_t beg = incl - pos, C = 0;
 #pragma unroll
@@ -2902,7 +2918,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
   const int q8 = NUa / 8, r8 = NUa % 8, xcd = b % 8, jj = b / 8;
   if (jj >= q8 + (xcd < r8 ? 1 : 0)) return false;  // idle workgroup (workgroup-uniform)
   const int u = xcd * q8 + min(xcd, r8) + jj;
-  const int64_t x0 = div_uniform((int64_t)u * C, NUa);
+  const int64_t x0 = pre_div((int64_t)u * C, NUa);
   const uint64_t own = __builtin_amdgcn_ballot_w64(beg <= x0 && x0 < beg + pos);  // one thread of one wave
   if (own) {  // that wave, in scalar code (wave-uniform)
     const int l = __builtin_ctzll(own);
@@ -2914,7 +2930,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
       v.ctx = readlane64(sv.ctx, l);
       v.q_len = __builtin_amdgcn_readlane(sv.q_len, l);
       v.kv_total = __builtin_amdgcn_readlane(sv.kv_total, l);
-      per_kvh = div_uniform(readlane64(pos, l), p.Hkv);
+      per_kvh = pre_div(readlane64(pos, l), p.Hkv);
     } else {
       const int end = __builtin_amdgcn_readlane(s1, l);
       for (;; ++sq) {
@@ -2924,7 +2940,7 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
         off -= p.Hkv * per_kvh;
       }
     }
-    const int kvh = (int)div_uniform(off, per_kvh);
+    const int kvh = (int)pre_div(off, per_kvh);
     off -= kvh * per_kvh;
     // the tile: the last one that starts at or before off
     const PreSeq s = pre_seq(p, v);
@@ -2940,8 +2956,16 @@ __device__ __forceinline__ bool prefill_start_as(const PAParams& p, int b, PreSt
       t_beg = readlane64(x, k);
       if (k < 63) break;
     }
+    int unit = u;
+    if constexpr (WIN) {
+      float tiles_of_all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPlanThreads / 64; ++w) tiles_of_all += ((const float*)(wsum + kPlanThreads / 64))[w];
+      if (pre_whole_tiles(C, (int64_t)p.Hkv * uni((int)tiles_of_all), NUa, p.NUP, pre_full_tile(p.G, PR, p.WND, p.SNK)))
+        unit += kWholeTiles;
+    }
     if (lane == 0)
-      *st = PreStart{C, x0, div_uniform((int64_t)(u + 1) * C, NUa), v.qs, v.ctx, u, t, (int)(off - t_beg), v.q_len,
+      *st = PreStart{C, x0, pre_div((int64_t)(u + 1) * C, NUa), v.qs, v.ctx, unit, t, (int)(off - t_beg), v.q_len,
                      v.kv_total, (uint16_t)sq, (uint16_t)kvh};
   }
   __syncthreads();
@@ -2964,7 +2988,7 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
   if constexpr (NX == 1) {
     if (p.ND > 0 && b >= p.ND) {
       __shared__ PreStart st;
-      __shared__ int64_t wsum[kPlanThreads / 64];
+      __shared__ int64_t wsum[kPlanWords];
       bool work;
       if (prefill_two_tiles<KV, D, WIN>() && p.PR == kWavesPerWG * 32)
         work = prefill_start<kWavesPerWG * 32, WIN>(p, b - p.ND, &st, wsum);
@@ -2988,8 +3012,8 @@ __global__ __launch_bounds__(256) void pa_decode_kernel(PAParams p) {
 // same amount of work whatever the mix of prompt lengths. A tile split between units leaves
 // partials: unit u keeps the piece of its first non-empty tile in slot 2u and of its last in
 // slot 2u + 1 (tiles in between are whole and written out), and the unit holding a split
-// tile's first piece records its merge job (in the record of its workgroup). Under a window, where tiles are short and
-// alike, the units take whole tiles where that is cheaper (pre_whole_tiles). Workgroups are
+// tile's first piece records its merge job (in the record of its workgroup). Under a window, where tiles are short, the
+// units take whole tiles where that is cheaper (pre_whole_tiles). Workgroups are
 // dealt to the 8 XCDs round-robin, so the units are numbered XCD by XCD: the units of one
 // XCD are contiguous in the flat space and read the same sequence's K/V through that
 // XCD's L2.
@@ -3010,7 +3034,7 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   }
   const int64_t C = uni64(st->C);
   const int NUa = (int)active_units(C, p.NUP);
-  const int u = uni(st->u);
+  const int u = WIN ? uni(st->u) % kWholeTiles : uni(st->u);
   int kvh = uni(st->kvh);
   int t = uni(st->t);
   int seq = uni(st->seq);
@@ -3030,16 +3054,16 @@ __device__ __forceinline__ void prefill_units(const PAParams& p, int b, char* ld
   // of every unit, so the pieces partition the chunks; a range inside the virtual prefix is
   // empty and skipped.
   int64_t a = uni(st->rem);
+  const bool whole_tiles = WIN && uni(st->u) >= kWholeTiles;
   if constexpr (!PLANNED) __syncthreads();  // every wave has read the start before the tile's loads overwrite it
-  bool first = true, whole_tiles = false;
-  if constexpr (WIN) whole_tiles = pre_whole_tiles(C, NUa, p.NUP, pre_full_tile(p.G, PR, p.WND, p.SNK));
+  bool first = true;
   for (;;) {
     const int64_t tw = kTileCost + n_t;
     if (whole_tiles) {
-      const int64_t mid = x - a + tw / 2;
-      if (mid >= x1) break;
+      const PreTurn turn = pre_tile_turn(x - a, tw, x, x1);
+      if (turn == kPreEnd) break;
       const int rest = (int)max((int64_t)0, x1 - (x - a + tw));
-      if (mid >= x) tile(sv, R, seq, kvh, t, 0, n_t, false, 0, rest, total);
+      if (turn == kPreTake) tile(sv, R, seq, kvh, t, 0, n_t, false, 0, rest, total);
     }
     const int64_t e = whole_tiles ? tw : min(tw, a + (x1 - x));
     const int c_lo = (int)max((int64_t)0, a - kTileCost), c_hi = (int)max((int64_t)0, e - kTileCost);

@@ -143,11 +143,20 @@ KVH_PLAN_FN int64_t pre_skips(const PreSeq& s, int G, int PR, int WND, int SNK, 
 
 // Whether the units of a windowed launch take whole tiles, each those whose middle (its first position + half of its
 // positions) lies in the unit's range, instead of splitting tiles where ranges meet. A split tile's pieces are written in
-// fp32 and read back by the merge, as long as kSplitCost chunk steps where all units hold pieces; whole tiles leave the
-// last of a unit's rounds of `tile` positions (a tile's where its rows see a whole window) part empty. Us split and whole,
-// by the steps left empty (32 heads over 8 of 128, bf16; prompt and window): 2 (3000, 512) 76 and 57, 13 (12000, 1024) 260
-// and 238, 22 (8191, 1024) 194 and 182, 32 (4096, 1024) 108.9 and 110.4, 48 (8191, 2048) 275 and 293. Chunks over 4000
-// tokens: 20 (400, 512) 42 and 31, 29 (512, 1024) 41 and 50; on a third of the units: 21 (40, 512) 26 and 30.
+// fp32 and read back by the merge, as long as kSplitCost chunk steps where all units hold pieces.
+//  * Tiles alike, a full one's positions each (where its rows see a whole window): whole ones leave the last of a unit's
+//    rounds part empty. Us split and whole, by the steps left empty (32 heads over 8 of 128, bf16; prompt and window): 2
+//    (3000, 512) 76 and 57, 13 (12000, 1024) 260 and 238, 22 (8191, 1024) 194 and 182, 32 (4096, 1024) 108.9 and 110.4, 48
+//    (8191, 2048) 275 and 293. Chunks over 4000 tokens: 20 (400, 512) 42 and 31, 29 (512, 1024) 41 and 50; on a third of the
+//    units: 21 (40, 512) 26 and 30.
+//  * Prompts of up to a few windows, whose first tiles are shorter (the mean is below 3/4 of a full one): where ranges
+//    meet a unit is left with a tile too many, and a launch of few tiles with one that outlasts the ranges; half a full tile,
+//    or what it is longer than a range. Three row tiles a wave, us split and whole by these steps: 67 (4600, 4096) 218 and
+//    240, (5000, 4096) 234 and 283, (8000, 4096) 417 and 445, 35 (2500, 2048) 92 and 102, three prompts of (2000, 2048) 147 and 171,
+//    26 (1400, 1024) 58 and 64, 19 (2000, 1024) 71 and 68, eight of (1000, 1024) 115 and 106, 11 eight of (500, 512) 56 and 49. Over
+//    ranges of 9/4 full tiles and more that evens out, between the two units of a CU too, where every split still costs:
+//    2.4 three of (3500, 2048) 299 and 284, 2.6 four of (3000, 2048) 332 and 301, 3.9 four of (5000, 4096) 820 and 794, but two of
+//    (8000, 4096) 803 and 832, 5.4 sixteen of (2000, 2048) 641 and 599; 2.0 three of (4000, 4096) 434 and 478.
 constexpr int kSplitCost = 26;
 
 constexpr int pre_full_tile(int G, int PR, int WND, int SNK) {
@@ -155,10 +164,35 @@ constexpr int pre_full_tile(int G, int PR, int WND, int SNK) {
                            ((int64_t)SNK + kPlanChunk - 1) / kPlanChunk);
 }
 
-// C positions over `units` of the launch's `all` units.
-KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t units, int64_t all, int tile) {
-  const int64_t per = C / units, left = per % tile;
+// x / y of non-negative numbers, in 32 bits where they fit.
+KVH_PLAN_FN int64_t pre_div(int64_t x, int64_t y) {
+  return ((uint64_t)x | (uint64_t)y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// `per` positions of tiles alike for each of `units` of the launch's `all` units; C positions over them.
+KVH_PLAN_FN bool pre_whole_rounds(int64_t per, int64_t units, int64_t all, int tile) {
+  const int64_t left = per - pre_div(per, tile) * tile;
   return left == 0 || (tile - left) * all <= kSplitCost * units;
+}
+KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t units, int64_t all, int tile) {
+  return pre_whole_rounds(pre_div(C, units), units, all, tile);
+}
+
+// C positions of any `tiles` tiles. (Rounds that a range passes by a part of a position leave some units a tile more: the
+// positions of a unit are rounded up.)
+KVH_PLAN_FN bool pre_whole_tiles(int64_t C, int64_t tiles, int64_t units, int64_t all, int tile) {
+  const int64_t per = pre_div(C + units - 1, units);
+  if (4 * C >= 3 * tiles * tile) return pre_whole_rounds(per, units, all, tile);
+  if (4 * C >= 9 * units * tile) return true;
+  return (2 * per < tile ? tile - per : tile / 2) * all <= kSplitCost * units;
+}
+
+// What a unit of positions x .. x1 - 1 (x: where it stands in the tile, or before it) does with a tile of tw positions from
+// beg on, where units take whole ones: nothing, as the unit before took it; take it; or end, as the next one does.
+enum PreTurn { kPreSkip, kPreTake, kPreEnd };
+KVH_PLAN_FN PreTurn pre_tile_turn(int64_t beg, int64_t tw, int64_t x, int64_t x1) {
+  const int64_t mid = beg + tw / 2;
+  return mid >= x1 ? kPreEnd : (mid >= x ? kPreTake : kPreSkip);
 }
 
 // 16-row tiles a wave takes under a window, 3 or 2, for `rows` query rows per kv head in `seqs` sequences: the cheaper by
