@@ -30,8 +30,12 @@ constexpr int linear4_lds(const Linear4Form& f) {
 //  * Up to 16 rows of x: one tile a group as long as the tiles fit the CUs once ((1; 4096 x 4096) 5.2, with two tiles a wave
 //    6.4), in sixteen slices of a long k ((8; 4096 x 14336) 10.9, in eight 11.8); two tiles behind that ((16; 6144 x 4096)
 //    7.1, one 10.5), as long as they fit the CUs once ((16; 8192 x 4096) 7.2, two groups 8.6), then two groups, which share x
-//    ((8; 8208 x 4096) 8.5, one group 11.2, (8; 9216 x 4096) 8.5 and 11.6, (8; 12288 x 4096) 8.7 and 11.9), or four
-//    where two would load the CUs unevenly ((g 8; 28672 x 4096) 14.4 and 15.1; but (8; 32768 x 4096) 17.9 and 15.5).
+//    ((8; 8208 x 4096) 8.5, one group 11.2, (8; 9216 x 4096) 8.5 and 11.6, (8; 12288 x 4096) 8.7 and 11.9). From 1024
+//    tiles on some CUs take two such workgroups and others one: four groups, one workgroup a CU, up to a full round of
+//    them gated ((g 16; 16448 x 4096) 12.8, two groups 14.0, (g 8; 28736 x 4096) 14.1 and 15.1, (g 8; 32768 x 4096) 15.5 and
+//    16.1), up to three quarters of one else, behind which the pairs are nearly even ((16; 16480 x 4096) 13.0 and 14.2,
+//    (16; 20480 x 4096) 13.6 and 14.7, (1; 24576 x 2048) 8.6 and 9.1; but (1; 24576 x 4096) 14.4 and 13.9,
+//    (8; 28672 x 4096) 15.9 and 14.8).
 //  * More rows: workgroups of 32, 64, 128 or 256 weight rows, the fewest whose number fits the CUs once, in four slices of
 //    k up to 64: (500; 2048 x 2048) 11.7 with 64, 16.0 with 128; (64; 12288 x 4096) 18.7, 22.1; (64; 6144 x 4096) 14.5 with
 //    32, 15.3 with 64, 16.5 with 128. Each reads all of x: wider ones where that is more than 128 MB in all (at 128,
@@ -51,7 +55,7 @@ inline Linear4Form linear4_form(int64_t tiles, int64_t blocks, int64_t m, bool g
       return blocks < 48 ? Linear4Form{8, 1, 1, 8, 2, 1} : Linear4Form{8, 1, 1, 16, 2, 1};
     }
     if (tiles <= 512 && !glu) return {16, 2, 1, 8, 2, 1};
-    return tiles > 1024 && tiles <= 1792 ? Linear4Form{16, 2, 4, 4, 2, 1} : Linear4Form{16, 2, 2, 4, 2, 1};
+    return tiles > 1024 && tiles <= (glu ? 2048 : 1536) ? Linear4Form{16, 2, 4, 4, 2, 1} : Linear4Form{16, 2, 2, 4, 2, 1};
   }
   if (m <= 32 && blocks < 48 && !glu) {
     if (tiles <= 256) return {32, 1, 1, 8, 1, 1};

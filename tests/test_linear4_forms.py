@@ -50,3 +50,11 @@ def test_few_rows_take_one_round(form, m, glu):
         for tiles in (*range(2, 530, 2), *range(530, 2049, 14), 2048):
             rows, rt, wr, _, _, lds = form(tiles, blocks, m, glu)
             assert -(-tiles // (rt * wr)) <= 256 * (160 * 1024 // lds), (tiles, blocks)
+
+
+def test_four_groups_up_to_a_round(form):
+    """Plain and gated, the form that was the faster one, and where the rule passes from one to the other."""
+    two, four = (16, 2, 2, 4, 2), (16, 2, 4, 4, 2)
+    for tiles, glu, want in ((1024, 0, two), (1026, 0, four), (1280, 0, four), (1536, 0, four), (1538, 0, two), (1792, 0, two), (2048, 0, two),
+                             (1024, 1, two), (1026, 1, four), (1792, 1, four), (1796, 1, four), (2048, 1, four), (2050, 1, two)):  # fmt: skip
+        assert form(tiles, 32, 8, glu)[:5] == want, (tiles, glu)
