@@ -476,8 +476,8 @@ KVH_API int kvh_gemv_silu_mul(const void* x, int64_t x_row_stride, const void* w
  *   codes  [n / 16][k / 128][4 j][16 r][4 u] dwords: row r of the tile, elements 32 u + 8 j + i of the block, i = 2 p in
  *          bits 4 p .. + 3 and i = 2 p + 1 in bits 16 + 4 p .. + 3
  *   scales [n / 16][k / 128][128 / group][16 r] dwords: s in the low half and 16 + z in the high half, both as dtype; 0 past k
- * x, codes and scales 16-byte aligned, x_row_stride a multiple of 8; y must not overlap x. An infinity in a row of x makes that row
- * of y NaN.
+ * x, codes and scales 16-byte aligned, x_row_stride a multiple of 8; y must not overlap x. Any finite x, and scales below 2^123; an
+ * infinity in a row of x makes that row of y NaN.
  * workspace: kvh_linear4_workspace_size bytes, 16-byte aligned, which may be 0; it needs no clearing, and calls that overlap
  * on one device need one each. The reference has no 4-bit weights.
  */

@@ -6,7 +6,8 @@
 // exponent of 16, so the MFMA multiplies by 16 + q, exact in either type, and nothing is rounded on the way. With ag the sum
 // of x (16 + q) over a group and X the sum of x, the group adds s (ag - (16 + z) X) to a row. x is the A operand, the weight
 // B: a lane then holds sums of one weight row alone, one dword of s and z serves its accumulators, and X, the product with
-// a B operand of ones, comes out in the accumulators' places.
+// a B operand of ones, comes out in the accumulators' places. bf16 operands have the exponents 2^12 lower and the sums are
+// multiplied by 2^12 at the end, which rounds nothing else: 128 x (16 + q) 2^-12 stays in the range of fp32 for any finite x.
 //
 // The weight lies in blocks of 16 rows by 128 c, one wave-wide load of 16 bytes a lane: lane (j, r) holds of row r the
 // elements 32 u + 8 j .. + 7 in dword u, the operand of step u, element 2 p in nibble p and 2 p + 1 in nibble 4 + p.
@@ -27,12 +28,13 @@ namespace {
 
 constexpr int kSteps = kW4Block / 32;  // MFMA steps of a block
 
-// The weight operand of one step, and the 1 of the type twice.
+// The weight operand of one step, in units of 1 / kUnit, and such a unit twice.
 template <class E>
 struct Code;
 template <>
 struct Code<BF16> {
-  static constexpr uint32_t kOne = 0x3f803f80u, kMask = 0x00780078u, k16 = 0x41804180u;
+  static constexpr uint32_t kOne = 0x39803980u, kMask = 0x00780078u, k16 = 0x3b803b80u;
+  static constexpr float kUnit = 4096.f;
   static __device__ __forceinline__ u32x4 operand(uint32_t w, uint32_t o) {
     return u32x4{((w << 3) & kMask) | o, ((w >> 1) & kMask) | o, ((w >> 5) & kMask) | o, ((w >> 9) & kMask) | o};
   }
@@ -40,12 +42,24 @@ struct Code<BF16> {
 template <>
 struct Code<F16> {
   static constexpr uint32_t kOne = 0x3c003c00u, kMask = 0x03c003c0u, k16 = 0x4c004c00u;
+  static constexpr float kUnit = 1.f;
   static __device__ __forceinline__ u32x4 operand(uint32_t w, uint32_t o) {
     return u32x4{((w << 6) & kMask) | o, ((w << 2) & kMask) | o, ((w >> 2) & kMask) | o, ((w >> 6) & kMask) | o};
   }
 };
 
 __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
+
+// Four sums of rows of W, as they are accumulated, as elements of y (GLU: those of a gate, and of its up rows in u).
+template <class E, bool GLU>
+__device__ __forceinline__ f32x4 finish(f32x4 v, const f32x4& u) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] *= Code<E>::kUnit;
+    if constexpr (GLU) v[e] = silu(v[e]) * (u[e] * Code<E>::kUnit);
+  }
+  return v;
+}
 
 // Four neighbouring elements of y, of which some may lie past its last column.
 template <class E>
@@ -287,10 +301,7 @@ __global__ __launch_bounds__(64 * WR * WK) void linear4_kernel(Linear4Args a) {
       if constexpr (GLU) *(f32x4*)(dst + (int64_t)half * 16) = u;
       continue;
     }
-    if constexpr (GLU)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = silu(v[e]) * u[e];
-    store_y<E>(a, row, col, v);
+    store_y<E>(a, row, col, finish<E, GLU>(v, u));
   }
 }
 
@@ -309,10 +320,8 @@ __global__ __launch_bounds__(256) void linear4_sum_kernel(Linear4Args a) {
     src += a.tiles * 8;
     u = *(const f32x4*)src;
     for (int z = 1; z < a.splits; ++z) u += *(const f32x4*)(src + z * step);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = silu(v[e]) * u[e];
   }
-  store_y<E>(a, row, 4 * c, v);
+  store_y<E>(a, row, 4 * c, finish<E, GLU>(v, u));
 }
 
 template <class E, int G, int ROWS, int RT, int WR, int WK, int S, bool GLU>
