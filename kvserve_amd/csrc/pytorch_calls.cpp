@@ -599,8 +599,10 @@ PyObject* linear4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     where.k = x;
     void* stream;
     if (!stream_of(where, &stream)) return nullptr;
-    const int st = f_linear4(x->data_ptr(), x->stride(0), codes->data_ptr(), scales->data_ptr(), out.data_ptr(),
-                             out.stride(0), m, n, k, group, gated, type, need ? ws.data_ptr() : nullptr, need, stream);
+    // the stride of a lone row may be anything
+    const int64_t xs = m > 1 ? x->stride(0) : k, ys = m > 1 ? out.stride(0) : (cols + 3) / 4 * 4;
+    const int st = f_linear4(x->data_ptr(), xs, codes->data_ptr(), scales->data_ptr(), out.data_ptr(), ys, m, n, k, group,
+                             gated, type, need ? ws.data_ptr() : nullptr, need, stream);
     return result(st, a[8], std::move(out));
   });
 }

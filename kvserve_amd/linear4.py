@@ -128,9 +128,11 @@ def _product(x: torch.Tensor, weight: Weight4, silu_mul: bool, out: torch.Tensor
     lib = _lib.load()
     need = lib.kvh_linear4_workspace_size(m, n, k, int(silu_mul))
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    # the stride of a lone row may be anything
+    x_stride, y_stride = (x.stride(0), out.stride(0)) if m > 1 else (k, -(-cols // 4) * 4)
     with _current(x.get_device()):
-        st = lib.kvh_linear4(x.data_ptr(), x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
-                             out.stride(0), m, n, k, weight.group, int(silu_mul), _lib.KVH_DTYPE[x.dtype],
+        st = lib.kvh_linear4(x.data_ptr(), x_stride, weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(),
+                             y_stride, m, n, k, weight.group, int(silu_mul), _lib.KVH_DTYPE[x.dtype],
                              ws.data_ptr() if ws is not None else None, need, _stream_handle(x.device))  # fmt: skip
     _lib.check(st, "kvh_linear4")
     return out
