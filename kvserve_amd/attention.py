@@ -597,11 +597,13 @@ class HipAttention:
         dtype = _dtype_code(qkv, k_cache, v_cache, out) if fmt == _CACHE_DTYPE else _dtype_code(qkv, out)
         if num_tokens == 0:
             return out
+        # the strides of a lone token may be anything
+        qkv_stride, q_stride = (qkv.stride(0), out.stride(0)) if num_tokens > 1 else (qkv.shape[1], 0)
         with _current(dev):
             st = _lib.load().kvh_norm_rope_and_cache(
-                qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                qkv.data_ptr(), qkv_stride, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
                 2 * cos.shape[1], int(interleaved), q_norm.data_ptr() if q_norm is not None else None,
-                k_norm.data_ptr() if k_norm is not None else None, float(eps), out.data_ptr(), out.stride(0), out.stride(1),
+                k_norm.data_ptr() if k_norm is not None else None, float(eps), out.data_ptr(), q_stride, out.stride(1),
                 *caches, slots.data_ptr(), num_tokens, num_blocks, num_heads, num_kv_heads, head_dim, block_size, fmt, ks, vs,
                 dtype, _stream_handle(qkv.device),
             )  # fmt: skip

@@ -554,9 +554,11 @@ PyObject* norm_rope_and_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (!output(a[12], sizes, *qkv, c, &out)) return nullptr;
     void* stream;
     if (!stream_of(c, &stream)) return nullptr;
-    const int st = f_norm_rope(qkv->data_ptr(), qkv->stride(0), (const int64_t*)pos->data_ptr(),
+    // the strides of a lone token may be anything
+    const int64_t qkv_stride = T > 1 ? qkv->stride(0) : qkv->size(1), q_stride = T > 1 ? out.stride(0) : 0;
+    const int st = f_norm_rope(qkv->data_ptr(), qkv_stride, (const int64_t*)pos->data_ptr(),
                                (const float*)cos->data_ptr(), (const float*)sin->data_ptr(), cos->size(0), rotary,
-                               a[11] == Py_True, norm[0], norm[1], (float)eps, out.data_ptr(), out.stride(0),
+                               a[11] == Py_True, norm[0], norm[1], (float)eps, out.data_ptr(), q_stride,
                                out.stride(1), ANY_ARGS(c), (const int64_t*)slots->data_ptr(), T, c.k->size(0), H,
                                c.kv_heads, c.head_dim, c.block_size, c.format, c.k_scale, c.v_scale, dtype, stream);
     return result(st, a[12], std::move(out));

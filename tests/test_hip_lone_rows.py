@@ -5,8 +5,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kvserve_amd import _lib, linear4, linear4_silu_mul
+from kvserve_amd import HipAttention, _lib, linear4, linear4_silu_mul
 from tests.test_hip_linear4 import _weight, _x
+from tests.test_hip_norm_rope import _caches
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,21 @@ def test_a_column_turned_round(hip_device, path):
     w, _, _ = _weight(48, 128, 32, torch.float16, hip_device)
     x = _x(1, 128, torch.float16, hip_device)
     assert torch.equal(linear4(x.reshape(128, 1).t(), w), linear4(x, w))
+
+
+@pytest.mark.parametrize("stride", [0, 1, 7, 2**40])
+@pytest.mark.parametrize("kv", ["own", "e4m3", "fp4"])
+def test_norm_rope_and_cache(hip_device, path, stride, kv):
+    dev = hip_device
+    qkv = torch.randn((1, 8 * 64), device=dev).bfloat16()
+    cos, sin = torch.rand((9, 32), device=dev), torch.rand((9, 32), device=dev)
+    got = []
+    for lone in (False, True):
+        k, v, scales = _caches(kv, 2, 16, 2, 64, torch.bfloat16, dev)
+        buf = torch.full((3, 4, 64), 5.0, dtype=qkv.dtype, device=dev)
+        x, out = (_lone(qkv, stride), _lone(buf[1:2], stride)) if lone else (qkv, buf[1:2])
+        one = torch.tensor([3], device=dev)
+        HipAttention.norm_rope_and_cache(x, one, cos, sin, k, v, one, 4, out=out, **scales)
+        got.append([buf, *(t.view(torch.uint8) for t in (k, v))])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert not (got[0][0][1] == 5).all() and (got[0][0][[0, 2]] == 5).all()
