@@ -68,7 +68,7 @@ class Weight4:
         pair = torch.stack((scales, (zeros.int() + 16).to(scales.dtype)), dim=-1).contiguous().view(torch.int32)[..., 0]
         full = torch.zeros((16 * tiles, blocks * (128 // group)), dtype=torch.int32, device=codes.device)
         full[:n, : k // group] = pair
-        return cls(packed.view(tiles, blocks, 256), full.view(tiles, 16, -1).transpose(1, 2).contiguous(), (n, k), group,
+        return cls(packed.view(tiles, blocks, 256), full.view(tiles, 16, full.shape[1]).transpose(1, 2).contiguous(), (n, k), group,
                    scales.dtype)  # fmt: skip
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -77,9 +77,9 @@ class Weight4:
         d = self.codes.view(tiles, blocks, 4, 16, 4).permute(0, 3, 1, 4, 2)[..., None]  # tile, row, block, u, j
         p = 4 * torch.arange(4, dtype=torch.int32, device=self.device)
         q = torch.stack(((d >> p) & 15, (d >> (p + 16)) & 15), dim=-1).reshape(16 * tiles, 128 * blocks)[:n, :k]
-        pair = self.scales.transpose(1, 2).reshape(16 * tiles, -1)[:n, : k // self.group]
+        pair = self.scales.transpose(1, 2).reshape(16 * tiles, self.scales.shape[1])[:n, : k // self.group]
         s, z = (half.to(torch.int16).view(self.dtype).float() for half in (pair, pair >> 16))
-        return ((q.view(n, -1, self.group) - (z - 16)[..., None]) * s[..., None]).view(n, k).to(dtype)
+        return ((q.view(n, k // self.group, self.group) - (z - 16)[..., None]) * s[..., None]).view(n, k).to(dtype)
 
     def to(self, device: torch.device | str) -> Weight4:
         return Weight4(self.codes.to(device), self.scales.to(device), self.shape, self.group, self.dtype)
