@@ -87,15 +87,17 @@ class Weight4:
 
 def quantize_weight4(weight: torch.Tensor, group: int = 128) -> Weight4:
     """A bf16 or fp16 weight [n, k] rounded to the nearest of 16 evenly spaced values over each group's range, zero among
-    them. k a multiple of `group`."""
+    them. k a multiple of `group`; a group's range below 15 * 2^123, which is checked, so it waits for the device."""
     _require(weight.dim() == 2 and weight.dtype in (torch.bfloat16, torch.float16), "weight must be bf16 or fp16 [n, k]")
     _require(group in GROUPS and weight.shape[1] % group == 0 and weight.shape[1] > 0,
              f"groups must be of {GROUPS} columns that divide k (got {group}, k = {weight.shape[1]})")  # fmt: skip
     codes, scales, zeros = [], [], []
     for part in weight.split(1024):
-        w = part.float().unflatten(1, (-1, group))
+        w = part.float().unflatten(1, (weight.shape[1] // group, group))
         lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
         s = ((hi - lo) / 15).to(weight.dtype)
+        # what kvh_linear4 takes; a NaN is in its group's range
+        _require(bool((s < 2.0**123).all()), "weight must be finite, its groups' ranges below 15 * 2^123")
         step = s.float().masked_fill(s == 0, 1.0)
         z = (-lo / step).round().clamp(0, 15)
         q = ((w / step[..., None]).round() + z[..., None]).clamp(0, 15).to(torch.uint8).flatten(1)

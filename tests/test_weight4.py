@@ -19,6 +19,32 @@ def test_no_rows(dtype, group):
         assert w.dequantize().shape == (0, 384) and w.to("cpu").shape == w.shape
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_quantised_weights_are_finite(dtype, value):
+    w = torch.ones((1500, 64), dtype=dtype)
+    quantize_weight4(w, 32)
+    w[1400, 63] = value
+    with pytest.raises(ValueError, match="finite"):
+        quantize_weight4(w, 32)
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.float16, 65504.0), (torch.bfloat16, 7.5e37)], ids=str)
+def test_largest_weights(dtype, top):
+    """Groups over the type's range, or up to the largest scale: within a step of 2 top / 15, and the scale's rounding."""
+    w = (torch.linspace(-1, 1, 64, dtype=torch.float64) * top).to(dtype).repeat(3, 1)
+    back = quantize_weight4(w, 64).dequantize(torch.float64)
+    step = 2 * top / 15
+    assert ((back - w.double()).abs() <= step * (1 + 15 * torch.finfo(dtype).eps / 2)).all()
+
+
+def test_ranges_past_the_scales():
+    top = torch.finfo(torch.bfloat16).max
+    for lo, hi in ((-top, top), (0.0, top), (-8e37, 8.1e37)):
+        with pytest.raises(ValueError, match="ranges"):
+            quantize_weight4(torch.tensor([[lo, hi] * 16], dtype=torch.bfloat16), 32)
+
+
 @pytest.mark.gpu
 def test_products_with_no_rows(hip_device):
     w = quantize_weight4(torch.zeros((0, 384), dtype=torch.bfloat16, device=hip_device))
