@@ -30,6 +30,7 @@ sinks; projections held in 4 bits (`quantize_projections4`) run on `linear4`.
 
 from __future__ import annotations
 
+import inspect
 import math
 from dataclasses import dataclass, field, replace
 from pathlib import Path
@@ -236,6 +237,11 @@ class StageOut(NamedTuple):
     normed: torch.Tensor | None  # [T, hidden] the layer's normalised input
 
 
+def _takes_windows(backend) -> bool:
+    args = inspect.signature(backend.forward).parameters
+    return {"window", "sinks"} <= args.keys() or any(a.kind == a.VAR_KEYWORD for a in args.values())
+
+
 class PagedLlama:
     """A Llama decoder over the flat paged batch, calling an attention backend with kvserve's
     interface (`write_kv` / `forward`, src/kvserve/attention.py:39-102)."""
@@ -245,6 +251,8 @@ class PagedLlama:
         if cfg.attention_sinks < 0 or (cfg.sliding_window is None and cfg.attention_sinks) or (
                 cfg.sliding_window is not None and cfg.sliding_window < 1):  # fmt: skip
             raise ValueError(f"window {cfg.sliding_window} with {cfg.attention_sinks} sinks")
+        if any(cfg.window(i) is not None for i in range(cfg.num_layers)) and not _takes_windows(backend):
+            raise ValueError("the backend has no sliding windows (forward takes no window and sinks)")
         self.cfg = cfg
         self.w = weights
         self.backend = backend
