@@ -253,6 +253,11 @@ class PagedLlama:
             raise ValueError(f"window {cfg.sliding_window} with {cfg.attention_sinks} sinks")
         if any(cfg.window(i) is not None for i in range(cfg.num_layers)) and not _takes_windows(backend):
             raise ValueError("the backend has no sliding windows (forward takes no window and sinks)")
+        rotary = cfg.head_dim if cfg.rotary_dim is None else cfg.rotary_dim
+        if not 0 <= rotary <= cfg.head_dim or rotary % 2:
+            raise ValueError(f"rotary_dim {rotary} of heads of {cfg.head_dim}")
+        if any((w is not None) != cfg.qk_norm for lw in weights.layers for w in (lw.q_norm, lw.k_norm)):
+            raise ValueError("norms of query and key heads in the config or in the weights, but not in both")
         self.cfg = cfg
         self.w = weights
         self.backend = backend

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from kvserve_amd.attention import HipAttention
-from kvserve_amd.engine.model import build_model
+from kvserve_amd.engine.model import PagedLlama, build_model, random_weights
 from tests.engine_backends import TorchRefAttention
 from tests.test_engine_operators import ALL, WindowedTorch
 
@@ -25,3 +25,21 @@ def test_backends_without_windows():
         build_model(ALL, "cpu", torch.float32, 64, backend=backend)
     full = replace(ALL, full_layers=tuple(range(ALL.num_layers)))  # no layer has the window
     build_model(full, "cpu", torch.float32, 64, backend=TorchRefAttention)
+
+
+@pytest.mark.parametrize("rotary", [-2, 31, 66])
+def test_rotated_elements(rotary):
+    with pytest.raises(ValueError, match="rotary_dim"):
+        build_model(replace(ALL, rotary_dim=rotary), "cpu", torch.float32, 64, backend=WindowedTorch)
+
+
+def test_norms_of_config_and_weights():
+    """Norms that one of the two lacks would be left out, or taken, without a word."""
+    plain = replace(ALL, qk_norm=False)
+    for cfg, of in ((ALL, plain), (plain, ALL)):
+        with pytest.raises(ValueError, match="norms"):
+            PagedLlama(cfg, random_weights(of, "cpu", torch.float32), WindowedTorch)
+    w = random_weights(ALL, "cpu", torch.float32)
+    w.layers[-1].k_norm = None
+    with pytest.raises(ValueError, match="norms"):
+        PagedLlama(ALL, w, WindowedTorch)
