@@ -306,9 +306,10 @@ class PagedLlama:
         return x, rms_norm(x, weight, eps)
 
     def _mlp(self, h: torch.Tensor, lw: LayerWeights) -> torch.Tensor:
-        if isinstance(lw.w_gate_up, Weight4) and h.is_cuda:
+        packed = isinstance(lw.w_gate_up, Weight4)
+        if packed and h.is_cuda and lw.w_gate_up.shape[0] % 32 == 0:  # (what linear4_silu_mul takes)
             return self._linear(linear4_silu_mul(h, lw.w_gate_up), lw.w_down)
-        if self.fused_ops:
+        if self.fused_ops and not packed:
             return self._linear(ops.mlp_act(h, lw.w_gate_up), lw.w_down)
         gate, up = self._linear(h, lw.w_gate_up).chunk(2, dim=-1)
         return self._linear(F.silu(gate) * up, lw.w_down)

@@ -9,8 +9,10 @@ import torch
 
 from kvserve_amd.attention import HipAttention
 from kvserve_amd.engine.model import PagedLlama, build_model, random_weights
+from kvserve_amd.engine.runner import ModelRunner
+from kvserve_amd.linear4 import quantize_weight4
 from tests.engine_backends import TorchRefAttention
-from tests.test_engine_operators import ALL, WindowedTorch
+from tests.test_engine_operators import ALL, POOLS, WindowedTorch, _error, _model, _run
 
 
 def test_backends_without_windows():
@@ -43,3 +45,14 @@ def test_norms_of_config_and_weights():
     w.layers[-1].k_norm = None
     with pytest.raises(ValueError, match="norms"):
         PagedLlama(ALL, w, WindowedTorch)
+
+
+@pytest.mark.gpu
+def test_gate_rows_that_fill_no_tile(hip_device):
+    """An MLP of 648: 40.5 tiles of gate rows, which linear4_silu_mul does not take."""
+    cfg = replace(ALL, intermediate_size=648)
+    model = _model(cfg, hip_device, torch.bfloat16, HipAttention)
+    for lw in model.w.layers:
+        lw.w_gate_up = quantize_weight4(lw.w_gate_up, 128)
+    errs = [_error(model, _run(ModelRunner(model, num_blocks=96, max_model_len=256, decode_graphs=g), cfg)) for g in (False, True)]
+    assert max(errs) < POOLS["bf16"][1], errs
