@@ -275,6 +275,8 @@ class PagedLlama:
         # torch, write_kv with v a strided view of the fused QKV output, then forward(out=...).
         fused = "norm_rope_and_cache" if self.head_rope else "rope_and_cache"
         offered = callable(getattr(backend, fused, None))
+        if self.head_rope and (rotary % 16 or cfg.head_dim % 8 or cfg.head_dim > 256):
+            offered = False  # shapes that norm_rope_and_cache does not take
         if fused_rope and not offered:
             raise ValueError(f"the backend has no fused RoPE + cache write ({fused})")
         self.fused_rope = offered if fused_rope is None else bool(fused_rope)

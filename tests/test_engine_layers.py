@@ -47,6 +47,21 @@ def test_norms_of_config_and_weights():
         PagedLlama(ALL, w, WindowedTorch)
 
 
+def test_rotations_that_the_kernel_does_not_take():
+    """Pairs that are no multiple of 8 go step by step, unless the fused kernel is asked for."""
+    cfg = replace(ALL, rotary_dim=24)
+    assert not build_model(cfg, "cpu", torch.float32, 64).fused_rope and build_model(ALL, "cpu", torch.float32, 64).fused_rope
+    with pytest.raises(ValueError, match="fused"):
+        build_model(cfg, "cpu", torch.float32, 64, fused_rope=True)
+
+
+@pytest.mark.gpu
+def test_rotations_step_by_step(hip_device):
+    cfg = replace(ALL, rotary_dim=24)
+    model = _model(cfg, hip_device, torch.bfloat16, HipAttention)
+    assert _error(model, _run(ModelRunner(model, num_blocks=96, max_model_len=256), cfg)) < POOLS["bf16"][1]
+
+
 @pytest.mark.gpu
 def test_gate_rows_that_fill_no_tile(hip_device):
     """An MLP of 648: 40.5 tiles of gate rows, which linear4_silu_mul does not take."""
