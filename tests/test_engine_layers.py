@@ -12,7 +12,7 @@ from kvserve_amd.engine.model import PagedLlama, build_model, random_weights
 from kvserve_amd.engine.runner import ModelRunner
 from kvserve_amd.linear4 import quantize_weight4
 from tests.engine_backends import TorchRefAttention
-from tests.test_engine_operators import ALL, POOLS, WindowedTorch, _error, _model, _run
+from tests.test_engine_operators import ALL, POOLS, STEPS, WindowedTorch, _error, _model, _run
 
 
 def test_backends_without_windows():
@@ -71,3 +71,26 @@ def test_gate_rows_that_fill_no_tile(hip_device):
         lw.w_gate_up = quantize_weight4(lw.w_gate_up, 128)
     errs = [_error(model, _run(ModelRunner(model, num_blocks=96, max_model_len=256, decode_graphs=g), cfg)) for g in (False, True)]
     assert max(errs) < POOLS["bf16"][1], errs
+
+
+NEAR = [
+    {"sliding_window": 23}, {"sliding_window": 25}, {"attention_sinks": 2}, {"attention_sinks": 4}, {"full_layers": ()},
+    {"full_layers": (1, 2)}, {"full_layers": (0,)}, {"rotary_dim": 48}, {"rope_interleaved": False},
+]  # fmt: skip
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pool", POOLS)
+def test_no_other_layers_are_nearer(hip_device, pool):
+    """The logits are nearer to the 64-bit model of their own config than to any that differs by one key of a window, one
+    sink, one layer or the rotation, over prompts that a window leaves keys out of: whatever the errors, a model that
+    computed one of the others would be nearer to that."""
+    dtype, _ = POOLS[pool]
+    model = _model(ALL, hip_device, torch.bfloat16, HipAttention, 128)
+    got = [g for g in _run(ModelRunner(model, num_blocks=96, max_model_len=256, kv_cache_dtype=dtype), ALL)
+           if len(g[0]) > ALL.sliding_window + ALL.attention_sinks + STEPS]  # fmt: skip
+    assert len(got) == 2
+    own = _error(model, got, dtype)
+    for over in NEAR:
+        model.cfg = replace(ALL, **over)
+        assert own < _error(model, got, dtype), over
