@@ -212,7 +212,7 @@ KVH_API int kvh_rope_and_cache_fp4(const void* qkv, int64_t qkv_tok_stride, cons
  * cos_table / sin_table: fp32 [max_positions, rotary_dim / 2], one entry for each pair (frequencies and factors of
  * stretched contexts are the tables'); unused with rotary_dim = 0. The queries are written to q_out, the keys and the
  * (untouched) values to the pool at slot_mapping[t] (slots outside the pool are skipped). Computed in fp32 and rounded
- * once: the queries to dtype, the keys to the cache's format.
+ * once: the queries to dtype, the keys to the cache's format. (Squares in fp32: a normed head needs |x| below 2^60.)
  * cache_format and scales as in kvh_paged_attention_window. head_dim a multiple of 8 (MXFP4: of 32) up to 256, rotary_dim
  * a multiple of 16 up to head_dim; pointers 16-byte aligned (E4M3 caches 8, MXFP4 ones 4) and rows' strides likewise.
  */
@@ -468,8 +468,8 @@ KVH_API int kvh_gemv_silu_mul(const void* x, int64_t x_row_stride, const void* w
 
 /*
  * linear4: y = x W^T with a weight held in 4 bits, W[r][c] = s[r][c / group] (q[r][c] - z[r][c / group]), codes q and zero points
- * z in 0 .. 15; x [m, k] and y [m, n] fp16 or bf16 (dtype), the scales of that type, sums in fp32, rounded once. m below 2^20,
- * n up to 2^28; group 32, 64 or 128, k a multiple of it. silu_mul: the rows of W are n / 2 gate rows, then as many up rows
+ * z in 0 .. 15; x [m, k] and y [m, n] fp16 or bf16 (dtype), the scales of that type, sums in fp32, rounded once. m up to
+ * 1048560, n up to 2^28; group 32, 64 or 128, k a multiple of it. silu_mul: the rows of W are n / 2 gate rows, then as many up rows
  * (n % 32 == 0), and
  *   y[i][j] = silu(g) * u, g and u the products with rows j and n / 2 + j, rounded once; y is [m, n / 2].
  * The weight is packed once (all sizes rounded up, little endian):

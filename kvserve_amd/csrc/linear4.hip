@@ -17,8 +17,10 @@
 // x goes through LDS a chunk at a time, one chunk ahead, for all waves of a workgroup: read by each wave from the caches it
 // took the loads' path from the weight (8 rows against (28672, 4096), gated: 18.9 us, so 14.0; 64 rows 83 and 30.5). Where the
 // weight has few rows its k is split over workgroups as well, whose sums a second launch adds in order: every further
-// workgroup of rows reads all of x. Few rows are bound by the codes (those 8: 4.4 TB/s),
-// many by MFMAs and conversion, which add up: 1000 rows against (8192, 4096) 0.8 PFLOP/s.
+// workgroup of rows reads all of x. Few rows are bound by the codes (those 8: 4.3 TB/s),
+// many by the vector instructions beside the MFMAs, about four to one (64 rows of x and 64 of the weight, a block in one
+// group: 68 MFMAs, 128 instructions that convert, 64 that multiply by s, 64 that take out z), of which two would hide: 1000 rows
+// against (8192, 4096) 0.77 PFLOP/s, in groups of 64 and 32, whose part grows with their number, 0.68 and 0.55.
 #include "kvh_device.h"
 #include "kvh_internal.h"
 #include "linear4.h"

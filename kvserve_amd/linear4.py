@@ -141,11 +141,12 @@ def _product(x: torch.Tensor, weight: Weight4, silu_mul: bool, out: torch.Tensor
 
 
 def linear4(x: torch.Tensor, weight: Weight4, out: torch.Tensor | None = None) -> torch.Tensor:
-    """x [m, k] @ weight.T as [m, n] (in `out` if given, which must not overlap x): bf16 or fp16, sums in fp32, rounded once. Any m."""
+    """x [m, k] @ weight.T as [m, n] (in `out` if given, which must not overlap x): bf16 or fp16, sums in fp32, rounded once. Up to
+    1048560 rows; an infinity in a row makes its result NaN. Forward only: the output carries no gradient."""
     return _product(x, weight, False, out)
 
 
 def linear4_silu_mul(x: torch.Tensor, weight: Weight4, out: torch.Tensor | None = None) -> torch.Tensor:
     """SiLU(x @ gate.T) * (x @ up.T) as [m, n / 2] of a weight whose first n / 2 rows are the gate's (n a multiple of 32);
-    rounded once, behind the product."""
+    rounded once, behind the product. Otherwise as linear4."""
     return _product(x, weight, True, out)
